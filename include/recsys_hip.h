@@ -768,6 +768,45 @@ int rx_zero_unused_slots(const int64_t* d_counts, int32_t G, int64_t capacity, i
 int rx_topk_codes(const float* d_scores, const int64_t* d_codes, int64_t rows, int32_t n,
                   int32_t k, int64_t* d_out, int device, void* stream);
 
+/* ------------------------------------------------------------------ list-wise log-probabilities
+ * For scores l [R, V] (fp32, or bf16 with bf16 = 1; rows `ld` elements apart) of which row r has the first
+ * lengths[r] columns (NULL: all; clamped to [0, V]):
+ *   lse[r] = log sum_v exp l_rv      logprob[r, t] = l_{r, y_rt} - lse[r]      entropy[r] = -sum_v p_rv log p_rv
+ * and the k largest scores of the row as log-probabilities with their columns, in descending order, the lower column
+ * first among equal scores.  A score of -inf is masked: it has no probability and is no alternative.  Where a row
+ * has fewer than k alternatives the rest is (-inf, -1).  A row with nothing left (length 0, or -inf throughout) gives
+ * lse -inf, entropy 0, logprob -inf and no gradient.  A target of -1 stands for "no target" (logprob 0); any other
+ * target outside [0, V) sets RX_ERR_INDEX and gives NaN; a masked one gives -inf.  NaN in a live column makes the row's
+ * results NaN (its alternatives are then unspecified, but valid columns), and so does +inf.
+ * Accumulation in fp32.  Loss and evaluation over lists and catalogues; the reference ranks on the host
+ * (recsys/utils.py:40-58) and has no softmax loss. */
+typedef struct {
+  const void* logits;
+  int64_t ld;                /* elements between rows, >= V */
+  int64_t R, V;              /* V < 2^31 - 64 */
+  const int64_t* lengths;    /* [R] or NULL */
+  const int64_t* targets;    /* [R, T] */
+  int32_t T;                 /* 0..1024 */
+  int32_t k;                 /* 0..64 */
+  int32_t bf16;
+  int32_t pad_;
+  float* logprob;            /* [R, T] */
+  float* lse;                /* [R] */
+  float* entropy;            /* [R] */
+  float* top_logprob;        /* [R, k] */
+  int64_t* top_index;        /* [R, k] */
+  float* stats;              /* [R, 4], 16-byte aligned: written by rx_logprob_fwd (NULL: left out), read by rx_logprob_bwd */
+} rx_logprob_args;
+size_t rx_logprob_workspace_bytes(int64_t R, int64_t V, int32_t k);
+int rx_logprob_fwd(const rx_logprob_args* args, void* ws, size_t ws_bytes, int32_t* err_flag, int device, void* stream);
+/* dlogits [R, V] (the scores' type, rows ld_d apart; columns past a row's end get 0) from the gradients of logprob
+ * [R, T], entropy [R] and lse [R] (each may be NULL = zero):
+ *   dl_v = sum_t g_t (1[v = y_t] - p_v) + g_lse p_v - g_H p_v (log p_v + H)
+ * over the targets that carry a probability.  Needs logits, lengths, targets and the stats of the forward call; the
+ * outputs of the forward call in `args` are not read. */
+int rx_logprob_bwd(const rx_logprob_args* args, const float* d_g_logprob, const float* d_g_entropy, const float* d_g_lse,
+                   void* d_dlogits, int64_t ld_d, int device, void* stream);
+
 /* ------------------------------------------------------------------ dense layers, bf16 activations in HBM
  * The Linear(+ReLU) stacks and DCN-v2 cross layers of recsys_amd.models.fields (a14; the towers of
  * recsys/models/neuralcf/deep_factorization_machine.py:6-24 in their bf16 option) with every

@@ -96,6 +96,12 @@ class SegTable(C.Structure):
                 ("n_rows", i64), ("sq_part", vp)]
 
 
+class LogProbArgs(C.Structure):
+    _fields_ = [("logits", vp), ("ld", i64), ("R", i64), ("V", i64), ("lengths", vp), ("targets", vp), ("T", i32), ("k", i32),
+                ("bf16", i32), ("pad_", i32), ("logprob", vp), ("lse", vp), ("entropy", vp), ("top_logprob", vp), ("top_index", vp),
+                ("stats", vp)]
+
+
 # name -> (restype, argtypes); must list every symbol of include/recsys_hip.h
 PROTOTYPES = {
     "rx_abi_version": (C.c_int, []),
@@ -198,6 +204,9 @@ PROTOTYPES = {
     "rx_zero_unused_slots": (C.c_int, [vp, i32, i64, i32, vp, vp, C.c_int, vp]),
     "rx_fm_flat_rows": (C.c_int, [vp, vp, i64, i32, vp, C.c_int, vp]),
     "rx_compose_slots": (C.c_int, [vp, vp, i64, i64, vp, vp, C.c_int, vp]),
+    "rx_logprob_workspace_bytes": (sz, [i64, i64, i32]),
+    "rx_logprob_fwd": (C.c_int, [C.POINTER(LogProbArgs), vp, sz, vp, C.c_int, vp]),
+    "rx_logprob_bwd": (C.c_int, [C.POINTER(LogProbArgs), vp, vp, vp, vp, i64, C.c_int, vp]),
     "rx_topk_codes": (C.c_int, [vp, vp, i64, i32, i32, vp, C.c_int, vp]),
 }
 

@@ -15,6 +15,7 @@ from typing import Optional, Sequence
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 import os
@@ -1028,3 +1029,35 @@ class BCEWithLogits(Function):
 
 def bce_with_logits(logits: Tensor, labels: Tensor) -> Tensor:
     return BCEWithLogits.apply(logits, labels)
+
+
+# ------------------------------------------------------------------ list-wise log-probabilities
+class LogProb(Function):
+    """ops.logprob_fwd with its gradient (rx_logprob_bwd) to the scores; the alternatives carry none."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, lengths, k):
+        out, stats = ops.logprob_fwd(logits, targets, lengths, k, want_stats=ctx.needs_input_grad[0])
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(out.top_logprob, out.top_index)
+        ctx.save_for_backward(logits, targets, lengths, stats)
+        return tuple(out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, gh, gl, _top, _idx):
+        logits, targets, lengths, stats = ctx.saved_tensors
+        if g is None and gh is None and gl is None:
+            return None, None, None, None
+        g, gh, gl = (None if t is None else t.contiguous() for t in (g, gh, gl))
+        return ops.logprob_bwd(logits, targets, lengths, stats, g, gh, gl), None, None, None
+
+
+def log_probs(logits: Tensor, targets: Tensor, lengths: Optional[Tensor] = None, k: int = 0) -> ops.LogProbs:
+    """Log-probabilities of ``targets`` ([R] or [R, T] columns; -1 = none) under the softmax over each row of ``logits``
+    ([R, V] fp32 or bf16; -inf masks a score, ``lengths`` [R] ends the rows), the rows' entropy, log-sum-exp and ``k`` best
+    alternatives (k <= 64, descending, the lower column first among equal scores).  ``logprob``, ``entropy`` and
+    ``lse`` are differentiable."""
+    if logits.dim() == 2 and ((logits.shape[1] > 1 and logits.stride(1) != 1) or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1])):
+        logits = logits.contiguous()
+    return ops.LogProbs(*LogProb.apply(logits, targets.contiguous(), None if lengths is None else lengths.contiguous(), k))

@@ -39,6 +39,24 @@ extern thread_local char rx_err_buf[512];
     RX_HIP(hipSetDevice(device));                        \
   } while (0)
 
+// The same for the length of a call: the caller's device is current again when the entry point returns.
+struct RxDeviceGuard {
+  int prev = -1;
+  ~RxDeviceGuard() { if (prev >= 0) (void)hipSetDevice(prev); }
+  hipError_t enter(int device) {
+    int cur = -1;
+    hipError_t e = hipGetDevice(&cur);
+    if (e != hipSuccess || cur == device) return e;
+    e = hipSetDevice(device);
+    if (e == hipSuccess) prev = cur;
+    return e;
+  }
+};
+#define RX_GUARD_DEVICE(device)                          \
+  RX_REQUIRE((device) >= 0, "negative device ordinal");  \
+  RxDeviceGuard rx_guard_;                               \
+  RX_HIP(rx_guard_.enter(device))
+
 #define RX_LAUNCH_CHECK() RX_HIP(hipGetLastError())
 
 static inline int64_t rx_cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }

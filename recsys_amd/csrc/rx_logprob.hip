@@ -1,0 +1,792 @@
+// List-wise log-probabilities (gfx950): for scores l [R, V], per row
+//   lse = log sum_v exp l_v,  logprob_t = l_{y_t} - lse,  H = lse - sum_v p_v l_v,  the k largest l_v,
+// and the gradient  dl_v = sum_t g_t (1[v = y_t] - p_v) + g_lse p_v - g_H p_v (log p_v + H).
+//
+// Both directions read every score once and are bound by that read (and the write of dl): the softmax statistics are
+// online.  Each lane keeps its own running reference m (log2 units), sum s = sum 2^(l' - m) and t = sum 2^(l' - m) (l' - m)
+// with l' = l log2(e); the reference moves only when a score exceeds it by 2^4, so the rescale is off the common path,
+// and lanes, wavefronts and column splits are joined at the end.  All sums are fp32, whatever the scores' type.
+// Alternatives: a wavefront keeps the 64 best keys (value, column) sorted across its lanes; scores that beat the k-th
+// one are collected in a small LDS buffer and merged 64 at a time, so a row costs one compare per 16 bytes in the
+// common case.  Keys order by value, then by the lower column, and are unique, so the result does not depend on
+// how the row was split.
+#include "rx_common.h"
+
+#define LP_SMALL 1024        // rows up to this width: one wavefront (or part of one) per row, scores in registers
+#define LP_TOP 64            // most alternatives per row
+#define LP_SPLIT_MIN 4096    // fewest columns worth a split of their own
+#define LP_SPLIT_MAX 256
+#define LP_L2E 1.44269504088896340736f
+#define LP_LN2 0.69314718055994530942f
+#define LP_BIG 1e38f         // beyond this l * log2(e) leaves fp32: such rows take the form exp((l - m) log2 e)
+#define LP_NINF (-__builtin_inff())
+
+struct LpPart {   // one split's share of a row
+  float raw;      // largest score
+  float m2;       // reference of s and t (log2 units; the score itself when |raw| > LP_BIG)
+  float s, t;
+};
+
+// ---------------------------------------------------------------- element access
+template <typename T> __device__ __forceinline__ float lp_elem(const T* p);
+template <> __device__ __forceinline__ float lp_elem<float>(const float* p) { return *p; }
+template <> __device__ __forceinline__ float lp_elem<uint16_t>(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
+
+template <typename T> struct LpVec { static constexpr int N = 16 / (int)sizeof(T); };
+
+template <typename T>
+__device__ __forceinline__ void lp_unpack(const uint4& q, float* v);
+template <>
+__device__ __forceinline__ void lp_unpack<float>(const uint4& q, float* v) {
+  v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y); v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
+}
+template <>
+__device__ __forceinline__ void lp_unpack<uint16_t>(const uint4& q, float* v) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+__device__ __forceinline__ uint16_t lp_to_bf16(float f) {   // round to nearest even; NaN stays NaN
+  const uint32_t u = __float_as_uint(f);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
+  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+template <typename T> __device__ __forceinline__ void lp_put(T* p, float f);
+template <> __device__ __forceinline__ void lp_put<float>(float* p, float f) { *p = f; }
+template <> __device__ __forceinline__ void lp_put<uint16_t>(uint16_t* p, float f) { *p = lp_to_bf16(f); }
+
+__device__ __forceinline__ float lp_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ---------------------------------------------------------------- alternatives
+// key: order-preserving image of the value above, complemented column below; larger key = better alternative
+__device__ __forceinline__ uint64_t lp_key(float v, int32_t col) {
+  const uint32_t u = __float_as_uint(v + 0.0f);            // -0 counts as 0
+  const uint32_t o = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return ((uint64_t)o << 32) | (uint32_t)~col;
+}
+__device__ __forceinline__ float lp_key_value(uint64_t key) {
+  const uint32_t o = (uint32_t)(key >> 32);
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+__device__ __forceinline__ int32_t lp_key_col(uint64_t key) { return (int32_t)~(uint32_t)key; }
+// key 0 is no score's key: value bits 0 would be the image of a negative NaN
+
+__device__ __forceinline__ uint64_t lp_shfl_xor64(uint64_t x, int m) {
+  const uint32_t lo = __shfl_xor((uint32_t)x, m, 64), hi = __shfl_xor((uint32_t)(x >> 32), m, 64);
+  return ((uint64_t)hi << 32) | lo;
+}
+// keys of the wavefront's lanes in ascending lane order (bitonic network, 21 compare-exchange steps)
+__device__ __forceinline__ uint64_t lp_sort_up(uint64_t x) {
+  const int lane = rx_lane();
+#pragma unroll
+  for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+    for (int st = size >> 1; st > 0; st >>= 1) {
+      const uint64_t o = lp_shfl_xor64(x, st);
+      const bool up = (lane & size) == 0 || size == 64;
+      const bool low = (lane & st) == 0;
+      x = ((x < o) == (up == low)) ? x : o;
+    }
+  return x;
+}
+// best 64 of `list` (descending over the lanes) and `cand` (ascending), descending
+__device__ __forceinline__ uint64_t lp_merge(uint64_t list, uint64_t cand) {
+  const int lane = rx_lane();
+  uint64_t x = list > cand ? list : cand;
+#pragma unroll
+  for (int st = 32; st > 0; st >>= 1) {
+    const uint64_t o = lp_shfl_xor64(x, st);
+    const bool low = (lane & st) == 0;
+    x = ((x > o) == low) ? x : o;
+  }
+  return x;
+}
+__device__ __forceinline__ uint64_t lp_lane64(uint64_t x, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, lane), hi = __builtin_amdgcn_readlane((uint32_t)(x >> 32), lane);
+  return ((uint64_t)hi << 32) | lo;
+}
+
+// One wavefront's list of alternatives: `list` sorted over the lanes, `buf` [128] candidates waiting in LDS.
+struct LpTop {
+  uint64_t list;
+  uint64_t* buf;
+  int cnt;
+  float thr;       // score of the k-th alternative, as of the last refresh(); -inf while there are fewer
+  __device__ __forceinline__ void init(uint64_t* b) { list = 0; buf = b; cnt = 0; thr = LP_NINF; }
+  __device__ __forceinline__ void take(uint64_t key) { list = lp_merge(list, lp_sort_up(key)); }
+  // lanes with `on` add their key; called by the whole wavefront
+  __device__ __forceinline__ void push(bool on, uint64_t key) {
+    const uint64_t mask = __ballot(on);
+    if (!mask) return;
+    if (on) buf[cnt + __popcll(mask & ((1ull << rx_lane()) - 1))] = key;
+    cnt += (int)__popcll(mask);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (cnt >= 64) {
+      const uint64_t a = buf[rx_lane()], b = buf[64 + rx_lane()];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      cnt -= 64;
+      if (rx_lane() < cnt) buf[rx_lane()] = b;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      take(a);
+    }
+  }
+  __device__ __forceinline__ void flush() {
+    if (!cnt) return;
+    take(rx_lane() < cnt ? buf[rx_lane()] : 0);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    cnt = 0;
+  }
+  // The filter admits only scores above the k-th of the list.  It is refreshed between two groups of columns, never
+  // inside one: all columns of the list are then lower than any column still to come, so an equal score may go.
+  __device__ __forceinline__ void refresh(int k) {
+    const uint64_t kth = lp_lane64(list, k - 1);
+    thr = kth ? lp_key_value(kth) : LP_NINF;
+  }
+};
+
+// ---------------------------------------------------------------- shared row pieces
+struct LpRow {
+  float raw, m2, s, t;   // final statistics of the row
+  float lse, H;
+  bool empty, big;
+};
+
+__device__ __forceinline__ LpRow lp_finish(float raw, float m2, float s, float t) {
+  LpRow r;
+  r.raw = raw; r.m2 = m2; r.s = s; r.t = t;
+  r.empty = raw == LP_NINF && s == s;        // nothing above -inf (and no NaN): no distribution
+  r.big = fabsf(raw) > LP_BIG && fabsf(raw) < __builtin_inff();
+  if (r.empty) { r.lse = LP_NINF; r.H = 0.f; return r; }
+  const float l2s = log2f(s);
+  r.lse = r.big ? m2 + l2s * LP_LN2 : (m2 + l2s) * LP_LN2;
+  r.H = (l2s - t / s) * LP_LN2;
+  return r;
+}
+// log-probability of a score, from the reference rather than from the rounded lse
+__device__ __forceinline__ float lp_of(const LpRow& r, float l) {
+  if (l == LP_NINF || r.empty) return LP_NINF;
+  if (!r.big && fabsf(l) > LP_BIG) return l - r.lse;     // a mask of the type's lowest value under an ordinary row
+  const float l2s = log2f(r.s);
+  return r.big ? (l - r.m2) - l2s * LP_LN2 : (fmaf(l, LP_L2E, -r.m2) - l2s) * LP_LN2;
+}
+// what the gradient needs of a row: (reference, log2 s, unit of the reference: 0 log2, 1 score; 2 = empty row, H).
+// Kept apart from lse, whose rounding would cost the probabilities a factor of 1 + |lse| 2^-24.
+__device__ __forceinline__ void lp_write_row(const rx_logprob_args& a, const LpRow& r, int64_t row) {
+  a.lse[row] = r.lse;
+  a.entropy[row] = r.H;
+  if (a.stats) reinterpret_cast<float4*>(a.stats)[row] = make_float4(r.m2, log2f(r.s), r.empty ? 2.f : r.big ? 1.f : 0.f, r.H);
+}
+__device__ __forceinline__ int32_t lp_live(const rx_logprob_args& a, int64_t row) {
+  if (!a.lengths) return (int32_t)a.V;
+  const int64_t n = a.lengths[row];
+  return (int32_t)(n < 0 ? 0 : n > a.V ? a.V : n);
+}
+template <typename T>
+__device__ __forceinline__ void lp_write_target(const rx_logprob_args& a, const LpRow& r, const T* l, int32_t n, int64_t row, int t, int32_t* err) {
+  const int64_t y = a.targets[row * a.T + t];
+  float out;
+  if (y == -1) out = 0.f;                                            // no target here
+  else if (!rx_row_ok(y, a.V, err)) out = __builtin_nanf("");
+  else out = y < n ? lp_of(r, lp_elem(l + y)) : LP_NINF;
+  a.logprob[row * a.T + t] = out;
+}
+__device__ __forceinline__ void lp_write_top(const rx_logprob_args& a, const LpRow& r, int64_t row, int i, uint64_t key) {
+  a.top_index[row * a.k + i] = key ? (int64_t)lp_key_col(key) : -1;
+  a.top_logprob[row * a.k + i] = key ? lp_of(r, lp_key_value(key)) : LP_NINF;
+}
+
+// ---------------------------------------------------------------- narrow rows: G lanes per row, PER scores per lane
+template <typename T, int G, int PER, bool TOP>
+__global__ void __launch_bounds__(RX_BLOCK)
+lp_small_kernel(rx_logprob_args a, int32_t* err) {
+  __shared__ uint64_t tops[TOP ? RX_BLOCK / 64 : 1][TOP ? 128 : 1];
+  const int sub = threadIdx.x & (G - 1);
+  const int64_t row = (int64_t)blockIdx.x * (RX_BLOCK / G) + threadIdx.x / G;
+  if (G == 64 && row >= a.R) return;             // whole wavefronts leave
+  const bool on = row < a.R;
+  const T* l = (const T*)a.logits + (on ? row : 0) * a.ld;
+  const int32_t n = on ? lp_live(a, row) : 0;
+  float v[PER], m = LP_NINF;
+#pragma unroll
+  for (int q = 0; q < PER; ++q) {
+    const int c = q * G + sub;
+    v[q] = c < n ? lp_elem(l + c) : LP_NINF;
+    m = fmaxf(m, v[q]);
+  }
+#pragma unroll
+  for (int x = G >> 1; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+  const float ref = m == LP_NINF ? 0.f : m;
+  float s = 0.f, t = 0.f;
+#pragma unroll
+  for (int q = 0; q < PER; ++q) {
+    const float d = (v[q] - ref) * LP_L2E, e = lp_exp2(d);
+    s += e;
+    t = fmaf(e, fmaxf(d, -1e4f), t);             // a masked score: e = 0 times a finite number
+  }
+#pragma unroll
+  for (int x = G >> 1; x > 0; x >>= 1) { s += __shfl_xor(s, x, 64); t += __shfl_xor(t, x, 64); }
+  // the reference is the score itself here, as for rows beyond LP_BIG
+  LpRow r = lp_finish(m, ref, s, t);
+  r.big = true;
+  if (!r.empty) r.lse = ref + log2f(s) * LP_LN2;
+  if (on && sub == 0) lp_write_row(a, r, row);
+  if (on)
+    for (int q = sub; q < a.T; q += G) lp_write_target<T>(a, r, l, n, row, q, err);
+  if constexpr (TOP) {
+    LpTop top;
+    top.init(tops[threadIdx.x >> 6]);
+#pragma unroll
+    for (int q = 0; q < PER; ++q) {
+      if (q * 64 < n) {                          // the row's (wavefront's) live columns
+        if (q == 0) top.take(v[0] > LP_NINF ? lp_key(v[0], sub) : 0);
+        else top.push(v[q] > top.thr, lp_key(v[q], q * 64 + sub));
+        top.refresh(a.k);
+      }
+    }
+    top.flush();
+    if (sub < a.k) lp_write_top(a, r, row, sub, top.list);
+  }
+}
+
+// ---------------------------------------------------------------- wide rows
+struct LpAcc {
+  float raw, m2, s, t;
+  __device__ __forceinline__ void init() { raw = LP_NINF; m2 = LP_NINF; s = 0.f; t = 0.f; }
+  __device__ __forceinline__ void rebase(float n) {          // move the reference to n (log2 units, finite or +inf)
+    if (m2 != LP_NINF) {
+      const float f = lp_exp2(m2 - n);
+      t = (t + s * (m2 - n)) * f;
+      s *= f;
+    }
+    m2 = n;
+  }
+  template <int N>
+  __device__ __forceinline__ float add(const float* v) {     // returns the largest of v
+    float mx = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) mx = fmaxf(mx, v[i]);
+    raw = fmaxf(raw, mx);
+    const float n2 = mx * LP_L2E;
+    const bool grow = n2 > m2 + 4.f;
+    if (__ballot(grow)) {
+      if (grow) rebase(n2);
+    }
+    const float ref = m2 == LP_NINF ? 0.f : -m2;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float d = fmaf(v[i], LP_L2E, ref), e = lp_exp2(d);
+      s += e;
+      t = fmaf(e, fmaxf(d, -1e4f), t);
+    }
+    return mx;
+  }
+  // Scores whose products with log2(e) leave fp32 (e.g. masks of the type's lowest value with nothing else in the
+  // row): the same sums relative to the known maximum.
+  template <int N>
+  __device__ __forceinline__ void add_big(const float* v, float m) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float d = (v[i] - m) * LP_L2E, e = lp_exp2(d);
+      s += e;
+      t = fmaf(e, fmaxf(d, -1e4f), t);
+    }
+  }
+};
+
+// Columns of a row as 16-byte vectors: `head` scores before the first 16-byte boundary, `nvec` vectors, the rest.
+template <typename T>
+__device__ __forceinline__ void lp_frame(const T* l, int32_t n, int32_t* head, int32_t* nvec) {
+  const int32_t h = (int32_t)((16 - ((uintptr_t)l & 15)) & 15) / (int32_t)sizeof(T);
+  *head = h < n ? h : n;
+  *nvec = (n - *head) / LpVec<T>::N;
+}
+
+// Calls f(v[N], first column of the lane, n valid...) over this wavefront's share of the columns [part of row], in
+// ascending groups: every column of one call is lower than every column of the next.
+template <typename T, typename F>
+__device__ __forceinline__ void lp_stream(const T* l, int32_t n, int split, int n_split, F f) {
+  constexpr int N = LpVec<T>::N;
+  int32_t head, nvec;
+  lp_frame(l, n, &head, &nvec);
+  const int lane = rx_lane(), wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const bool first = split == 0 && wave == 0;
+  if (first && head) {
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = LP_NINF;
+    if (lane < head) v[0] = lp_elem(l + lane);
+    f(v, lane);
+  }
+  const int32_t chunk = (nvec + n_split - 1) / n_split;
+  const int32_t lo = split * chunk < nvec ? split * chunk : nvec;
+  const int32_t hi = lo + chunk < nvec ? lo + chunk : nvec;
+  const uint4* p = reinterpret_cast<const uint4*>(l + head);
+  for (int32_t b = lo + wave * 64; b < hi; b += waves * 64) {
+    const int32_t q = b + lane;
+    float v[N];
+    if (q < hi) lp_unpack<T>(p[q], v);
+    else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = LP_NINF;
+    }
+    f(v, head + q * N);
+  }
+  const int32_t tail = head + nvec * N;
+  if (first && tail < n) {
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = LP_NINF;
+    if (lane < n - tail) v[0] = lp_elem(l + tail + lane);
+    f(v, tail + lane);
+  }
+}
+
+__device__ __forceinline__ void lp_join(LpPart& x, const LpPart& y) {
+  const float raw = fmaxf(x.raw, y.raw);
+  const bool big = fabsf(raw) > LP_BIG && fabsf(raw) < __builtin_inff();
+  // references in one unit: with the maximum beyond LP_BIG only sums taken relative to scores beyond it count
+  if (big) {
+    auto w = [&](const LpPart& p, float* s, float* t) {
+      if (p.raw == LP_NINF && p.s == p.s) { *s = 0.f; *t = 0.f; return; }
+      if (!(fabsf(p.raw) > LP_BIG)) {                    // ordinary scores below a maximum beyond LP_BIG
+        if (p.s == p.s && raw > 0.f) { *s = 0.f; *t = 0.f; } else { *s = p.s; *t = p.t; }
+        return;
+      }
+      const float d = (p.m2 - raw) * LP_L2E, f = lp_exp2(d);
+      *s = p.s * f;
+      *t = (p.t + p.s * fmaxf(d, -1e4f)) * f;
+    };
+    float s0, t0, s1, t1;
+    w(x, &s0, &t0);
+    w(y, &s1, &t1);
+    x.raw = raw; x.m2 = raw; x.s = s0 + s1; x.t = t0 + t1;
+    return;
+  }
+  auto scaled = [&](const LpPart& p, float m, float* s, float* t) {
+    if (p.m2 == LP_NINF || (fabsf(p.raw) > LP_BIG && p.raw < 0.f)) {   // empty, or far below the maximum (NaN goes through)
+      *s = p.s == p.s ? 0.f : p.s;
+      *t = p.s == p.s ? 0.f : p.t;
+      return;
+    }
+    const float f = lp_exp2(p.m2 - m);
+    *t = (p.t + p.s * (p.m2 - m)) * f;
+    *s = p.s * f;
+  };
+  const bool xb = fabsf(x.raw) > LP_BIG && x.raw < 0.f, yb = fabsf(y.raw) > LP_BIG && y.raw < 0.f;
+  const float m = fmaxf(xb ? LP_NINF : x.m2, yb ? LP_NINF : y.m2);
+  float s0, t0, s1, t1;
+  scaled(x, m, &s0, &t0);
+  scaled(y, m, &s1, &t1);
+  x.raw = raw; x.m2 = m; x.s = s0 + s1; x.t = t0 + t1;
+}
+__device__ __forceinline__ LpPart lp_wave_join(LpPart p) {
+  for (int x = 32; x > 0; x >>= 1) {
+    LpPart o;
+    o.raw = __shfl_xor(p.raw, x, 64); o.m2 = __shfl_xor(p.m2, x, 64);
+    o.s = __shfl_xor(p.s, x, 64); o.t = __shfl_xor(p.t, x, 64);
+    // the same operand order on both sides keeps the lanes' copies bit-identical
+    if (rx_lane() & x) { LpPart q = o; lp_join(q, p); p = q; } else lp_join(p, o);
+  }
+  return p;
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(RX_BLOCK)
+lp_wide_kernel(rx_logprob_args a, LpPart* parts, uint64_t* lists, int n_split, int32_t* err) {
+  constexpr int N = LpVec<T>::N, W = RX_BLOCK / 64;
+  __shared__ LpPart sh[W];
+  __shared__ uint64_t tops[TOP ? W : 1][TOP ? 128 : 1];
+  const int64_t row = blockIdx.x / n_split;
+  const int split = blockIdx.x % n_split;
+  const int wave = threadIdx.x >> 6, lane = rx_lane();
+  const T* l = (const T*)a.logits + row * a.ld;
+  const int32_t n = lp_live(a, row);
+  LpAcc acc;
+  acc.init();
+  LpTop top;
+  if constexpr (TOP) top.init(tops[wave]);
+  lp_stream<T>(l, n, split, n_split, [&](const float* v, int32_t col) {
+    const float mx = acc.add<N>(v);
+    if constexpr (TOP) {
+      if (__ballot(mx > top.thr)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) top.push(v[i] > top.thr, lp_key(v[i], col + i));
+        top.refresh(a.k);
+      }
+    }
+  });
+  // the largest score of the workgroup decides, uniformly, whether the sums have to be taken again
+  float raw = acc.raw;
+  for (int x = 32; x > 0; x >>= 1) raw = fmaxf(raw, __shfl_xor(raw, x, 64));
+  if (lane == 0) sh[wave].raw = raw;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < W; ++w) raw = fmaxf(raw, sh[w].raw);
+  __syncthreads();
+  LpPart p;
+  if (fabsf(raw) > LP_BIG && fabsf(raw) < __builtin_inff()) {
+    acc.s = 0.f; acc.t = 0.f;
+    lp_stream<T>(l, n, split, n_split, [&](const float* v, int32_t) { acc.add_big<N>(v, raw); });
+    p.raw = raw; p.m2 = raw; p.s = acc.s; p.t = acc.t;
+  } else {
+    p.raw = acc.raw; p.m2 = acc.m2; p.s = acc.s; p.t = acc.t;
+  }
+  p = lp_wave_join(p);
+  if (lane == 0) sh[wave] = p;
+  if constexpr (TOP) {
+    top.flush();
+    tops[wave][lane] = top.list;
+  }
+  __syncthreads();
+  p = sh[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) lp_join(p, sh[w]);
+  if constexpr (TOP) {
+    if (wave == 0)
+      for (int w = 1; w < W; ++w) top.list = lp_merge(top.list, tops[w][63 - lane]);
+  }
+  if (n_split > 1) {
+    if (threadIdx.x == 0) parts[blockIdx.x] = p;
+    if constexpr (TOP) {
+      if (wave == 0 && lane < a.k) lists[(int64_t)blockIdx.x * a.k + lane] = top.list;
+    }
+    return;
+  }
+  const LpRow r = lp_finish(p.raw, p.m2, p.s, p.t);
+  if (threadIdx.x == 0) lp_write_row(a, r, row);
+  for (int t = threadIdx.x; t < a.T; t += RX_BLOCK) lp_write_target<T>(a, r, l, n, row, t, err);
+  if constexpr (TOP) {
+    if (wave == 0 && lane < a.k) lp_write_top(a, r, row, lane, top.list);
+  }
+}
+
+// One workgroup per row joins the splits.  A list's k-th key bounds the row's k-th key from below, so the largest of
+// them filters the candidates before anything is merged.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(RX_BLOCK)
+lp_join_kernel(rx_logprob_args a, const LpPart* parts, const uint64_t* lists, int n_split, int32_t* err) {
+  constexpr int W = RX_BLOCK / 64;
+  __shared__ LpPart sh[W];
+  __shared__ uint64_t bound[W];
+  __shared__ uint64_t tops[TOP ? W : 1][TOP ? 128 : 1];
+  const int64_t row = blockIdx.x;
+  const int wave = threadIdx.x >> 6, lane = rx_lane();
+  const T* l = (const T*)a.logits + row * a.ld;
+  const int32_t n = lp_live(a, row);
+  LpPart p;
+  p.raw = LP_NINF; p.m2 = LP_NINF; p.s = 0.f; p.t = 0.f;
+  if ((int)threadIdx.x < n_split) p = parts[row * n_split + threadIdx.x];
+  p = lp_wave_join(p);
+  if (lane == 0) sh[wave] = p;
+  if constexpr (TOP) {
+    uint64_t th = (int)threadIdx.x < n_split ? lists[(row * n_split + threadIdx.x) * a.k + a.k - 1] : 0;
+    for (int x = 32; x > 0; x >>= 1) { const uint64_t o = lp_shfl_xor64(th, x); th = th > o ? th : o; }
+    if (lane == 0) bound[wave] = th;
+  }
+  __syncthreads();
+  p = sh[0];
+#pragma unroll
+  for (int w = 1; w < W; ++w) lp_join(p, sh[w]);
+  const LpRow r = lp_finish(p.raw, p.m2, p.s, p.t);
+  if (threadIdx.x == 0) lp_write_row(a, r, row);
+  for (int t = threadIdx.x; t < a.T; t += RX_BLOCK) lp_write_target<T>(a, r, l, n, row, t, err);
+  if constexpr (TOP) {
+    uint64_t th = bound[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) th = th > bound[w] ? th : bound[w];
+    LpTop top;
+    top.init(tops[wave]);
+    const int total = n_split * a.k;
+    const uint64_t* mine = lists + row * n_split * (int64_t)a.k;
+    for (int b = wave * 64; b < total; b += RX_BLOCK) {
+      const uint64_t key = b + lane < total ? mine[b + lane] : 0;
+      top.push(key != 0 && key >= th, key);
+    }
+    top.flush();
+    tops[wave][lane] = top.list;
+    __syncthreads();
+    if (wave == 0) {
+      for (int w = 1; w < W; ++w) top.list = lp_merge(top.list, tops[w][63 - lane]);
+      if (lane < a.k) lp_write_top(a, r, row, lane, top.list);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- gradient
+// dl = p (A - g_H log p),  A = g_lse - sum_t g_t - g_H H, and the targets' own share on top.  A target that carries no
+// probability (-1, a masked score, a column past the row's end) takes no part; a row with nothing left gets zeros.
+struct LpGrad {
+  float ref, l2s, A, gh2;      // gh2 = g_H ln 2: log p is held in log2 units
+  bool dead, big;
+  template <bool BIG>
+  __device__ __forceinline__ float of(float l) const {
+    const float d = (BIG ? (l - ref) * LP_L2E : fmaf(l, LP_L2E, -ref)) - l2s, p = lp_exp2(d);
+    return p * fmaf(-gh2, fmaxf(d, -1e4f), A);
+  }
+  __device__ __forceinline__ float any(float l) const { return big ? of<true>(l) : of<false>(l); }
+};
+template <typename T>
+__device__ __forceinline__ bool lp_target_on(const rx_logprob_args& a, const T* l, int32_t n, int64_t row, int t, int64_t* y) {
+  *y = a.targets[row * a.T + t];
+  return *y >= 0 && *y < n && lp_elem(l + *y) != LP_NINF;
+}
+__device__ __forceinline__ LpGrad lp_grad_row(const rx_logprob_args& a, const float* gh, const float* gl, float gsum, int64_t row) {
+  const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
+  LpGrad r;
+  const float h = gh ? gh[row] : 0.f;
+  r.ref = st.x; r.l2s = st.y;
+  r.gh2 = h * LP_LN2;
+  r.A = (gl ? gl[row] : 0.f) - gsum - h * st.w;
+  r.dead = st.z == 2.f;
+  r.big = st.z != 0.f;
+  return r;
+}
+// the whole gradient of target t's column: its share of the softmax and every gradient that names the column; written
+// by the first target that does
+template <typename T>
+__device__ __forceinline__ void lp_fix_target(const rx_logprob_args& a, const LpGrad& r, const T* l, T* d, int32_t n,
+                                              const float* g, int64_t row, int t, int32_t lo, int32_t hi) {
+  int64_t y;
+  if (r.dead || !lp_target_on(a, l, n, row, t, &y) || y < lo || y >= hi) return;
+  float sum = 0.f;
+  for (int u = 0; u < a.T; ++u) {
+    if (a.targets[row * a.T + u] != y) continue;
+    if (u < t) return;
+    sum += g[row * a.T + u];
+  }
+  lp_put<T>(d + y, r.any(lp_elem(l + y)) + sum);
+}
+
+template <typename T, int G, int PER>
+__global__ void __launch_bounds__(RX_BLOCK)
+lp_bwd_small_kernel(rx_logprob_args a, const float* __restrict__ g, const float* __restrict__ gh, const float* __restrict__ gl,
+                    T* __restrict__ dl, int64_t ld_d) {
+  const int sub = threadIdx.x & (G - 1);
+  const int64_t row = (int64_t)blockIdx.x * (RX_BLOCK / G) + threadIdx.x / G;
+  if (G == 64 && row >= a.R) return;
+  const bool on = row < a.R;
+  const int64_t rr = on ? row : 0;
+  const T* l = (const T*)a.logits + rr * a.ld;
+  T* d = dl + rr * ld_d;
+  const int32_t n = on ? lp_live(a, row) : 0;
+  float gs = 0.f;
+  if (g && on)
+    for (int t = sub; t < a.T; t += G) {
+      int64_t y;
+      if (lp_target_on(a, l, n, row, t, &y)) gs += g[row * a.T + t];
+    }
+#pragma unroll
+  for (int x = G >> 1; x > 0; x >>= 1) gs += __shfl_xor(gs, x, 64);
+  if (!on) return;
+  const LpGrad r = lp_grad_row(a, gh, gl, gs, row);
+  float v[PER];
+#pragma unroll
+  for (int q = 0; q < PER; ++q) {
+    const int c = q * G + sub;
+    v[q] = c < n && !r.dead ? r.any(lp_elem(l + c)) : 0.f;
+  }
+  if (g && !r.dead) {
+    // every lane looks at all targets: its own columns take their gradients in ascending target order
+    for (int t = 0; t < a.T; ++t) {
+      int64_t y;
+      if (!lp_target_on(a, l, n, row, t, &y)) continue;
+      const float gt = g[row * a.T + t];
+#pragma unroll
+      for (int q = 0; q < PER; ++q)
+        if (y == q * G + sub) v[q] += gt;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < PER; ++q)
+    if (q * G + sub < a.V) lp_put<T>(d + q * G + sub, v[q]);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(RX_BLOCK)
+lp_bwd_wide_kernel(rx_logprob_args a, const float* __restrict__ g, const float* __restrict__ gh, const float* __restrict__ gl,
+                   T* __restrict__ dl, int64_t ld_d, int n_split) {
+  constexpr int N = LpVec<T>::N;
+  __shared__ float part[RX_BLOCK / 64];
+  const int64_t row = blockIdx.x / n_split;
+  const int split = blockIdx.x % n_split;
+  const T* l = (const T*)a.logits + row * a.ld;
+  T* d = dl + row * ld_d;
+  const int32_t n = lp_live(a, row), V = (int32_t)a.V;
+  float gs = 0.f;
+  if (g) {
+    for (int t = threadIdx.x; t < a.T; t += RX_BLOCK) {
+      int64_t y;
+      if (lp_target_on(a, l, n, row, t, &y)) gs += g[row * a.T + t];
+    }
+    gs = rx_wave_sum(gs);
+    if (rx_lane() == 0) part[threadIdx.x >> 6] = gs;
+    __syncthreads();
+    gs = part[0] + part[1] + part[2] + part[3];
+  }
+  const LpGrad r = lp_grad_row(a, gh, gl, gs, row);
+  // the vectors follow the stores' alignment; scores that lie differently are read one by one
+  const int32_t head = min((int32_t)((16 - ((uintptr_t)d & 15)) & 15) / (int32_t)sizeof(T), V);
+  const int32_t nvec = (V - head) / N;
+  const bool same = ((((uintptr_t)l) ^ ((uintptr_t)d)) & 15) == 0;
+  const int32_t chunk = (nvec + n_split - 1) / n_split;
+  const int32_t lo = min(split * chunk, nvec), hi = min(lo + chunk, nvec);
+  for (int32_t q = lo + threadIdx.x; q < hi; q += RX_BLOCK) {
+    const int32_t c = head + q * N;
+    float v[N];
+    if (c + N <= n && !r.dead) {
+      if (same) lp_unpack<T>(*reinterpret_cast<const uint4*>(l + c), v);
+      else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = lp_elem(l + c + i);
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = r.any(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = c + i < n && !r.dead ? r.any(lp_elem(l + c + i)) : 0.f;
+    }
+    uint4 o;
+    if constexpr (sizeof(T) == 4) {
+      o = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = (uint32_t)lp_to_bf16(v[2 * i]) | ((uint32_t)lp_to_bf16(v[2 * i + 1]) << 16);
+      o = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    *reinterpret_cast<uint4*>(d + c) = o;
+  }
+  // columns outside the vectors, with the first and the last split
+  const int32_t tail = head + nvec * N;
+  if (split == 0 && (int)threadIdx.x < head) {
+    const int c = threadIdx.x;
+    lp_put<T>(d + c, c < n && !r.dead ? r.any(lp_elem(l + c)) : 0.f);
+  }
+  if (split == n_split - 1 && (int)threadIdx.x < V - tail) {
+    const int c = tail + threadIdx.x;
+    lp_put<T>(d + c, c < n && !r.dead ? r.any(lp_elem(l + c)) : 0.f);
+  }
+  if (!g) return;
+  __syncthreads();           // the targets' columns are written again, after everything else of this split
+  const int32_t c0 = split == 0 ? 0 : head + lo * N, c1 = split == n_split - 1 ? V : head + hi * N;
+  for (int t = threadIdx.x; t < a.T; t += RX_BLOCK) lp_fix_target<T>(a, r, l, d, n, g, row, t, c0, c1);
+}
+
+// ---------------------------------------------------------------- host
+static int lp_splits(int64_t R, int64_t V) {
+  // Enough workgroups to fill the chip (4 per CU) when there are few rows, each with at least LP_SPLIT_MIN columns.
+  int64_t want = rx_cdiv(1024, R > 0 ? R : 1), most = V / LP_SPLIT_MIN;
+  if (want > most) want = most;
+  if (want > LP_SPLIT_MAX) want = LP_SPLIT_MAX;
+  return want < 1 ? 1 : (int)want;
+}
+
+static int lp_check(const rx_logprob_args* a, const char* who) {
+  RX_REQUIRE(a, "%s: null argument", who);
+  RX_REQUIRE(a->R >= 0 && a->V >= 1 && a->V < (1ll << 31) - 64 && a->ld >= a->V, "%s: bad shape R=%lld V=%lld ld=%lld", who,
+             (long long)a->R, (long long)a->V, (long long)a->ld);
+  RX_REQUIRE(a->T >= 0 && a->T <= 1024, "%s: T=%d targets per row (at most 1024)", who, a->T);
+  RX_REQUIRE(a->R * (int64_t)lp_splits(a->R, a->V) < (1ll << 31), "%s: R=%lld rows are more than one launch takes", who, (long long)a->R);
+  RX_REQUIRE(a->bf16 == 0 || a->bf16 == 1, "%s: bad element type %d", who, a->bf16);
+  if (a->R == 0) return 0;
+  RX_REQUIRE(a->logits && (a->T == 0 || a->targets), "%s: null argument", who);
+  RX_REQUIRE(((uintptr_t)a->stats & 15) == 0, "%s: stats must be 16-byte aligned", who);
+  RX_REQUIRE(((uintptr_t)a->logits & (a->bf16 ? 1 : 3)) == 0, "%s: logits are not aligned to their elements", who);
+  return 0;
+}
+
+extern "C" size_t rx_logprob_workspace_bytes(int64_t R, int64_t V, int32_t k) {
+  if (R <= 0 || V <= LP_SMALL || k < 0 || k > LP_TOP) return 0;
+  const int n = lp_splits(R, V);
+  return n > 1 ? (size_t)R * n * (sizeof(LpPart) + 8 * (size_t)k) : 0;
+}
+
+template <typename T, bool TOP>
+static void lp_launch_small(const rx_logprob_args& a, int32_t* err, hipStream_t st) {
+#define LP_GO(G, PER)                                                                                              \
+  hipLaunchKernelGGL((lp_small_kernel<T, G, PER, TOP>), dim3((unsigned)rx_cdiv(a.R, RX_BLOCK / (G))), dim3(RX_BLOCK), 0, st, a, err)
+  if constexpr (!TOP) {
+    if (a.V <= 8) { LP_GO(8, 1); return; }
+    if (a.V <= 32) { LP_GO(32, 1); return; }
+  }
+  if (a.V <= 64) LP_GO(64, 1);
+  else if (a.V <= 128) LP_GO(64, 2);
+  else if (a.V <= 256) LP_GO(64, 4);
+  else if (a.V <= 512) LP_GO(64, 8);
+  else LP_GO(64, 16);
+#undef LP_GO
+}
+
+template <typename T>
+static void lp_launch_fwd(const rx_logprob_args& a, void* ws, int32_t* err, hipStream_t st) {
+  if (a.V <= LP_SMALL) {
+    if (a.k) lp_launch_small<T, true>(a, err, st);
+    else lp_launch_small<T, false>(a, err, st);
+    return;
+  }
+  const int n = lp_splits(a.R, a.V);
+  LpPart* parts = (LpPart*)ws;
+  uint64_t* lists = (uint64_t*)(parts + (n > 1 ? a.R * n : 0));
+  const dim3 grid((unsigned)(a.R * n)), blk(RX_BLOCK);
+  if (a.k) {
+    hipLaunchKernelGGL((lp_wide_kernel<T, true>), grid, blk, 0, st, a, parts, lists, n, err);
+    if (n > 1) hipLaunchKernelGGL((lp_join_kernel<T, true>), dim3((unsigned)a.R), blk, 0, st, a, parts, lists, n, err);
+  } else {
+    hipLaunchKernelGGL((lp_wide_kernel<T, false>), grid, blk, 0, st, a, parts, lists, n, err);
+    if (n > 1) hipLaunchKernelGGL((lp_join_kernel<T, false>), dim3((unsigned)a.R), blk, 0, st, a, parts, lists, n, err);
+  }
+}
+
+extern "C" int rx_logprob_fwd(const rx_logprob_args* args, void* ws, size_t ws_bytes, int32_t* err_flag, int device, void* stream) {
+  if (lp_check(args, "rx_logprob_fwd")) return 1;
+  const rx_logprob_args a = *args;
+  RX_REQUIRE(a.k >= 0 && a.k <= LP_TOP, "rx_logprob_fwd: k=%d alternatives (at most %d)", a.k, LP_TOP);
+  if (a.R == 0) return 0;
+  RX_REQUIRE(a.lse && a.entropy && (a.T == 0 || a.logprob) && (a.k == 0 || (a.top_logprob && a.top_index)), "rx_logprob_fwd: null output");
+  const size_t need = rx_logprob_workspace_bytes(a.R, a.V, a.k);
+  RX_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0), "rx_logprob_fwd: workspace of %zu bytes, %zu needed",
+             ws_bytes, need);
+  RX_GUARD_DEVICE(device);
+  if (a.bf16) lp_launch_fwd<uint16_t>(a, ws, err_flag, (hipStream_t)stream);
+  else lp_launch_fwd<float>(a, ws, err_flag, (hipStream_t)stream);
+  RX_LAUNCH_CHECK();
+  return 0;
+}
+
+template <typename T>
+static void lp_launch_bwd(const rx_logprob_args& a, const float* g, const float* gh, const float* gl, T* dl, int64_t ld, hipStream_t st) {
+#define LP_GO(G, PER)                                                                                                     \
+  hipLaunchKernelGGL((lp_bwd_small_kernel<T, G, PER>), dim3((unsigned)rx_cdiv(a.R, RX_BLOCK / (G))), dim3(RX_BLOCK), 0, st, a, g, gh, \
+                     gl, dl, ld)
+  if (a.V <= 8) LP_GO(8, 1);
+  else if (a.V <= 32) LP_GO(32, 1);
+  else if (a.V <= 64) LP_GO(64, 1);
+  else if (a.V <= 128) LP_GO(64, 2);
+  else if (a.V <= 256) LP_GO(64, 4);
+  else if (a.V <= 512) LP_GO(64, 8);
+  else if (a.V <= LP_SMALL) LP_GO(64, 16);
+  else {
+    const int n = lp_splits(a.R, a.V);
+    hipLaunchKernelGGL((lp_bwd_wide_kernel<T>), dim3((unsigned)(a.R * n)), dim3(RX_BLOCK), 0, st, a, g, gh, gl, dl, ld, n);
+  }
+#undef LP_GO
+}
+
+extern "C" int rx_logprob_bwd(const rx_logprob_args* args, const float* d_g_logprob, const float* d_g_entropy, const float* d_g_lse,
+                              void* d_dlogits, int64_t ld_d, int device, void* stream) {
+  if (lp_check(args, "rx_logprob_bwd")) return 1;
+  const rx_logprob_args a = *args;
+  RX_REQUIRE(ld_d >= a.V, "rx_logprob_bwd: row stride %lld below V=%lld", (long long)ld_d, (long long)a.V);
+  if (a.R == 0) return 0;
+  RX_REQUIRE(a.stats && d_dlogits && ((uintptr_t)d_dlogits & (a.bf16 ? 1 : 3)) == 0, "rx_logprob_bwd: bad gradient buffer");
+  RX_GUARD_DEVICE(device);
+  if (a.T == 0) d_g_logprob = nullptr;
+  if (a.bf16) lp_launch_bwd<uint16_t>(a, d_g_logprob, d_g_entropy, d_g_lse, (uint16_t*)d_dlogits, ld_d, (hipStream_t)stream);
+  else lp_launch_bwd<float>(a, d_g_logprob, d_g_entropy, d_g_lse, (float*)d_dlogits, ld_d, (hipStream_t)stream);
+  RX_LAUNCH_CHECK();
+  return 0;
+}

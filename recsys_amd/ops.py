@@ -8,12 +8,12 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import FMArgs, GatherSeg, MFArgs, check, lib
+from ._lib import FMArgs, GatherSeg, LogProbArgs, MFArgs, check, lib
 
 Tensor = torch.Tensor
 
@@ -1385,6 +1385,102 @@ def topk_codes(scores: Tensor, codes: Optional[Tensor], k: int) -> Tensor:
     check(lib.rx_topk_codes(_p(scores), _p(codes), rows, n, k, _p(out), _dev(scores), _stream(scores)),
           "rx_topk_codes")
     return out
+
+
+# ------------------------------------------------------------------ list-wise log-probabilities
+LOGPROB_MAX_TOP = 64          # alternatives per row
+LOGPROB_MAX_TARGETS = 1024    # targets per row
+
+
+class LogProbs(NamedTuple):
+    """Per-row results over scores [R, V]; ``logprob`` has the shape of the targets, the alternatives are [R, k]."""
+    logprob: Tensor
+    entropy: Tensor
+    lse: Tensor
+    top_logprob: Tensor
+    top_index: Tensor
+
+
+def _score_rows(t: Tensor, name: str) -> Tuple[Tensor, int]:
+    """fp32 or bf16 [R, V] on the GPU with unit inner stride and rows that do not overlap: (tensor, row stride)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a tensor on the GPU, got device {t.device}")
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
+    if t.dim() != 2:
+        raise ValueError(f"{name}: expected 2 dimensions, got shape {tuple(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: columns must have unit stride")
+    ld = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if ld < t.shape[1]:
+        raise ValueError(f"{name}: rows must not overlap")
+    return t, ld
+
+
+def _logprob_args(logits: Tensor, targets: Tensor, lengths: Optional[Tensor], k: int) -> Tuple[LogProbArgs, int, int, int]:
+    _, ld = _score_rows(logits, "logits")
+    R, V = logits.shape
+    _idx(targets, "targets")
+    if targets.dim() not in (1, 2) or targets.shape[0] != R:
+        raise ValueError(f"targets: expected shape [{R}] or [{R}, T], got {tuple(targets.shape)}")
+    T = targets.shape[1] if targets.dim() == 2 else 1
+    if T > LOGPROB_MAX_TARGETS:
+        raise ValueError(f"targets: at most {LOGPROB_MAX_TARGETS} per row, got {T}")
+    if not 0 <= k <= LOGPROB_MAX_TOP:
+        raise ValueError(f"k: expected 0..{LOGPROB_MAX_TOP}, got {k}")
+    if V < 1:
+        raise ValueError("logits: rows without columns")
+    if lengths is not None:
+        _idx(lengths, "lengths")
+        if tuple(lengths.shape) != (R,):
+            raise ValueError(f"lengths: expected shape [{R}], got {tuple(lengths.shape)}")
+    _same_device(logits, targets, lengths)
+    a = LogProbArgs(logits.data_ptr(), ld, R, V, 0 if lengths is None else lengths.data_ptr(), targets.data_ptr(), T, k,
+                    int(logits.dtype == torch.bfloat16))
+    return a, R, V, T
+
+
+def logprob_fwd(logits: Tensor, targets: Tensor, lengths: Optional[Tensor] = None, k: int = 0,
+                want_stats: bool = False) -> Tuple[LogProbs, Optional[Tensor]]:
+    """Log-probabilities of ``targets`` ([R] or [R, T]; -1 = none) under the softmax over each row's scores (the first
+    ``lengths[r]`` columns of row r; all without ``lengths``), the rows' entropy and log-sum-exp, and their ``k`` best
+    alternatives (rx_logprob_fwd).  Returns (LogProbs, stats for :func:`logprob_bwd` or None)."""
+    a, R, V, T = _logprob_args(logits, targets, lengths, k)
+    dev = logits.device
+    f = lambda *shape: torch.empty(*shape, dtype=torch.float32, device=dev)
+    out = LogProbs(f(targets.shape), f(R), f(R), f(R, k), torch.empty(R, k, dtype=torch.int64, device=dev))
+    stats = f(R, 4) if want_stats else None
+    a.logprob, a.entropy, a.lse = out.logprob.data_ptr(), out.entropy.data_ptr(), out.lse.data_ptr()
+    a.top_logprob, a.top_index = out.top_logprob.data_ptr(), out.top_index.data_ptr()
+    a.stats = 0 if stats is None else stats.data_ptr()
+    need = int(lib.rx_logprob_workspace_bytes(R, V, k))
+    ws = _ws(need, dev) if need else None
+    check(lib.rx_logprob_fwd(C.byref(a), _p(ws), need, _p(_err_flag(dev)), _dev(logits), _stream(logits)), "rx_logprob_fwd")
+    _after_index_op(dev)
+    return out, stats
+
+
+def logprob_bwd(logits: Tensor, targets: Tensor, lengths: Optional[Tensor], stats: Tensor, g_logprob: Optional[Tensor] = None,
+                g_entropy: Optional[Tensor] = None, g_lse: Optional[Tensor] = None) -> Tensor:
+    """Gradient of the scores, in their type, from the gradients of logprob / entropy / lse (fp32; None = zero) and
+    the stats of the forward call (rx_logprob_bwd)."""
+    a, R, V, T = _logprob_args(logits, targets, lengths, 0)
+    _req(stats, torch.float32, "stats", 2)
+    if tuple(stats.shape) != (R, 4):
+        raise ValueError(f"stats: expected shape [{R}, 4], got {tuple(stats.shape)}")
+    for t, name, n in ((g_logprob, "g_logprob", R * T), (g_entropy, "g_entropy", R), (g_lse, "g_lse", R)):
+        if t is not None:
+            _req(t, torch.float32, name)
+            if t.numel() != n:
+                raise ValueError(f"{name}: expected {n} elements, got {t.numel()}")
+    _same_device(logits, stats, g_logprob, g_entropy, g_lse)
+    a.stats = stats.data_ptr()
+    dl = torch.empty(R, V, dtype=logits.dtype, device=logits.device)
+    check(lib.rx_logprob_bwd(C.byref(a), _p(g_logprob), _p(g_entropy), _p(g_lse), _p(dl), V, _dev(logits), _stream(logits)),
+          "rx_logprob_bwd")
+    return dl
 
 
 # ------------------------------------------------------------------ batching
