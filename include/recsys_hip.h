@@ -807,6 +807,59 @@ int rx_logprob_fwd(const rx_logprob_args* args, void* ws, size_t ws_bytes, int32
 int rx_logprob_bwd(const rx_logprob_args* args, const float* d_g_logprob, const float* d_g_entropy, const float* d_g_lse,
                    void* d_dlogits, int64_t ld_d, int device, void* stream);
 
+/* ------------------------------------------------------------------ softmax over a whole catalogue
+ * Scores s_rv = x_r . t_v + b_v of rows x [R, D] against all V rows of a table, never stored:
+ *   lse[r] = log sum_v exp s_rv,  logprob[r] = s_{r, y_r} - lse[r]     (natural logarithms, fp32)
+ * x and the table are fp32, or bf16 with bf16 = 1; the bias is fp32 [V] or NULL.  D up to 256, any value; rows ld_x /
+ * ld_t elements apart.  fp32 operands are multiplied to fp32 accuracy.  A target of -1 stands for "no target" (logprob 0, no
+ * gradient through it); any other target outside [0, V) sets RX_ERR_INDEX and gives NaN.  A bias of -inf takes an item
+ * out; a target that is out gives -inf and no gradient, and a row with no item left gives lse -inf and no gradient.
+ * `stats` [R, 2] and `mean` [R, D] fp32 (both may be NULL) are what rx_catalog_bwd needs: the row's softmax
+ * reference and sum, and sum_v p_rv t_v (only for the gradient of x).
+ * The full-catalogue counterpart of the sampled BCE loss (recsys/models/matrix_factorization/vanilla_mf.py:35-39). */
+typedef struct {
+  const void* x;
+  const void* table;
+  int64_t ld_x, ld_t;
+  const float* bias;
+  const int64_t* targets;    /* [R] */
+  int64_t R, V;              /* R up to 2^24, V up to 2^30 */
+  int32_t D;
+  int32_t bf16;
+} rx_catalog_args;
+size_t rx_catalog_fwd_workspace_bytes(int64_t R, int64_t V, int32_t D, int32_t bf16, int32_t want_mean);
+int rx_catalog_fwd(const rx_catalog_args* args, float* d_logprob, float* d_lse, float* d_stats, float* d_mean, void* ws,
+                   size_t ws_bytes, int32_t* err_flag, int device, void* stream);
+/* Gradients from those of logprob [R] and lse [R] (each may be NULL = zero), with c_r = g_lse_r - g_r:
+ *   dx_r = g_r t_{y_r} + c_r mean_r       dtable_v = sum_r c_r p_rv x_r + sum_{r: y_r = v} g_r x_r
+ *   dbias_v = sum_r c_r p_rv + sum_{r: y_r = v} g_r
+ * d_dx [R, D] / d_dtable [V, D] (the operands' type, 16-byte aligned table gradient, rows back to back) or NULL; with a bias
+ * d_dbias [V] comes with d_dtable.  Deterministic: no atomics.  Workspace only with d_dtable. */
+size_t rx_catalog_bwd_workspace_bytes(int64_t R, int64_t V, int32_t D, int32_t bf16, int32_t want_bias);
+int rx_catalog_bwd(const rx_catalog_args* args, const float* d_stats, const float* d_mean, const float* d_g_logprob,
+                   const float* d_g_lse, void* d_dx, void* d_dtable, float* d_dbias, void* ws, size_t ws_bytes, int device,
+                   void* stream);
+
+/* ------------------------------------------------------------------ orthogonalised updates
+ * Newton-Schulz orthogonalisation of a list of fp32 matrices G [rows, cols], row-major and back to back, into out
+ * (may not overlap):  X = G / (|G|_F + eps), then `steps` times
+ *   A = X X^T,  X <- a X + (b A + c A A) X      (on G^T when rows > cols)
+ * which drives the singular values of G towards 1 and leaves its singular vectors.  Products to fp32 accuracy.
+ * At most RX_ORTHO_MAX matrices per call, none empty, rows and cols up to 16384.  A matrix of zeros gives zeros.
+ * The dense half of a train step (the reference steps every tower with Adam, recsys/pipelines/neuralcf/neumf.py:10). */
+#define RX_ORTHO_MAX 24
+typedef struct {
+  const float* g[RX_ORTHO_MAX];
+  float* out[RX_ORTHO_MAX];
+  int32_t rows[RX_ORTHO_MAX];
+  int32_t cols[RX_ORTHO_MAX];
+  int32_t count;
+  int32_t steps;             /* 1..32 */
+  float a, b, c, eps;
+} rx_ortho_args;
+size_t rx_orthogonalize_workspace_bytes(const rx_ortho_args* args);
+int rx_orthogonalize(const rx_ortho_args* args, void* ws, size_t ws_bytes, int device, void* stream);
+
 /* ------------------------------------------------------------------ dense layers, bf16 activations in HBM
  * The Linear(+ReLU) stacks and DCN-v2 cross layers of recsys_amd.models.fields (a14; the towers of
  * recsys/models/neuralcf/deep_factorization_machine.py:6-24 in their bf16 option) with every

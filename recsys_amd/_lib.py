@@ -102,6 +102,19 @@ class LogProbArgs(C.Structure):
                 ("stats", vp)]
 
 
+class CatalogArgs(C.Structure):
+    _fields_ = [("x", vp), ("table", vp), ("ld_x", i64), ("ld_t", i64), ("bias", vp), ("targets", vp), ("R", i64), ("V", i64),
+                ("D", i32), ("bf16", i32)]
+
+
+RX_ORTHO_MAX = 24
+
+
+class OrthoArgs(C.Structure):
+    _fields_ = [("g", vp * RX_ORTHO_MAX), ("out", vp * RX_ORTHO_MAX), ("rows", i32 * RX_ORTHO_MAX), ("cols", i32 * RX_ORTHO_MAX),
+                ("count", i32), ("steps", i32), ("a", f32), ("b", f32), ("c", f32), ("eps", f32)]
+
+
 # name -> (restype, argtypes); must list every symbol of include/recsys_hip.h
 PROTOTYPES = {
     "rx_abi_version": (C.c_int, []),
@@ -207,6 +220,12 @@ PROTOTYPES = {
     "rx_logprob_workspace_bytes": (sz, [i64, i64, i32]),
     "rx_logprob_fwd": (C.c_int, [C.POINTER(LogProbArgs), vp, sz, vp, C.c_int, vp]),
     "rx_logprob_bwd": (C.c_int, [C.POINTER(LogProbArgs), vp, vp, vp, vp, i64, C.c_int, vp]),
+    "rx_catalog_fwd_workspace_bytes": (sz, [i64, i64, i32, i32, i32]),
+    "rx_catalog_fwd": (C.c_int, [C.POINTER(CatalogArgs), vp, vp, vp, vp, vp, sz, vp, C.c_int, vp]),
+    "rx_catalog_bwd_workspace_bytes": (sz, [i64, i64, i32, i32, i32]),
+    "rx_catalog_bwd": (C.c_int, [C.POINTER(CatalogArgs), vp, vp, vp, vp, vp, vp, vp, vp, sz, C.c_int, vp]),
+    "rx_orthogonalize_workspace_bytes": (sz, [C.POINTER(OrthoArgs)]),
+    "rx_orthogonalize": (C.c_int, [C.POINTER(OrthoArgs), vp, sz, C.c_int, vp]),
     "rx_topk_codes": (C.c_int, [vp, vp, i64, i32, i32, vp, C.c_int, vp]),
 }
 

@@ -1061,3 +1061,69 @@ def log_probs(logits: Tensor, targets: Tensor, lengths: Optional[Tensor] = None,
     if logits.dim() == 2 and ((logits.shape[1] > 1 and logits.stride(1) != 1) or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1])):
         logits = logits.contiguous()
     return ops.LogProbs(*LogProb.apply(logits, targets.contiguous(), None if lengths is None else lengths.contiguous(), k))
+
+
+# ------------------------------------------------------------------ softmax over a whole catalogue
+_ALL_ROWS: dict = {}
+
+
+def all_rows(n_rows: int, device) -> SortedIndex:
+    """The index list 0 .. n_rows - 1 as its own sort, for a gradient that touches every row of a table."""
+    key = (int(n_rows), torch.device(device))
+    si = _ALL_ROWS.get(key)
+    if si is None:
+        i32 = torch.arange(n_rows + 1, dtype=torch.int32, device=device)
+        si = SortedIndex(n_rows, n_rows, i32[:n_rows], i32[:n_rows], torch.arange(n_rows, device=device), i32,
+                         torch.full((1,), n_rows, dtype=torch.int32, device=device))
+        if not (torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing()):
+            if torch.device(device).type == "cuda":
+                torch.cuda.current_stream(device).synchronize()      # once: any stream may read it from here on
+            _ALL_ROWS[key] = si          # a recording keeps its own copy in its pool
+            while len(_ALL_ROWS) > 16:
+                _ALL_ROWS.pop(next(iter(_ALL_ROWS)))
+    return si
+
+
+def full_table_backward(param: Tensor, grad: Tensor):
+    """A gradient for every row of ``param``: handed on as it is, or applied through the parameter's fused sparse
+    rule (all rows touched) when it carries one."""
+    if getattr(param, "_rx_sparse", None) is None:
+        return grad
+    rows = param.shape[0]
+    return table_backward(param, all_rows(rows, param.device), grad.reshape(rows, -1), dim=grad.numel() // rows)
+
+
+class CatalogLogProb(Function):
+    """ops.catalog_fwd with its gradients (rx_catalog_bwd) to x, the table and the bias."""
+
+    @staticmethod
+    def forward(ctx, x, table, targets, bias):
+        need_x, need_t, _, need_b = ctx.needs_input_grad
+        logprob, lse, stats, mean = ops.catalog_fwd(x, table, targets, bias, want_stats=need_x or need_t or need_b, want_mean=need_x)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, table, targets, bias, stats, mean)
+        ctx.params = (table, bias)         # the objects that may carry a sparse rule
+        return logprob, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, gl):
+        x, table, targets, bias, stats, mean = ctx.saved_tensors
+        need_x, need_t, _, need_b = ctx.needs_input_grad
+        if g is None and gl is None:
+            return None, None, None, None
+        g, gl = (None if t is None else t.contiguous() for t in (g, gl))
+        dx, dt, db = ops.catalog_bwd(x, table, targets, bias, stats, mean, g, gl, want_x=need_x, want_table=need_t or need_b)
+        dt = full_table_backward(ctx.params[0], dt) if need_t else None
+        db = full_table_backward(ctx.params[1], db) if need_b else None
+        return dx, dt, None, db
+
+
+def catalog_logprob(x: Tensor, table: Tensor, targets: Tensor, bias: Optional[Tensor] = None):
+    """(logprob [R], lse [R]): log-probabilities of one item per row (-1 = none) under the softmax over all rows of ``table``
+    of ``x @ table.T + bias``, and the log-sum-exp.  ``x`` [R, D] and ``table`` [V, D] both fp32 or both bf16, D <= 256,
+    ``bias`` [V] fp32; the [R, V] scores are never stored.  Differentiable in all three (a table with a fused sparse rule
+    takes its step, on every row)."""
+    if x.dim() == 2 and ((x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
+        x = x.contiguous()
+    return CatalogLogProb.apply(x, table, targets.contiguous(), bias)

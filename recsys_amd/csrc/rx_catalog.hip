@@ -1,0 +1,832 @@
+// Softmax over a whole item catalogue (gfx950): scores s_rv = x_r . t_v + b_v of rows x [R, D] against a table
+// t [V, D], never stored.
+//   forward   lse_r = log sum_v exp s_rv,  logprob_r = s_{r,y_r} - lse_r,  mean_r = sum_v p_rv t_v
+//   backward  dx_r = g_r t_{y_r} + c_r mean_r,   dt_v = sum_r c_r p_rv x_r + sum_{r: y_r = v} g_r x_r,   c_r = g_lse_r - g_r
+// The rows' expectation mean_r does not depend on the gradient, so the forward pass takes it along (online softmax with
+// the table as keys and values) and a train step costs four products of 2 R V D operations: scores and mean forward,
+// scores and dt backward.
+//
+// Both passes are one loop.  One side is stationary (forward: rows, backward: items): its vectors sit in registers as
+// matrix operands, 32 per wavefront and block, one per lane column.  The other side streams through LDS in tiles, kept
+// twice: row-major for the scores, transposed for the second product.  Scores come out of the matrix unit with the
+// streaming index along a lane's registers and the stationary index across the lanes, so the softmax reference and sum
+// are one number per lane, and the weights go straight back in as the other operand of the second product: its
+// contraction index may run in any order, and the transposed tile is laid out in the order the registers have.
+//
+// fp32 operands are cut into three bf16 planes (8 + 8 + 8 significant bits) and the six plane products down to
+// 2^-24 of the result are added in fp32: fp32 accuracy from the bf16 matrix rate (fp32 matrix instructions run at 1/16
+// of it, six products at 1/6).  bf16 operands take one plane; there the weights of the second product are rounded
+// to bf16 as well, 2^-9 relative and independent from term to term, as much as the result's own rounding.
+// Scores, references, sums, means and gradients accumulate in fp32.
+#include "rx_common.h"
+
+typedef __bf16 ct_h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 ct_h2 __attribute__((ext_vector_type(2)));
+typedef float ct_f2 __attribute__((ext_vector_type(2)));
+typedef float ct_acc __attribute__((ext_vector_type(16)));
+
+#define CT_L2E 1.44269504088896340736f
+#define CT_LN2 0.69314718055994530942f
+#define CT_NINF (-__builtin_inff())
+#define CT_MAXD 256
+#define CT_LIM 3.0e38f       // |bias * log2 e| is held inside fp32: masks of the type's lowest value stay finite
+#define CT_SLACK 24.f        // the online reference moves only when a score exceeds it by 2^24
+#define CT_THREADS 256
+#define CT_WAVES 4
+
+struct CtRow {               // what the backward pass needs of a row
+  float m2, l2s, z, sgn;     // p_rv |c_r| = 2^(s log2 e - m2 - l2s), z = m2 + l2s, sgn = sign of c_r
+  float g;                   // gradient of logprob (0 where the row has no target)
+  int32_t y;                 // target or -1
+  int32_t pad0, pad1;
+};
+
+union CtFrag { uint4 u; uint2 d[2]; ct_h8 h; };
+
+__device__ __forceinline__ uint32_t ct_pk(float a, float b) {
+  ct_f2 v = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, ct_h2));
+}
+__device__ __forceinline__ float ct_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float ct_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+
+// two floats -> their words in PL planes
+template <int PL>
+__device__ __forceinline__ void ct_cut2(float a, float b, uint32_t* w) {
+  w[0] = ct_pk(a, b);
+  if constexpr (PL == 3) {
+    a -= ct_lo(w[0]); b -= ct_hi(w[0]);
+    w[1] = ct_pk(a, b);
+    a -= ct_lo(w[1]); b -= ct_hi(w[1]);
+    w[2] = ct_pk(a, b);
+  }
+}
+template <int PL>
+__device__ __forceinline__ void ct_cut8(const float* v, CtFrag* f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w[PL];
+    ct_cut2<PL>(v[2 * i], v[2 * i + 1], w);
+#pragma unroll
+    for (int p = 0; p < PL; ++p) reinterpret_cast<uint32_t*>(&f[p])[i] = w[p];
+  }
+}
+// acc += A B over the planes, the smallest products first
+template <int PL>
+__device__ __forceinline__ ct_acc ct_mma(const CtFrag* a, const CtFrag* b, ct_acc c) {
+#define CT_MM(i, j) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i].h, b[j].h, c, 0, 0, 0)
+  if constexpr (PL == 3) {
+    CT_MM(2, 0); CT_MM(0, 2); CT_MM(1, 1); CT_MM(1, 0); CT_MM(0, 1);
+  }
+  CT_MM(0, 0);
+#undef CT_MM
+  return c;
+}
+
+// ---------------------------------------------------------------- global reads
+template <typename T> __device__ __forceinline__ float ct_elem(const T* p);
+template <> __device__ __forceinline__ float ct_elem<float>(const float* p) { return *p; }
+template <> __device__ __forceinline__ float ct_elem<uint16_t>(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
+
+// four consecutive elements [d, d + 4) of a row, zeros past D
+template <typename T>
+__device__ __forceinline__ float4 ct_load4(const T* row, int d, int D, bool vec) {
+  if (vec && d + 4 <= D) {
+    if constexpr (sizeof(T) == 4) return *reinterpret_cast<const float4*>(row + d);
+    else {
+      const uint2 q = *reinterpret_cast<const uint2*>(row + d);
+      return make_float4(ct_lo(q.x), ct_hi(q.x), ct_lo(q.y), ct_hi(q.y));
+    }
+  }
+  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (d < D) r.x = ct_elem(row + d);
+  if (d + 1 < D) r.y = ct_elem(row + d + 1);
+  if (d + 2 < D) r.z = ct_elem(row + d + 2);
+  if (d + 3 < D) r.w = ct_elem(row + d + 3);
+  return r;
+}
+
+// stationary operands of one block of 32 vectors: lane column l & 31, element ks * 16 + 8 (l >> 5) + j
+template <typename T, int PL, int DP>
+__device__ __forceinline__ void ct_stationary(const T* base, int64_t ld, int64_t row, int64_t rows, int D, bool vec, CtFrag (*f)[PL]) {
+  const int h = rx_lane() >> 5;
+  const T* p = base + (row < rows ? row : 0) * ld;
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) {
+    float v[8];
+    const int d = ks * 16 + h * 8;
+    float4 a = ct_load4(p, d, row < rows ? D : 0, vec), b = ct_load4(p, d + 4, row < rows ? D : 0, vec);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    ct_cut8<PL>(v, f[ks]);
+  }
+}
+
+// ---------------------------------------------------------------- streaming tiles
+// A tile of BN vectors in LDS: rm[PL][BN][DP + 8] row-major and, with TR, tr[PL][DP][BN + 8] transposed.  In the
+// transposed copy the 16 vectors of a contraction step lie as {0-3, 8-11, 4-7, 12-15}: the order in which the two
+// halves of a wavefront hold the scores.  Row strides are odd multiples of 16 bytes: 16-byte reads down the rows meet every
+// bank equally often.
+template <int PL, int DP, int BN, bool TR>
+struct CtTile {
+  static constexpr int RS = DP + 8, TS = BN + 8;
+  static constexpr int RM = PL * BN * RS, TM = TR ? PL * DP * TS : 0;    // 16-bit elements
+  static constexpr int BYTES = (RM + TM) * 2;
+  static constexpr int BLOCKS = BN * DP / 16, PER = (BLOCKS + CT_THREADS - 1) / CT_THREADS;   // 4 x 4 blocks, per thread
+};
+
+template <typename T, int PL, int DP, int BN, bool TR>
+struct CtStage {
+  typedef CtTile<PL, DP, BN, TR> Tile;
+  float4 v[Tile::PER][4];
+  // vectors [row0, row0 + BN) of the streaming side, zeros past `rows`
+  __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row0, int64_t rows, int D, bool vec) {
+#pragma unroll
+    for (int q = 0; q < Tile::PER; ++q) {
+      const int blk = q * CT_THREADS + threadIdx.x;
+      const int d = blk % (DP / 4) * 4, i = blk / (DP / 4) * 4;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t row = row0 + i + k;
+        const bool on = row < rows && (Tile::BLOCKS % CT_THREADS == 0 || blk < Tile::BLOCKS);
+        v[q][k] = ct_load4(base + (on ? row : 0) * ld, d, on ? D : 0, vec);
+      }
+    }
+  }
+  // into LDS; `flip` (may be null): sign words of the tile's vectors, applied to the transposed copy
+  __device__ __forceinline__ void store(uint16_t* rm, uint16_t* tr, const uint32_t* flip) {
+#pragma unroll
+    for (int q = 0; q < Tile::PER; ++q) {
+      const int blk = q * CT_THREADS + threadIdx.x;
+      if (Tile::BLOCKS % CT_THREADS != 0 && blk >= Tile::BLOCKS) continue;
+      const int d = blk % (DP / 4) * 4, ib = blk / (DP / 4);
+      uint32_t w[4][2][PL];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        ct_cut2<PL>(v[q][k].x, v[q][k].y, w[k][0]);
+        ct_cut2<PL>(v[q][k].z, v[q][k].w, w[k][1]);
+      }
+#pragma unroll
+      for (int p = 0; p < PL; ++p)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<uint2*>(rm + (p * BN + ib * 4 + k) * Tile::RS + d) = make_uint2(w[k][0][p], w[k][1][p]);
+      if constexpr (TR) {
+        if (flip) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t f = flip[ib * 4 + k];
+#pragma unroll
+            for (int p = 0; p < PL; ++p) { w[k][0][p] ^= f; w[k][1][p] ^= f; }
+          }
+        }
+        const int pos = (ib >> 2) * 16 + ((ib & 1) * 2 + ((ib >> 1) & 1)) * 4;
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;     // upper or lower halves of two words
+            const uint32_t a = __builtin_amdgcn_perm(w[1][e >> 1][p], w[0][e >> 1][p], sel);
+            const uint32_t b = __builtin_amdgcn_perm(w[3][e >> 1][p], w[2][e >> 1][p], sel);
+            *reinterpret_cast<uint2*>(tr + (p * DP + d + e) * Tile::TS + pos) = make_uint2(a, b);
+          }
+      }
+    }
+  }
+};
+
+// scores of 32 streaming vectors [it * 32, + 32) of the tile against the stationary block
+template <int PL, int DP, int BN, bool TR>
+__device__ __forceinline__ ct_acc ct_scores(const uint16_t* rm, int it, const CtFrag (*st)[PL]) {
+  typedef CtTile<PL, DP, BN, TR> Tile;
+  const int l31 = rx_lane() & 31, h = rx_lane() >> 5;
+  ct_acc s = {};
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) {
+    CtFrag a[PL];
+#pragma unroll
+    for (int p = 0; p < PL; ++p) a[p].u = *reinterpret_cast<const uint4*>(rm + (p * BN + it * 32 + l31) * Tile::RS + ks * 16 + h * 8);
+    s = ct_mma<PL>(a, st[ks], s);
+  }
+  return s;
+}
+// out[db] += transposed tile (dims db * 32 ..) x weights, w[16] in the scores' register order
+template <int PL, int DP, int BN>
+__device__ __forceinline__ void ct_weigh(const uint16_t* tr, int it, const float* w, ct_acc* out) {
+  typedef CtTile<PL, DP, BN, true> Tile;
+  const int l31 = rx_lane() & 31, h = rx_lane() >> 5;
+#pragma unroll
+  for (int k2 = 0; k2 < 2; ++k2) {
+    CtFrag b[PL];
+    ct_cut8<PL>(w + k2 * 8, b);
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) {
+      CtFrag a[PL];
+#pragma unroll
+      for (int p = 0; p < PL; ++p)
+        a[p].u = *reinterpret_cast<const uint4*>(tr + (p * DP + db * 32 + l31) * Tile::TS + it * 32 + k2 * 16 + h * 8);
+      out[db] = ct_mma<PL>(a, b, out[db]);
+    }
+  }
+}
+
+__device__ __forceinline__ float ct_bias2(float b) {      // bias in log2 units; -inf stays, anything else stays finite
+  return b == CT_NINF ? CT_NINF : fminf(fmaxf(b * CT_L2E, -CT_LIM), CT_LIM);
+}
+
+// Which split and which stationary tile a workgroup takes.  Workgroups are dealt to the 8 XCDs in turn; with the splits
+// dealt the same way all tiles of one split meet its part of the streaming side in one L2.
+__device__ __forceinline__ void ct_place(int tiles, int n_split, int* tile, int* split) {
+  const int b = blockIdx.x;
+  if (n_split % 8 == 0) {
+    *split = b % 8 + 8 * (b / (8 * tiles));
+    *tile = b / 8 % tiles;
+  } else {
+    *split = b / tiles;
+    *tile = b % tiles;
+  }
+}
+
+// ---------------------------------------------------------------- forward
+struct CtFwd {
+  const void *x, *t;
+  int64_t ld_x, ld_t, R, V;
+  const float* bias;
+  int D, tiles, n_split;
+  int64_t per_split;           // items per split, a multiple of the tile
+  bool vec;
+  float2* part;                // [n_split][R]: reference, sum
+  float* out;                  // [n_split][R][D]: sum of weight * t_v
+};
+
+template <typename T, int PL, int DP, int MB, int BN, bool MEAN, bool BIAS, int OCC>
+__global__ void __launch_bounds__(CT_THREADS, OCC) ct_fwd_kernel(CtFwd a) {
+  typedef CtTile<PL, DP, BN, MEAN> Tile;
+  extern __shared__ __align__(16) uint8_t ct_lds[];
+  uint16_t* rm = reinterpret_cast<uint16_t*>(ct_lds);
+  uint16_t* tr = rm + Tile::RM;
+  float* lb = reinterpret_cast<float*>(ct_lds + Tile::BYTES);
+  int tile, split;
+  ct_place(a.tiles, a.n_split, &tile, &split);
+  const int wave = threadIdx.x >> 6, l31 = rx_lane() & 31, h = rx_lane() >> 5;
+  const int64_t row0 = ((int64_t)tile * CT_WAVES + wave) * (32 * MB);
+  CtFrag st[MB][DP / 16][PL];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+    ct_stationary<T, PL, DP>((const T*)a.x, a.ld_x, row0 + mb * 32 + l31, a.R, a.D, a.vec, st[mb]);
+  ct_acc o[MB][MEAN ? DP / 32 : 1] = {};
+  float ref[MB], sum[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) { ref[mb] = CT_NINF; sum[mb] = 0.f; }
+  const int64_t v0 = split * a.per_split, v1 = v0 + a.per_split < a.V ? v0 + a.per_split : a.V;
+  CtStage<T, PL, DP, BN, MEAN> stage;
+  float nb = 0.f;
+  if (v0 < v1) {
+    stage.load((const T*)a.t, a.ld_t, v0, v1, a.D, a.vec);
+    if (BIAS && threadIdx.x < BN) nb = v0 + threadIdx.x < v1 ? ct_bias2(a.bias[v0 + threadIdx.x]) : CT_NINF;
+  }
+  for (int64_t v = v0; v < v1; v += BN) {
+    __syncthreads();
+    stage.store(rm, tr, nullptr);
+    if (BIAS && threadIdx.x < BN) lb[threadIdx.x] = nb;
+    __syncthreads();
+    if (v + BN < v1) {
+      stage.load((const T*)a.t, a.ld_t, v + BN, v1, a.D, a.vec);
+      if (BIAS && threadIdx.x < BN) nb = v + BN + threadIdx.x < v1 ? ct_bias2(a.bias[v + BN + threadIdx.x]) : CT_NINF;
+    }
+    const bool whole = v + BN <= v1;
+#pragma unroll
+    for (int it = 0; it < BN / 32; ++it) {
+      float bb[16];
+      if constexpr (BIAS) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4 f = *reinterpret_cast<const float4*>(lb + it * 32 + 8 * q + 4 * h);
+          bb[4 * q] = f.x; bb[4 * q + 1] = f.y; bb[4 * q + 2] = f.z; bb[4 * q + 3] = f.w;
+        }
+      }
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        const ct_acc s = ct_scores<PL, DP, BN, MEAN>(rm, it, st[mb]);
+        float w[16], mx = CT_NINF;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          w[i] = BIAS ? fmaf(s[i], CT_L2E, bb[i]) : s[i] * CT_L2E;
+          if (!whole && v + it * 32 + 8 * (i / 4) + 4 * h + i % 4 >= v1) w[i] = CT_NINF;
+          mx = fmaxf(mx, w[i]);
+        }
+        if (__ballot(mx > ref[mb] + CT_SLACK)) {          // rare after the first tile
+          const float n = fmaxf(mx, __shfl_xor(mx, 32, 64));
+          if (n > ref[mb] + CT_SLACK) {                   // both halves of a row decide alike
+            if (ref[mb] != CT_NINF) {
+              const float f = __builtin_amdgcn_exp2f(ref[mb] - n);
+              sum[mb] *= f;
+              if constexpr (MEAN) {
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) o[mb][db][i] *= f;
+              }
+            }
+            ref[mb] = n;
+          }
+        }
+        const float r0 = ref[mb] == CT_NINF ? 0.f : ref[mb];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          w[i] = __builtin_amdgcn_exp2f(w[i] - r0);
+          sum[mb] += w[i];
+        }
+        if constexpr (MEAN) ct_weigh<PL, DP, BN>(tr, it, w, o[mb]);
+      }
+    }
+  }
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    const float total = sum[mb] + __shfl_xor(sum[mb], 32, 64);
+    const int64_t row = row0 + mb * 32 + l31;
+    if (row >= a.R) continue;
+    if (h == 0) a.part[(int64_t)split * a.R + row] = make_float2(ref[mb], total);
+    if constexpr (MEAN) {
+      float* out = a.out + ((int64_t)split * a.R + row) * a.D;
+      const bool v4 = a.D % 4 == 0;
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int d = db * 32 + 8 * q + 4 * h;
+          if (v4 && d < a.D) *reinterpret_cast<float4*>(out + d) = make_float4(o[mb][db][4 * q], o[mb][db][4 * q + 1], o[mb][db][4 * q + 2], o[mb][db][4 * q + 3]);
+          else
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (d + i < a.D) out[d + i] = o[mb][db][4 * q + i];
+        }
+    }
+  }
+}
+
+// One wavefront per row: joins the splits and takes the target's score as a plain dot product.
+struct CtJoin {
+  const void *x, *t;
+  int64_t ld_x, ld_t, R, V;
+  const float* bias;
+  const int64_t* targets;
+  int D, n_split;
+  const float2* part;
+  const float* out;
+  float *logprob, *lse, *stats, *mean;
+};
+template <typename T>
+__device__ __forceinline__ float ct_dot(const T* x, const T* t, int D) {
+  float s = 0.f;
+  for (int d = rx_lane(); d < D; d += 64) s = fmaf(ct_elem(x + d), ct_elem(t + d), s);
+  return rx_wave_sum(s);
+}
+template <typename T>
+__global__ void __launch_bounds__(CT_THREADS) ct_join_kernel(CtJoin a, int32_t* err) {
+  const int64_t row = (int64_t)blockIdx.x * CT_WAVES + (threadIdx.x >> 6);
+  if (row >= a.R) return;
+  const int lane = rx_lane();
+  float ref = CT_NINF;
+  for (int q = lane; q < a.n_split; q += 64) ref = fmaxf(ref, a.part[(int64_t)q * a.R + row].x);
+  for (int x = 32; x > 0; x >>= 1) ref = fmaxf(ref, __shfl_xor(ref, x, 64));
+  const float r0 = ref == CT_NINF ? 0.f : ref;
+  float s = 0.f;
+  for (int q = lane; q < a.n_split; q += 64) {
+    const float2 p = a.part[(int64_t)q * a.R + row];
+    s += p.y * __builtin_amdgcn_exp2f(p.x - r0);
+  }
+  s = rx_wave_sum(s);
+  const bool empty = s == 0.f;
+  const float l2s = empty ? 0.f : log2f(s), lse = empty ? CT_NINF : (r0 + l2s) * CT_LN2;
+  if (a.mean) {
+    const float inv = empty ? 0.f : 1.f / s;
+    for (int d = lane; d < a.D; d += 64) {
+      float m = 0.f;
+      for (int q = 0; q < a.n_split; ++q)
+        m = fmaf(a.out[((int64_t)q * a.R + row) * a.D + d], __builtin_amdgcn_exp2f(a.part[(int64_t)q * a.R + row].x - r0), m);
+      a.mean[row * a.D + d] = m * inv;
+    }
+  }
+  const int64_t y = a.targets[row];
+  const bool ok = y >= 0 && y < a.V;
+  float lp;
+  if (ok) {
+    const float dot = ct_dot((const T*)a.x + row * a.ld_x, (const T*)a.t + y * a.ld_t, a.D);
+    const float b = a.bias ? a.bias[y] : 0.f, b2 = ct_bias2(b);
+    if (empty || b == CT_NINF) lp = CT_NINF;
+    else if (fabsf(b2) == CT_LIM && fabsf(r0) < 1e38f) lp = dot + b - lse;      // a mask of the type's lowest value
+    else lp = (fmaf(dot, CT_L2E, b2) - r0 - l2s) * CT_LN2;
+  } else lp = y == -1 ? 0.f : __builtin_nanf("");
+  if (lane == 0) {
+    if (!ok && y != -1 && err) atomicOr(err, RX_ERR_INDEX);
+    a.logprob[row] = lp;
+    a.lse[row] = lse;
+    if (a.stats) reinterpret_cast<float2*>(a.stats)[row] = make_float2(r0, empty ? __builtin_inff() : l2s);
+  }
+}
+
+// ---------------------------------------------------------------- backward
+struct CtPrep {
+  const void* t;
+  int64_t ld_t, R, V;
+  const float* bias;
+  const int64_t* targets;
+  int D;
+  const float *stats, *mean, *g, *gl;
+  void* dx;
+  CtRow* rows;
+};
+// dx, and the rows as the table's pass wants them; one wavefront per row
+template <typename T>
+__global__ void __launch_bounds__(CT_THREADS) ct_prep_kernel(CtPrep a) {
+  const int64_t row = (int64_t)blockIdx.x * CT_WAVES + (threadIdx.x >> 6);
+  if (row >= a.R) return;
+  const float2 st = reinterpret_cast<const float2*>(a.stats)[row];
+  int64_t y = a.targets[row];
+  const bool dead = st.y == __builtin_inff();
+  if (dead || y < 0 || y >= a.V || (a.bias && a.bias[y] == CT_NINF)) y = -1;      // nothing depends on such a target
+  const float g = y >= 0 && a.g ? a.g[row] : 0.f;
+  const float c = dead ? 0.f : (a.gl ? a.gl[row] : 0.f) - g;
+  if (rx_lane() == 0 && a.rows) {
+    CtRow r;
+    r.sgn = c < 0.f ? -1.f : 1.f;
+    r.m2 = st.x;
+    r.l2s = c == 0.f ? __builtin_inff() : st.y - log2f(fabsf(c));
+    r.z = r.m2 + r.l2s;
+    r.g = g;
+    r.y = (int32_t)y;
+    r.pad0 = r.pad1 = 0;
+    a.rows[row] = r;
+  }
+  if (a.dx) {
+    const T* t = (const T*)a.t + (y < 0 ? 0 : y) * a.ld_t;
+    for (int d = rx_lane(); d < a.D; d += 64) {
+      const float v = (y < 0 ? 0.f : g * ct_elem(t + d)) + (c == 0.f ? 0.f : c * a.mean[row * a.D + d]);
+      if constexpr (sizeof(T) == 4) ((float*)a.dx)[row * a.D + d] = v;
+      else ((uint16_t*)a.dx)[row * a.D + d] = (uint16_t)ct_pk(v, v);
+    }
+  }
+}
+
+struct CtBwd {
+  const void *x, *t;
+  int64_t ld_x, ld_t, R, V;
+  const float* bias;
+  const CtRow* rows;
+  int D, tiles, n_split;
+  int64_t per_split;           // rows per split, a multiple of the tile
+  bool vec;
+  void* dt;                    // [V][D] in the table's type, or fp32 [n_split][V][D]
+  float* db;                   // [V], or [n_split][V]
+  bool partial;
+};
+
+template <typename T, int PL, int DP, int MB, int BN, bool BIAS, int OCC>
+__global__ void __launch_bounds__(CT_THREADS, OCC) ct_bwd_kernel(CtBwd a) {
+  typedef CtTile<PL, DP, BN, true> Tile;
+  extern __shared__ __align__(16) uint8_t ct_lds[];
+  uint16_t* rm = reinterpret_cast<uint16_t*>(ct_lds);
+  uint16_t* tr = rm + Tile::RM;
+  float* lz = reinterpret_cast<float*>(ct_lds + Tile::BYTES);      // z, or m2 with a bias
+  float* ll = lz + BN;                                             // l2s (bias)
+  float* lsg = ll + BN;                                            // sign of c (bias)
+  float* lg = lsg + BN;
+  int32_t* ly = reinterpret_cast<int32_t*>(lg + BN);
+  uint32_t* lf = reinterpret_cast<uint32_t*>(ly + BN);             // sign words
+  int tile, split;
+  ct_place(a.tiles, a.n_split, &tile, &split);
+  const int wave = threadIdx.x >> 6, lane = rx_lane(), l31 = lane & 31, h = lane >> 5;
+  const int64_t item0 = ((int64_t)tile * CT_WAVES + wave) * (32 * MB);
+  CtFrag st[MB][DP / 16][PL];
+  float b2[MB], dbias[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    const int64_t item = item0 + mb * 32 + l31;
+    ct_stationary<T, PL, DP>((const T*)a.t, a.ld_t, item, a.V, a.D, a.vec, st[mb]);
+    b2[mb] = BIAS && item < a.V ? ct_bias2(a.bias[item]) : 0.f;
+    dbias[mb] = 0.f;
+  }
+  ct_acc o[MB][DP / 32] = {};
+  const int64_t r0 = split * a.per_split, r1 = r0 + a.per_split < a.R ? r0 + a.per_split : a.R;
+  CtStage<T, PL, DP, BN, true> stage;
+  CtRow info;
+  auto fetch = [&](int64_t r) {
+    stage.load((const T*)a.x, a.ld_x, r, r1, a.D, a.vec);
+    if (threadIdx.x < BN) {
+      if (r + threadIdx.x < r1) info = a.rows[r + threadIdx.x];
+      else { info.m2 = 0.f; info.l2s = info.z = __builtin_inff(); info.sgn = 1.f; info.g = 0.f; info.y = -1; }
+    }
+  };
+  if (r0 < r1) fetch(r0);
+  for (int64_t r = r0; r < r1; r += BN) {
+    __syncthreads();
+    if (threadIdx.x < BN) {
+      lz[threadIdx.x] = BIAS ? info.m2 : info.z;
+      if (BIAS) { ll[threadIdx.x] = info.l2s; lsg[threadIdx.x] = info.sgn; }
+      lg[threadIdx.x] = info.g;
+      ly[threadIdx.x] = info.y;
+      lf[threadIdx.x] = info.sgn < 0.f ? 0x80008000u : 0u;
+    }
+    __syncthreads();
+    stage.store(rm, tr, lf);
+    __syncthreads();
+    if (r + BN < r1) fetch(r + BN);
+#pragma unroll
+    for (int it = 0; it < BN / 32; ++it) {
+      float zz[16], z2[BIAS ? 16 : 1], sg[BIAS ? 16 : 1];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4 f = *reinterpret_cast<const float4*>(lz + it * 32 + 8 * q + 4 * h);
+        zz[4 * q] = f.x; zz[4 * q + 1] = f.y; zz[4 * q + 2] = f.z; zz[4 * q + 3] = f.w;
+        if constexpr (BIAS) {
+          const float4 e = *reinterpret_cast<const float4*>(ll + it * 32 + 8 * q + 4 * h);
+          z2[4 * q] = e.x; z2[4 * q + 1] = e.y; z2[4 * q + 2] = e.z; z2[4 * q + 3] = e.w;
+          const float4 n = *reinterpret_cast<const float4*>(lsg + it * 32 + 8 * q + 4 * h);
+          sg[4 * q] = n.x; sg[4 * q + 1] = n.y; sg[4 * q + 2] = n.z; sg[4 * q + 3] = n.w;
+        }
+      }
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        const ct_acc s = ct_scores<PL, DP, BN, true>(rm, it, st[mb]);
+        float w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if constexpr (BIAS) {
+            w[i] = __builtin_amdgcn_exp2f((fmaf(s[i], CT_L2E, b2[mb]) - zz[i]) - z2[i]);
+            dbias[mb] = fmaf(w[i], sg[i], dbias[mb]);
+          } else {
+            w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], CT_L2E, -zz[i]));
+          }
+        }
+        ct_weigh<PL, DP, BN>(tr, it, w, o[mb]);
+      }
+    }
+    // targets of this tile among the wavefront's items: g_r x_r on top, in the order of the rows
+    const int64_t rel = lane < BN && ly[lane] >= 0 ? ly[lane] - item0 : -1;
+    uint64_t hits = __ballot(rel >= 0 && rel < 32 * MB);
+    while (hits) {
+      const int i = __builtin_ctzll(hits);
+      hits &= hits - 1;
+      const int li = __builtin_amdgcn_readlane((int)rel, i);
+      const float g = lg[i];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        const float c = li == mb * 32 + l31 ? g : 0.f;
+        if (BIAS && h == 0) dbias[mb] += c;
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float e[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int p = PL - 1; p >= 0; --p) {
+              const uint2 u = *reinterpret_cast<const uint2*>(rm + (p * BN + i) * Tile::RS + db * 32 + 8 * q + 4 * h);
+              e[0] += ct_lo(u.x); e[1] += ct_hi(u.x); e[2] += ct_lo(u.y); e[3] += ct_hi(u.y);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[mb][db][4 * q + k] = c != 0.f ? fmaf(c, e[k], o[mb][db][4 * q + k]) : o[mb][db][4 * q + k];
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    const float total = dbias[mb] + __shfl_xor(dbias[mb], 32, 64);
+    const int64_t item = item0 + mb * 32 + l31;
+    if (item >= a.V) continue;
+    const int64_t at = (a.partial ? (int64_t)split * a.V : 0) + item;
+    if (BIAS && h == 0) a.db[at] = total;
+    const bool v4 = a.D % 4 == 0;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int d = db * 32 + 8 * q + 4 * h;
+        const float e[4] = {o[mb][db][4 * q], o[mb][db][4 * q + 1], o[mb][db][4 * q + 2], o[mb][db][4 * q + 3]};
+        if (sizeof(T) == 4 || a.partial) {
+          float* p = (float*)a.dt + at * a.D + d;
+          if (v4 && d < a.D) *reinterpret_cast<float4*>(p) = make_float4(e[0], e[1], e[2], e[3]);
+          else
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (d + i < a.D) p[i] = e[i];
+        } else {
+          uint16_t* p = (uint16_t*)a.dt + at * a.D + d;
+          if (v4 && d < a.D) *reinterpret_cast<uint2*>(p) = make_uint2(ct_pk(e[0], e[1]), ct_pk(e[2], e[3]));
+          else
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (d + i < a.D) p[i] = (uint16_t)ct_pk(e[i], e[i]);
+        }
+      }
+  }
+}
+
+// sums of n_split partial arrays of n elements, in split order
+template <typename T>
+__global__ void __launch_bounds__(CT_THREADS) ct_sum_kernel(const float* __restrict__ part, int64_t n, int n_split, T* __restrict__ out) {
+  for (int64_t i = (int64_t)blockIdx.x * CT_THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * CT_THREADS) {
+    float s = 0.f;
+    for (int q = 0; q < n_split; ++q) s += part[q * n + i];
+    if constexpr (sizeof(T) == 4) out[i] = s;
+    else out[i] = (uint16_t)ct_pk(s, s);
+  }
+}
+
+// ---------------------------------------------------------------- host
+static int ct_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+static int ct_mb(bool bf16, int dp) { return bf16 && dp <= 64 ? 2 : 1; }
+static int ct_bn(bool bf16, int dp) { return bf16 ? (dp <= 128 ? 64 : 32) : (dp <= 64 ? 64 : 32); }
+
+struct CtPlan {
+  int tiles, n_split;
+  int64_t per_split;
+};
+// `fixed` vectors are stationary, `moving` ones stream: enough splits of the stream for four workgroups per CU, each of
+// at least two tiles; multiples of 8 (one XCD each) where there are that many.
+static CtPlan ct_plan(int64_t fixed, int64_t moving, int bm, int bn) {
+  CtPlan p;
+  p.tiles = (int)rx_cdiv(fixed, bm);
+  int64_t n = rx_cdiv(1024, p.tiles);
+  const int64_t most = rx_cdiv(moving, 2 * bn);
+  if (n > most) n = most;
+  if (n > 8) n = n / 8 * 8;
+  if (n < 1) n = 1;
+  p.per_split = rx_cdiv(rx_cdiv(moving, n), bn) * bn;
+  p.n_split = (int)rx_cdiv(moving, p.per_split);
+  if (p.n_split < 1) p.n_split = 1;
+  return p;
+}
+
+static int ct_check(const rx_catalog_args* a, const char* who) {
+  RX_REQUIRE(a, "%s: null argument", who);
+  RX_REQUIRE(a->R >= 0 && a->R <= (1 << 24) && a->V >= 1 && a->V <= (1ll << 30) && a->D >= 1 && a->D <= CT_MAXD,
+             "%s: bad shape R=%lld V=%lld D=%d (R up to 2^24, V up to 2^30, D up to %d)", who, (long long)a->R, (long long)a->V, a->D, CT_MAXD);
+  RX_REQUIRE(a->ld_x >= a->D && a->ld_t >= a->D, "%s: row strides %lld, %lld below D=%d", who, (long long)a->ld_x, (long long)a->ld_t, a->D);
+  RX_REQUIRE(a->bf16 == 0 || a->bf16 == 1, "%s: bad element type %d", who, a->bf16);
+  if (a->R == 0) return 0;
+  RX_REQUIRE(a->x && a->table && a->targets, "%s: null argument", who);
+  const uintptr_t al = a->bf16 ? 1 : 3;
+  RX_REQUIRE(((uintptr_t)a->x & al) == 0 && ((uintptr_t)a->table & al) == 0, "%s: x or table not aligned to their elements", who);
+  return 0;
+}
+static bool ct_vec(const rx_catalog_args* a) {      // 4-element loads
+  const uintptr_t al = a->bf16 ? 7 : 15;
+  return a->D % 4 == 0 && a->ld_x % 4 == 0 && a->ld_t % 4 == 0 && ((uintptr_t)a->x & al) == 0 && ((uintptr_t)a->table & al) == 0;
+}
+
+static CtPlan ct_fwd_plan(int64_t R, int64_t V, int D, int bf16) {
+  const int dp = ct_dp(D);
+  return ct_plan(R, V, CT_WAVES * 32 * ct_mb(bf16, dp), ct_bn(bf16, dp));
+}
+static CtPlan ct_bwd_plan(int64_t R, int64_t V, int D, int bf16) {
+  const int dp = ct_dp(D);
+  return ct_plan(V, R, CT_WAVES * 32 * ct_mb(bf16, dp), ct_bn(bf16, dp));
+}
+
+extern "C" size_t rx_catalog_fwd_workspace_bytes(int64_t R, int64_t V, int32_t D, int32_t bf16, int32_t want_mean) {
+  if (R <= 0 || V <= 0 || D < 1 || D > CT_MAXD) return 0;
+  const CtPlan p = ct_fwd_plan(R, V, D, bf16);
+  return rx_align_up((size_t)p.n_split * R * sizeof(float2), 256) + (want_mean ? (size_t)p.n_split * R * D * 4 : 0);
+}
+extern "C" size_t rx_catalog_bwd_workspace_bytes(int64_t R, int64_t V, int32_t D, int32_t bf16, int32_t want_bias) {
+  if (R <= 0 || V <= 0 || D < 1 || D > CT_MAXD) return 0;
+  const CtPlan p = ct_bwd_plan(R, V, D, bf16);
+  return rx_align_up((size_t)R * sizeof(CtRow), 256) +
+         (p.n_split > 1 ? rx_align_up((size_t)p.n_split * V * D * 4, 256) + (want_bias ? (size_t)p.n_split * V * 4 : 0) : 0);
+}
+
+
+template <typename T, int PL, int DP, int MB, int BN, bool MEAN, bool BIAS, int OCC>
+static int ct_go_fwd(const CtFwd& f, hipStream_t st) {
+  auto kernel = ct_fwd_kernel<T, PL, DP, MB, BN, MEAN, BIAS, OCC>;
+  const int lds = CtTile<PL, DP, BN, MEAN>::BYTES + (BIAS ? BN * 4 : 0);
+  if (lds > 64 * 1024) RX_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(f.tiles * f.n_split)), dim3(CT_THREADS), lds, st, f);
+  return 0;
+}
+template <typename T, int PL, int DP, int MB, int BN, int OCC>
+static int ct_pick_fwd(const CtFwd& f, hipStream_t st) {
+  if (f.out) return f.bias ? ct_go_fwd<T, PL, DP, MB, BN, true, true, OCC>(f, st) : ct_go_fwd<T, PL, DP, MB, BN, true, false, OCC>(f, st);
+  return f.bias ? ct_go_fwd<T, PL, DP, MB, BN, false, true, OCC>(f, st) : ct_go_fwd<T, PL, DP, MB, BN, false, false, OCC>(f, st);
+}
+template <typename T, int PL, int DP, int MB, int BN, int OCC>
+static int ct_pick_bwd(const CtBwd& f, hipStream_t st) {
+  const int lds = CtTile<PL, DP, BN, true>::BYTES + 6 * BN * 4;
+  if (f.db) {
+    auto kernel = ct_bwd_kernel<T, PL, DP, MB, BN, true, OCC>;
+    if (lds > 64 * 1024) RX_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(f.tiles * f.n_split)), dim3(CT_THREADS), lds, st, f);
+  } else {
+    auto kernel = ct_bwd_kernel<T, PL, DP, MB, BN, false, OCC>;
+    if (lds > 64 * 1024) RX_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(f.tiles * f.n_split)), dim3(CT_THREADS), lds, st, f);
+  }
+  return 0;
+}
+
+extern "C" int rx_catalog_fwd(const rx_catalog_args* args, float* d_logprob, float* d_lse, float* d_stats, float* d_mean, void* ws,
+                              size_t ws_bytes, int32_t* err_flag, int device, void* stream) {
+  if (ct_check(args, "rx_catalog_fwd")) return 1;
+  const rx_catalog_args a = *args;
+  if (a.R == 0) return 0;
+  RX_REQUIRE(d_logprob && d_lse, "rx_catalog_fwd: null output");
+  RX_REQUIRE(((uintptr_t)d_stats & 7) == 0, "rx_catalog_fwd: stats must be 8-byte aligned");
+  const size_t need = rx_catalog_fwd_workspace_bytes(a.R, a.V, a.D, a.bf16, d_mean != nullptr);
+  RX_REQUIRE(ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0, "rx_catalog_fwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
+  RX_GUARD_DEVICE(device);
+  const CtPlan p = ct_fwd_plan(a.R, a.V, a.D, a.bf16);
+  float2* part = (float2*)ws;
+  float* out = d_mean ? (float*)((uint8_t*)ws + rx_align_up((size_t)p.n_split * a.R * sizeof(float2), 256)) : nullptr;
+  CtFwd f = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, a.D, p.tiles, p.n_split, p.per_split, ct_vec(&a), part, out};
+  hipStream_t st = (hipStream_t)stream;
+  int rc;
+  if (a.bf16) {
+    switch (ct_dp(a.D)) {
+      case 32: rc = ct_pick_fwd<uint16_t, 1, 32, 2, 64, 2>(f, st); break;
+      case 64: rc = ct_pick_fwd<uint16_t, 1, 64, 2, 64, 2>(f, st); break;
+      case 128: rc = ct_pick_fwd<uint16_t, 1, 128, 1, 64, 2>(f, st); break;
+      default: rc = ct_pick_fwd<uint16_t, 1, 256, 1, 32, 1>(f, st);
+    }
+  } else {
+    switch (ct_dp(a.D)) {
+      case 32: rc = ct_pick_fwd<float, 3, 32, 1, 64, 2>(f, st); break;
+      case 64: rc = ct_pick_fwd<float, 3, 64, 1, 64, 2>(f, st); break;
+      case 128: rc = ct_pick_fwd<float, 3, 128, 1, 32, 1>(f, st); break;
+      default: rc = ct_pick_fwd<float, 3, 256, 1, 32, 1>(f, st);
+    }
+  }
+  if (rc) return rc;
+  RX_LAUNCH_CHECK();
+  CtJoin j = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, a.targets, a.D, p.n_split, part, out, d_logprob, d_lse, d_stats, d_mean};
+  const dim3 grid((unsigned)rx_cdiv(a.R, CT_WAVES));
+  if (a.bf16) hipLaunchKernelGGL(ct_join_kernel<uint16_t>, grid, dim3(CT_THREADS), 0, st, j, err_flag);
+  else hipLaunchKernelGGL(ct_join_kernel<float>, grid, dim3(CT_THREADS), 0, st, j, err_flag);
+  RX_LAUNCH_CHECK();
+  return 0;
+}
+
+extern "C" int rx_catalog_bwd(const rx_catalog_args* args, const float* d_stats, const float* d_mean, const float* d_g_logprob,
+                              const float* d_g_lse, void* d_dx, void* d_dtable, float* d_dbias, void* ws, size_t ws_bytes, int device,
+                              void* stream) {
+  if (ct_check(args, "rx_catalog_bwd")) return 1;
+  const rx_catalog_args a = *args;
+  if (a.R == 0) return 0;
+  RX_REQUIRE(d_stats && ((uintptr_t)d_stats & 7) == 0, "rx_catalog_bwd: stats missing or not 8-byte aligned");
+  RX_REQUIRE(!d_dx || d_mean, "rx_catalog_bwd: the gradient of x needs the means of the forward call");
+  RX_REQUIRE(!d_dbias || (a.bias && d_dtable), "rx_catalog_bwd: the bias gradient needs a bias and comes with the table's");
+  RX_REQUIRE(((uintptr_t)d_dtable & 15) == 0 && ((uintptr_t)d_dx & (a.bf16 ? 1 : 3)) == 0, "rx_catalog_bwd: gradient buffers not aligned");
+  const bool want_t = d_dtable != nullptr;
+  const size_t need = want_t ? rx_catalog_bwd_workspace_bytes(a.R, a.V, a.D, a.bf16, d_dbias != nullptr) : 0;
+  RX_REQUIRE(!want_t || (ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0), "rx_catalog_bwd: workspace of %zu bytes, %zu needed",
+             ws_bytes, need);
+  RX_GUARD_DEVICE(device);
+  hipStream_t st = (hipStream_t)stream;
+  CtRow* rows = want_t ? (CtRow*)ws : nullptr;
+  CtPrep q = {a.table, a.ld_t, a.R, a.V, a.bias, a.targets, a.D, d_stats, d_mean, d_g_logprob, d_g_lse, d_dx, rows};
+  const dim3 grid((unsigned)rx_cdiv(a.R, CT_WAVES));
+  if (a.bf16) hipLaunchKernelGGL(ct_prep_kernel<uint16_t>, grid, dim3(CT_THREADS), 0, st, q);
+  else hipLaunchKernelGGL(ct_prep_kernel<float>, grid, dim3(CT_THREADS), 0, st, q);
+  RX_LAUNCH_CHECK();
+  if (!want_t) return 0;
+  const CtPlan p = ct_bwd_plan(a.R, a.V, a.D, a.bf16);
+  uint8_t* w = (uint8_t*)ws + rx_align_up((size_t)a.R * sizeof(CtRow), 256);
+  const bool partial = p.n_split > 1;
+  float* pt = (float*)w;
+  float* pb = (float*)(w + rx_align_up((size_t)p.n_split * a.V * a.D * 4, 256));
+  // with a bias but no gradient asked for it, the pass still needs the bias: its sums then go to the partial's place
+  CtBwd f = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, rows, a.D, p.tiles, p.n_split, p.per_split, ct_vec(&a),
+             partial ? (void*)pt : d_dtable, partial ? (d_dbias ? pb : nullptr) : d_dbias, partial};
+  RX_REQUIRE(!a.bias || f.db, "rx_catalog_bwd: with a bias the table's gradient comes with the bias gradient");
+  int rc;
+  if (a.bf16) {
+    switch (ct_dp(a.D)) {
+      case 32: rc = ct_pick_bwd<uint16_t, 1, 32, 2, 64, 2>(f, st); break;
+      case 64: rc = ct_pick_bwd<uint16_t, 1, 64, 2, 64, 2>(f, st); break;
+      case 128: rc = ct_pick_bwd<uint16_t, 1, 128, 1, 64, 2>(f, st); break;
+      default: rc = ct_pick_bwd<uint16_t, 1, 256, 1, 32, 1>(f, st);
+    }
+  } else {
+    switch (ct_dp(a.D)) {
+      case 32: rc = ct_pick_bwd<float, 3, 32, 1, 64, 2>(f, st); break;
+      case 64: rc = ct_pick_bwd<float, 3, 64, 1, 64, 2>(f, st); break;
+      case 128: rc = ct_pick_bwd<float, 3, 128, 1, 32, 1>(f, st); break;
+      default: rc = ct_pick_bwd<float, 3, 256, 1, 32, 1>(f, st);
+    }
+  }
+  if (rc) return rc;
+  RX_LAUNCH_CHECK();
+  if (partial) {
+    const int64_t n = a.V * a.D;
+    const dim3 g((unsigned)(rx_cdiv(n, CT_THREADS) < 4096 ? rx_cdiv(n, CT_THREADS) : 4096));
+    if (a.bf16) hipLaunchKernelGGL(ct_sum_kernel<uint16_t>, g, dim3(CT_THREADS), 0, st, pt, n, p.n_split, (uint16_t*)d_dtable);
+    else hipLaunchKernelGGL(ct_sum_kernel<float>, g, dim3(CT_THREADS), 0, st, pt, n, p.n_split, (float*)d_dtable);
+    RX_LAUNCH_CHECK();
+    if (d_dbias) {
+      const dim3 gb((unsigned)(rx_cdiv(a.V, CT_THREADS) < 4096 ? rx_cdiv(a.V, CT_THREADS) : 4096));
+      hipLaunchKernelGGL(ct_sum_kernel<float>, gb, dim3(CT_THREADS), 0, st, pb, a.V, p.n_split, d_dbias);
+      RX_LAUNCH_CHECK();
+    }
+  }
+  return 0;
+}

@@ -690,7 +690,9 @@ static int lp_check(const rx_logprob_args* a, const char* who) {
   RX_REQUIRE(a->R >= 0 && a->V >= 1 && a->V < (1ll << 31) - 64 && a->ld >= a->V, "%s: bad shape R=%lld V=%lld ld=%lld", who,
              (long long)a->R, (long long)a->V, (long long)a->ld);
   RX_REQUIRE(a->T >= 0 && a->T <= 1024, "%s: T=%d targets per row (at most 1024)", who, a->T);
-  RX_REQUIRE(a->R * (int64_t)lp_splits(a->R, a->V) < (1ll << 31), "%s: R=%lld rows are more than one launch takes", who, (long long)a->R);
+  // a launch takes fewer than 2^32 threads
+  const int64_t per = a->V > LP_SMALL ? 1 : a->V <= 8 && a->k == 0 ? RX_BLOCK / 8 : RX_BLOCK / 64;
+  RX_REQUIRE(a->R <= ((1ll << 24) - 1) * per / lp_splits(a->R, a->V), "%s: R=%lld rows are more than one launch takes", who, (long long)a->R);
   RX_REQUIRE(a->bf16 == 0 || a->bf16 == 1, "%s: bad element type %d", who, a->bf16);
   if (a->R == 0) return 0;
   RX_REQUIRE(a->logits && (a->T == 0 || a->targets), "%s: null argument", who);

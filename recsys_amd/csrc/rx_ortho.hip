@@ -1,0 +1,479 @@
+// Newton-Schulz orthogonalisation of weight updates (gfx950):  X = G / (|G|_F + eps), then `steps` times
+//   A = X X^T,  B = b A + c A A,  X <- a X + B X          (m = min(rows, cols) rows after a transpose, n = max columns)
+//
+// The products take all the time: m^2 n + m^3 + 2 m^2 n operations per step, A and A A being symmetric (only tiles on and
+// below the diagonal are computed, the others are their mirror images).  Small singular values grow by up to a^steps = 485,
+// and so do rounding errors along them: bf16 products would leave errors of the size of the result there, so the products
+// keep fp32 accuracy.
+//   * Matrices that fit one workgroup's LDS take all steps in one launch, on fp32 matrix instructions: such lists are
+//     bound by launches, not by products.
+//   * The others share three launches per step, whatever their number.  X, X^T, A and B live in the workspace as three
+//     bf16 planes each (8 + 8 + 8 significant bits), cut once in the epilogue that makes them; six plane products give
+//     fp32 accuracy at 1/6 of the bf16 rate where fp32 matrix instructions have 1/16.  With X^T kept beside X
+//     all three products read both operands along the contraction.
+#include "rx_common.h"
+
+typedef __bf16 ns_h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 ns_h2 __attribute__((ext_vector_type(2)));
+typedef float ns_f2 __attribute__((ext_vector_type(2)));
+typedef float ns_f4 __attribute__((ext_vector_type(4)));
+typedef float ns_acc __attribute__((ext_vector_type(16)));
+
+#define NS_MAXDIM 16384
+#define NS_SMALL_M 96
+#define NS_SMALL_LDS (152 * 1024)
+#define NS_SMALL_THREADS 512
+#define NS_PARTS 64            // norm partials per matrix
+
+// ---------------------------------------------------------------- small matrices: one workgroup each
+struct NsSmall {
+  const float* g[RX_ORTHO_MAX];
+  float* out[RX_ORTHO_MAX];
+  int32_t rows[RX_ORTHO_MAX], cols[RX_ORTHO_MAX];
+  int32_t steps;
+  float a, b, c, eps;
+};
+static inline int ns_up(int x, int a) { return (x + a - 1) / a * a; }
+static size_t ns_small_lds(int rows, int cols) {
+  const int m = ns_up(rows < cols ? rows : cols, 16), n = ns_up(rows < cols ? cols : rows, 16);
+  return ((size_t)m * (n + 4) + 2 * (size_t)m * (m + 4)) * 4;
+}
+static bool ns_is_small(int rows, int cols) {
+  return (rows < cols ? rows : cols) <= NS_SMALL_M && ns_small_lds(rows, cols) <= NS_SMALL_LDS;
+}
+
+// C (m x m, symmetric) tiles on and below the diagonal of s U U^T + t W, both images written; U [m][K] in LDS
+__device__ __forceinline__ void ns_small_gram(const float* U, int ldu, int K, int mt, float s, float t, const float* W, float* C, int ldc) {
+  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = rx_lane(), l15 = lane & 15, q = lane >> 4;
+  const int tiles = mt * (mt + 1) / 2;
+  for (int x = wave; x < tiles; x += waves) {
+    int i = 0;
+    while ((i + 1) * (i + 2) / 2 <= x) ++i;
+    const int j = x - i * (i + 1) / 2;
+    const float* ui = U + (i * 16 + l15) * ldu + q;
+    const float* uj = U + (j * 16 + l15) * ldu + q;
+    ns_f4 acc0 = {}, acc1 = {};
+    int k = 0;
+    for (; k + 8 <= K; k += 8) {
+      acc0 = __builtin_amdgcn_mfma_f32_16x16x4f32(ui[k], uj[k], acc0, 0, 0, 0);
+      acc1 = __builtin_amdgcn_mfma_f32_16x16x4f32(ui[k + 4], uj[k + 4], acc1, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = i * 16 + q * 4 + e, c = j * 16 + l15;
+      float v = s * (acc0[e] + acc1[e]);
+      if (W) v = fmaf(t, W[r * ldc + c], v);
+      C[r * ldc + c] = v;
+      C[c * ldc + r] = v;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(NS_SMALL_THREADS) ns_small_kernel(NsSmall a) {
+  extern __shared__ __align__(16) float ns_lds[];
+  __shared__ double part[NS_SMALL_THREADS / 64];
+  const float* g = a.g[blockIdx.x];
+  float* out = a.out[blockIdx.x];
+  const int rows = a.rows[blockIdx.x], cols = a.cols[blockIdx.x];
+  const bool flip = rows > cols;
+  const int m = flip ? cols : rows, n = flip ? rows : cols;
+  const int mp = (m + 15) & ~15, np = (n + 15) & ~15, ldx = np + 4, ldc = mp + 4, mt = mp / 16;
+  float* X = ns_lds;
+  float* A = X + mp * ldx;
+  float* B = A + mp * ldc;
+  const int lane = rx_lane(), wave = threadIdx.x >> 6, waves = blockDim.x >> 6, l15 = lane & 15, q = lane >> 4;
+  for (int i = threadIdx.x; i < mp * ldx; i += blockDim.x) X[i] = 0.f;
+  __syncthreads();
+  double ss = 0.0;
+  for (int i = threadIdx.x; i < rows * cols; i += blockDim.x) {
+    const int r = i / cols, c = i - r * cols;
+    const float v = g[i];
+    ss = fma((double)v, (double)v, ss);
+    X[flip ? c * ldx + r : r * ldx + c] = v;
+  }
+  ss = rx_wave_sum_f64(ss);
+  if (lane == 0) part[wave] = ss;
+  __syncthreads();
+  ss = 0.0;
+  for (int w = 0; w < waves; ++w) ss += part[w];
+  const float div = (float)(sqrt(ss) + (double)a.eps);
+  for (int i = threadIdx.x; i < mp * ldx; i += blockDim.x) X[i] /= i % ldx < n && i / ldx < m ? div : 1.f;   // padding stays 0
+  __syncthreads();
+  for (int step = 0; step < a.steps; ++step) {
+    ns_small_gram(X, ldx, np, mt, 1.f, 0.f, nullptr, A, ldc);
+    __syncthreads();
+    ns_small_gram(A, ldc, mp, mt, a.c, a.b, A, B, ldc);
+    __syncthreads();
+    // a wavefront owns 16 columns of X: all of them are read before any is written
+    for (int cb = wave; cb < np / 16; cb += waves) {
+      float x[NS_SMALL_M / 4];                     // rows q + 4 k of the lane's column
+      float* col = X + cb * 16 + l15;
+#pragma unroll
+      for (int k = 0; k < NS_SMALL_M / 4; ++k) x[k] = k * 4 < mp ? col[(k * 4 + q) * ldx] : 0.f;
+      ns_f4 acc[NS_SMALL_M / 16];
+#pragma unroll
+      for (int i = 0; i < NS_SMALL_M / 16; ++i) {
+        acc[i] = ns_f4{};
+        if (i < mt) {
+          const float* bi = B + (i * 16 + l15) * ldc + q;
+#pragma unroll
+          for (int k = 0; k < NS_SMALL_M / 4; ++k)
+            if (k * 4 < mp) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(bi[k * 4], x[k], acc[i], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NS_SMALL_M / 16; ++i)
+        if (i < mt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float* p = col + (i * 16 + q * 4 + e) * ldx;
+            *p = fmaf(a.a, *p, acc[i][e]);
+          }
+        }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < rows * cols; i += blockDim.x) {
+    const int r = i / cols, c = i - r * cols;
+    out[i] = X[flip ? c * ldx + r : r * ldx + c];
+  }
+}
+
+// ---------------------------------------------------------------- large matrices: planes
+struct NsMat {
+  const float* g;
+  float* out;
+  int32_t rows, cols;          // as given
+  int32_t m, n, mp, np;        // working shape, and padded to the tile
+  uint16_t *x[2], *xt[2];      // [3][mp][np], [3][np][mp], alternating by step
+  uint16_t *A, *B;             // [3][mp][mp]
+  int32_t tiles_sym, tiles_x;
+  int32_t pad_;
+};
+struct NsList {
+  NsMat mat[RX_ORTHO_MAX];
+  int32_t count, steps, tile, pad_;
+  float a, b, c, eps;
+  double* parts;               // [count][NS_PARTS]
+};
+
+__device__ __forceinline__ uint32_t ns_pk(float a, float b) {
+  ns_f2 v = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, ns_h2));
+}
+__device__ __forceinline__ float ns_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float ns_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ void ns_cut2(float a, float b, uint32_t* w) {
+#pragma unroll
+  for (int p = 0; p < 3; ++p) {
+    w[p] = ns_pk(a, b);
+    a -= ns_lo(w[p]);
+    b -= ns_hi(w[p]);
+  }
+}
+__device__ __forceinline__ float ns_join(const uint16_t* p, int64_t plane, int64_t at) {
+  return (__uint_as_float((uint32_t)p[2 * plane + at] << 16) + __uint_as_float((uint32_t)p[plane + at] << 16)) + __uint_as_float((uint32_t)p[at] << 16);
+}
+
+__global__ void __launch_bounds__(RX_BLOCK) ns_norm_kernel(NsList a) {
+  const int mi = blockIdx.x / NS_PARTS, pt = blockIdx.x % NS_PARTS;
+  const NsMat& t = a.mat[mi];
+  const int64_t n = (int64_t)t.rows * t.cols;
+  double s = 0.0;
+  for (int64_t i = (int64_t)pt * RX_BLOCK + threadIdx.x; i < n; i += (int64_t)NS_PARTS * RX_BLOCK) {
+    const double v = t.g[i];
+    s = fma(v, v, s);
+  }
+  __shared__ double w[RX_BLOCK / 64];
+  s = rx_wave_sum_f64(s);
+  if (rx_lane() == 0) w[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) a.parts[blockIdx.x] = ((w[0] + w[1]) + w[2]) + w[3];
+}
+
+// planes of X and X^T from G, 64 x 64 at a time, padding included
+__global__ void __launch_bounds__(RX_BLOCK) ns_init_kernel(NsList a) {
+  __shared__ float tl[64][65];
+  int mi = 0, b = blockIdx.x;
+  for (; mi < a.count; ++mi) {
+    const int k = (a.mat[mi].mp / 64) * (a.mat[mi].np / 64);
+    if (b < k) break;
+    b -= k;
+  }
+  if (mi == a.count) return;
+  const NsMat& t = a.mat[mi];
+  double ss = 0.0;
+  for (int i = 0; i < NS_PARTS; ++i) ss += a.parts[mi * NS_PARTS + i];
+  const float div = (float)(sqrt(ss) + (double)a.eps);
+  const int r0 = b / (t.np / 64) * 64, c0 = b % (t.np / 64) * 64;      // of X
+  const bool flip = t.rows > t.cols;
+  for (int i = threadIdx.x; i < 64 * 64; i += RX_BLOCK) {
+    const int y = i / 64, x = i % 64;
+    const int r = flip ? c0 + y : r0 + y, c = flip ? r0 + x : c0 + x;  // of G: rows of it are read along
+    const float v = r < t.rows && c < t.cols ? t.g[(int64_t)r * t.cols + c] / div : 0.f;
+    if (flip) tl[x][y] = v;
+    else tl[y][x] = v;
+  }
+  __syncthreads();
+  const int64_t plane = (int64_t)t.mp * t.np;
+  for (int i = threadIdx.x; i < 64 * 32; i += RX_BLOCK) {
+    const int y = i / 32, x = i % 32 * 2;
+    uint32_t w[3];
+    ns_cut2(tl[y][x], tl[y][x + 1], w);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *reinterpret_cast<uint32_t*>(t.x[0] + p * plane + (int64_t)(r0 + y) * t.np + c0 + x) = w[p];
+    ns_cut2(tl[x][y], tl[x + 1][y], w);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *reinterpret_cast<uint32_t*>(t.xt[0] + p * plane + (int64_t)(c0 + y) * t.mp + r0 + x) = w[p];
+  }
+}
+
+// One T x T tile of P Q^T from planes P [3][.][K], Q [3][.][K]: four wavefronts, (T / 2)^2 each.
+#define NS_BK 32
+#define NS_LDK (NS_BK + 8)
+template <int T>
+struct NsTile {
+  static constexpr int NB = T / 64;
+  static constexpr int CH = 2 * 3 * T * (NS_BK / 8) / RX_BLOCK;       // 16-byte chunks per thread and step
+};
+
+enum { NS_MODE_A, NS_MODE_B, NS_MODE_X };
+
+// chunk x of a step: 16 bytes of a row, the rows of a plane, the planes of an operand
+template <int T>
+__device__ __forceinline__ void ns_fetch(uint4 (&pre)[NsTile<T>::CH], const uint16_t* P, int64_t pp, const uint16_t* Q, int64_t pq, int K, int k0) {
+#pragma unroll
+  for (int q = 0; q < NsTile<T>::CH; ++q) {
+    const int x = q * RX_BLOCK + threadIdx.x;
+    const int ch = x % (NS_BK / 8), row = x / (NS_BK / 8) % T, pl = x / (NS_BK / 8) / T % 3, op = x / (NS_BK / 8) / T / 3;
+    const uint16_t* src = op ? Q + pl * pq : P + pl * pp;
+    pre[q] = *reinterpret_cast<const uint4*>(src + (int64_t)row * K + k0 + ch * 8);
+  }
+}
+
+template <int T, int MODE>
+__global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step) {
+  constexpr int NB = NsTile<T>::NB, CH = NsTile<T>::CH;
+  __shared__ __align__(16) uint16_t lds[2][3][T][NS_LDK];
+  int mi = 0, b = blockIdx.x;
+  for (; mi < a.count; ++mi) {
+    const int k = MODE == NS_MODE_X ? a.mat[mi].tiles_x : a.mat[mi].tiles_sym;
+    if (b < k) break;
+    b -= k;
+  }
+  if (mi == a.count) return;
+  const NsMat& t = a.mat[mi];
+  const int cur = step & 1;
+  int ti, tj;
+  if (MODE == NS_MODE_X) {
+    ti = b / (t.np / T);
+    tj = b % (t.np / T);
+  } else {                     // lower triangle
+    ti = 0;
+    int x = b;
+    while (x > ti) x -= ++ti;
+    tj = x;
+  }
+  const uint16_t *P, *Q;
+  int64_t pp, pq;
+  int K;
+  if (MODE == NS_MODE_A) { P = Q = t.x[cur]; pp = pq = (int64_t)t.mp * t.np; K = t.np; }
+  else if (MODE == NS_MODE_B) { P = Q = t.A; pp = pq = (int64_t)t.mp * t.mp; K = t.mp; }
+  else { P = t.B; pp = (int64_t)t.mp * t.mp; Q = t.xt[cur]; pq = (int64_t)t.np * t.mp; K = t.mp; }
+  P += (int64_t)ti * T * K;
+  Q += (int64_t)tj * T * K;
+  const int lane = rx_lane(), l31 = lane & 31, h = lane >> 5, wave = threadIdx.x >> 6;
+  const int wi = wave >> 1, wj = wave & 1;
+  uint4 pre[CH];
+  ns_acc acc[NB][NB] = {};
+  ns_fetch<T>(pre, P, pp, Q, pq, K, 0);
+  for (int k0 = 0; k0 < K; k0 += NS_BK) {
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < CH; ++q) {
+      const int x = q * RX_BLOCK + threadIdx.x;
+      const int ch = x % (NS_BK / 8), row = x / (NS_BK / 8) % T, pl = x / (NS_BK / 8) / T % 3, op = x / (NS_BK / 8) / T / 3;
+      *reinterpret_cast<uint4*>(&lds[op][pl][row][ch * 8]) = pre[q];
+    }
+    __syncthreads();
+    if (k0 + NS_BK < K) ns_fetch<T>(pre, P, pp, Q, pq, K, k0 + NS_BK);
+#pragma unroll
+    for (int ks = 0; ks < NS_BK; ks += 16) {
+      ns_h8 fa[NB][3], fb[NB][3];
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+          fa[i][p] = *reinterpret_cast<const ns_h8*>(&lds[0][p][(wi * NB + i) * 32 + l31][ks + h * 8]);
+          fb[i][p] = *reinterpret_cast<const ns_h8*>(&lds[1][p][(wj * NB + i) * 32 + l31][ks + h * 8]);
+        }
+      constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+      for (int u = 0; u < 6; ++u)
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i][PA[u]], fb[j][PB[u]], acc[i][j], 0, 0, 0);
+    }
+  }
+  // lane: column tj * T + .. + l31, rows 8 q + 4 h + k
+  const bool last = MODE == NS_MODE_X && step + 1 == a.steps;
+  const bool flip = t.rows > t.cols;
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = ti * T + (wi * NB + i) * 32 + 8 * q + 4 * h, c = tj * T + (wj * NB + j) * 32 + l31;
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[k] = acc[i][j][4 * q + k];
+          if (MODE == NS_MODE_B) v[k] = fmaf(a.b, ns_join(t.A, (int64_t)t.mp * t.mp, (int64_t)(r + k) * t.mp + c), a.c * v[k]);
+          if (MODE == NS_MODE_X) v[k] = fmaf(a.a, ns_join(t.x[cur], (int64_t)t.mp * t.np, (int64_t)(r + k) * t.np + c), v[k]);
+        }
+        if (last) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (r + k < t.m && c < t.n) t.out[flip ? (int64_t)c * t.cols + r + k : (int64_t)(r + k) * t.cols + c] = v[k];
+          continue;
+        }
+        uint32_t w0[3], w1[3];
+        ns_cut2(v[0], v[1], w0);
+        ns_cut2(v[2], v[3], w1);
+        uint16_t* row_major = MODE == NS_MODE_A ? t.A : MODE == NS_MODE_B ? t.B : t.x[cur ^ 1];
+        uint16_t* mirror = MODE == NS_MODE_A ? t.A : MODE == NS_MODE_B ? t.B : t.xt[cur ^ 1];
+        const int64_t ldr = MODE == NS_MODE_X ? t.np : t.mp, plane = (int64_t)t.mp * ldr;
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+          *reinterpret_cast<uint2*>(mirror + p * plane + (int64_t)c * t.mp + r) = make_uint2(w0[p], w1[p]);
+          if (MODE == NS_MODE_X || ti != tj) {           // a diagonal tile is its own mirror image
+            uint16_t* d = row_major + p * plane + (int64_t)r * ldr + c;
+            d[0] = (uint16_t)w0[p];
+            d[ldr] = (uint16_t)(w0[p] >> 16);
+            d[2 * ldr] = (uint16_t)w1[p];
+            d[3 * ldr] = (uint16_t)(w1[p] >> 16);
+          }
+        }
+      }
+}
+
+// ---------------------------------------------------------------- host
+static int ns_check(const rx_ortho_args* a) {
+  RX_REQUIRE(a, "rx_orthogonalize: null argument");
+  RX_REQUIRE(a->count >= 0 && a->count <= RX_ORTHO_MAX, "rx_orthogonalize: %d matrices (at most %d)", a->count, RX_ORTHO_MAX);
+  RX_REQUIRE(a->steps >= 1 && a->steps <= 32, "rx_orthogonalize: steps=%d (1..32)", a->steps);
+  for (int i = 0; i < a->count; ++i) {
+    RX_REQUIRE(a->rows[i] >= 1 && a->cols[i] >= 1 && a->rows[i] <= NS_MAXDIM && a->cols[i] <= NS_MAXDIM,
+               "rx_orthogonalize: matrix %d is %d x %d (1..%d)", i, a->rows[i], a->cols[i], NS_MAXDIM);
+  }
+  return 0;
+}
+
+// Tile: 128 once the largest product of the list fills the chip with such tiles, 64 for the parallelism otherwise.
+static void ns_plan(const rx_ortho_args* a, NsList* l, size_t* bytes, uint8_t* ws) {
+  memset(l, 0, sizeof(*l));
+  int order[RX_ORTHO_MAX], k = 0;
+  for (int i = 0; i < a->count; ++i)
+    if (!ns_is_small(a->rows[i], a->cols[i])) {
+      int at = k++;
+      auto cost = [&](int x) { return a->rows[x] < a->cols[x] ? a->rows[x] : a->cols[x]; };
+      while (at > 0 && cost(order[at - 1]) < cost(i)) { order[at] = order[at - 1]; --at; }   // longest contractions first
+      order[at] = i;
+    }
+  int64_t big = 0;
+  for (int i = 0; i < k; ++i) big += rx_cdiv(a->rows[order[i]], 128) * rx_cdiv(a->cols[order[i]], 128);
+  l->tile = big >= 256 ? 128 : 64;
+  l->count = k;
+  l->steps = a->steps;
+  l->a = a->a; l->b = a->b; l->c = a->c; l->eps = a->eps;
+  size_t at = 0;
+  auto take = [&](size_t n) { uint8_t* p = ws ? ws + at : nullptr; at += rx_align_up(n, 256); return p; };
+  l->parts = (double*)take(sizeof(double) * NS_PARTS * (size_t)k);
+  for (int i = 0; i < k; ++i) {
+    NsMat& t = l->mat[i];
+    t.g = a->g[order[i]]; t.out = a->out[order[i]];
+    t.rows = a->rows[order[i]]; t.cols = a->cols[order[i]];
+    t.m = t.rows < t.cols ? t.rows : t.cols;
+    t.n = t.rows < t.cols ? t.cols : t.rows;
+    t.mp = ns_up(t.m, l->tile); t.np = ns_up(t.n, l->tile);
+    const int tm = t.mp / l->tile;
+    t.tiles_sym = tm * (tm + 1) / 2;
+    t.tiles_x = tm * (t.np / l->tile);
+    const size_t mn = (size_t)t.mp * t.np * 6, mm = (size_t)t.mp * t.mp * 6;
+    for (int q = 0; q < 2; ++q) { t.x[q] = (uint16_t*)take(mn); t.xt[q] = (uint16_t*)take(mn); }
+    t.A = (uint16_t*)take(mm);
+    t.B = (uint16_t*)take(mm);
+  }
+  *bytes = k ? at : 0;
+}
+
+extern "C" size_t rx_orthogonalize_workspace_bytes(const rx_ortho_args* args) {
+  if (ns_check(args)) return 0;
+  NsList l;
+  size_t bytes;
+  ns_plan(args, &l, &bytes, nullptr);
+  return bytes;
+}
+
+template <int T>
+static void ns_run(const NsList& l, hipStream_t st) {
+  unsigned sym = 0, full = 0;
+  for (int i = 0; i < l.count; ++i) { sym += l.mat[i].tiles_sym; full += l.mat[i].tiles_x; }
+  for (int s = 0; s < l.steps; ++s) {
+    hipLaunchKernelGGL((ns_gemm_kernel<T, NS_MODE_A>), dim3(sym), dim3(RX_BLOCK), 0, st, l, s);
+    hipLaunchKernelGGL((ns_gemm_kernel<T, NS_MODE_B>), dim3(sym), dim3(RX_BLOCK), 0, st, l, s);
+    hipLaunchKernelGGL((ns_gemm_kernel<T, NS_MODE_X>), dim3(full), dim3(RX_BLOCK), 0, st, l, s);
+  }
+}
+
+extern "C" int rx_orthogonalize(const rx_ortho_args* args, void* ws, size_t ws_bytes, int device, void* stream) {
+  if (ns_check(args)) return 1;
+  const rx_ortho_args a = *args;
+  if (a.count == 0) return 0;
+  for (int i = 0; i < a.count; ++i) {
+    RX_REQUIRE(a.g[i] && a.out[i] && (((uintptr_t)a.g[i] | (uintptr_t)a.out[i]) & 3) == 0, "rx_orthogonalize: matrix %d: null or unaligned pointer", i);
+    for (int j = 0; j < a.count; ++j) {
+      const uintptr_t o = (uintptr_t)a.out[i], oe = o + (size_t)a.rows[i] * a.cols[i] * 4;
+      const uintptr_t g = (uintptr_t)a.g[j], ge = g + (size_t)a.rows[j] * a.cols[j] * 4;
+      RX_REQUIRE(oe <= g || ge <= o, "rx_orthogonalize: output %d overlaps input %d", i, j);
+      const uintptr_t p = (uintptr_t)a.out[j], pe = p + (size_t)a.rows[j] * a.cols[j] * 4;
+      RX_REQUIRE(i == j || oe <= p || pe <= o, "rx_orthogonalize: outputs %d and %d overlap", i, j);
+    }
+  }
+  NsList l;
+  size_t need;
+  ns_plan(&a, &l, &need, (uint8_t*)ws);
+  RX_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 255) == 0), "rx_orthogonalize: workspace of %zu bytes, %zu needed",
+             ws_bytes, need);
+  RX_GUARD_DEVICE(device);
+  hipStream_t st = (hipStream_t)stream;
+  NsSmall s;
+  memset(&s, 0, sizeof(s));
+  s.steps = a.steps; s.a = a.a; s.b = a.b; s.c = a.c; s.eps = a.eps;
+  int k = 0;
+  size_t lds = 0;
+  for (int i = 0; i < a.count; ++i)
+    if (ns_is_small(a.rows[i], a.cols[i])) {
+      s.g[k] = a.g[i]; s.out[k] = a.out[i]; s.rows[k] = a.rows[i]; s.cols[k] = a.cols[i];
+      const size_t b = ns_small_lds(a.rows[i], a.cols[i]);
+      if (b > lds) lds = b;
+      ++k;
+    }
+  if (k) {
+    if (lds > 64 * 1024) RX_HIP(hipFuncSetAttribute((const void*)ns_small_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    hipLaunchKernelGGL(ns_small_kernel, dim3(k), dim3(NS_SMALL_THREADS), lds, st, s);
+    RX_LAUNCH_CHECK();
+  }
+  if (l.count == 0) return 0;
+  unsigned blocks = 0;
+  for (int i = 0; i < l.count; ++i) blocks += (l.mat[i].mp / 64) * (l.mat[i].np / 64);
+  hipLaunchKernelGGL(ns_norm_kernel, dim3(l.count * NS_PARTS), dim3(RX_BLOCK), 0, st, l);
+  hipLaunchKernelGGL(ns_init_kernel, dim3(blocks), dim3(RX_BLOCK), 0, st, l);
+  if (l.tile == 128) ns_run<128>(l, st);
+  else ns_run<64>(l, st);
+  RX_LAUNCH_CHECK();
+  return 0;
+}

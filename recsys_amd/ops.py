@@ -13,7 +13,7 @@ from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from ._lib import FMArgs, GatherSeg, LogProbArgs, MFArgs, check, lib
+from ._lib import CatalogArgs, FMArgs, GatherSeg, LogProbArgs, MFArgs, OrthoArgs, check, lib
 
 Tensor = torch.Tensor
 
@@ -1481,6 +1481,126 @@ def logprob_bwd(logits: Tensor, targets: Tensor, lengths: Optional[Tensor], stat
     check(lib.rx_logprob_bwd(C.byref(a), _p(g_logprob), _p(g_entropy), _p(g_lse), _p(dl), V, _dev(logits), _stream(logits)),
           "rx_logprob_bwd")
     return dl
+
+
+# ------------------------------------------------------------------ softmax over a whole catalogue
+CATALOG_MAX_DIM = 256
+
+
+def _catalog_args(x: Tensor, table: Tensor, targets: Tensor, bias: Optional[Tensor]) -> CatalogArgs:
+    _, ld_x = _score_rows(x, "x")
+    _, ld_t = _score_rows(table, "table")
+    if x.dtype != table.dtype:
+        raise TypeError(f"x is {x.dtype}, the table {table.dtype}")
+    (R, D), V = x.shape, table.shape[0]
+    if table.shape[1] != D:
+        raise ValueError(f"x has {D} columns, the table {table.shape[1]}")
+    if not 1 <= D <= CATALOG_MAX_DIM:
+        raise ValueError(f"embedding width {D}: expected 1..{CATALOG_MAX_DIM}")
+    if V < 1:
+        raise ValueError("table: no rows")
+    _idx(targets, "targets")
+    if tuple(targets.shape) != (R,):
+        raise ValueError(f"targets: expected shape [{R}], got {tuple(targets.shape)}")
+    if bias is not None:
+        _req(bias, torch.float32, "bias", 1)
+        if bias.shape[0] != V:
+            raise ValueError(f"bias: expected {V} elements, got {bias.shape[0]}")
+    _same_device(x, table, targets, bias)
+    return CatalogArgs(x.data_ptr(), table.data_ptr(), ld_x, ld_t, 0 if bias is None else bias.data_ptr(), targets.data_ptr(), R, V, D,
+                       int(x.dtype == torch.bfloat16))
+
+
+def catalog_fwd(x: Tensor, table: Tensor, targets: Tensor, bias: Optional[Tensor] = None, want_stats: bool = False,
+                want_mean: bool = False):
+    """Log-probability of one item per row (-1 = none) under the softmax of ``x @ table.T + bias`` over all rows of the
+    table, and the rows' log-sum-exp; the scores are never stored (rx_catalog_fwd).  Returns (logprob, lse, stats or None,
+    mean or None): stats and mean are what :func:`catalog_bwd` needs, the mean only for the gradient of ``x``."""
+    a = _catalog_args(x, table, targets, bias)
+    dev = x.device
+    f = lambda *shape: torch.empty(*shape, dtype=torch.float32, device=dev)
+    logprob, lse = f(a.R), f(a.R)
+    stats = f(a.R, 2) if want_stats else None
+    mean = f(a.R, a.D) if want_mean else None
+    ws = _ws(int(lib.rx_catalog_fwd_workspace_bytes(a.R, a.V, a.D, a.bf16, int(want_mean))), dev)
+    check(lib.rx_catalog_fwd(C.byref(a), _p(logprob), _p(lse), _p(stats), _p(mean), _p(ws), ws.numel(), _p(_err_flag(dev)), _dev(x),
+                             _stream(x)), "rx_catalog_fwd")
+    _after_index_op(dev)
+    return logprob, lse, stats, mean
+
+
+def catalog_bwd(x: Tensor, table: Tensor, targets: Tensor, bias: Optional[Tensor], stats: Tensor, mean: Optional[Tensor],
+                g_logprob: Optional[Tensor] = None, g_lse: Optional[Tensor] = None, want_x: bool = True, want_table: bool = True):
+    """(dx or None, dtable or None, dbias or None) from the gradients of logprob and lse (fp32 [R]; None = zero) and the
+    forward call's stats and mean (rx_catalog_bwd).  With a bias its gradient comes with the table's."""
+    a = _catalog_args(x, table, targets, bias)
+    _req(stats, torch.float32, "stats", 2)
+    if tuple(stats.shape) != (a.R, 2):
+        raise ValueError(f"stats: expected shape [{a.R}, 2], got {tuple(stats.shape)}")
+    if want_x:
+        if mean is None:
+            raise ValueError("the gradient of x needs the means of the forward call")
+        _req(mean, torch.float32, "mean", 2)
+        if tuple(mean.shape) != (a.R, a.D):
+            raise ValueError(f"mean: expected shape [{a.R}, {a.D}], got {tuple(mean.shape)}")
+    for t, name in ((g_logprob, "g_logprob"), (g_lse, "g_lse")):
+        if t is not None:
+            _req(t, torch.float32, name)
+            if t.numel() != a.R:
+                raise ValueError(f"{name}: expected {a.R} elements, got {t.numel()}")
+    _same_device(x, stats, mean, g_logprob, g_lse)
+    dev = x.device
+    if a.R == 0:
+        return (torch.zeros(0, a.D, dtype=x.dtype, device=dev) if want_x else None,
+                torch.zeros(a.V, a.D, dtype=x.dtype, device=dev) if want_table else None,
+                torch.zeros(a.V, dtype=torch.float32, device=dev) if want_table and bias is not None else None)
+    dx = torch.empty(a.R, a.D, dtype=x.dtype, device=dev) if want_x else None
+    dt = torch.empty(a.V, a.D, dtype=x.dtype, device=dev) if want_table else None
+    db = torch.empty(a.V, dtype=torch.float32, device=dev) if want_table and bias is not None else None
+    ws = _ws(int(lib.rx_catalog_bwd_workspace_bytes(a.R, a.V, a.D, a.bf16, int(db is not None))), dev) if want_table else None
+    check(lib.rx_catalog_bwd(C.byref(a), _p(stats), _p(mean), _p(g_logprob), _p(g_lse), _p(dx), _p(dt), _p(db), _p(ws),
+                             0 if ws is None else ws.numel(), _dev(x), _stream(x)), "rx_catalog_bwd")
+    return dx, dt, db
+
+
+# ------------------------------------------------------------------ orthogonalised updates
+ORTHO_COEFFS = (3.4445, -4.7750, 2.0315)     # a, b, c of X <- a X + (b A + c A A) X, A = X X^T
+
+
+def orthogonalize(mats: Sequence[Tensor], steps: int = 5, coeffs=ORTHO_COEFFS, eps: float = 1e-7,
+                  out: Optional[Sequence[Tensor]] = None) -> List[Tensor]:
+    """Newton-Schulz orthogonalisation of fp32 matrices (rx_orthogonalize): ``X = G / (|G|_F + eps)``, then ``steps`` times
+    ``X <- a X + (b A + c A A) X`` with ``A = X X^T``, which drives the singular values towards 1.  Lists of any length,
+    all matrices of a chunk of 24 in the same launches; ``out``: where the results go (must not overlap the inputs)."""
+    mats = list(mats)
+    if out is None:
+        out = [torch.empty_like(m, memory_format=torch.contiguous_format) for m in mats]
+    out = list(out)
+    if len(out) != len(mats):
+        raise ValueError("orthogonalize: as many outputs as matrices")
+    if not 1 <= steps <= 32:
+        raise ValueError(f"orthogonalize: steps={steps} (1..32)")
+    if len(coeffs) != 3:
+        raise ValueError("orthogonalize: three coefficients")
+    for i, (m, o) in enumerate(zip(mats, out)):
+        _req(m, torch.float32, f"matrix {i}", 2)
+        _req(o, torch.float32, f"out {i}", 2)
+        if m.shape != o.shape:
+            raise ValueError(f"orthogonalize: out {i} has shape {tuple(o.shape)}, the matrix {tuple(m.shape)}")
+        if m.numel() == 0:
+            raise ValueError(f"orthogonalize: matrix {i} is empty")
+        _same_device(mats[0], m, o)
+    for i in range(0, len(mats), _lib.RX_ORTHO_MAX):
+        a = OrthoArgs()
+        part = list(zip(mats, out))[i:i + _lib.RX_ORTHO_MAX]
+        for k, (m, o) in enumerate(part):
+            a.g[k], a.out[k], a.rows[k], a.cols[k] = m.data_ptr(), o.data_ptr(), m.shape[0], m.shape[1]
+        a.count, a.steps, a.eps = len(part), steps, eps
+        a.a, a.b, a.c = coeffs
+        need = int(lib.rx_orthogonalize_workspace_bytes(C.byref(a)))
+        ws = _ws(need, mats[0].device) if need else None
+        check(lib.rx_orthogonalize(C.byref(a), _p(ws), need, _dev(mats[0]), _stream(mats[0])), "rx_orthogonalize")
+    return out
 
 
 # ------------------------------------------------------------------ batching
