@@ -859,6 +859,25 @@ typedef struct {
 } rx_ortho_args;
 size_t rx_orthogonalize_workspace_bytes(const rx_ortho_args* args);
 int rx_orthogonalize(const rx_ortho_args* args, void* ws, size_t ws_bytes, int device, void* stream);
+/* The whole step of a list of weight matrices in the same launches, with `scale` a device factor on the gradients (the
+ * clip factor; NULL: 1):  mom <- momentum mom + scale g;  u = scale g + momentum mom (nesterov) or mom;
+ * w <- w - lr NewtonSchulz(u).  No two buffers may overlap. */
+typedef struct {
+  const float* g[RX_ORTHO_MAX];
+  float* w[RX_ORTHO_MAX];
+  float* mom[RX_ORTHO_MAX];
+  float lr[RX_ORTHO_MAX];
+  int32_t rows[RX_ORTHO_MAX];
+  int32_t cols[RX_ORTHO_MAX];
+  int32_t count;
+  int32_t steps;
+  int32_t nesterov;
+  float momentum;
+  float a, b, c, eps;
+  const float* scale;
+} rx_muon_args;
+size_t rx_muon_step_workspace_bytes(const rx_muon_args* args);
+int rx_muon_step(const rx_muon_args* args, void* ws, size_t ws_bytes, int device, void* stream);
 
 /* ------------------------------------------------------------------ dense layers, bf16 activations in HBM
  * The Linear(+ReLU) stacks and DCN-v2 cross layers of recsys_amd.models.fields (a14; the towers of

@@ -115,6 +115,12 @@ class OrthoArgs(C.Structure):
                 ("count", i32), ("steps", i32), ("a", f32), ("b", f32), ("c", f32), ("eps", f32)]
 
 
+class MuonArgs(C.Structure):
+    _fields_ = [("g", vp * RX_ORTHO_MAX), ("w", vp * RX_ORTHO_MAX), ("mom", vp * RX_ORTHO_MAX), ("lr", f32 * RX_ORTHO_MAX),
+                ("rows", i32 * RX_ORTHO_MAX), ("cols", i32 * RX_ORTHO_MAX), ("count", i32), ("steps", i32), ("nesterov", i32),
+                ("momentum", f32), ("a", f32), ("b", f32), ("c", f32), ("eps", f32), ("scale", vp)]
+
+
 # name -> (restype, argtypes); must list every symbol of include/recsys_hip.h
 PROTOTYPES = {
     "rx_abi_version": (C.c_int, []),
@@ -226,6 +232,8 @@ PROTOTYPES = {
     "rx_catalog_bwd": (C.c_int, [C.POINTER(CatalogArgs), vp, vp, vp, vp, vp, vp, vp, vp, sz, C.c_int, vp]),
     "rx_orthogonalize_workspace_bytes": (sz, [C.POINTER(OrthoArgs)]),
     "rx_orthogonalize": (C.c_int, [C.POINTER(OrthoArgs), vp, sz, C.c_int, vp]),
+    "rx_muon_step_workspace_bytes": (sz, [C.POINTER(MuonArgs)]),
+    "rx_muon_step": (C.c_int, [C.POINTER(MuonArgs), vp, sz, C.c_int, vp]),
     "rx_topk_codes": (C.c_int, [vp, vp, i64, i32, i32, vp, C.c_int, vp]),
 }
 

@@ -1063,6 +1063,34 @@ def log_probs(logits: Tensor, targets: Tensor, lengths: Optional[Tensor] = None,
     return ops.LogProbs(*LogProb.apply(logits, targets.contiguous(), None if lengths is None else lengths.contiguous(), k))
 
 
+class MeanNLL(Function):
+    """-mean(logprob) as an fp64 scalar (rx_reduce_sum: no library reduction in a recorded step)."""
+
+    @staticmethod
+    def forward(ctx, logprob):
+        ctx.shape = logprob.shape
+        return ops.reduce_sum(logprob.contiguous())[0].double() * (-1.0 / logprob.numel())
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        n = 1
+        for d in ctx.shape:
+            n *= d
+        return (g * (-1.0 / n)).to(torch.float32).expand(ctx.shape)
+
+
+def mean_nll(logprob: Tensor) -> Tensor:
+    if logprob.numel() == 0:
+        raise ValueError("mean_nll: no log-probabilities")
+    return MeanNLL.apply(logprob)
+
+
+def gather_rows(table: Tensor, idx: Tensor) -> Tensor:
+    """table[idx] for idx [B] through rx_gather_concat, with the deterministic table backward."""
+    return GatherConcat.apply([(0, idx, 0, 1, 1, 0, 0)], idx.shape[0], table.shape[1], table)
+
+
 # ------------------------------------------------------------------ softmax over a whole catalogue
 _ALL_ROWS: dict = {}
 

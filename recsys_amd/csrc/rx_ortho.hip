@@ -29,10 +29,19 @@ typedef float ns_acc __attribute__((ext_vector_type(16)));
 struct NsSmall {
   const float* g[RX_ORTHO_MAX];
   float* out[RX_ORTHO_MAX];
+  float *mom[RX_ORTHO_MAX], *w[RX_ORTHO_MAX];
+  float alpha[RX_ORTHO_MAX];
   int32_t rows[RX_ORTHO_MAX], cols[RX_ORTHO_MAX];
-  int32_t steps;
-  float a, b, c, eps;
+  int32_t steps, nesterov;
+  float a, b, c, eps, mu;
+  const float* scale;
 };
+// What is orthogonalised of a gradient value: the value itself, or with momentum (m: in the new, out the stored one)
+// u = s g + mu m, m = mu m + s g.
+__device__ __forceinline__ float ns_update(float g, float* m, float mu, int nesterov) {
+  *m = fmaf(mu, *m, g);
+  return nesterov ? fmaf(mu, *m, g) : *m;
+}
 static inline int ns_up(int x, int a) { return (x + a - 1) / a * a; }
 static size_t ns_small_lds(int rows, int cols) {
   const int m = ns_up(rows < cols ? rows : cols, 16), n = ns_up(rows < cols ? cols : rows, 16);
@@ -85,9 +94,16 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS) ns_small_kernel(NsSmall a) {
   for (int i = threadIdx.x; i < mp * ldx; i += blockDim.x) X[i] = 0.f;
   __syncthreads();
   double ss = 0.0;
+  float* mom = a.mom[blockIdx.x];
+  const float sc = a.scale ? *a.scale : 1.f;
   for (int i = threadIdx.x; i < rows * cols; i += blockDim.x) {
     const int r = i / cols, c = i - r * cols;
-    const float v = g[i];
+    float v = g[i];
+    if (mom) {
+      float m = mom[i];
+      v = ns_update(v * sc, &m, a.mu, a.nesterov);
+      mom[i] = m;
+    }
     ss = fma((double)v, (double)v, ss);
     X[flip ? c * ldx + r : r * ldx + c] = v;
   }
@@ -133,27 +149,32 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS) ns_small_kernel(NsSmall a) {
     }
     __syncthreads();
   }
+  float* w = a.w[blockIdx.x];
+  const float alpha = a.alpha[blockIdx.x];
   for (int i = threadIdx.x; i < rows * cols; i += blockDim.x) {
     const int r = i / cols, c = i - r * cols;
-    out[i] = X[flip ? c * ldx + r : r * ldx + c];
+    const float v = X[flip ? c * ldx + r : r * ldx + c];
+    if (w) w[i] = fmaf(-alpha, v, w[i]);
+    else out[i] = v;
   }
 }
 
 // ---------------------------------------------------------------- large matrices: planes
 struct NsMat {
   const float* g;
-  float* out;
+  float *out, *mom, *w;
   int32_t rows, cols;          // as given
   int32_t m, n, mp, np;        // working shape, and padded to the tile
   uint16_t *x[2], *xt[2];      // [3][mp][np], [3][np][mp], alternating by step
   uint16_t *A, *B;             // [3][mp][mp]
   int32_t tiles_sym, tiles_x;
-  int32_t pad_;
+  float alpha;
 };
 struct NsList {
   NsMat mat[RX_ORTHO_MAX];
-  int32_t count, steps, tile, pad_;
-  float a, b, c, eps;
+  int32_t count, steps, tile, nesterov;
+  float a, b, c, eps, mu;
+  const float* scale;
   double* parts;               // [count][NS_PARTS]
 };
 
@@ -179,9 +200,16 @@ __global__ void __launch_bounds__(RX_BLOCK) ns_norm_kernel(NsList a) {
   const int mi = blockIdx.x / NS_PARTS, pt = blockIdx.x % NS_PARTS;
   const NsMat& t = a.mat[mi];
   const int64_t n = (int64_t)t.rows * t.cols;
+  const float sc = a.scale ? *a.scale : 1.f;
   double s = 0.0;
   for (int64_t i = (int64_t)pt * RX_BLOCK + threadIdx.x; i < n; i += (int64_t)NS_PARTS * RX_BLOCK) {
-    const double v = t.g[i];
+    float u = t.g[i];
+    if (t.mom) {
+      float m = t.mom[i];
+      u = ns_update(u * sc, &m, a.mu, a.nesterov);
+      t.mom[i] = m;
+    }
+    const double v = u;
     s = fma(v, v, s);
   }
   __shared__ double w[RX_BLOCK / 64];
@@ -205,12 +233,19 @@ __global__ void __launch_bounds__(RX_BLOCK) ns_init_kernel(NsList a) {
   double ss = 0.0;
   for (int i = 0; i < NS_PARTS; ++i) ss += a.parts[mi * NS_PARTS + i];
   const float div = (float)(sqrt(ss) + (double)a.eps);
+  const float sc = a.scale ? *a.scale : 1.f;
   const int r0 = b / (t.np / 64) * 64, c0 = b % (t.np / 64) * 64;      // of X
   const bool flip = t.rows > t.cols;
   for (int i = threadIdx.x; i < 64 * 64; i += RX_BLOCK) {
     const int y = i / 64, x = i % 64;
     const int r = flip ? c0 + y : r0 + y, c = flip ? r0 + x : c0 + x;  // of G: rows of it are read along
-    const float v = r < t.rows && c < t.cols ? t.g[(int64_t)r * t.cols + c] / div : 0.f;
+    float v = 0.f;
+    if (r < t.rows && c < t.cols) {
+      const int64_t at = (int64_t)r * t.cols + c;
+      v = t.g[at];
+      if (t.mom) v = a.nesterov ? fmaf(a.mu, t.mom[at], v * sc) : t.mom[at];     // the norm's pass stored the new momentum
+      v /= div;
+    }
     if (flip) tl[x][y] = v;
     else tl[y][x] = v;
   }
@@ -337,7 +372,11 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
         if (last) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (r + k < t.m && c < t.n) t.out[flip ? (int64_t)c * t.cols + r + k : (int64_t)(r + k) * t.cols + c] = v[k];
+            if (r + k < t.m && c < t.n) {
+              const int64_t at = flip ? (int64_t)c * t.cols + r + k : (int64_t)(r + k) * t.cols + c;
+              if (t.w) t.w[at] = fmaf(-t.alpha, v[k], t.w[at]);
+              else t.out[at] = v[k];
+            }
           continue;
         }
         uint32_t w0[3], w1[3];
@@ -361,41 +400,53 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
 }
 
 // ---------------------------------------------------------------- host
-static int ns_check(const rx_ortho_args* a) {
-  RX_REQUIRE(a, "rx_orthogonalize: null argument");
-  RX_REQUIRE(a->count >= 0 && a->count <= RX_ORTHO_MAX, "rx_orthogonalize: %d matrices (at most %d)", a->count, RX_ORTHO_MAX);
-  RX_REQUIRE(a->steps >= 1 && a->steps <= 32, "rx_orthogonalize: steps=%d (1..32)", a->steps);
-  for (int i = 0; i < a->count; ++i) {
-    RX_REQUIRE(a->rows[i] >= 1 && a->cols[i] >= 1 && a->rows[i] <= NS_MAXDIM && a->cols[i] <= NS_MAXDIM,
-               "rx_orthogonalize: matrix %d is %d x %d (1..%d)", i, a->rows[i], a->cols[i], NS_MAXDIM);
-  }
+struct NsArgs {                // rx_ortho_args and rx_muon_args in one form
+  const float* g[RX_ORTHO_MAX];
+  float *out[RX_ORTHO_MAX], *mom[RX_ORTHO_MAX], *w[RX_ORTHO_MAX];
+  float alpha[RX_ORTHO_MAX];
+  int32_t rows[RX_ORTHO_MAX], cols[RX_ORTHO_MAX];
+  int32_t count, steps, nesterov;
+  float a, b, c, eps, mu;
+  const float* scale;
+};
+
+static int ns_check(const char* who, const int32_t* rows, const int32_t* cols, int count, int steps) {
+  RX_REQUIRE(count >= 0 && count <= RX_ORTHO_MAX, "%s: %d matrices (at most %d)", who, count, RX_ORTHO_MAX);
+  RX_REQUIRE(steps >= 1 && steps <= 32, "%s: steps=%d (1..32)", who, steps);
+  for (int i = 0; i < count; ++i)
+    RX_REQUIRE(rows[i] >= 1 && cols[i] >= 1 && rows[i] <= NS_MAXDIM && cols[i] <= NS_MAXDIM, "%s: matrix %d is %d x %d (1..%d)", who, i,
+               rows[i], cols[i], NS_MAXDIM);
   return 0;
 }
 
 // Tile: 128 once the largest product of the list fills the chip with such tiles, 64 for the parallelism otherwise.
-static void ns_plan(const rx_ortho_args* a, NsList* l, size_t* bytes, uint8_t* ws) {
+static void ns_plan(const NsArgs& a, NsList* l, size_t* bytes, uint8_t* ws) {
   memset(l, 0, sizeof(*l));
   int order[RX_ORTHO_MAX], k = 0;
-  for (int i = 0; i < a->count; ++i)
-    if (!ns_is_small(a->rows[i], a->cols[i])) {
+  for (int i = 0; i < a.count; ++i)
+    if (!ns_is_small(a.rows[i], a.cols[i])) {
       int at = k++;
-      auto cost = [&](int x) { return a->rows[x] < a->cols[x] ? a->rows[x] : a->cols[x]; };
+      auto cost = [&](int x) { return a.rows[x] < a.cols[x] ? a.rows[x] : a.cols[x]; };
       while (at > 0 && cost(order[at - 1]) < cost(i)) { order[at] = order[at - 1]; --at; }   // longest contractions first
       order[at] = i;
     }
   int64_t big = 0;
-  for (int i = 0; i < k; ++i) big += rx_cdiv(a->rows[order[i]], 128) * rx_cdiv(a->cols[order[i]], 128);
+  for (int i = 0; i < k; ++i) big += rx_cdiv(a.rows[order[i]], 128) * rx_cdiv(a.cols[order[i]], 128);
   l->tile = big >= 256 ? 128 : 64;
   l->count = k;
-  l->steps = a->steps;
-  l->a = a->a; l->b = a->b; l->c = a->c; l->eps = a->eps;
+  l->steps = a.steps;
+  l->nesterov = a.nesterov;
+  l->mu = a.mu;
+  l->scale = a.scale;
+  l->a = a.a; l->b = a.b; l->c = a.c; l->eps = a.eps;
   size_t at = 0;
   auto take = [&](size_t n) { uint8_t* p = ws ? ws + at : nullptr; at += rx_align_up(n, 256); return p; };
   l->parts = (double*)take(sizeof(double) * NS_PARTS * (size_t)k);
   for (int i = 0; i < k; ++i) {
     NsMat& t = l->mat[i];
-    t.g = a->g[order[i]]; t.out = a->out[order[i]];
-    t.rows = a->rows[order[i]]; t.cols = a->cols[order[i]];
+    const int o = order[i];
+    t.g = a.g[o]; t.out = a.out[o]; t.mom = a.mom[o]; t.w = a.w[o]; t.alpha = a.alpha[o];
+    t.rows = a.rows[o]; t.cols = a.cols[o];
     t.m = t.rows < t.cols ? t.rows : t.cols;
     t.n = t.rows < t.cols ? t.cols : t.rows;
     t.mp = ns_up(t.m, l->tile); t.np = ns_up(t.n, l->tile);
@@ -410,14 +461,6 @@ static void ns_plan(const rx_ortho_args* a, NsList* l, size_t* bytes, uint8_t* w
   *bytes = k ? at : 0;
 }
 
-extern "C" size_t rx_orthogonalize_workspace_bytes(const rx_ortho_args* args) {
-  if (ns_check(args)) return 0;
-  NsList l;
-  size_t bytes;
-  ns_plan(args, &l, &bytes, nullptr);
-  return bytes;
-}
-
 template <int T>
 static void ns_run(const NsList& l, hipStream_t st) {
   unsigned sym = 0, full = 0;
@@ -429,35 +472,23 @@ static void ns_run(const NsList& l, hipStream_t st) {
   }
 }
 
-extern "C" int rx_orthogonalize(const rx_ortho_args* args, void* ws, size_t ws_bytes, int device, void* stream) {
-  if (ns_check(args)) return 1;
-  const rx_ortho_args a = *args;
-  if (a.count == 0) return 0;
-  for (int i = 0; i < a.count; ++i) {
-    RX_REQUIRE(a.g[i] && a.out[i] && (((uintptr_t)a.g[i] | (uintptr_t)a.out[i]) & 3) == 0, "rx_orthogonalize: matrix %d: null or unaligned pointer", i);
-    for (int j = 0; j < a.count; ++j) {
-      const uintptr_t o = (uintptr_t)a.out[i], oe = o + (size_t)a.rows[i] * a.cols[i] * 4;
-      const uintptr_t g = (uintptr_t)a.g[j], ge = g + (size_t)a.rows[j] * a.cols[j] * 4;
-      RX_REQUIRE(oe <= g || ge <= o, "rx_orthogonalize: output %d overlaps input %d", i, j);
-      const uintptr_t p = (uintptr_t)a.out[j], pe = p + (size_t)a.rows[j] * a.cols[j] * 4;
-      RX_REQUIRE(i == j || oe <= p || pe <= o, "rx_orthogonalize: outputs %d and %d overlap", i, j);
-    }
-  }
+static int ns_go(const char* who, const NsArgs& a, void* ws, size_t ws_bytes, int device, void* stream) {
   NsList l;
   size_t need;
-  ns_plan(&a, &l, &need, (uint8_t*)ws);
-  RX_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 255) == 0), "rx_orthogonalize: workspace of %zu bytes, %zu needed",
-             ws_bytes, need);
+  ns_plan(a, &l, &need, (uint8_t*)ws);
+  RX_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 255) == 0), "%s: workspace of %zu bytes, %zu needed", who, ws_bytes, need);
   RX_GUARD_DEVICE(device);
   hipStream_t st = (hipStream_t)stream;
   NsSmall s;
   memset(&s, 0, sizeof(s));
-  s.steps = a.steps; s.a = a.a; s.b = a.b; s.c = a.c; s.eps = a.eps;
+  s.steps = a.steps; s.nesterov = a.nesterov; s.mu = a.mu; s.scale = a.scale;
+  s.a = a.a; s.b = a.b; s.c = a.c; s.eps = a.eps;
   int k = 0;
   size_t lds = 0;
   for (int i = 0; i < a.count; ++i)
     if (ns_is_small(a.rows[i], a.cols[i])) {
-      s.g[k] = a.g[i]; s.out[k] = a.out[i]; s.rows[k] = a.rows[i]; s.cols[k] = a.cols[i];
+      s.g[k] = a.g[i]; s.out[k] = a.out[i]; s.mom[k] = a.mom[i]; s.w[k] = a.w[i]; s.alpha[k] = a.alpha[i];
+      s.rows[k] = a.rows[i]; s.cols[k] = a.cols[i];
       const size_t b = ns_small_lds(a.rows[i], a.cols[i]);
       if (b > lds) lds = b;
       ++k;
@@ -476,4 +507,80 @@ extern "C" int rx_orthogonalize(const rx_ortho_args* args, void* ws, size_t ws_b
   else ns_run<64>(l, st);
   RX_LAUNCH_CHECK();
   return 0;
+}
+
+static size_t ns_bytes(const int32_t* rows, const int32_t* cols, int count, int steps) {
+  NsArgs a;
+  memset(&a, 0, sizeof(a));
+  a.count = count; a.steps = steps;
+  memcpy(a.rows, rows, sizeof(a.rows));
+  memcpy(a.cols, cols, sizeof(a.cols));
+  NsList l;
+  size_t bytes;
+  ns_plan(a, &l, &bytes, nullptr);
+  return bytes;
+}
+
+// two ranges of n and m floats share memory
+static bool ns_overlap(const float* p, size_t n, const float* q, size_t m) {
+  return (uintptr_t)p < (uintptr_t)(q + m) && (uintptr_t)q < (uintptr_t)(p + n);
+}
+
+extern "C" size_t rx_orthogonalize_workspace_bytes(const rx_ortho_args* a) {
+  if (!a || ns_check("rx_orthogonalize", a->rows, a->cols, a->count, a->steps)) return 0;
+  return ns_bytes(a->rows, a->cols, a->count, a->steps);
+}
+
+extern "C" int rx_orthogonalize(const rx_ortho_args* args, void* ws, size_t ws_bytes, int device, void* stream) {
+  RX_REQUIRE(args, "rx_orthogonalize: null argument");
+  if (ns_check("rx_orthogonalize", args->rows, args->cols, args->count, args->steps)) return 1;
+  NsArgs a;
+  memset(&a, 0, sizeof(a));
+  for (int i = 0; i < args->count; ++i) {
+    const size_t n = (size_t)args->rows[i] * args->cols[i];
+    RX_REQUIRE(args->g[i] && args->out[i] && (((uintptr_t)args->g[i] | (uintptr_t)args->out[i]) & 3) == 0,
+               "rx_orthogonalize: matrix %d: null or unaligned pointer", i);
+    for (int j = 0; j < args->count; ++j) {
+      const size_t m = (size_t)args->rows[j] * args->cols[j];
+      RX_REQUIRE(args->g[j] && !ns_overlap(args->out[i], n, args->g[j], m), "rx_orthogonalize: output %d overlaps input %d", i, j);
+      RX_REQUIRE(i == j || !ns_overlap(args->out[i], n, args->out[j], m), "rx_orthogonalize: outputs %d and %d overlap", i, j);
+    }
+    a.g[i] = args->g[i]; a.out[i] = args->out[i]; a.rows[i] = args->rows[i]; a.cols[i] = args->cols[i];
+  }
+  a.count = args->count; a.steps = args->steps;
+  a.a = args->a; a.b = args->b; a.c = args->c; a.eps = args->eps;
+  if (a.count == 0) return 0;
+  return ns_go("rx_orthogonalize", a, ws, ws_bytes, device, stream);
+}
+
+extern "C" size_t rx_muon_step_workspace_bytes(const rx_muon_args* a) {
+  if (!a || ns_check("rx_muon_step", a->rows, a->cols, a->count, a->steps)) return 0;
+  return ns_bytes(a->rows, a->cols, a->count, a->steps);
+}
+
+extern "C" int rx_muon_step(const rx_muon_args* args, void* ws, size_t ws_bytes, int device, void* stream) {
+  RX_REQUIRE(args, "rx_muon_step: null argument");
+  if (ns_check("rx_muon_step", args->rows, args->cols, args->count, args->steps)) return 1;
+  RX_REQUIRE(((uintptr_t)args->scale & 3) == 0, "rx_muon_step: unaligned scale");
+  NsArgs a;
+  memset(&a, 0, sizeof(a));
+  for (int i = 0; i < args->count; ++i) {
+    const size_t n = (size_t)args->rows[i] * args->cols[i];
+    RX_REQUIRE(args->g[i] && args->w[i] && args->mom[i] && (((uintptr_t)args->g[i] | (uintptr_t)args->w[i] | (uintptr_t)args->mom[i]) & 3) == 0,
+               "rx_muon_step: matrix %d: null or unaligned pointer", i);
+    for (int j = 0; j < args->count; ++j) {
+      const size_t m = (size_t)args->rows[j] * args->cols[j];
+      RX_REQUIRE(args->g[j] && args->mom[j] && !ns_overlap(args->w[i], n, args->g[j], m) && !ns_overlap(args->mom[i], n, args->g[j], m) &&
+                     !ns_overlap(args->w[i], n, args->mom[j], m) &&
+                     (i == j || (!ns_overlap(args->w[i], n, args->w[j], m) && !ns_overlap(args->mom[i], n, args->mom[j], m))),
+                 "rx_muon_step: buffers of matrices %d and %d overlap", i, j);
+    }
+    a.g[i] = args->g[i]; a.w[i] = args->w[i]; a.mom[i] = args->mom[i]; a.alpha[i] = args->lr[i];
+    a.rows[i] = args->rows[i]; a.cols[i] = args->cols[i];
+  }
+  a.count = args->count; a.steps = args->steps; a.nesterov = args->nesterov != 0;
+  a.a = args->a; a.b = args->b; a.c = args->c; a.eps = args->eps; a.mu = args->momentum;
+  a.scale = args->scale;
+  if (a.count == 0) return 0;
+  return ns_go("rx_muon_step", a, ws, ws_bytes, device, stream);
 }

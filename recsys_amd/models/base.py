@@ -20,6 +20,51 @@ class HotPathModule(nn.Module):
     optimizer updates row-wise); everything else in ``parameters()`` is dense."""
 
     _sparse_names: List[str] = []
+    objective = "bce"
+
+    def set_objective(self, name: str) -> "HotPathModule":
+        """What ``loss(inputs)`` -- and with it every train loop and recorded step -- minimises: ``"bce"`` (the reference's),
+        ``"softmax"`` (``softmax_loss``: the positive against its own list) or ``"catalog"`` (``catalog_loss``: the positive
+        against every item; models whose score is a product of a user-side vector with the item's)."""
+        if name not in ("bce", "softmax", "catalog"):
+            raise ValueError(f"unknown objective {name!r}")
+        if name == "catalog" and type(self)._catalog_query is HotPathModule._catalog_query:
+            raise ValueError(f"{type(self).__name__}: the scores are not a product with an item table")
+        self.objective = name
+        return self
+
+    def _objective_loss(self, inputs):
+        return self.softmax_loss(inputs) if self.objective == "softmax" else self.catalog_loss(inputs)
+
+    def softmax_loss(self, inputs):
+        """Mean of -log softmax of the positive over its list of scores (rx_logprob_*).  The positive is column 0, where the
+        loader puts it (recsys/dataset.py:172-181), or column ``inputs["target"]`` [B]; with ``inputs["list_length"]`` [B]
+        only that many columns of a row count.  fp64 like the BCE loss; at least two candidates per row."""
+        logits = self(inputs)
+        if logits.dim() != 2 or logits.shape[0] == 0 or logits.shape[1] < 2:
+            raise ValueError(f"softmax_loss: expected scores [B, N] with B >= 1 and N >= 2, got {tuple(logits.shape)}")
+        target = inputs.get("target")
+        if target is None:
+            target = torch.zeros(logits.shape[0], dtype=torch.int64, device=logits.device)
+        return rxa.mean_nll(rxa.log_probs(logits, target, lengths=inputs.get("list_length")).logprob)
+
+    def _catalog_query(self, inputs):
+        """(x [B, D], item table [V, D], item bias [V] or None): scores over the catalogue are x . table[v] + bias[v], up to
+        a constant per row."""
+        raise NotImplementedError
+
+    def catalog_loss(self, inputs):
+        """Mean of -log softmax of the positive (column 0 of ``item_code``, or ``item_code`` [B]) over the whole item
+        catalogue, without the [B, n_items] scores (rx_catalog_*).  Terms that are the same for every item of a row (user
+        and global bias, the user's temporal term) drop out of it and take no gradient.  Embedding width up to 256."""
+        if type(self)._catalog_query is HotPathModule._catalog_query:
+            raise ValueError(f"{type(self).__name__}: the scores are not a product with an item table")
+        items = as_index(inputs["item_code"], "item_code")
+        if items.shape[0] == 0:
+            raise ValueError("catalog_loss: empty batch")
+        x, table, bias = self._catalog_query(inputs)
+        target = items[:, 0].contiguous() if items.dim() == 2 else items
+        return rxa.mean_nll(rxa.catalog_logprob(x, table, target, bias=bias)[0])
 
     def sparse_parameters(self) -> Iterator[nn.Parameter]:
         named = dict(self.named_parameters())
@@ -45,6 +90,10 @@ class HotPathModule(nn.Module):
         return res
 
     def loss(self, inputs, *args, **kwargs):
+        if self.objective != "bce":
+            if args and args[0] or kwargs.get("pointwise"):
+                raise ValueError(f"objective {self.objective!r} is list-wise")
+            return self._objective_loss(inputs)
         labels = inputs["label"]
         logits = self(inputs, *args, **kwargs)
         return rxa.bce_with_logits(logits, labels)

@@ -119,6 +119,8 @@ class FieldFM(_FieldTable):
     def loss(self, inputs):
         """BCE loss.  With field groups in use the logits, the loss and the per-sample backward
         records come out of one launch (autograd.FMLoss); otherwise the generic two-step path."""
+        if self.objective != "bce":
+            return super().loss(inputs)
         ex, base, item, item_base = self._split(inputs)
         feat = self.feature_embedding.weight
         labels = inputs["label"]

@@ -34,9 +34,11 @@ class VanillaMF(HotPathModule):
     def _index_lists(self, inputs):
         if inputs.get("item_code") is None:
             return []
-        lists = [(as_index(inputs["user_code"], "user_code"), self.n_users),
-                 (as_index(inputs["item_code"], "item_code"), self.n_items)]
+        lists = [(as_index(inputs["user_code"], "user_code"), self.n_users)]
         e = self._extras(inputs)
+        if self.objective == "catalog":      # every item row takes a gradient: nothing to sort on that side
+            return lists + ([(e["occs"], e["O"].shape[0])] if e["occs"] is not None else [])
+        lists.append((as_index(inputs["item_code"], "item_code"), self.n_items))
         if e["occs"] is not None:
             lists.append((e["occs"], e["O"].shape[0]))
         if e["temps"] is not None:
@@ -59,6 +61,8 @@ class VanillaMF(HotPathModule):
     def loss(self, inputs):
         """BCE loss (vanilla_mf.py:35-39).  On the GPU with one label per logit the logits, the loss and
         dL/dlogit come out of one launch (autograd.MFLoss); otherwise the generic two-step path."""
+        if self.objective != "bce":
+            return self._objective_loss(inputs)
         labels, items = inputs["label"], inputs.get("item_code")
         users = inputs["user_code"]
         if (_FUSED_LOSS and items is not None and isinstance(labels, torch.Tensor) and labels.is_cuda and users.is_cuda
@@ -69,6 +73,14 @@ class VanillaMF(HotPathModule):
                                     self.user_embedding.weight, self.item_embedding.weight, e["O"], e["UT"], e["T"],
                                     e["user_bias"], e["item_bias"], e["bias"], None, None, labels)
         return super().loss(inputs)
+
+    def _catalog_query(self, inputs):
+        users = as_index(inputs["user_code"], "user_code")
+        x = rxa.gather_rows(self.user_embedding.weight, users)
+        e = self._extras(inputs)
+        if e["occs"] is not None:
+            x = x + rxa.gather_rows(e["O"], e["occs"])
+        return x, self.item_embedding.weight, e["item_bias"]
 
 
 class BiasMF(VanillaMF):

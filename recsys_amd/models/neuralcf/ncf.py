@@ -58,8 +58,14 @@ class GMF(HotPathModule):
     def _index_lists(self, inputs):
         if inputs.get("item_code") is None:
             return []
-        return [(as_index(inputs["user_code"], "user_code"), self.n_users),
-                (as_index(inputs["item_code"], "item_code"), self.n_items)]
+        lists = [(as_index(inputs["user_code"], "user_code"), self.n_users)]
+        if self.objective != "catalog":      # there every item row takes a gradient: nothing to sort on that side
+            lists.append((as_index(inputs["item_code"], "item_code"), self.n_items))
+        return lists
+
+    def _catalog_query(self, inputs):
+        users = as_index(inputs["user_code"], "user_code")
+        return rxa.gather_rows(self.user_embedding.weight, users) * self.linear.weight, self.item_embedding.weight, None
 
     def forward(self, inputs, pointwise=False):
         users = as_index(inputs["user_code"], "user_code")
@@ -77,6 +83,8 @@ class GMF(HotPathModule):
     def loss(self, inputs, pointwise=False):
         """BCE loss (gmf.py:41-45); list-wise on the GPU the forward launch also forms the loss and dL/dlogit
         (autograd.MFLoss)."""
+        if self.objective != "bce":
+            return super().loss(inputs, pointwise)
         labels, items, users = inputs["label"], inputs.get("item_code"), inputs["user_code"]
         if (not pointwise and os.environ.get("RX_NO_FUSED_MF_LOSS") != "1" and items is not None and isinstance(labels, torch.Tensor)
                 and labels.is_cuda and users.is_cuda and labels.dtype in (torch.float32, torch.float64) and items.dim() == 2
@@ -177,7 +185,7 @@ class NeuMF(HotPathModule):
                 and ops.neumf_step_supported(self.embedding_dim, items.shape[1]))
 
     def loss(self, inputs, pointwise=False):
-        if not pointwise and inputs.get("item_code") is not None and "label" in inputs:
+        if self.objective == "bce" and not pointwise and inputs.get("item_code") is not None and "label" in inputs:
             users = as_index(inputs["user_code"], "user_code")
             items = as_index(inputs["item_code"], "item_code")
             labels = inputs["label"]

@@ -13,7 +13,7 @@ from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from ._lib import CatalogArgs, FMArgs, GatherSeg, LogProbArgs, MFArgs, OrthoArgs, check, lib
+from ._lib import CatalogArgs, FMArgs, GatherSeg, LogProbArgs, MFArgs, MuonArgs, OrthoArgs, check, lib
 
 Tensor = torch.Tensor
 
@@ -1601,6 +1601,43 @@ def orthogonalize(mats: Sequence[Tensor], steps: int = 5, coeffs=ORTHO_COEFFS, e
         ws = _ws(need, mats[0].device) if need else None
         check(lib.rx_orthogonalize(C.byref(a), _p(ws), need, _dev(mats[0]), _stream(mats[0])), "rx_orthogonalize")
     return out
+
+
+def muon_step(ws: Sequence[Tensor], gs: Sequence[Tensor], moms: Sequence[Tensor], lrs: Sequence[float], momentum: float = 0.95,
+              nesterov: bool = True, scale: Optional[Tensor] = None, steps: int = 5, coeffs=ORTHO_COEFFS, eps: float = 1e-7) -> None:
+    """Momentum, Newton-Schulz and the weight update of a list of fp32 matrices (rx_muon_step), in place:
+    ``mom <- momentum mom + s g``, ``w <- w - lr NewtonSchulz(s g + momentum mom)`` (nesterov; of ``mom`` without), with s
+    the device factor ``scale`` (the clip factor) and one learning rate per matrix."""
+    n = len(ws)
+    if not len(gs) == len(moms) == len(lrs) == n:
+        raise ValueError("muon_step: as many gradients, momenta and learning rates as matrices")
+    for i, (w, g, m) in enumerate(zip(ws, gs, moms)):
+        for t, name in ((w, "weight"), (g, "gradient"), (m, "momentum")):
+            _req(t, torch.float32, f"{name} {i}", 2)
+            if t.shape != w.shape:
+                raise ValueError(f"muon_step: {name} {i} has shape {tuple(t.shape)}, the weight {tuple(w.shape)}")
+        if w.numel() == 0:
+            raise ValueError(f"muon_step: matrix {i} is empty")
+        _same_device(ws[0], w, g, m)
+    if scale is not None:
+        _req(scale, torch.float32, "scale")
+        if scale.numel() != 1:
+            raise ValueError("scale: one element")
+        if n:
+            _same_device(ws[0], scale)
+    for i in range(0, n, _lib.RX_ORTHO_MAX):
+        a = MuonArgs()
+        c = min(n - i, _lib.RX_ORTHO_MAX)
+        for k in range(c):
+            w = ws[i + k]
+            a.g[k], a.w[k], a.mom[k], a.lr[k] = gs[i + k].data_ptr(), w.data_ptr(), moms[i + k].data_ptr(), float(lrs[i + k])
+            a.rows[k], a.cols[k] = w.shape
+        a.count, a.steps, a.nesterov, a.momentum, a.eps = c, steps, int(nesterov), momentum, eps
+        a.a, a.b, a.c = coeffs
+        a.scale = 0 if scale is None else scale.data_ptr()
+        need = int(lib.rx_muon_step_workspace_bytes(C.byref(a)))
+        buf = _ws(need, ws[0].device) if need else None
+        check(lib.rx_muon_step(C.byref(a), _p(buf), need, _dev(ws[0]), _stream(ws[0])), "rx_muon_step")
 
 
 # ------------------------------------------------------------------ batching

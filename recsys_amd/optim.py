@@ -159,7 +159,10 @@ class FusedOptimizer:
 
     ``kind`` in {"sgd", "adagrad", "rowwise_adagrad"} applies to the parameters the model lists
     in ``model.sparse_parameters()``; all other parameters are stepped densely with
-    ``dense_kind`` (default: "sgd" for sgd, "adagrad" otherwise; "adam" allowed).
+    ``dense_kind`` (default: "sgd" for sgd, "adagrad" otherwise; "adam" and "muon" allowed).
+    ``dense_kind="muon"``: weight matrices (both sides of two or more) take momentum steps along the orthogonalised
+    update (ops.muon_step: ``momentum``, Nesterov form, learning rate ``lr * sqrt(max(1, rows / cols))``), everything
+    else (biases, normalisation, one-row layers) takes Adam with ``adam_lr`` (default ``lr``).
     ``speculative``: whether clipped SGD over field groups takes its step inside the backward's reduce and redoes
     rows only if the clip bites (default: only for models without dense parameters).
     ``kind="dense_adam"``: no sparse rule at all -- dense table gradients and Adam on every parameter,
@@ -168,16 +171,18 @@ class FusedOptimizer:
 
     def __init__(self, model, kind: str = "sgd", lr: float = 0.01, eps: float = 1e-10,
                  clip_norm: Optional[float] = None, dense_kind: Optional[str] = None,
-                 betas=(0.9, 0.999), adam_eps: float = 1e-8, speculative: Optional[bool] = None):
+                 betas=(0.9, 0.999), adam_eps: float = 1e-8, speculative: Optional[bool] = None,
+                 momentum: float = 0.95, adam_lr: Optional[float] = None):
         if kind not in _MODES and kind != "dense_adam":
             raise ValueError(f"unknown sparse optimizer {kind!r}")
         self.kind, self.lr, self.eps, self.clip_norm = kind, lr, eps, clip_norm
         self.dense_kind = dense_kind or ("sgd" if kind == "sgd" else "adam" if kind == "dense_adam" else "adagrad")
-        if self.dense_kind not in ("sgd", "adagrad", "adam"):
+        if self.dense_kind not in ("sgd", "adagrad", "adam", "muon"):
             raise ValueError(f"unknown dense optimizer {self.dense_kind!r}")
         if kind == "dense_adam" and self.dense_kind != "adam":
             raise ValueError("kind='dense_adam' steps every parameter with Adam")
         self.betas, self.adam_eps = betas, adam_eps
+        self.momentum, self.adam_lr = momentum, adam_lr
         # kind="dense_adam": what the reference's pipelines build -- torch.optim.Adam over ALL parameters behind
         # clip_grad_norm_ (recsys/pipelines/neuralcf/neumf.py:10, recsys/utils.py:101-103).  No parameter carries a
         # sparse rule: the tables' gradients come out of the backward pass as dense [rows, dim] arrays (sort +
@@ -199,7 +204,7 @@ class FusedOptimizer:
         if self.dense_kind == "adagrad":
             for p in self.dense:
                 self._dense_state_for(p)
-        elif self.dense_kind == "adam":
+        elif self.dense_kind in ("adam", "muon"):
             for p in self.dense:
                 self._dense_state_for(p)
         # Clipped SGD taken speculatively inside the reduce (see _rule_apply_fm) pays when the clip is idle and costs a
@@ -222,7 +227,7 @@ class FusedOptimizer:
         # inside a step: a counter created (and filled) while a graph is being recorded would be reset to the
         # recording's value by every replay.
         self._step_dev = None
-        if self.dense_kind == "adam" and self.dense and self.dense[0].is_cuda:
+        if self.dense_kind in ("adam", "muon") and self.dense and self.dense[0].is_cuda:
             self._step_dev = torch.zeros(1, dtype=torch.int32, device=self.dense[0].device)
         self.last_total_norm: Optional[torch.Tensor] = None
 
@@ -399,7 +404,7 @@ class FusedOptimizer:
             if (rule.mode, rule.lr, rule.eps, compact.shape[1]) != (r0.mode, r0.lr, r0.eps, d0):
                 return False
             seen.add(id(param))
-        if self.dense_kind == "adam":
+        if self.dense_kind in ("adam", "muon"):
             return False
         # every block of the fused launch adds up all partial sums before it touches a row: a gain for the small
         # lists of the MF / NCF families (launch-bound tails), a loss once the lists are long -- 0.65 against 0.55 ms
@@ -442,12 +447,17 @@ class FusedOptimizer:
         self._sq_used += need
         return out
 
+    def _is_muon(self, p) -> bool:
+        return self.dense_kind == "muon" and p.dim() == 2 and min(p.shape) >= 2
+
     def _dense_state_for(self, p):
         st = self._dense_state.get(id(p))
         if st is None:
             if self.dense_kind == "adagrad":
                 st = torch.zeros_like(p.data, memory_format=torch.contiguous_format)
-            elif self.dense_kind == "adam":
+            elif self._is_muon(p):
+                st = torch.zeros_like(p.data, memory_format=torch.contiguous_format)
+            elif self.dense_kind in ("adam", "muon"):
                 st = (torch.zeros_like(p.data, memory_format=torch.contiguous_format), torch.zeros_like(p.data, memory_format=torch.contiguous_format))
             else:
                 return None
@@ -462,12 +472,22 @@ class FusedOptimizer:
         w = p.data
         if self.dense_kind == "sgd":
             ops.dense_sgd(w, g, self.lr, scale)
+        elif self._is_muon(p):
+            self._muon_all([(p, g)], scale)
         elif self.dense_kind == "adagrad":
             ops.dense_adagrad(w, g, self._dense_state_for(p), self.lr, self.eps, scale)
         else:
             st = self._dense_state_for(p)
-            ops.dense_adam(w, g, st[0], st[1], self.lr, self.betas[0], self.betas[1], self.adam_eps,
+            ops.dense_adam(w, g, st[0], st[1], self._adam_lr(), self.betas[0], self.betas[1], self.adam_eps,
                            self._step_dev if self._step_dev is not None else self._step, scale)
+
+    def _adam_lr(self) -> float:
+        return self.adam_lr if self.dense_kind == "muon" and self.adam_lr is not None else self.lr
+
+    def _muon_all(self, live, scale):
+        lrs = [self.lr * max(1.0, p.shape[0] / p.shape[1]) ** 0.5 for p, _ in live]
+        ops.muon_step([p.data for p, _ in live], [g for _, g in live], [self._dense_state_for(p) for p, _ in live], lrs,
+                      momentum=self.momentum, scale=scale)
 
     def _dense_step_all(self, scale):
         """All dense parameters in launches of up to 24 tensors (same bits as one launch per tensor)."""
@@ -478,13 +498,18 @@ class FusedOptimizer:
             for p, _ in live:
                 self._dense_update(p, scale)
             return
-        if self.dense_kind == "adam":
+        if self.dense_kind == "muon":
+            mats = [e for e in live if self._is_muon(e[0])]
+            if mats:
+                self._muon_all(mats, scale)
+            live = [e for e in live if not self._is_muon(e[0])]
+        if self.dense_kind in ("adam", "muon"):
             step = self._step_dev if self._step_dev is not None else self._step
             for i in range(0, len(live), _lib.RX_MULTI_MAX):
                 chunk = live[i:i + _lib.RX_MULTI_MAX]
                 st = [self._dense_state_for(p) for p, _ in chunk]
                 ops.multi_dense_adam([p.data for p, _ in chunk], [g for _, g in chunk], [x[0] for x in st], [x[1] for x in st],
-                                     self.lr, self.betas[0], self.betas[1], self.adam_eps, step, scale)
+                                     self._adam_lr(), self.betas[0], self.betas[1], self.adam_eps, step, scale)
             return
         mode = _lib.RX_SEG_SGD if self.dense_kind == "sgd" else _lib.RX_SEG_ADAGRAD
         for i in range(0, len(live), _lib.RX_MULTI_MAX):
@@ -514,7 +539,7 @@ class FusedOptimizer:
             for p in self.dense:           # dense gradients may have been made on a branch stream: read here
                 if p.grad is not None:
                     p.grad.record_stream(cur)
-        if self.dense_kind == "adam" and self.dense:
+        if self.dense_kind in ("adam", "muon") and self.dense:
             # the step count also lives on the device, advanced on the stream: a recorded graph of this
             # step then reads the count of the replay, not the one of the recording
             if self._step_dev is not None:

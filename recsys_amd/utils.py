@@ -46,6 +46,34 @@ def topk(scores, array=None, subset=None, k=10):
     return order if array is None else np.take_along_axis(array, order, axis=1)
 
 
+def recommend(model, inputs, k=10, exclude=None):
+    """The ``k`` best items of every row of ``inputs`` with their log-probabilities: (codes [B, k] int64, logprob [B, k], entropy
+    [B]), best first, the lower code first among equal scores; (-1, -inf) where a row has fewer items.  Over the whole
+    catalogue when ``inputs["item_code"]`` is None (models that score every item then), else over each row's own candidates.
+    ``exclude`` [B, E]: positions in the score row (codes, for the whole catalogue) left out; -1 = nothing."""
+    from . import autograd as rxa
+    with torch.no_grad():
+        scores = model(inputs)
+        B, V = scores.shape
+        if exclude is not None:
+            exclude = torch.as_tensor(exclude, device=scores.device).long()
+            if exclude.dim() != 2 or exclude.shape[0] != B:
+                raise ValueError(f"exclude: expected shape [{B}, E], got {tuple(exclude.shape)}")
+            if not torch.cuda.is_current_stream_capturing() and exclude.numel() and bool(((exclude < -1) | (exclude >= V)).any()):
+                raise IndexError("exclude: position out of range")
+            # a spare last column takes the -1 entries
+            wide = torch.cat([scores, scores.new_zeros(B, 1)], 1)
+            wide.scatter_(1, torch.where(exclude < 0, torch.full_like(exclude, V), exclude), float("-inf"))
+            scores = wide[:, :V]
+        none = torch.full((B,), -1, dtype=torch.int64, device=scores.device)
+        out = rxa.log_probs(scores, none, k=k)
+        codes = out.top_index
+        items = inputs.get("item_code")
+        if items is not None:
+            codes = torch.where(codes < 0, codes, torch.gather(items, 1, codes.clamp(min=0)))
+    return codes, out.top_logprob, out.entropy
+
+
 def load_model(model, device, **kwargs):
     return model(**kwargs).to(device)
 
