@@ -17,13 +17,14 @@ typedef __bf16 ns_h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 ns_h2 __attribute__((ext_vector_type(2)));
 typedef float ns_f2 __attribute__((ext_vector_type(2)));
 typedef float ns_f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t ns_u4 __attribute__((ext_vector_type(4)));   // HIP's uint4 kept the prefetch registers in scratch
 typedef float ns_acc __attribute__((ext_vector_type(16)));
 
 #define NS_MAXDIM 16384
 #define NS_SMALL_M 96
 #define NS_SMALL_LDS (152 * 1024)
 #define NS_SMALL_THREADS 512
-#define NS_PARTS 64            // norm partials per matrix
+#define NS_PARTS 256           // norm partials per matrix
 
 // ---------------------------------------------------------------- small matrices: one workgroup each
 struct NsSmall {
@@ -231,7 +232,11 @@ __global__ void __launch_bounds__(RX_BLOCK) ns_init_kernel(NsList a) {
   if (mi == a.count) return;
   const NsMat& t = a.mat[mi];
   double ss = 0.0;
-  for (int i = 0; i < NS_PARTS; ++i) ss += a.parts[mi * NS_PARTS + i];
+  __shared__ double wsum[RX_BLOCK / 64];
+  ss = rx_wave_sum_f64(a.parts[mi * NS_PARTS + threadIdx.x]);
+  if (rx_lane() == 0) wsum[threadIdx.x >> 6] = ss;
+  __syncthreads();
+  ss = ((wsum[0] + wsum[1]) + wsum[2]) + wsum[3];
   const float div = (float)(sqrt(ss) + (double)a.eps);
   const float sc = a.scale ? *a.scale : 1.f;
   const int r0 = b / (t.np / 64) * 64, c0 = b % (t.np / 64) * 64;      // of X
@@ -276,13 +281,13 @@ enum { NS_MODE_A, NS_MODE_B, NS_MODE_X };
 
 // chunk x of a step: 16 bytes of a row, the rows of a plane, the planes of an operand
 template <int T>
-__device__ __forceinline__ void ns_fetch(uint4 (&pre)[NsTile<T>::CH], const uint16_t* P, int64_t pp, const uint16_t* Q, int64_t pq, int K, int k0) {
+__device__ __forceinline__ void ns_fetch(ns_u4 (&pre)[NsTile<T>::CH], const uint16_t* P, int64_t pp, const uint16_t* Q, int64_t pq, int K, int k0) {
 #pragma unroll
   for (int q = 0; q < NsTile<T>::CH; ++q) {
     const int x = q * RX_BLOCK + threadIdx.x;
     const int ch = x % (NS_BK / 8), row = x / (NS_BK / 8) % T, pl = x / (NS_BK / 8) / T % 3, op = x / (NS_BK / 8) / T / 3;
     const uint16_t* src = op ? Q + pl * pq : P + pl * pp;
-    pre[q] = *reinterpret_cast<const uint4*>(src + (int64_t)row * K + k0 + ch * 8);
+    pre[q] = *reinterpret_cast<const ns_u4*>(src + (int64_t)row * K + k0 + ch * 8);
   }
 }
 
@@ -290,7 +295,9 @@ template <int T, int MODE>
 __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step) {
   constexpr int NB = NsTile<T>::NB, CH = NsTile<T>::CH;
   __shared__ __align__(16) uint16_t lds[2][3][T][NS_LDK];
-  int mi = 0, b = blockIdx.x;
+  // workgroups are dealt to the 8 XCDs in turn: each XCD takes a run of neighbouring tiles, which share operand rows in its L2
+  const int per = (gridDim.x + 7) / 8;
+  int mi = 0, b = (blockIdx.x % 8) * per + blockIdx.x / 8;
   for (; mi < a.count; ++mi) {
     const int k = MODE == NS_MODE_X ? a.mat[mi].tiles_x : a.mat[mi].tiles_sym;
     if (b < k) break;
@@ -319,7 +326,7 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
   Q += (int64_t)tj * T * K;
   const int lane = rx_lane(), l31 = lane & 31, h = lane >> 5, wave = threadIdx.x >> 6;
   const int wi = wave >> 1, wj = wave & 1;
-  uint4 pre[CH];
+  ns_u4 pre[CH];
   ns_acc acc[NB][NB] = {};
   ns_fetch<T>(pre, P, pp, Q, pq, K, 0);
   for (int k0 = 0; k0 < K; k0 += NS_BK) {
@@ -328,7 +335,7 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
     for (int q = 0; q < CH; ++q) {
       const int x = q * RX_BLOCK + threadIdx.x;
       const int ch = x % (NS_BK / 8), row = x / (NS_BK / 8) % T, pl = x / (NS_BK / 8) / T % 3, op = x / (NS_BK / 8) / T / 3;
-      *reinterpret_cast<uint4*>(&lds[op][pl][row][ch * 8]) = pre[q];
+      *reinterpret_cast<ns_u4*>(&lds[op][pl][row][ch * 8]) = pre[q];
     }
     __syncthreads();
     if (k0 + NS_BK < K) ns_fetch<T>(pre, P, pp, Q, pq, K, k0 + NS_BK);
@@ -465,7 +472,10 @@ template <int T>
 static void ns_run(const NsList& l, hipStream_t st) {
   unsigned sym = 0, full = 0;
   for (int i = 0; i < l.count; ++i) { sym += l.mat[i].tiles_sym; full += l.mat[i].tiles_x; }
+  sym = (sym + 7) / 8 * 8;
+  full = (full + 7) / 8 * 8;
   for (int s = 0; s < l.steps; ++s) {
+    // a multiple of 8: the tiles are dealt to the XCDs in runs
     hipLaunchKernelGGL((ns_gemm_kernel<T, NS_MODE_A>), dim3(sym), dim3(RX_BLOCK), 0, st, l, s);
     hipLaunchKernelGGL((ns_gemm_kernel<T, NS_MODE_B>), dim3(sym), dim3(RX_BLOCK), 0, st, l, s);
     hipLaunchKernelGGL((ns_gemm_kernel<T, NS_MODE_X>), dim3(full), dim3(RX_BLOCK), 0, st, l, s);
