@@ -13,15 +13,22 @@
 // are one number per lane, and the weights go straight back in as the other operand of the second product: its
 // contraction index may run in any order, and the transposed tile is laid out in the order the registers have.
 //
-// fp32 operands are cut into three bf16 planes (8 + 8 + 8 significant bits) and the six plane products down to
-// 2^-24 of the result are added in fp32: fp32 accuracy from the bf16 matrix rate (fp32 matrix instructions run at 1/16
-// of it, six products at 1/6).  bf16 operands take one plane; there the weights of the second product are rounded
-// to bf16 as well, 2^-9 relative and independent from term to term, as much as the result's own rounding.
+// fp32 operands are cut into two fp16 planes (11 + 11 significant bits: the value to 2^-24) and multiplied as high high +
+// high low + low high in fp32: fp32 accuracy (what is left out is below 2^-24 of a term) from three products at the 16-bit
+// matrix rate, where fp32 matrix instructions run at 1/16 of it and three bf16 planes would take six products.  fp16 has no
+// range to spare, so everything is scaled by powers of two first, which costs no accuracy: a stationary vector by its
+// own largest element, a streaming tile by the tile's (both to 2^14 .. 2^15: elements down to 2^-15 of the largest keep
+// all their bits, smaller ones an absolute error of 2^-40 of it), and the weights by a running reference per stationary
+// vector (the softmax's own in the forward pass).  The factors fold into numbers the loop has anyway.
+// bf16 operands take one plane, exactly; there the weights of the second product are rounded to bf16 as well, 2^-9
+// relative and independent from term to term, as much as the result's own rounding.
 // Scores, references, sums, means and gradients accumulate in fp32.
 #include "rx_common.h"
 
 typedef __bf16 ct_h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 ct_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 ct_f8 __attribute__((ext_vector_type(8)));
+typedef _Float16 ct_p2 __attribute__((ext_vector_type(2)));
 typedef float ct_f2 __attribute__((ext_vector_type(2)));
 typedef float ct_acc __attribute__((ext_vector_type(16)));
 
@@ -30,7 +37,10 @@ typedef float ct_acc __attribute__((ext_vector_type(16)));
 #define CT_NINF (-__builtin_inff())
 #define CT_MAXD 256
 #define CT_LIM 3.0e38f       // |bias * log2 e| is held inside fp32: masks of the type's lowest value stay finite
-#define CT_SLACK 24.f        // the online reference moves only when a score exceeds it by 2^24
+// A running reference is set so that the largest weight is 2^CT_BASE and moves when one passes 2^CT_TOP: fp16 weights stay
+// below 2^16 (a weight and a target's share on top of it), bf16 ones have room.
+#define CT_BASE(PL) ((PL) == 2 ? 6.f : 0.f)
+#define CT_TOP(PL) ((PL) == 2 ? 14.f : 24.f)
 #define CT_THREADS 256
 #define CT_WAVES 4
 
@@ -41,7 +51,7 @@ struct CtRow {               // what the backward pass needs of a row
   int32_t pad0, pad1;
 };
 
-union CtFrag { uint4 u; uint2 d[2]; ct_h8 h; };
+union CtFrag { uint4 u; ct_h8 h; ct_f8 f; };
 
 __device__ __forceinline__ uint32_t ct_pk(float a, float b) {
   ct_f2 v = {a, b};
@@ -50,16 +60,35 @@ __device__ __forceinline__ uint32_t ct_pk(float a, float b) {
 __device__ __forceinline__ float ct_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float ct_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// two floats -> their words in PL planes
+// two floats -> their words in PL planes (1: bf16, 2: fp16)
 template <int PL>
 __device__ __forceinline__ void ct_cut2(float a, float b, uint32_t* w) {
-  w[0] = ct_pk(a, b);
-  if constexpr (PL == 3) {
-    a -= ct_lo(w[0]); b -= ct_hi(w[0]);
-    w[1] = ct_pk(a, b);
-    a -= ct_lo(w[1]); b -= ct_hi(w[1]);
-    w[2] = ct_pk(a, b);
+  if constexpr (PL == 1) {
+    w[0] = ct_pk(a, b);
+  } else {
+    ct_f2 v = {a, b};
+    const ct_p2 h = __builtin_convertvector(v, ct_p2);
+    ct_f2 r = {a - (float)h.x, b - (float)h.y};
+    w[0] = __builtin_bit_cast(uint32_t, h);
+    w[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, ct_p2));
   }
+}
+// power of two that takes a largest magnitude (its bits) to [2^14, 2^15); infinities and NaN stay what they are
+__device__ __forceinline__ float ct_scale(uint32_t peak) {
+  const int e = 268 - (int)(peak >> 23);
+  return __uint_as_float((uint32_t)(e < 227 ? e : 227) << 23);
+}
+__device__ __forceinline__ float ct_inverse(float scale) { return __uint_as_float((254u << 23) - __float_as_uint(scale)); }
+__device__ __forceinline__ float ct_log2(float scale) { return (float)((int)(__float_as_uint(scale) >> 23) - 127); }
+__device__ __forceinline__ uint32_t ct_abs(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t ct_umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+// largest of the wavefront, in every lane
+__device__ __forceinline__ uint32_t ct_wave_umax(uint32_t v) {
+#define CT_DPP(c) v = ct_umax(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, c, 0xf, 0xf, true))
+  CT_DPP(0x111); CT_DPP(0x112); CT_DPP(0x114); CT_DPP(0x118);      // rows of 16: shifts by 1, 2, 4, 8
+  CT_DPP(0x142); CT_DPP(0x143);                                   // on to the next row, on to the upper half
+#undef CT_DPP
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 template <int PL>
 __device__ __forceinline__ void ct_cut8(const float* v, CtFrag* f) {
@@ -74,13 +103,13 @@ __device__ __forceinline__ void ct_cut8(const float* v, CtFrag* f) {
 // acc += A B over the planes, the smallest products first
 template <int PL>
 __device__ __forceinline__ ct_acc ct_mma(const CtFrag* a, const CtFrag* b, ct_acc c) {
-#define CT_MM(i, j) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i].h, b[j].h, c, 0, 0, 0)
-  if constexpr (PL == 3) {
-    CT_MM(2, 0); CT_MM(0, 2); CT_MM(1, 1); CT_MM(1, 0); CT_MM(0, 1);
+  if constexpr (PL == 2) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1].f, b[0].f, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0].f, b[1].f, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0].f, b[0].f, c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0].h, b[0].h, c, 0, 0, 0);
   }
-  CT_MM(0, 0);
-#undef CT_MM
-  return c;
 }
 
 // ---------------------------------------------------------------- global reads
@@ -106,19 +135,35 @@ __device__ __forceinline__ float4 ct_load4(const T* row, int d, int D, bool vec)
   return r;
 }
 
-// stationary operands of one block of 32 vectors: lane column l & 31, element ks * 16 + 8 (l >> 5) + j
+// stationary operands of one block of 32 vectors: lane column l & 31, element ks * 16 + 8 (l >> 5) + j; returns what the
+// scores have to be multiplied with to undo the vector's scale
 template <typename T, int PL, int DP>
-__device__ __forceinline__ void ct_stationary(const T* base, int64_t ld, int64_t row, int64_t rows, int D, bool vec, CtFrag (*f)[PL]) {
+__device__ __forceinline__ float ct_stationary(const T* base, int64_t ld, int64_t row, int64_t rows, int D, bool vec, CtFrag (*f)[PL]) {
   const int h = rx_lane() >> 5;
   const T* p = base + (row < rows ? row : 0) * ld;
+  const int n = row < rows ? D : 0;
+  float scale = 1.f;
+  if constexpr (PL == 2) {
+    uint32_t peak = 0;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      const float4 a = ct_load4(p, ks * 16 + h * 8, n, vec), b = ct_load4(p, ks * 16 + h * 8 + 4, n, vec);
+      peak = ct_umax(ct_umax(peak, ct_umax(ct_abs(a.x), ct_abs(a.y))), ct_umax(ct_abs(a.z), ct_abs(a.w)));
+      peak = ct_umax(ct_umax(peak, ct_umax(ct_abs(b.x), ct_abs(b.y))), ct_umax(ct_abs(b.z), ct_abs(b.w)));
+    }
+    scale = ct_scale(ct_umax(peak, (uint32_t)__shfl_xor((int)peak, 32, 64)));
+  }
 #pragma unroll
   for (int ks = 0; ks < DP / 16; ++ks) {
-    float v[8];
-    const int d = ks * 16 + h * 8;
-    float4 a = ct_load4(p, d, row < rows ? D : 0, vec), b = ct_load4(p, d + 4, row < rows ? D : 0, vec);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    const float4 a = ct_load4(p, ks * 16 + h * 8, n, vec), b = ct_load4(p, ks * 16 + h * 8 + 4, n, vec);
+    float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if constexpr (PL == 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= scale;
+    }
     ct_cut8<PL>(v, f[ks]);
   }
+  return ct_inverse(scale);
 }
 
 // ---------------------------------------------------------------- streaming tiles
@@ -152,8 +197,18 @@ struct CtStage {
       }
     }
   }
-  // into LDS; `flip` (may be null): sign words of the tile's vectors, applied to the transposed copy
-  __device__ __forceinline__ void store(uint16_t* rm, uint16_t* tr, const uint32_t* flip) {
+  // bits of the largest magnitude the wavefront holds
+  __device__ __forceinline__ uint32_t peak() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int q = 0; q < Tile::PER; ++q)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        m = ct_umax(ct_umax(m, ct_umax(ct_abs(v[q][k].x), ct_abs(v[q][k].y))), ct_umax(ct_abs(v[q][k].z), ct_abs(v[q][k].w)));
+    return ct_wave_umax(m);
+  }
+  // into LDS, times `scale`; `flip` (may be null): sign words of the tile's vectors, applied to the transposed copy
+  __device__ __forceinline__ void store(uint16_t* rm, uint16_t* tr, const uint32_t* flip, float scale) {
 #pragma unroll
     for (int q = 0; q < Tile::PER; ++q) {
       const int blk = q * CT_THREADS + threadIdx.x;
@@ -162,8 +217,10 @@ struct CtStage {
       uint32_t w[4][2][PL];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        ct_cut2<PL>(v[q][k].x, v[q][k].y, w[k][0]);
-        ct_cut2<PL>(v[q][k].z, v[q][k].w, w[k][1]);
+        float4 e = v[q][k];
+        if constexpr (PL == 2) { e.x *= scale; e.y *= scale; e.z *= scale; e.w *= scale; }
+        ct_cut2<PL>(e.x, e.y, w[k][0]);
+        ct_cut2<PL>(e.z, e.w, w[k][1]);
       }
 #pragma unroll
       for (int p = 0; p < PL; ++p)
@@ -206,6 +263,7 @@ __device__ __forceinline__ ct_acc ct_scores(const uint16_t* rm, int it, const Ct
 #pragma unroll
     for (int p = 0; p < PL; ++p) a[p].u = *reinterpret_cast<const uint4*>(rm + (p * BN + it * 32 + l31) * Tile::RS + ks * 16 + h * 8);
     s = ct_mma<PL>(a, st[ks], s);
+    if constexpr (DP == 256) __builtin_amdgcn_sched_barrier(0);      // registers are full: no fragments ahead of their use
   }
   return s;
 }
@@ -225,10 +283,16 @@ __device__ __forceinline__ void ct_weigh(const uint16_t* tr, int it, const float
       for (int p = 0; p < PL; ++p)
         a[p].u = *reinterpret_cast<const uint4*>(tr + (p * DP + db * 32 + l31) * Tile::TS + it * 32 + k2 * 16 + h * 8);
       out[db] = ct_mma<PL>(a, b, out[db]);
+      if constexpr (DP == 256) __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
 
+// element e of four neighbouring LDS floats: one 16-byte read for the four of them
+__device__ __forceinline__ float ct_at(const float* p, int e) {
+  const float4 f = *reinterpret_cast<const float4*>(p);
+  return e == 0 ? f.x : e == 1 ? f.y : e == 2 ? f.z : f.w;
+}
 __device__ __forceinline__ float ct_bias2(float b) {      // bias in log2 units; -inf stays, anything else stays finite
   return b == CT_NINF ? CT_NINF : fminf(fmaxf(b * CT_L2E, -CT_LIM), CT_LIM);
 }
@@ -265,18 +329,11 @@ __global__ void __launch_bounds__(CT_THREADS, OCC) ct_fwd_kernel(CtFwd a) {
   uint16_t* rm = reinterpret_cast<uint16_t*>(ct_lds);
   uint16_t* tr = rm + Tile::RM;
   float* lb = reinterpret_cast<float*>(ct_lds + Tile::BYTES);
+  uint32_t* lm = reinterpret_cast<uint32_t*>(lb + BN);
   int tile, split;
   ct_place(a.tiles, a.n_split, &tile, &split);
   const int wave = threadIdx.x >> 6, l31 = rx_lane() & 31, h = rx_lane() >> 5;
   const int64_t row0 = ((int64_t)tile * CT_WAVES + wave) * (32 * MB);
-  CtFrag st[MB][DP / 16][PL];
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb)
-    ct_stationary<T, PL, DP>((const T*)a.x, a.ld_x, row0 + mb * 32 + l31, a.R, a.D, a.vec, st[mb]);
-  ct_acc o[MB][MEAN ? DP / 32 : 1] = {};
-  float ref[MB], sum[MB];
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) { ref[mb] = CT_NINF; sum[mb] = 0.f; }
   const int64_t v0 = split * a.per_split, v1 = v0 + a.per_split < a.V ? v0 + a.per_split : a.V;
   CtStage<T, PL, DP, BN, MEAN> stage;
   float nb = 0.f;
@@ -284,9 +341,26 @@ __global__ void __launch_bounds__(CT_THREADS, OCC) ct_fwd_kernel(CtFwd a) {
     stage.load((const T*)a.t, a.ld_t, v0, v1, a.D, a.vec);
     if (BIAS && threadIdx.x < BN) nb = v0 + threadIdx.x < v1 ? ct_bias2(a.bias[v0 + threadIdx.x]) : CT_NINF;
   }
+  CtFrag st[MB][DP / 16][PL];
+  ct_acc o[MB][MEAN ? DP / 32 : 1] = {};
+  // w = 2^((score - ref) + (kt - kr)), kt the tile's scale undone; sum: of w / 2^kt.  Without a bias kt is part of the
+  // score and kr stays 0: one operation less per score.  A bias may be a mask of 1e38, which would swallow it.
+  float inv[MB], ref[MB], kr[MB], sum[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.x, a.ld_x, row0 + mb * 32 + l31, a.R, a.D, a.vec, st[mb]);
+    ref[mb] = CT_NINF;
+    kr[mb] = sum[mb] = 0.f;
+  }
   for (int64_t v = v0; v < v1; v += BN) {
+    if constexpr (PL == 2) {
+      const uint32_t m = stage.peak();
+      if (rx_lane() == 0) lm[wave] = m;
+    }
     __syncthreads();
-    stage.store(rm, tr, nullptr);
+    const float scale = PL == 2 ? ct_scale(ct_umax(ct_umax(lm[0], lm[1]), ct_umax(lm[2], lm[3]))) : 1.f;
+    const float kt = PL == 2 ? -ct_log2(scale) : 0.f;
+    stage.store(rm, tr, nullptr, scale);
     if (BIAS && threadIdx.x < BN) lb[threadIdx.x] = nb;
     __syncthreads();
     if (v + BN < v1) {
@@ -294,31 +368,29 @@ __global__ void __launch_bounds__(CT_THREADS, OCC) ct_fwd_kernel(CtFwd a) {
       if (BIAS && threadIdx.x < BN) nb = v + BN + threadIdx.x < v1 ? ct_bias2(a.bias[v + BN + threadIdx.x]) : CT_NINF;
     }
     const bool whole = v + BN <= v1;
+    const float back = ct_inverse(scale);
 #pragma unroll
     for (int it = 0; it < BN / 32; ++it) {
-      float bb[16];
-      if constexpr (BIAS) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 f = *reinterpret_cast<const float4*>(lb + it * 32 + 8 * q + 4 * h);
-          bb[4 * q] = f.x; bb[4 * q + 1] = f.y; bb[4 * q + 2] = f.z; bb[4 * q + 3] = f.w;
-        }
-      }
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
         const ct_acc s = ct_scores<PL, DP, BN, MEAN>(rm, it, st[mb]);
+        const float mul = PL == 2 ? inv[mb] * back : CT_L2E;
         float w[16], mx = CT_NINF;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          w[i] = BIAS ? fmaf(s[i], CT_L2E, bb[i]) : s[i] * CT_L2E;
+          if constexpr (BIAS) w[i] = fmaf(s[i], mul, ct_at(lb + it * 32 + 8 * (i / 4) + 4 * h, i % 4));
+          else w[i] = PL == 2 ? fmaf(s[i], mul, kt) : s[i] * mul;
           if (!whole && v + it * 32 + 8 * (i / 4) + 4 * h + i % 4 >= v1) w[i] = CT_NINF;
           mx = fmaxf(mx, w[i]);
         }
-        if (__ballot(mx > ref[mb] + CT_SLACK)) {          // rare after the first tile
+        const float kb = PL == 2 && BIAS ? kt : 0.f;
+        const float base = ref[mb] == CT_NINF ? CT_NINF : ref[mb] - (kb - kr[mb]);
+        if (__ballot(mx > base + CT_TOP(PL))) {               // rare after the first tile
           const float n = fmaxf(mx, __shfl_xor(mx, 32, 64));
-          if (n > ref[mb] + CT_SLACK) {                   // both halves of a row decide alike
+          if (n > base + CT_TOP(PL)) {                        // both halves of a row decide alike
+            const float nk = BIAS ? kb - CT_BASE(PL) : 0.f, nr = BIAS ? n : n - CT_BASE(PL);
             if (ref[mb] != CT_NINF) {
-              const float f = __builtin_amdgcn_exp2f(ref[mb] - n);
+              const float f = __builtin_amdgcn_exp2f((ref[mb] - nr) + (kr[mb] - nk));
               sum[mb] *= f;
               if constexpr (MEAN) {
 #pragma unroll
@@ -327,14 +399,15 @@ __global__ void __launch_bounds__(CT_THREADS, OCC) ct_fwd_kernel(CtFwd a) {
                   for (int i = 0; i < 16; ++i) o[mb][db][i] *= f;
               }
             }
-            ref[mb] = n;
+            ref[mb] = nr;
+            kr[mb] = nk;
           }
         }
-        const float r0 = ref[mb] == CT_NINF ? 0.f : ref[mb];
+        const float r0 = ref[mb] == CT_NINF ? 0.f : ref[mb], dk = kb - kr[mb];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          w[i] = __builtin_amdgcn_exp2f(w[i] - r0);
-          sum[mb] += w[i];
+          w[i] = __builtin_amdgcn_exp2f(PL == 2 && BIAS ? (w[i] - r0) + dk : w[i] - r0);
+          sum[mb] = PL == 2 ? fmaf(w[i], scale, sum[mb]) : sum[mb] + w[i];
         }
         if constexpr (MEAN) ct_weigh<PL, DP, BN>(tr, it, w, o[mb]);
       }
@@ -342,7 +415,17 @@ __global__ void __launch_bounds__(CT_THREADS, OCC) ct_fwd_kernel(CtFwd a) {
   }
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
-    const float total = sum[mb] + __shfl_xor(sum[mb], 32, 64);
+    float total = sum[mb] + __shfl_xor(sum[mb], 32, 64);
+    if constexpr (PL == 2 && BIAS) {                          // back to plain 2^(score - ref)
+      const float f = __builtin_amdgcn_exp2f(kr[mb]);
+      total *= f;
+      if constexpr (MEAN) {
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[mb][db][i] *= f;
+      }
+    }
     const int64_t row = row0 + mb * 32 + l31;
     if (row >= a.R) continue;
     if (h == 0) a.part[(int64_t)split * a.R + row] = make_float2(ref[mb], total);
@@ -489,24 +572,15 @@ __global__ void __launch_bounds__(CT_THREADS, OCC) ct_bwd_kernel(CtBwd a) {
   uint16_t* tr = rm + Tile::RM;
   float* lz = reinterpret_cast<float*>(ct_lds + Tile::BYTES);      // z, or m2 with a bias
   float* ll = lz + BN;                                             // l2s (bias)
-  float* lsg = ll + BN;                                            // sign of c (bias)
-  float* lg = lsg + BN;
+  float* lsg = ll + BN;                                            // sign of c, with the tile's scale undone (bias)
+  float* lg = lsg + BN;                                            // g times that sign
   int32_t* ly = reinterpret_cast<int32_t*>(lg + BN);
   uint32_t* lf = reinterpret_cast<uint32_t*>(ly + BN);             // sign words
+  uint32_t* lm = lf + BN;
   int tile, split;
   ct_place(a.tiles, a.n_split, &tile, &split);
   const int wave = threadIdx.x >> 6, lane = rx_lane(), l31 = lane & 31, h = lane >> 5;
   const int64_t item0 = ((int64_t)tile * CT_WAVES + wave) * (32 * MB);
-  CtFrag st[MB][DP / 16][PL];
-  float b2[MB], dbias[MB];
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    const int64_t item = item0 + mb * 32 + l31;
-    ct_stationary<T, PL, DP>((const T*)a.t, a.ld_t, item, a.V, a.D, a.vec, st[mb]);
-    b2[mb] = BIAS && item < a.V ? ct_bias2(a.bias[item]) : 0.f;
-    dbias[mb] = 0.f;
-  }
-  ct_acc o[MB][DP / 32] = {};
   const int64_t r0 = split * a.per_split, r1 = r0 + a.per_split < a.R ? r0 + a.per_split : a.R;
   CtStage<T, PL, DP, BN, true> stage;
   CtRow info;
@@ -518,75 +592,116 @@ __global__ void __launch_bounds__(CT_THREADS, OCC) ct_bwd_kernel(CtBwd a) {
     }
   };
   if (r0 < r1) fetch(r0);
+  CtFrag st[MB][DP / 16][PL];
+  float inv[MB], b2[MB], dbias[MB], ref[MB];      // ref: of w = 2^(log2 (|c| p) + kt - ref); PL == 1 keeps it at 0
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    const int64_t item = item0 + mb * 32 + l31;
+    inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.t, a.ld_t, item, a.V, a.D, a.vec, st[mb]);
+    b2[mb] = BIAS && item < a.V ? ct_bias2(a.bias[item]) : 0.f;
+    dbias[mb] = 0.f;
+    ref[mb] = PL == 2 ? CT_NINF : 0.f;
+  }
+  ct_acc o[MB][DP / 32] = {};
   for (int64_t r = r0; r < r1; r += BN) {
+    if constexpr (PL == 2) {
+      const uint32_t m = stage.peak();
+      if (lane == 0) lm[wave] = m;
+    }
     __syncthreads();
+    const float scale = PL == 2 ? ct_scale(ct_umax(ct_umax(lm[0], lm[1]), ct_umax(lm[2], lm[3]))) : 1.f;
+    const float kt = PL == 2 ? -ct_log2(scale) : 0.f;
     if (threadIdx.x < BN) {
-      lz[threadIdx.x] = BIAS ? info.m2 : info.z;
-      if (BIAS) { ll[threadIdx.x] = info.l2s; lsg[threadIdx.x] = info.sgn; }
-      lg[threadIdx.x] = info.g;
+      lz[threadIdx.x] = BIAS ? info.m2 : info.z - kt;
+      if (BIAS) { ll[threadIdx.x] = info.l2s - kt; lsg[threadIdx.x] = info.sgn * scale; }
+      lg[threadIdx.x] = info.g * info.sgn;
       ly[threadIdx.x] = info.y;
       lf[threadIdx.x] = info.sgn < 0.f ? 0x80008000u : 0u;
     }
     __syncthreads();
-    stage.store(rm, tr, lf);
+    stage.store(rm, tr, lf, scale);
     __syncthreads();
     if (r + BN < r1) fetch(r + BN);
+    const float back = ct_inverse(scale);
+    // rows of this tile whose target is among the wavefront's items
+    const int64_t rel = lane < BN && ly[lane] >= 0 ? ly[lane] - item0 : -1;
+    const uint64_t hits = __ballot(rel >= 0 && rel < 32 * MB);
 #pragma unroll
     for (int it = 0; it < BN / 32; ++it) {
-      float zz[16], z2[BIAS ? 16 : 1], sg[BIAS ? 16 : 1];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4 f = *reinterpret_cast<const float4*>(lz + it * 32 + 8 * q + 4 * h);
-        zz[4 * q] = f.x; zz[4 * q + 1] = f.y; zz[4 * q + 2] = f.z; zz[4 * q + 3] = f.w;
-        if constexpr (BIAS) {
-          const float4 e = *reinterpret_cast<const float4*>(ll + it * 32 + 8 * q + 4 * h);
-          z2[4 * q] = e.x; z2[4 * q + 1] = e.y; z2[4 * q + 2] = e.z; z2[4 * q + 3] = e.w;
-          const float4 n = *reinterpret_cast<const float4*>(lsg + it * 32 + 8 * q + 4 * h);
-          sg[4 * q] = n.x; sg[4 * q + 1] = n.y; sg[4 * q + 2] = n.z; sg[4 * q + 3] = n.w;
-        }
-      }
+      const bool hit = (uint32_t)(hits >> (it * 32)) != 0;
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
         const ct_acc s = ct_scores<PL, DP, BN, true>(rm, it, st[mb]);
-        float w[16];
+        const float mul = PL == 2 ? inv[mb] * back : CT_L2E;
+        float w[16], mx = CT_NINF;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          if constexpr (BIAS) {
-            w[i] = __builtin_amdgcn_exp2f((fmaf(s[i], CT_L2E, b2[mb]) - zz[i]) - z2[i]);
-            dbias[mb] = fmaf(w[i], sg[i], dbias[mb]);
-          } else {
-            w[i] = __builtin_amdgcn_exp2f(fmaf(s[i], CT_L2E, -zz[i]));
+          const int k = it * 32 + 8 * (i / 4) + 4 * h;
+          if constexpr (BIAS) w[i] = (fmaf(s[i], mul, b2[mb]) - ct_at(lz + k, i % 4)) - ct_at(ll + k, i % 4);
+          else w[i] = fmaf(s[i], mul, -ct_at(lz + k, i % 4));
+          if (PL == 2) mx = fmaxf(mx, w[i]);
+        }
+        const int64_t mine = item0 + mb * 32 + l31;
+        if constexpr (PL == 2) {
+          if (hit) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int k = it * 32 + 8 * (i / 4) + 4 * h + i % 4;
+              if (ly[k] == mine) mx = fmaxf(mx, log2f(fabsf(lg[k])) + kt);
+            }
+          }
+          if (__ballot(mx > ref[mb] + CT_TOP(PL))) {
+            const float n = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            if (n > ref[mb] + CT_TOP(PL)) {
+              if (ref[mb] != CT_NINF) {
+                const float f = __builtin_amdgcn_exp2f(ref[mb] - (n - CT_BASE(PL)));
+                dbias[mb] *= f;
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) o[mb][db][i] *= f;
+              }
+              ref[mb] = n - CT_BASE(PL);
+            }
           }
         }
+        const float rf = ref[mb] == CT_NINF ? 0.f : ref[mb];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = __builtin_amdgcn_exp2f(PL == 2 ? w[i] - rf : w[i]);
+        if (hit) {                // the target's own share: sgn(c) g on top of |c| p, both still to meet sgn(c) x
+          const float up = PL == 2 ? __builtin_amdgcn_exp2f(kt - rf) : 1.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int k = it * 32 + 8 * (i / 4) + 4 * h + i % 4;
+            if (ly[k] == mine) w[i] = fmaf(lg[k], up, w[i]);
+          }
+        }
+        if constexpr (BIAS) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dbias[mb] = fmaf(w[i], ct_at(lsg + it * 32 + 8 * (i / 4) + 4 * h, i % 4), dbias[mb]);
+        }
         ct_weigh<PL, DP, BN>(tr, it, w, o[mb]);
+        if (PL == 1 && hit) {     // a target's share is as large as the whole gradient: what bf16 dropped of these weights goes in too
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const uint32_t u = ct_pk(w[i], w[i + 1]);
+            w[i] -= ct_lo(u);
+            w[i + 1] -= ct_hi(u);
+          }
+          ct_weigh<PL, DP, BN>(tr, it, w, o[mb]);
+        }
       }
     }
-    // targets of this tile among the wavefront's items: g_r x_r on top, in the order of the rows
-    const int64_t rel = lane < BN && ly[lane] >= 0 ? ly[lane] - item0 : -1;
-    uint64_t hits = __ballot(rel >= 0 && rel < 32 * MB);
-    while (hits) {
-      const int i = __builtin_ctzll(hits);
-      hits &= hits - 1;
-      const int li = __builtin_amdgcn_readlane((int)rel, i);
-      const float g = lg[i];
+  }
+  if constexpr (PL == 2) {        // back from the references, in two steps: 2^ref alone may be below the smallest number
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-        const float c = li == mb * 32 + l31 ? g : 0.f;
-        if (BIAS && h == 0) dbias[mb] += c;
+    for (int mb = 0; mb < MB; ++mb) {
+      const float f = ref[mb] == CT_NINF ? 1.f : __builtin_amdgcn_exp2f(0.5f * ref[mb]);
+      dbias[mb] = dbias[mb] * f * f;
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
+      for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float e[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int p = PL - 1; p >= 0; --p) {
-              const uint2 u = *reinterpret_cast<const uint2*>(rm + (p * BN + i) * Tile::RS + db * 32 + 8 * q + 4 * h);
-              e[0] += ct_lo(u.x); e[1] += ct_hi(u.x); e[2] += ct_lo(u.y); e[3] += ct_hi(u.y);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) o[mb][db][4 * q + k] = c != 0.f ? fmaf(c, e[k], o[mb][db][4 * q + k]) : o[mb][db][4 * q + k];
-          }
-      }
+        for (int i = 0; i < 16; ++i) o[mb][db][i] = o[mb][db][i] * f * f;
     }
   }
 #pragma unroll
@@ -622,13 +737,18 @@ __global__ void __launch_bounds__(CT_THREADS, OCC) ct_bwd_kernel(CtBwd a) {
   }
 }
 
-// sums of n_split partial arrays of n elements, in split order
+// sums of n_split partial arrays in split order: n elements of the table gradient, nb of the bias gradient behind them
 template <typename T>
-__global__ void __launch_bounds__(CT_THREADS) ct_sum_kernel(const float* __restrict__ part, int64_t n, int n_split, T* __restrict__ out) {
-  for (int64_t i = (int64_t)blockIdx.x * CT_THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * CT_THREADS) {
+__global__ void __launch_bounds__(CT_THREADS) ct_sum_kernel(const float* __restrict__ part, int64_t n, const float* __restrict__ part_b,
+                                                            int64_t nb, int n_split, T* __restrict__ out, float* __restrict__ out_b) {
+  for (int64_t i = (int64_t)blockIdx.x * CT_THREADS + threadIdx.x; i < n + nb; i += (int64_t)gridDim.x * CT_THREADS) {
+    const bool b = i >= n;
+    const float* p = b ? part_b + (i - n) : part + i;
+    const int64_t step = b ? nb : n;
     float s = 0.f;
-    for (int q = 0; q < n_split; ++q) s += part[q * n + i];
-    if constexpr (sizeof(T) == 4) out[i] = s;
+    for (int q = 0; q < n_split; ++q) s += p[q * step];
+    if (b) out_b[i - n] = s;
+    else if constexpr (sizeof(T) == 4) out[i] = s;
     else out[i] = (uint16_t)ct_pk(s, s);
   }
 }
@@ -636,6 +756,8 @@ __global__ void __launch_bounds__(CT_THREADS) ct_sum_kernel(const float* __restr
 // ---------------------------------------------------------------- host
 static int ct_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 static int ct_mb(bool bf16, int dp) { return bf16 && dp <= 64 ? 2 : 1; }
+// two blocks with a bias do not fit the registers of two wavefronts per SIMD
+static int ct_bwd_mb(bool bf16, int dp, bool bias) { return bias && dp == 64 ? 1 : ct_mb(bf16, dp); }
 static int ct_bn(bool bf16, int dp) { return bf16 ? (dp <= 128 ? 64 : 32) : (dp <= 64 ? 64 : 32); }
 
 struct CtPlan {
@@ -643,14 +765,14 @@ struct CtPlan {
   int64_t per_split;
 };
 // `fixed` vectors are stationary, `moving` ones stream: enough splits of the stream for four workgroups per CU, each of
-// at least two tiles; multiples of 8 (one XCD each) where there are that many.
+// at least two tiles; multiples of 8 (one XCD each) where there are many.
 static CtPlan ct_plan(int64_t fixed, int64_t moving, int bm, int bn) {
   CtPlan p;
   p.tiles = (int)rx_cdiv(fixed, bm);
   int64_t n = rx_cdiv(1024, p.tiles);
   const int64_t most = rx_cdiv(moving, 2 * bn);
   if (n > most) n = most;
-  if (n > 8) n = n / 8 * 8;
+  if (n > 64) n = n / 8 * 8;
   if (n < 1) n = 1;
   p.per_split = rx_cdiv(rx_cdiv(moving, n), bn) * bn;
   p.n_split = (int)rx_cdiv(moving, p.per_split);
@@ -679,9 +801,9 @@ static CtPlan ct_fwd_plan(int64_t R, int64_t V, int D, int bf16) {
   const int dp = ct_dp(D);
   return ct_plan(R, V, CT_WAVES * 32 * ct_mb(bf16, dp), ct_bn(bf16, dp));
 }
-static CtPlan ct_bwd_plan(int64_t R, int64_t V, int D, int bf16) {
+static CtPlan ct_bwd_plan(int64_t R, int64_t V, int D, int bf16, bool bias) {
   const int dp = ct_dp(D);
-  return ct_plan(V, R, CT_WAVES * 32 * ct_mb(bf16, dp), ct_bn(bf16, dp));
+  return ct_plan(V, R, CT_WAVES * 32 * ct_bwd_mb(bf16, dp, bias), ct_bn(bf16, dp));
 }
 
 extern "C" size_t rx_catalog_fwd_workspace_bytes(int64_t R, int64_t V, int32_t D, int32_t bf16, int32_t want_mean) {
@@ -691,7 +813,7 @@ extern "C" size_t rx_catalog_fwd_workspace_bytes(int64_t R, int64_t V, int32_t D
 }
 extern "C" size_t rx_catalog_bwd_workspace_bytes(int64_t R, int64_t V, int32_t D, int32_t bf16, int32_t want_bias) {
   if (R <= 0 || V <= 0 || D < 1 || D > CT_MAXD) return 0;
-  const CtPlan p = ct_bwd_plan(R, V, D, bf16);
+  const CtPlan p = ct_bwd_plan(R, V, D, bf16, want_bias != 0);
   return rx_align_up((size_t)R * sizeof(CtRow), 256) +
          (p.n_split > 1 ? rx_align_up((size_t)p.n_split * V * D * 4, 256) + (want_bias ? (size_t)p.n_split * V * 4 : 0) : 0);
 }
@@ -700,7 +822,7 @@ extern "C" size_t rx_catalog_bwd_workspace_bytes(int64_t R, int64_t V, int32_t D
 template <typename T, int PL, int DP, int MB, int BN, bool MEAN, bool BIAS, int OCC>
 static int ct_go_fwd(const CtFwd& f, hipStream_t st) {
   auto kernel = ct_fwd_kernel<T, PL, DP, MB, BN, MEAN, BIAS, OCC>;
-  const int lds = CtTile<PL, DP, BN, MEAN>::BYTES + (BIAS ? BN * 4 : 0);
+  const int lds = CtTile<PL, DP, BN, MEAN>::BYTES + BN * 4 + 16;
   if (lds > 64 * 1024) RX_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
   hipLaunchKernelGGL(kernel, dim3((unsigned)(f.tiles * f.n_split)), dim3(CT_THREADS), lds, st, f);
   return 0;
@@ -712,9 +834,9 @@ static int ct_pick_fwd(const CtFwd& f, hipStream_t st) {
 }
 template <typename T, int PL, int DP, int MB, int BN, int OCC>
 static int ct_pick_bwd(const CtBwd& f, hipStream_t st) {
-  const int lds = CtTile<PL, DP, BN, true>::BYTES + 6 * BN * 4;
+  const int lds = CtTile<PL, DP, BN, true>::BYTES + 6 * BN * 4 + 16;
   if (f.db) {
-    auto kernel = ct_bwd_kernel<T, PL, DP, MB, BN, true, OCC>;
+    auto kernel = ct_bwd_kernel<T, PL, DP, DP == 64 ? 1 : MB, BN, true, OCC>;
     if (lds > 64 * 1024) RX_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     hipLaunchKernelGGL(kernel, dim3((unsigned)(f.tiles * f.n_split)), dim3(CT_THREADS), lds, st, f);
   } else {
@@ -750,10 +872,10 @@ extern "C" int rx_catalog_fwd(const rx_catalog_args* args, float* d_logprob, flo
     }
   } else {
     switch (ct_dp(a.D)) {
-      case 32: rc = ct_pick_fwd<float, 3, 32, 1, 64, 2>(f, st); break;
-      case 64: rc = ct_pick_fwd<float, 3, 64, 1, 64, 2>(f, st); break;
-      case 128: rc = ct_pick_fwd<float, 3, 128, 1, 32, 1>(f, st); break;
-      default: rc = ct_pick_fwd<float, 3, 256, 1, 32, 1>(f, st);
+      case 32: rc = ct_pick_fwd<float, 2, 32, 1, 64, 2>(f, st); break;
+      case 64: rc = ct_pick_fwd<float, 2, 64, 1, 64, 2>(f, st); break;
+      case 128: rc = ct_pick_fwd<float, 2, 128, 1, 32, 1>(f, st); break;
+      default: rc = ct_pick_fwd<float, 2, 256, 1, 32, 1>(f, st);
     }
   }
   if (rc) return rc;
@@ -789,7 +911,7 @@ extern "C" int rx_catalog_bwd(const rx_catalog_args* args, const float* d_stats,
   else hipLaunchKernelGGL(ct_prep_kernel<float>, grid, dim3(CT_THREADS), 0, st, q);
   RX_LAUNCH_CHECK();
   if (!want_t) return 0;
-  const CtPlan p = ct_bwd_plan(a.R, a.V, a.D, a.bf16);
+  const CtPlan p = ct_bwd_plan(a.R, a.V, a.D, a.bf16, d_dbias != nullptr);
   uint8_t* w = (uint8_t*)ws + rx_align_up((size_t)a.R * sizeof(CtRow), 256);
   const bool partial = p.n_split > 1;
   float* pt = (float*)w;
@@ -808,25 +930,20 @@ extern "C" int rx_catalog_bwd(const rx_catalog_args* args, const float* d_stats,
     }
   } else {
     switch (ct_dp(a.D)) {
-      case 32: rc = ct_pick_bwd<float, 3, 32, 1, 64, 2>(f, st); break;
-      case 64: rc = ct_pick_bwd<float, 3, 64, 1, 64, 2>(f, st); break;
-      case 128: rc = ct_pick_bwd<float, 3, 128, 1, 32, 1>(f, st); break;
-      default: rc = ct_pick_bwd<float, 3, 256, 1, 32, 1>(f, st);
+      case 32: rc = ct_pick_bwd<float, 2, 32, 1, 64, 2>(f, st); break;
+      case 64: rc = ct_pick_bwd<float, 2, 64, 1, 64, 2>(f, st); break;
+      case 128: rc = ct_pick_bwd<float, 2, 128, 1, 32, 1>(f, st); break;
+      default: rc = ct_pick_bwd<float, 2, 256, 1, 32, 1>(f, st);
     }
   }
   if (rc) return rc;
   RX_LAUNCH_CHECK();
   if (partial) {
-    const int64_t n = a.V * a.D;
-    const dim3 g((unsigned)(rx_cdiv(n, CT_THREADS) < 4096 ? rx_cdiv(n, CT_THREADS) : 4096));
-    if (a.bf16) hipLaunchKernelGGL(ct_sum_kernel<uint16_t>, g, dim3(CT_THREADS), 0, st, pt, n, p.n_split, (uint16_t*)d_dtable);
-    else hipLaunchKernelGGL(ct_sum_kernel<float>, g, dim3(CT_THREADS), 0, st, pt, n, p.n_split, (float*)d_dtable);
+    const int64_t n = a.V * a.D, nb = d_dbias ? a.V : 0;
+    const dim3 g((unsigned)(rx_cdiv(n + nb, CT_THREADS) < 8192 ? rx_cdiv(n + nb, CT_THREADS) : 8192));
+    if (a.bf16) hipLaunchKernelGGL(ct_sum_kernel<uint16_t>, g, dim3(CT_THREADS), 0, st, pt, n, pb, nb, p.n_split, (uint16_t*)d_dtable, d_dbias);
+    else hipLaunchKernelGGL(ct_sum_kernel<float>, g, dim3(CT_THREADS), 0, st, pt, n, pb, nb, p.n_split, (float*)d_dtable, d_dbias);
     RX_LAUNCH_CHECK();
-    if (d_dbias) {
-      const dim3 gb((unsigned)(rx_cdiv(a.V, CT_THREADS) < 4096 ? rx_cdiv(a.V, CT_THREADS) : 4096));
-      hipLaunchKernelGGL(ct_sum_kernel<float>, gb, dim3(CT_THREADS), 0, st, pb, a.V, p.n_split, d_dbias);
-      RX_LAUNCH_CHECK();
-    }
   }
   return 0;
 }
