@@ -25,6 +25,8 @@
 // Scores, references, sums, means and gradients accumulate in fp32.
 #include "rx_common.h"
 
+#include <type_traits>
+
 typedef __bf16 ct_h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 ct_h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 ct_f8 __attribute__((ext_vector_type(8)));
@@ -41,6 +43,11 @@ typedef float ct_acc __attribute__((ext_vector_type(16)));
 // below 2^16 (a weight and a target's share on top of it), bf16 ones have room.
 #define CT_BASE(PL) ((PL) == 2 ? 6.f : 0.f)
 #define CT_TOP(PL) ((PL) == 2 ? 14.f : 24.f)
+#ifndef CT_NW64
+#define CT_NW64 4
+#define CT_NW32 4
+#define CT_OCC128 2
+#endif
 #define CT_THREADS 256
 #define CT_WAVES 4
 
@@ -67,9 +74,11 @@ __device__ __forceinline__ void ct_cut2(float a, float b, uint32_t* w) {
     w[0] = ct_pk(a, b);
   } else {
     ct_f2 v = {a, b};
-    const ct_p2 h = __builtin_convertvector(v, ct_p2);
-    ct_f2 r = {a - (float)h.x, b - (float)h.y};
-    w[0] = __builtin_bit_cast(uint32_t, h);
+    w[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, ct_p2));
+    // a - high, b - high in one mixed-precision instruction each (the compiler converts back and subtracts)
+    ct_f2 r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r.x) : "v"(w[0]), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r.y) : "v"(w[0]), "v"(b));
     w[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, ct_p2));
   }
 }
@@ -135,6 +144,17 @@ __device__ __forceinline__ float4 ct_load4(const T* row, int d, int D, bool vec)
   return r;
 }
 
+// the same four bf16 elements as two words
+__device__ __forceinline__ uint2 ct_words4(const uint16_t* row, int d, int D, bool vec) {
+  if (vec && d + 4 <= D) return *reinterpret_cast<const uint2*>(row + d);
+  uint2 r = make_uint2(0u, 0u);
+  if (d < D) r.x = row[d];
+  if (d + 1 < D) r.x |= (uint32_t)row[d + 1] << 16;
+  if (d + 2 < D) r.y = row[d + 2];
+  if (d + 3 < D) r.y |= (uint32_t)row[d + 3] << 16;
+  return r;
+}
+
 // stationary operands of one block of 32 vectors: lane column l & 31, element ks * 16 + 8 (l >> 5) + j; returns what the
 // scores have to be multiplied with to undo the vector's scale
 template <typename T, int PL, int DP>
@@ -167,33 +187,44 @@ __device__ __forceinline__ float ct_stationary(const T* base, int64_t ld, int64_
 }
 
 // ---------------------------------------------------------------- streaming tiles
-// A tile of BN vectors in LDS: rm[PL][BN][DP + 8] row-major and, with TR, tr[PL][DP][BN + 8] transposed.  In the
+// A tile of BN vectors in LDS: rm[PL][BN][DP + 8] row-major and, with TR, tr[PL][DP][BN] transposed.  In the
 // transposed copy the 16 vectors of a contraction step lie as {0-3, 8-11, 4-7, 12-15}: the order in which the two
-// halves of a wavefront hold the scores.  Row strides are odd multiples of 16 bytes: 16-byte reads down the rows meet every
-// bank equally often.
-template <int PL, int DP, int BN, bool TR>
+// halves of a wavefront hold the scores.  Row-major rows are an odd multiple of 16 bytes apart, so that 16-byte reads down
+// the rows meet every bank equally often; the transposed copy, written 8 bytes at a time by threads four rows apart as
+// well as read down its rows, permutes the 16-byte chunks of a row instead (ct_swz).
+template <int PL, int DP, int BN, bool TR, int NT>
 struct CtTile {
-  static constexpr int RS = DP + 8, TS = BN + 8;
+  static constexpr int RS = DP + 8, TS = BN;
   static constexpr int RM = PL * BN * RS, TM = TR ? PL * DP * TS : 0;    // 16-bit elements
   static constexpr int BYTES = (RM + TM) * 2;
-  static constexpr int BLOCKS = BN * DP / 16, PER = (BLOCKS + CT_THREADS - 1) / CT_THREADS;   // 4 x 4 blocks, per thread
+  static constexpr int BLOCKS = BN * DP / 16, PER = (BLOCKS + NT - 1) / NT;   // 4 x 4 blocks, per thread
 };
 
-template <typename T, int PL, int DP, int BN, bool TR>
+// chunk of row d that holds chunk c: eight neighbouring rows, and eight rows four apart, take different banks
+template <int BN>
+__device__ __forceinline__ int ct_swz(int d, int c) {
+  if constexpr (BN == 64) return c ^ ((((d & 3) << 1) | ((d >> 2) & 1)) ^ ((d >> 3) & 7));
+  else return c ^ (((d & 2) | ((d >> 2) & 1)) ^ ((d >> 3) & 3));
+}
+
+template <typename T, int PL, int DP, int BN, bool TR, int NT>
 struct CtStage {
-  typedef CtTile<PL, DP, BN, TR> Tile;
-  float4 v[Tile::PER][4];
+  typedef CtTile<PL, DP, BN, TR, NT> Tile;
+  // as they lie in memory: four floats, or four bf16 in two words, of four vectors
+  typedef typename std::conditional<sizeof(T) == 4, float4, uint2>::type Quad;
+  Quad v[Tile::PER][4];
   // vectors [row0, row0 + BN) of the streaming side, zeros past `rows`
   __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row0, int64_t rows, int D, bool vec) {
 #pragma unroll
     for (int q = 0; q < Tile::PER; ++q) {
-      const int blk = q * CT_THREADS + threadIdx.x;
+      const int blk = q * NT + threadIdx.x;
       const int d = blk % (DP / 4) * 4, i = blk / (DP / 4) * 4;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int64_t row = row0 + i + k;
-        const bool on = row < rows && (Tile::BLOCKS % CT_THREADS == 0 || blk < Tile::BLOCKS);
-        v[q][k] = ct_load4(base + (on ? row : 0) * ld, d, on ? D : 0, vec);
+        const bool on = row < rows && (Tile::BLOCKS % NT == 0 || blk < Tile::BLOCKS);
+        if constexpr (sizeof(T) == 4) v[q][k] = ct_load4(base + (on ? row : 0) * ld, d, on ? D : 0, vec);
+        else v[q][k] = ct_words4(base + (on ? row : 0) * ld, d, on ? D : 0, vec);
       }
     }
   }
@@ -204,23 +235,27 @@ struct CtStage {
     for (int q = 0; q < Tile::PER; ++q)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        m = ct_umax(ct_umax(m, ct_umax(ct_abs(v[q][k].x), ct_abs(v[q][k].y))), ct_umax(ct_abs(v[q][k].z), ct_abs(v[q][k].w)));
+        if constexpr (PL == 2)
+          m = ct_umax(ct_umax(m, ct_umax(ct_abs(v[q][k].x), ct_abs(v[q][k].y))), ct_umax(ct_abs(v[q][k].z), ct_abs(v[q][k].w)));
     return ct_wave_umax(m);
   }
   // into LDS, times `scale`; `flip` (may be null): sign words of the tile's vectors, applied to the transposed copy
   __device__ __forceinline__ void store(uint16_t* rm, uint16_t* tr, const uint32_t* flip, float scale) {
 #pragma unroll
     for (int q = 0; q < Tile::PER; ++q) {
-      const int blk = q * CT_THREADS + threadIdx.x;
-      if (Tile::BLOCKS % CT_THREADS != 0 && blk >= Tile::BLOCKS) continue;
+      const int blk = q * NT + threadIdx.x;
+      if (Tile::BLOCKS % NT != 0 && blk >= Tile::BLOCKS) continue;
       const int d = blk % (DP / 4) * 4, ib = blk / (DP / 4);
       uint32_t w[4][2][PL];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float4 e = v[q][k];
-        if constexpr (PL == 2) { e.x *= scale; e.y *= scale; e.z *= scale; e.w *= scale; }
-        ct_cut2<PL>(e.x, e.y, w[k][0]);
-        ct_cut2<PL>(e.z, e.w, w[k][1]);
+        if constexpr (PL == 2) {
+          ct_cut2<PL>(v[q][k].x * scale, v[q][k].y * scale, w[k][0]);
+          ct_cut2<PL>(v[q][k].z * scale, v[q][k].w * scale, w[k][1]);
+        } else {
+          w[k][0][0] = v[q][k].x;
+          w[k][1][0] = v[q][k].y;
+        }
       }
 #pragma unroll
       for (int p = 0; p < PL; ++p)
@@ -244,7 +279,7 @@ struct CtStage {
             const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;     // upper or lower halves of two words
             const uint32_t a = __builtin_amdgcn_perm(w[1][e >> 1][p], w[0][e >> 1][p], sel);
             const uint32_t b = __builtin_amdgcn_perm(w[3][e >> 1][p], w[2][e >> 1][p], sel);
-            *reinterpret_cast<uint2*>(tr + (p * DP + d + e) * Tile::TS + pos) = make_uint2(a, b);
+            *reinterpret_cast<uint2*>(tr + (p * DP + d + e) * Tile::TS + ct_swz<BN>(d + e, pos >> 3) * 8 + (pos & 4)) = make_uint2(a, b);
           }
       }
     }
@@ -252,9 +287,9 @@ struct CtStage {
 };
 
 // scores of 32 streaming vectors [it * 32, + 32) of the tile against the stationary block
-template <int PL, int DP, int BN, bool TR>
+template <int PL, int DP, int BN>
 __device__ __forceinline__ ct_acc ct_scores(const uint16_t* rm, int it, const CtFrag (*st)[PL]) {
-  typedef CtTile<PL, DP, BN, TR> Tile;
+  typedef CtTile<PL, DP, BN, true, 256> Tile;
   const int l31 = rx_lane() & 31, h = rx_lane() >> 5;
   ct_acc s = {};
 #pragma unroll
@@ -270,7 +305,7 @@ __device__ __forceinline__ ct_acc ct_scores(const uint16_t* rm, int it, const Ct
 // out[db] += transposed tile (dims db * 32 ..) x weights, w[16] in the scores' register order
 template <int PL, int DP, int BN>
 __device__ __forceinline__ void ct_weigh(const uint16_t* tr, int it, const float* w, ct_acc* out) {
-  typedef CtTile<PL, DP, BN, true> Tile;
+  typedef CtTile<PL, DP, BN, true, 256> Tile;
   const int l31 = rx_lane() & 31, h = rx_lane() >> 5;
 #pragma unroll
   for (int k2 = 0; k2 < 2; ++k2) {
@@ -281,7 +316,7 @@ __device__ __forceinline__ void ct_weigh(const uint16_t* tr, int it, const float
       CtFrag a[PL];
 #pragma unroll
       for (int p = 0; p < PL; ++p)
-        a[p].u = *reinterpret_cast<const uint4*>(tr + (p * DP + db * 32 + l31) * Tile::TS + it * 32 + k2 * 16 + h * 8);
+        a[p].u = *reinterpret_cast<const uint4*>(tr + (p * DP + db * 32 + l31) * Tile::TS + ct_swz<BN>(db * 32 + l31, it * 4 + k2 * 2 + h) * 8);
       out[db] = ct_mma<PL>(a, b, out[db]);
       if constexpr (DP == 256) __builtin_amdgcn_sched_barrier(0);
     }
@@ -322,25 +357,47 @@ struct CtFwd {
   float* out;                  // [n_split][R][D]: sum of weight * t_v
 };
 
-template <typename T, int PL, int DP, int MB, int BN, bool MEAN, bool BIAS, int OCC>
-__global__ void __launch_bounds__(CT_THREADS, OCC) ct_fwd_kernel(CtFwd a) {
-  typedef CtTile<PL, DP, BN, MEAN> Tile;
+// The loop has one barrier per tile: while tile i is worked on, tile i + 1 goes from registers into the other LDS buffer
+// and tile i + 2 from memory into the registers; its largest magnitude is known one barrier before its scale is needed.
+template <typename T, int PL, int DP, int MB, int BN, bool MEAN, bool BIAS, int NW, int OCC>
+__global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
+  typedef CtTile<PL, DP, BN, MEAN, NW * 64> Tile;
   extern __shared__ __align__(16) uint8_t ct_lds[];
-  uint16_t* rm = reinterpret_cast<uint16_t*>(ct_lds);
-  uint16_t* tr = rm + Tile::RM;
-  float* lb = reinterpret_cast<float*>(ct_lds + Tile::BYTES);
-  uint32_t* lm = reinterpret_cast<uint32_t*>(lb + BN);
+  float* lb = reinterpret_cast<float*>(ct_lds + 2 * Tile::BYTES);           // [2][BN] bias
+  uint32_t* lm = reinterpret_cast<uint32_t*>(lb + 2 * BN);                  // [2][NW] largest magnitudes
   int tile, split;
   ct_place(a.tiles, a.n_split, &tile, &split);
   const int wave = threadIdx.x >> 6, l31 = rx_lane() & 31, h = rx_lane() >> 5;
-  const int64_t row0 = ((int64_t)tile * CT_WAVES + wave) * (32 * MB);
+  const int64_t row0 = ((int64_t)tile * NW + wave) * (32 * MB);
   const int64_t v0 = split * a.per_split, v1 = v0 + a.per_split < a.V ? v0 + a.per_split : a.V;
-  CtStage<T, PL, DP, BN, MEAN> stage;
+  const int n = (int)((v1 - v0 + BN - 1) / BN);             // tiles of this split, at least one
+  CtStage<T, PL, DP, BN, MEAN, NW * 64> stage;
   float nb = 0.f;
-  if (v0 < v1) {
-    stage.load((const T*)a.t, a.ld_t, v0, v1, a.D, a.vec);
-    if (BIAS && threadIdx.x < BN) nb = v0 + threadIdx.x < v1 ? ct_bias2(a.bias[v0 + threadIdx.x]) : CT_NINF;
-  }
+  auto fetch = [&](int i) {
+    const int64_t v = v0 + (int64_t)i * BN;
+    stage.load((const T*)a.t, a.ld_t, v, v1, a.D, a.vec);
+    if (BIAS && threadIdx.x < BN) nb = v + threadIdx.x < v1 ? ct_bias2(a.bias[v + threadIdx.x]) : CT_NINF;
+  };
+  auto publish = [&](int i) {
+    if constexpr (PL == 2) {
+      const uint32_t m = stage.peak();
+      if (rx_lane() == 0) lm[(i & 1) * NW + wave] = m;
+    }
+  };
+  auto put = [&](int i) -> float {                          // tile i into its buffer; returns its scale
+    float scale = 1.f;
+    if constexpr (PL == 2) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) m = ct_umax(m, lm[(i & 1) * NW + w]);
+      scale = ct_scale(m);
+    }
+    uint16_t* rm = reinterpret_cast<uint16_t*>(ct_lds + (i & 1) * Tile::BYTES);
+    stage.store(rm, rm + Tile::RM, nullptr, scale);
+    if (BIAS && threadIdx.x < BN) lb[(i & 1) * BN + threadIdx.x] = nb;
+    return scale;
+  };
+  fetch(0);
   CtFrag st[MB][DP / 16][PL];
   ct_acc o[MB][MEAN ? DP / 32 : 1] = {};
   // w = 2^((score - ref) + (kt - kr)), kt the tile's scale undone; sum: of w / 2^kt.  Without a bias kt is part of the
@@ -352,43 +409,53 @@ __global__ void __launch_bounds__(CT_THREADS, OCC) ct_fwd_kernel(CtFwd a) {
     ref[mb] = CT_NINF;
     kr[mb] = sum[mb] = 0.f;
   }
-  for (int64_t v = v0; v < v1; v += BN) {
-    if constexpr (PL == 2) {
-      const uint32_t m = stage.peak();
-      if (rx_lane() == 0) lm[wave] = m;
+  publish(0);
+  __syncthreads();
+  float scale = put(0), next = 1.f;
+  if (n > 1) {
+    fetch(1);
+    publish(1);
+  }
+  __syncthreads();
+  for (int i = 0; i < n; ++i) {
+    if (i + 1 < n) {
+      next = put(i + 1);
+      if (i + 2 < n) fetch(i + 2);
     }
-    __syncthreads();
-    const float scale = PL == 2 ? ct_scale(ct_umax(ct_umax(lm[0], lm[1]), ct_umax(lm[2], lm[3]))) : 1.f;
-    const float kt = PL == 2 ? -ct_log2(scale) : 0.f;
-    stage.store(rm, tr, nullptr, scale);
-    if (BIAS && threadIdx.x < BN) lb[threadIdx.x] = nb;
-    __syncthreads();
-    if (v + BN < v1) {
-      stage.load((const T*)a.t, a.ld_t, v + BN, v1, a.D, a.vec);
-      if (BIAS && threadIdx.x < BN) nb = v + BN + threadIdx.x < v1 ? ct_bias2(a.bias[v + BN + threadIdx.x]) : CT_NINF;
-    }
-    const bool whole = v + BN <= v1;
-    const float back = ct_inverse(scale);
+    const uint16_t* rm = reinterpret_cast<const uint16_t*>(ct_lds + (i & 1) * Tile::BYTES);
+    const uint16_t* tr = rm + Tile::RM;
+    const float* bb = lb + (i & 1) * BN;
+    const float kt = PL == 2 ? -ct_log2(scale) : 0.f, back = ct_inverse(scale);
+    const int64_t left = v1 - v0 - (int64_t)i * BN;
+    const int live = left < BN ? (int)left : BN;
 #pragma unroll
     for (int it = 0; it < BN / 32; ++it) {
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
-        const ct_acc s = ct_scores<PL, DP, BN, MEAN>(rm, it, st[mb]);
+        const ct_acc s = ct_scores<PL, DP, BN>(rm, it, st[mb]);
         const float mul = PL == 2 ? inv[mb] * back : CT_L2E;
-        float w[16], mx = CT_NINF;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if constexpr (BIAS) w[i] = fmaf(s[i], mul, ct_at(lb + it * 32 + 8 * (i / 4) + 4 * h, i % 4));
-          else w[i] = PL == 2 ? fmaf(s[i], mul, kt) : s[i] * mul;
-          if (!whole && v + it * 32 + 8 * (i / 4) + 4 * h + i % 4 >= v1) w[i] = CT_NINF;
-          mx = fmaxf(mx, w[i]);
-        }
+        float r0 = ref[mb] == CT_NINF ? 0.f : ref[mb];
         const float kb = PL == 2 && BIAS ? kt : 0.f;
-        const float base = ref[mb] == CT_NINF ? CT_NINF : ref[mb] - (kb - kr[mb]);
+        float w[16], mx = CT_NINF;
+        // without a bias: relative to the reference at once
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          if constexpr (BIAS) w[e] = fmaf(s[e], mul, ct_at(bb + it * 32 + 8 * (e / 4) + 4 * h, e % 4));
+          else w[e] = fmaf(s[e], mul, (PL == 2 ? kt : 0.f) - r0);
+        }
+        if (live < BN) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (it * 32 + 8 * (e / 4) + 4 * h + e % 4 >= live) w[e] = CT_NINF;
+          asm volatile("");         // a branch: the comparisons are for the last tile only
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, w[e]);
+        const float base = ref[mb] == CT_NINF ? CT_NINF : BIAS ? ref[mb] - (kb - kr[mb]) : 0.f;
         if (__ballot(mx > base + CT_TOP(PL))) {               // rare after the first tile
-          const float n = fmaxf(mx, __shfl_xor(mx, 32, 64));
-          if (n > base + CT_TOP(PL)) {                        // both halves of a row decide alike
-            const float nk = BIAS ? kb - CT_BASE(PL) : 0.f, nr = BIAS ? n : n - CT_BASE(PL);
+          const float m = fmaxf(mx, __shfl_xor(mx, 32, 64));
+          if (m > base + CT_TOP(PL)) {                        // both halves of a row decide alike
+            const float nk = BIAS ? kb - CT_BASE(PL) : 0.f, nr = BIAS ? m : (m + r0) - CT_BASE(PL);
             if (ref[mb] != CT_NINF) {
               const float f = __builtin_amdgcn_exp2f((ref[mb] - nr) + (kr[mb] - nk));
               sum[mb] *= f;
@@ -396,22 +463,29 @@ __global__ void __launch_bounds__(CT_THREADS, OCC) ct_fwd_kernel(CtFwd a) {
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) o[mb][db][i] *= f;
+                  for (int e = 0; e < 16; ++e) o[mb][db][e] *= f;
               }
             }
-            ref[mb] = nr;
+            if constexpr (!BIAS) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) w[e] -= nr - r0;
+            }
+            ref[mb] = r0 = nr;
             kr[mb] = nk;
           }
         }
-        const float r0 = ref[mb] == CT_NINF ? 0.f : ref[mb], dk = kb - kr[mb];
+        const float dk = kb - kr[mb];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          w[i] = __builtin_amdgcn_exp2f(PL == 2 && BIAS ? (w[i] - r0) + dk : w[i] - r0);
-          sum[mb] = PL == 2 ? fmaf(w[i], scale, sum[mb]) : sum[mb] + w[i];
+        for (int e = 0; e < 16; ++e) {
+          w[e] = __builtin_amdgcn_exp2f(!BIAS ? w[e] : PL == 2 ? (w[e] - r0) + dk : w[e] - r0);
+          sum[mb] = PL == 2 ? fmaf(w[e], scale, sum[mb]) : sum[mb] + w[e];
         }
         if constexpr (MEAN) ct_weigh<PL, DP, BN>(tr, it, w, o[mb]);
       }
     }
+    if (i + 2 < n) publish(i);
+    scale = next;
+    __syncthreads();
   }
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
@@ -564,34 +638,57 @@ struct CtBwd {
   bool partial;
 };
 
-template <typename T, int PL, int DP, int MB, int BN, bool BIAS, int OCC>
-__global__ void __launch_bounds__(CT_THREADS, OCC) ct_bwd_kernel(CtBwd a) {
-  typedef CtTile<PL, DP, BN, true> Tile;
+template <typename T, int PL, int DP, int MB, int BN, bool BIAS, int NW, int OCC>
+__global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
+  typedef CtTile<PL, DP, BN, true, NW * 64> Tile;
   extern __shared__ __align__(16) uint8_t ct_lds[];
-  uint16_t* rm = reinterpret_cast<uint16_t*>(ct_lds);
-  uint16_t* tr = rm + Tile::RM;
-  float* lz = reinterpret_cast<float*>(ct_lds + Tile::BYTES);      // z, or m2 with a bias
-  float* ll = lz + BN;                                             // l2s (bias)
-  float* lsg = ll + BN;                                            // sign of c, with the tile's scale undone (bias)
-  float* lg = lsg + BN;                                            // g times that sign
-  int32_t* ly = reinterpret_cast<int32_t*>(lg + BN);
-  uint32_t* lf = reinterpret_cast<uint32_t*>(ly + BN);             // sign words
-  uint32_t* lm = lf + BN;
+  float* lz0 = reinterpret_cast<float*>(ct_lds + 2 * Tile::BYTES); // [2][6][BN], see below
+  uint32_t* lm = reinterpret_cast<uint32_t*>(lz0 + 12 * BN);       // [2][NW] largest magnitudes
   int tile, split;
   ct_place(a.tiles, a.n_split, &tile, &split);
   const int wave = threadIdx.x >> 6, lane = rx_lane(), l31 = lane & 31, h = lane >> 5;
-  const int64_t item0 = ((int64_t)tile * CT_WAVES + wave) * (32 * MB);
+  const int64_t item0 = ((int64_t)tile * NW + wave) * (32 * MB);
   const int64_t r0 = split * a.per_split, r1 = r0 + a.per_split < a.R ? r0 + a.per_split : a.R;
-  CtStage<T, PL, DP, BN, true> stage;
+  const int n = (int)((r1 - r0 + BN - 1) / BN);             // tiles of this split, at least one
+  CtStage<T, PL, DP, BN, true, NW * 64> stage;
   CtRow info;
-  auto fetch = [&](int64_t r) {
+  auto fetch = [&](int i) {
+    const int64_t r = r0 + (int64_t)i * BN;
     stage.load((const T*)a.x, a.ld_x, r, r1, a.D, a.vec);
     if (threadIdx.x < BN) {
       if (r + threadIdx.x < r1) info = a.rows[r + threadIdx.x];
       else { info.m2 = 0.f; info.l2s = info.z = __builtin_inff(); info.sgn = 1.f; info.g = 0.f; info.y = -1; }
     }
   };
-  if (r0 < r1) fetch(r0);
+  auto publish = [&](int i) {      // before the barrier in front of put(i): the largest magnitude, the sign words
+    if constexpr (PL == 2) {
+      const uint32_t m = stage.peak();
+      if (lane == 0) lm[(i & 1) * NW + wave] = m;
+    }
+    if (threadIdx.x < BN) reinterpret_cast<uint32_t*>(lz0 + (i & 1) * 6 * BN)[5 * BN + threadIdx.x] = info.sgn < 0.f ? 0x80008000u : 0u;
+  };
+  auto put = [&](int i) -> float {
+    float scale = 1.f;
+    if constexpr (PL == 2) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) m = ct_umax(m, lm[(i & 1) * NW + w]);
+      scale = ct_scale(m);
+    }
+    const float kt = PL == 2 ? -ct_log2(scale) : 0.f;
+    float* lz = lz0 + (i & 1) * 6 * BN;
+    if (threadIdx.x < BN) {
+      float* p = lz + threadIdx.x;
+      p[0] = BIAS ? info.m2 : info.z - kt;
+      if (BIAS) { p[BN] = info.l2s - kt; p[2 * BN] = info.sgn * scale; }     // sign of c, with the tile's scale undone
+      p[3 * BN] = info.g * info.sgn;
+      reinterpret_cast<int32_t*>(p)[4 * BN] = info.y;
+    }
+    uint16_t* rm = reinterpret_cast<uint16_t*>(ct_lds + (i & 1) * Tile::BYTES);
+    stage.store(rm, rm + Tile::RM, reinterpret_cast<const uint32_t*>(lz + 5 * BN), scale);
+    return scale;
+  };
+  fetch(0);
   CtFrag st[MB][DP / 16][PL];
   float inv[MB], b2[MB], dbias[MB], ref[MB];      // ref: of w = 2^(log2 (|c| p) + kt - ref); PL == 1 keeps it at 0
 #pragma unroll
@@ -603,26 +700,25 @@ __global__ void __launch_bounds__(CT_THREADS, OCC) ct_bwd_kernel(CtBwd a) {
     ref[mb] = PL == 2 ? CT_NINF : 0.f;
   }
   ct_acc o[MB][DP / 32] = {};
-  for (int64_t r = r0; r < r1; r += BN) {
-    if constexpr (PL == 2) {
-      const uint32_t m = stage.peak();
-      if (lane == 0) lm[wave] = m;
+  publish(0);
+  __syncthreads();
+  float scale = put(0), next = 1.f;
+  if (n > 1) {
+    fetch(1);
+    publish(1);
+  }
+  __syncthreads();
+  for (int i = 0; i < n; ++i) {
+    if (i + 1 < n) {
+      next = put(i + 1);
+      if (i + 2 < n) fetch(i + 2);
     }
-    __syncthreads();
-    const float scale = PL == 2 ? ct_scale(ct_umax(ct_umax(lm[0], lm[1]), ct_umax(lm[2], lm[3]))) : 1.f;
-    const float kt = PL == 2 ? -ct_log2(scale) : 0.f;
-    if (threadIdx.x < BN) {
-      lz[threadIdx.x] = BIAS ? info.m2 : info.z - kt;
-      if (BIAS) { ll[threadIdx.x] = info.l2s - kt; lsg[threadIdx.x] = info.sgn * scale; }
-      lg[threadIdx.x] = info.g * info.sgn;
-      ly[threadIdx.x] = info.y;
-      lf[threadIdx.x] = info.sgn < 0.f ? 0x80008000u : 0u;
-    }
-    __syncthreads();
-    stage.store(rm, tr, lf, scale);
-    __syncthreads();
-    if (r + BN < r1) fetch(r + BN);
-    const float back = ct_inverse(scale);
+    const uint16_t* rm = reinterpret_cast<const uint16_t*>(ct_lds + (i & 1) * Tile::BYTES);
+    const uint16_t* tr = rm + Tile::RM;
+    const float* lz = lz0 + (i & 1) * 6 * BN;             // z, or m2 with a bias
+    const float *ll = lz + BN, *lsg = lz + 2 * BN, *lg = lz + 3 * BN;
+    const int32_t* ly = reinterpret_cast<const int32_t*>(lz + 4 * BN);
+    const float kt = PL == 2 ? -ct_log2(scale) : 0.f, back = ct_inverse(scale);
     // rows of this tile whose target is among the wavefront's items
     const int64_t rel = lane < BN && ly[lane] >= 0 ? ly[lane] - item0 : -1;
     const uint64_t hits = __ballot(rel >= 0 && rel < 32 * MB);
@@ -631,22 +727,22 @@ __global__ void __launch_bounds__(CT_THREADS, OCC) ct_bwd_kernel(CtBwd a) {
       const bool hit = (uint32_t)(hits >> (it * 32)) != 0;
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
-        const ct_acc s = ct_scores<PL, DP, BN, true>(rm, it, st[mb]);
+        const ct_acc s = ct_scores<PL, DP, BN>(rm, it, st[mb]);
         const float mul = PL == 2 ? inv[mb] * back : CT_L2E;
         float w[16], mx = CT_NINF;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int k = it * 32 + 8 * (i / 4) + 4 * h;
-          if constexpr (BIAS) w[i] = (fmaf(s[i], mul, b2[mb]) - ct_at(lz + k, i % 4)) - ct_at(ll + k, i % 4);
-          else w[i] = fmaf(s[i], mul, -ct_at(lz + k, i % 4));
-          if (PL == 2) mx = fmaxf(mx, w[i]);
+        for (int e = 0; e < 16; ++e) {
+          const int k = it * 32 + 8 * (e / 4) + 4 * h;
+          if constexpr (BIAS) w[e] = (fmaf(s[e], mul, b2[mb]) - ct_at(lz + k, e % 4)) - ct_at(ll + k, e % 4);
+          else w[e] = fmaf(s[e], mul, -ct_at(lz + k, e % 4));
+          if (PL == 2) mx = fmaxf(mx, w[e]);
         }
         const int64_t mine = item0 + mb * 32 + l31;
         if constexpr (PL == 2) {
           if (hit) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int k = it * 32 + 8 * (i / 4) + 4 * h + i % 4;
+            for (int e = 0; e < 16; ++e) {
+              const int k = it * 32 + 8 * (e / 4) + 4 * h + e % 4;
               if (ly[k] == mine) mx = fmaxf(mx, log2f(fabsf(lg[k])) + kt);
             }
           }
@@ -659,7 +755,7 @@ __global__ void __launch_bounds__(CT_THREADS, OCC) ct_bwd_kernel(CtBwd a) {
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) o[mb][db][i] *= f;
+                  for (int e = 0; e < 16; ++e) o[mb][db][e] *= f;
               }
               ref[mb] = n - CT_BASE(PL);
             }
@@ -667,31 +763,34 @@ __global__ void __launch_bounds__(CT_THREADS, OCC) ct_bwd_kernel(CtBwd a) {
         }
         const float rf = ref[mb] == CT_NINF ? 0.f : ref[mb];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = __builtin_amdgcn_exp2f(PL == 2 ? w[i] - rf : w[i]);
+        for (int e = 0; e < 16; ++e) w[e] = __builtin_amdgcn_exp2f(PL == 2 ? w[e] - rf : w[e]);
         if (hit) {                // the target's own share: sgn(c) g on top of |c| p, both still to meet sgn(c) x
           const float up = PL == 2 ? __builtin_amdgcn_exp2f(kt - rf) : 1.f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int k = it * 32 + 8 * (i / 4) + 4 * h + i % 4;
-            if (ly[k] == mine) w[i] = fmaf(lg[k], up, w[i]);
+          for (int e = 0; e < 16; ++e) {
+            const int k = it * 32 + 8 * (e / 4) + 4 * h + e % 4;
+            if (ly[k] == mine) w[e] = fmaf(lg[k], up, w[e]);
           }
         }
         if constexpr (BIAS) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) dbias[mb] = fmaf(w[i], ct_at(lsg + it * 32 + 8 * (i / 4) + 4 * h, i % 4), dbias[mb]);
+          for (int e = 0; e < 16; ++e) dbias[mb] = fmaf(w[e], ct_at(lsg + it * 32 + 8 * (e / 4) + 4 * h, e % 4), dbias[mb]);
         }
         ct_weigh<PL, DP, BN>(tr, it, w, o[mb]);
         if (PL == 1 && hit) {     // a target's share is as large as the whole gradient: what bf16 dropped of these weights goes in too
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const uint32_t u = ct_pk(w[i], w[i + 1]);
-            w[i] -= ct_lo(u);
-            w[i + 1] -= ct_hi(u);
+          for (int e = 0; e < 16; e += 2) {
+            const uint32_t u = ct_pk(w[e], w[e + 1]);
+            w[e] -= ct_lo(u);
+            w[e + 1] -= ct_hi(u);
           }
           ct_weigh<PL, DP, BN>(tr, it, w, o[mb]);
         }
       }
     }
+    if (i + 2 < n) publish(i);
+    scale = next;
+    __syncthreads();
   }
   if constexpr (PL == 2) {        // back from the references, in two steps: 2^ref alone may be below the smallest number
 #pragma unroll
@@ -755,10 +854,20 @@ __global__ void __launch_bounds__(CT_THREADS) ct_sum_kernel(const float* __restr
 
 // ---------------------------------------------------------------- host
 static int ct_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
-static int ct_mb(bool bf16, int dp) { return bf16 && dp <= 64 ? 2 : 1; }
-// two blocks with a bias do not fit the registers of two wavefronts per SIMD
-static int ct_bwd_mb(bool bf16, int dp, bool bias) { return bias && dp == 64 ? 1 : ct_mb(bf16, dp); }
-static int ct_bn(bool bf16, int dp) { return bf16 ? (dp <= 128 ? 64 : 32) : (dp <= 64 ? 64 : 32); }
+// X(T, PL, DP, MB, BN, NW, OCC): the kernels there are, one per element type and padded width
+#define CT_KERNELS(X, bf16, dp)                                                  \
+  (bf16 ? dp == 32 ? X(uint16_t, 1, 32, 2, 64, 4, 2)                             \
+          : dp == 64 ? X(uint16_t, 1, 64, 2, 64, 4, 2)                           \
+          : dp == 128 ? X(uint16_t, 1, 128, 1, 64, 4, 2)                         \
+                      : X(uint16_t, 1, 256, 1, 32, 4, 1)                         \
+   : dp == 32 ? X(float, 2, 32, 1, 64, CT_NW32, 2)                               \
+   : dp == 64 ? X(float, 2, 64, 1, 64, CT_NW64, 2)                               \
+   : dp == 128 ? X(float, 2, 128, 1, 32, 4, CT_OCC128)                           \
+               : X(float, 2, 256, 1, 32, 4, 1))
+
+// stationary vectors per workgroup and streaming ones per tile, of the kernels in CT_KERNELS
+#define CT_BM(T, PL, DP, MB, BN, NW, OCC) ((NW) * 32 * (MB))
+#define CT_BN(T, PL, DP, MB, BN, NW, OCC) (BN)
 
 struct CtPlan {
   int tiles, n_split;
@@ -799,11 +908,13 @@ static bool ct_vec(const rx_catalog_args* a) {      // 4-element loads
 
 static CtPlan ct_fwd_plan(int64_t R, int64_t V, int D, int bf16) {
   const int dp = ct_dp(D);
-  return ct_plan(R, V, CT_WAVES * 32 * ct_mb(bf16, dp), ct_bn(bf16, dp));
+  return ct_plan(R, V, CT_KERNELS(CT_BM, bf16, dp), CT_KERNELS(CT_BN, bf16, dp));
 }
 static CtPlan ct_bwd_plan(int64_t R, int64_t V, int D, int bf16, bool bias) {
   const int dp = ct_dp(D);
-  return ct_plan(V, R, CT_WAVES * 32 * ct_bwd_mb(bf16, dp, bias), ct_bn(bf16, dp));
+  // two blocks and a bias do not fit the registers of two wavefronts per SIMD: one there (ct_pick_bwd)
+  const int bm = CT_KERNELS(CT_BM, bf16, dp) / (bf16 && dp == 64 && bias ? 2 : 1);
+  return ct_plan(V, R, bm, CT_KERNELS(CT_BN, bf16, dp));
 }
 
 extern "C" size_t rx_catalog_fwd_workspace_bytes(int64_t R, int64_t V, int32_t D, int32_t bf16, int32_t want_mean) {
@@ -819,32 +930,35 @@ extern "C" size_t rx_catalog_bwd_workspace_bytes(int64_t R, int64_t V, int32_t D
 }
 
 
-template <typename T, int PL, int DP, int MB, int BN, bool MEAN, bool BIAS, int OCC>
+template <typename K>
+static int ct_allow_lds(K kernel, int bytes) {
+  if (bytes > 64 * 1024) RX_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  return 0;
+}
+template <typename T, int PL, int DP, int MB, int BN, int NW, int OCC, bool MEAN, bool BIAS>
 static int ct_go_fwd(const CtFwd& f, hipStream_t st) {
-  auto kernel = ct_fwd_kernel<T, PL, DP, MB, BN, MEAN, BIAS, OCC>;
-  const int lds = CtTile<PL, DP, BN, MEAN>::BYTES + BN * 4 + 16;
-  if (lds > 64 * 1024) RX_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(f.tiles * f.n_split)), dim3(CT_THREADS), lds, st, f);
+  auto kernel = ct_fwd_kernel<T, PL, DP, MB, BN, MEAN, BIAS, NW, OCC>;
+  const int lds = 2 * CtTile<PL, DP, BN, MEAN, NW * 64>::BYTES + 2 * BN * 4 + 2 * NW * 4;
+  if (ct_allow_lds(kernel, lds)) return 1;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(f.tiles * f.n_split)), dim3(NW * 64), lds, st, f);
   return 0;
 }
-template <typename T, int PL, int DP, int MB, int BN, int OCC>
+template <typename T, int PL, int DP, int MB, int BN, int NW, int OCC>
 static int ct_pick_fwd(const CtFwd& f, hipStream_t st) {
-  if (f.out) return f.bias ? ct_go_fwd<T, PL, DP, MB, BN, true, true, OCC>(f, st) : ct_go_fwd<T, PL, DP, MB, BN, true, false, OCC>(f, st);
-  return f.bias ? ct_go_fwd<T, PL, DP, MB, BN, false, true, OCC>(f, st) : ct_go_fwd<T, PL, DP, MB, BN, false, false, OCC>(f, st);
+  if (f.out) return f.bias ? ct_go_fwd<T, PL, DP, MB, BN, NW, OCC, true, true>(f, st) : ct_go_fwd<T, PL, DP, MB, BN, NW, OCC, true, false>(f, st);
+  return f.bias ? ct_go_fwd<T, PL, DP, MB, BN, NW, OCC, false, true>(f, st) : ct_go_fwd<T, PL, DP, MB, BN, NW, OCC, false, false>(f, st);
 }
-template <typename T, int PL, int DP, int MB, int BN, int OCC>
-static int ct_pick_bwd(const CtBwd& f, hipStream_t st) {
-  const int lds = CtTile<PL, DP, BN, true>::BYTES + 6 * BN * 4 + 16;
-  if (f.db) {
-    auto kernel = ct_bwd_kernel<T, PL, DP, DP == 64 ? 1 : MB, BN, true, OCC>;
-    if (lds > 64 * 1024) RX_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(f.tiles * f.n_split)), dim3(CT_THREADS), lds, st, f);
-  } else {
-    auto kernel = ct_bwd_kernel<T, PL, DP, MB, BN, false, OCC>;
-    if (lds > 64 * 1024) RX_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(f.tiles * f.n_split)), dim3(CT_THREADS), lds, st, f);
-  }
+template <typename T, int PL, int DP, int MB, int BN, int NW, int OCC, bool BIAS>
+static int ct_go_bwd(const CtBwd& f, hipStream_t st) {
+  auto kernel = ct_bwd_kernel<T, PL, DP, MB, BN, BIAS, NW, OCC>;
+  const int lds = 2 * CtTile<PL, DP, BN, true, NW * 64>::BYTES + 12 * BN * 4 + 2 * NW * 4;
+  if (ct_allow_lds(kernel, lds)) return 1;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(f.tiles * f.n_split)), dim3(NW * 64), lds, st, f);
   return 0;
+}
+template <typename T, int PL, int DP, int MB, int BN, int NW, int OCC>
+static int ct_pick_bwd(const CtBwd& f, hipStream_t st) {
+  return f.db ? ct_go_bwd<T, PL, DP, DP == 64 ? 1 : MB, BN, NW, OCC, true>(f, st) : ct_go_bwd<T, PL, DP, MB, BN, NW, OCC, false>(f, st);
 }
 
 extern "C" int rx_catalog_fwd(const rx_catalog_args* args, float* d_logprob, float* d_lse, float* d_stats, float* d_mean, void* ws,
@@ -862,22 +976,9 @@ extern "C" int rx_catalog_fwd(const rx_catalog_args* args, float* d_logprob, flo
   float* out = d_mean ? (float*)((uint8_t*)ws + rx_align_up((size_t)p.n_split * a.R * sizeof(float2), 256)) : nullptr;
   CtFwd f = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, a.D, p.tiles, p.n_split, p.per_split, ct_vec(&a), part, out};
   hipStream_t st = (hipStream_t)stream;
-  int rc;
-  if (a.bf16) {
-    switch (ct_dp(a.D)) {
-      case 32: rc = ct_pick_fwd<uint16_t, 1, 32, 2, 64, 2>(f, st); break;
-      case 64: rc = ct_pick_fwd<uint16_t, 1, 64, 2, 64, 2>(f, st); break;
-      case 128: rc = ct_pick_fwd<uint16_t, 1, 128, 1, 64, 2>(f, st); break;
-      default: rc = ct_pick_fwd<uint16_t, 1, 256, 1, 32, 1>(f, st);
-    }
-  } else {
-    switch (ct_dp(a.D)) {
-      case 32: rc = ct_pick_fwd<float, 2, 32, 1, 64, 2>(f, st); break;
-      case 64: rc = ct_pick_fwd<float, 2, 64, 1, 64, 2>(f, st); break;
-      case 128: rc = ct_pick_fwd<float, 2, 128, 1, 32, 1>(f, st); break;
-      default: rc = ct_pick_fwd<float, 2, 256, 1, 32, 1>(f, st);
-    }
-  }
+#define CT_GO(...) ct_pick_fwd<__VA_ARGS__>(f, st)
+  const int rc = CT_KERNELS(CT_GO, a.bf16, ct_dp(a.D));
+#undef CT_GO
   if (rc) return rc;
   RX_LAUNCH_CHECK();
   CtJoin j = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, a.targets, a.D, p.n_split, part, out, d_logprob, d_lse, d_stats, d_mean};
@@ -920,22 +1021,9 @@ extern "C" int rx_catalog_bwd(const rx_catalog_args* args, const float* d_stats,
   CtBwd f = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, rows, a.D, p.tiles, p.n_split, p.per_split, ct_vec(&a),
              partial ? (void*)pt : d_dtable, partial ? (d_dbias ? pb : nullptr) : d_dbias, partial};
   RX_REQUIRE(!a.bias || f.db, "rx_catalog_bwd: with a bias the table's gradient comes with the bias gradient");
-  int rc;
-  if (a.bf16) {
-    switch (ct_dp(a.D)) {
-      case 32: rc = ct_pick_bwd<uint16_t, 1, 32, 2, 64, 2>(f, st); break;
-      case 64: rc = ct_pick_bwd<uint16_t, 1, 64, 2, 64, 2>(f, st); break;
-      case 128: rc = ct_pick_bwd<uint16_t, 1, 128, 1, 64, 2>(f, st); break;
-      default: rc = ct_pick_bwd<uint16_t, 1, 256, 1, 32, 1>(f, st);
-    }
-  } else {
-    switch (ct_dp(a.D)) {
-      case 32: rc = ct_pick_bwd<float, 2, 32, 1, 64, 2>(f, st); break;
-      case 64: rc = ct_pick_bwd<float, 2, 64, 1, 64, 2>(f, st); break;
-      case 128: rc = ct_pick_bwd<float, 2, 128, 1, 32, 1>(f, st); break;
-      default: rc = ct_pick_bwd<float, 2, 256, 1, 32, 1>(f, st);
-    }
-  }
+#define CT_GO(...) ct_pick_bwd<__VA_ARGS__>(f, st)
+  const int rc = CT_KERNELS(CT_GO, a.bf16, ct_dp(a.D));
+#undef CT_GO
   if (rc) return rc;
   RX_LAUNCH_CHECK();
   if (partial) {
