@@ -13,6 +13,7 @@
 #include "rx_common.h"
 
 #define LP_SMALL 1024        // rows up to this width: one wavefront (or part of one) per row, scores in registers
+#define LP_WIDE 256          // threads per split of a wide row
 #define LP_TOP 64            // most alternatives per row
 #define LP_SPLIT_MIN 4096    // fewest columns worth a split of their own
 #define LP_SPLIT_MAX 256
@@ -20,6 +21,8 @@
 #define LP_LN2 0.69314718055994530942f
 #define LP_BIG 1e38f         // beyond this l * log2(e) leaves fp32: such rows take the form exp((l - m) log2 e)
 #define LP_NINF (-__builtin_inff())
+
+typedef uint32_t lp_u4 __attribute__((ext_vector_type(4)));
 
 struct LpPart {   // one split's share of a row
   float raw;      // largest score
@@ -35,13 +38,13 @@ template <> __device__ __forceinline__ float lp_elem<uint16_t>(const uint16_t* p
 template <typename T> struct LpVec { static constexpr int N = 16 / (int)sizeof(T); };
 
 template <typename T>
-__device__ __forceinline__ void lp_unpack(const uint4& q, float* v);
+__device__ __forceinline__ void lp_unpack(const lp_u4& q, float* v);
 template <>
-__device__ __forceinline__ void lp_unpack<float>(const uint4& q, float* v) {
+__device__ __forceinline__ void lp_unpack<float>(const lp_u4& q, float* v) {
   v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y); v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
 }
 template <>
-__device__ __forceinline__ void lp_unpack<uint16_t>(const uint4& q, float* v) {
+__device__ __forceinline__ void lp_unpack<uint16_t>(const lp_u4& q, float* v) {
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -59,6 +62,44 @@ template <typename T> __device__ __forceinline__ void lp_put(T* p, float f);
 template <> __device__ __forceinline__ void lp_put<float>(float* p, float f) { *p = f; }
 template <> __device__ __forceinline__ void lp_put<uint16_t>(uint16_t* p, float f) { *p = lp_to_bf16(f); }
 
+// of loaded values; fmaxf would quiet each of them first.  NaN loses against a number.
+__device__ __forceinline__ float lp_max3(float a, float b, float c) {
+  float d;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
+// value of lane ^ M without going through LDS: quad permutes, row mirrors and rotations, and the swaps of 16 and 32 lanes
+template <int M>
+__device__ __forceinline__ uint32_t lp_xor(uint32_t x) {
+#define LP_DPP(v, c) (uint32_t)__builtin_amdgcn_mov_dpp((int)(v), c, 0xf, 0xf, true)
+  if constexpr (M == 1) return LP_DPP(x, 0xB1);                     // quad_perm 1,0,3,2
+  else if constexpr (M == 2) return LP_DPP(x, 0x4E);                // quad_perm 2,3,0,1
+  else if constexpr (M == 4) return LP_DPP(LP_DPP(x, 0x141), 0x1B); // half row mirrored (^ 7), quads reversed (^ 3)
+  else if constexpr (M == 8) return LP_DPP(x, 0x128);               // row rotated by 8
+  else if constexpr (M == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return (rx_lane() & 16) ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return (rx_lane() & 32) ? r[0] : r[1];
+  }
+#undef LP_DPP
+}
+template <int M>
+__device__ __forceinline__ float lp_xorf(float v) { return __uint_as_float(lp_xor<M>(__float_as_uint(v))); }
+// largest / sum over G neighbouring lanes, in each of them
+template <int G>
+__device__ __forceinline__ float lp_max(float v) {
+  if constexpr (G > 1) {
+    const float o = lp_xorf<G / 2>(v);
+    return lp_max<G / 2>(lp_max3(v, o, o));
+  } else return v;
+}
+template <int G>
+__device__ __forceinline__ float lp_sum(float v) {
+  if constexpr (G > 1) return lp_sum<G / 2>(v + lp_xorf<G / 2>(v));
+  else return v;
+}
 __device__ __forceinline__ float lp_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ---------------------------------------------------------------- alternatives
@@ -72,38 +113,50 @@ __device__ __forceinline__ float lp_key_value(uint64_t key) {
   const uint32_t o = (uint32_t)(key >> 32);
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
+// the next smaller score (of a finite one or +inf)
+__device__ __forceinline__ float lp_below(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return __uint_as_float(v > 0.f ? u - 1 : v < 0.f ? u + 1 : 0x80000001u);
+}
 __device__ __forceinline__ int32_t lp_key_col(uint64_t key) { return (int32_t)~(uint32_t)key; }
 // key 0 is no score's key: value bits 0 would be the image of a negative NaN
 
-__device__ __forceinline__ uint64_t lp_shfl_xor64(uint64_t x, int m) {
-  const uint32_t lo = __shfl_xor((uint32_t)x, m, 64), hi = __shfl_xor((uint32_t)(x >> 32), m, 64);
-  return ((uint64_t)hi << 32) | lo;
+template <int M>
+__device__ __forceinline__ uint64_t lp_xor64(uint64_t x) {
+  return ((uint64_t)lp_xor<M>((uint32_t)(x >> 32)) << 32) | lp_xor<M>((uint32_t)x);
+}
+// compare-exchange with lane ^ ST: lanes with `small` keep the smaller key
+template <int ST>
+__device__ __forceinline__ uint64_t lp_exchange(uint64_t x, bool small) {
+  const uint64_t o = lp_xor64<ST>(x);
+  return ((x < o) == small) ? x : o;
+}
+template <int SIZE, int ST>
+__device__ __forceinline__ uint64_t lp_stage(uint64_t x) {
+  const int lane = rx_lane();
+  const bool up = SIZE == 64 || (lane & SIZE) == 0, low = (lane & ST) == 0;
+  x = lp_exchange<ST>(x, up == low);
+  if constexpr (ST > 1) return lp_stage<SIZE, ST / 2>(x);
+  else return x;
 }
 // keys of the wavefront's lanes in ascending lane order (bitonic network, 21 compare-exchange steps)
 __device__ __forceinline__ uint64_t lp_sort_up(uint64_t x) {
-  const int lane = rx_lane();
-#pragma unroll
-  for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-    for (int st = size >> 1; st > 0; st >>= 1) {
-      const uint64_t o = lp_shfl_xor64(x, st);
-      const bool up = (lane & size) == 0 || size == 64;
-      const bool low = (lane & st) == 0;
-      x = ((x < o) == (up == low)) ? x : o;
-    }
-  return x;
+  x = lp_stage<2, 1>(x);
+  x = lp_stage<4, 2>(x);
+  x = lp_stage<8, 4>(x);
+  x = lp_stage<16, 8>(x);
+  x = lp_stage<32, 16>(x);
+  return lp_stage<64, 32>(x);
 }
 // best 64 of `list` (descending over the lanes) and `cand` (ascending), descending
+template <int ST>
+__device__ __forceinline__ uint64_t lp_down(uint64_t x) {
+  x = lp_exchange<ST>(x, (rx_lane() & ST) != 0);
+  if constexpr (ST > 1) return lp_down<ST / 2>(x);
+  else return x;
+}
 __device__ __forceinline__ uint64_t lp_merge(uint64_t list, uint64_t cand) {
-  const int lane = rx_lane();
-  uint64_t x = list > cand ? list : cand;
-#pragma unroll
-  for (int st = 32; st > 0; st >>= 1) {
-    const uint64_t o = lp_shfl_xor64(x, st);
-    const bool low = (lane & st) == 0;
-    x = ((x > o) == low) ? x : o;
-  }
-  return x;
+  return lp_down<32>(list > cand ? list : cand);
 }
 __device__ __forceinline__ uint64_t lp_lane64(uint64_t x, int lane) {
   const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, lane), hi = __builtin_amdgcn_readlane((uint32_t)(x >> 32), lane);
@@ -217,8 +270,7 @@ lp_small_kernel(rx_logprob_args a, int32_t* err) {
     v[q] = c < n ? lp_elem(l + c) : LP_NINF;
     m = fmaxf(m, v[q]);
   }
-#pragma unroll
-  for (int x = G >> 1; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+  m = lp_max<G>(m);
   const float ref = m == LP_NINF ? 0.f : m;
   float s = 0.f, t = 0.f;
 #pragma unroll
@@ -227,8 +279,8 @@ lp_small_kernel(rx_logprob_args a, int32_t* err) {
     s += e;
     t = fmaf(e, fmaxf(d, -1e4f), t);             // a masked score: e = 0 times a finite number
   }
-#pragma unroll
-  for (int x = G >> 1; x > 0; x >>= 1) { s += __shfl_xor(s, x, 64); t += __shfl_xor(t, x, 64); }
+  s = lp_sum<G>(s);
+  t = lp_sum<G>(t);
   // the reference is the score itself here, as for rows beyond LP_BIG
   LpRow r = lp_finish(m, ref, s, t);
   r.big = true;
@@ -237,6 +289,31 @@ lp_small_kernel(rx_logprob_args a, int32_t* err) {
   if (on)
     for (int q = sub; q < a.T; q += G) lp_write_target<T>(a, r, l, n, row, q, err);
   if constexpr (TOP) {
+    // A round takes the largest score left and its lowest column: about 15 + 3 PER instructions, against 400 for sorting
+    // and merging 64 keys.
+    if (a.k * (15 + 3 * PER) <= 400 * PER) {
+      uint64_t mine = 0;
+      for (int j = 0; j < a.k; ++j) {
+        float best = v[0];
+#pragma unroll
+        for (int q = 1; q < PER; ++q) best = lp_max3(best, v[q], v[q]);
+        best = lp_max<64>(best);
+        if (!(best > LP_NINF)) break;
+        int32_t col = -1;
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+          const uint64_t at = __ballot(v[q] == best);
+          if (col < 0 && at) {
+            const int ln = __builtin_ctzll(at);
+            col = q * 64 + ln;
+            if (rx_lane() == ln) v[q] = LP_NINF;
+          }
+        }
+        if (rx_lane() == j) mine = lp_key(best, col);
+      }
+      if (sub < a.k) lp_write_top(a, r, row, sub, mine);
+      return;
+    }
     LpTop top;
     top.init(tops[threadIdx.x >> 6]);
 #pragma unroll
@@ -266,10 +343,11 @@ struct LpAcc {
   }
   template <int N>
   __device__ __forceinline__ float add(const float* v) {     // returns the largest of v
-    float mx = v[0];
+    float mx = lp_max3(v[0], v[1], v[2]);
 #pragma unroll
-    for (int i = 1; i < N; ++i) mx = fmaxf(mx, v[i]);
-    raw = fmaxf(raw, mx);
+    for (int i = 3; i + 1 < N; i += 2) mx = lp_max3(mx, v[i], v[i + 1]);
+    mx = lp_max3(mx, v[N - 1], v[N - 1]);
+    raw = lp_max3(raw, mx, mx);
     const float n2 = mx * LP_L2E;
     const bool grow = n2 > m2 + 4.f;
     if (__ballot(grow)) {
@@ -305,8 +383,10 @@ __device__ __forceinline__ void lp_frame(const T* l, int32_t n, int32_t* head, i
   *nvec = (n - *head) / LpVec<T>::N;
 }
 
-// Calls f(v[N], first column of the lane, n valid...) over this wavefront's share of the columns [part of row], in
-// ascending groups: every column of one call is lower than every column of the next.
+// Calls f(v[2 N], column of v[0]) over this wavefront's share of the columns [part of row], in ascending groups: every
+// column of one call is lower than every column of the next.  v[N] .. are LP_NEXT(T) columns further on.  A call's
+// 32 bytes per lane are loaded one call ahead.
+#define LP_NEXT(T) (64 * LpVec<T>::N)
 template <typename T, typename F>
 __device__ __forceinline__ void lp_stream(const T* l, int32_t n, int split, int n_split, F f) {
   constexpr int N = LpVec<T>::N;
@@ -314,32 +394,43 @@ __device__ __forceinline__ void lp_stream(const T* l, int32_t n, int split, int 
   lp_frame(l, n, &head, &nvec);
   const int lane = rx_lane(), wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const bool first = split == 0 && wave == 0;
+  float v[2 * N];
   if (first && head) {
-    float v[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = LP_NINF;
+    for (int i = 0; i < 2 * N; ++i) v[i] = LP_NINF;
     if (lane < head) v[0] = lp_elem(l + lane);
     f(v, lane);
   }
   const int32_t chunk = (nvec + n_split - 1) / n_split;
   const int32_t lo = split * chunk < nvec ? split * chunk : nvec;
   const int32_t hi = lo + chunk < nvec ? lo + chunk : nvec;
-  const uint4* p = reinterpret_cast<const uint4*>(l + head);
-  for (int32_t b = lo + wave * 64; b < hi; b += waves * 64) {
-    const int32_t q = b + lane;
-    float v[N];
-    if (q < hi) lp_unpack<T>(p[q], v);
-    else {
+  const lp_u4* p = reinterpret_cast<const lp_u4*>(l + head);
+  lp_u4 q0 = {}, q1 = {};
+  int32_t b = lo + wave * 128;
+  if (b + lane < hi) q0 = p[b + lane];
+  if (b + 64 + lane < hi) q1 = p[b + 64 + lane];
+  for (; b < hi; b += waves * 128) {
+    const int32_t c = b + waves * 128;
+    lp_u4 n0 = {}, n1 = {};
+    if (c + lane < hi) n0 = p[c + lane];
+    if (c + 64 + lane < hi) n1 = p[c + 64 + lane];
+    lp_unpack<T>(q0, v);
+    lp_unpack<T>(q1, v + N);
+    if (b + 128 > hi) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = LP_NINF;
+      for (int i = 0; i < N; ++i) {
+        if (b + lane >= hi) v[i] = LP_NINF;
+        if (b + 64 + lane >= hi) v[N + i] = LP_NINF;
+      }
     }
-    f(v, head + q * N);
+    f(v, head + (b + lane) * N);
+    q0 = n0;
+    q1 = n1;
   }
   const int32_t tail = head + nvec * N;
   if (first && tail < n) {
-    float v[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = LP_NINF;
+    for (int i = 0; i < 2 * N; ++i) v[i] = LP_NINF;
     if (lane < n - tail) v[0] = lp_elem(l + tail + lane);
     f(v, tail + lane);
   }
@@ -383,7 +474,18 @@ __device__ __forceinline__ void lp_join(LpPart& x, const LpPart& y) {
   scaled(y, m, &s1, &t1);
   x.raw = raw; x.m2 = m; x.s = s0 + s1; x.t = t0 + t1;
 }
-__device__ __forceinline__ LpPart lp_wave_join(LpPart p) {
+// Joins the lanes' shares.  `big`: uniform, some share is relative to a score beyond LP_BIG.
+__device__ __forceinline__ LpPart lp_wave_join(LpPart p, bool big) {
+  if (!big) {
+    const float raw = lp_max<64>(p.raw), m = lp_max<64>(p.m2);
+    const bool none = p.m2 == LP_NINF;           // s is 0, or NaN
+    const float d = none ? 0.f : p.m2 - m, f = none ? 1.f : lp_exp2(d);
+    p.t = lp_sum<64>((p.t + p.s * d) * f);
+    p.s = lp_sum<64>(p.s * f);
+    p.raw = raw;
+    p.m2 = m;
+    return p;
+  }
   for (int x = 32; x > 0; x >>= 1) {
     LpPart o;
     o.raw = __shfl_xor(p.raw, x, 64); o.m2 = __shfl_xor(p.m2, x, 64);
@@ -395,9 +497,9 @@ __device__ __forceinline__ LpPart lp_wave_join(LpPart p) {
 }
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(RX_BLOCK)
+__global__ void __launch_bounds__(LP_WIDE)
 lp_wide_kernel(rx_logprob_args a, LpPart* parts, uint64_t* lists, int n_split, int32_t* err) {
-  constexpr int N = LpVec<T>::N, W = RX_BLOCK / 64;
+  constexpr int N = LpVec<T>::N, W = LP_WIDE / 64;
   __shared__ LpPart sh[W];
   __shared__ uint64_t tops[TOP ? W : 1][TOP ? 128 : 1];
   const int64_t row = blockIdx.x / n_split;
@@ -410,32 +512,39 @@ lp_wide_kernel(rx_logprob_args a, LpPart* parts, uint64_t* lists, int n_split, i
   LpTop top;
   if constexpr (TOP) top.init(tops[wave]);
   lp_stream<T>(l, n, split, n_split, [&](const float* v, int32_t col) {
-    const float mx = acc.add<N>(v);
+    const float mx = acc.add<2 * N>(v);
     if constexpr (TOP) {
       if (__ballot(mx > top.thr)) {
+        // no list yet: k lanes hold a score that large, so only scores from the k-th largest lane maximum up can be in it
+        float lim = top.thr;
+        if (lim == LP_NINF) {
+          const uint64_t kth = lp_lane64(lp_sort_up(mx > LP_NINF ? lp_key(mx, 0) : 0), 64 - a.k);
+          if (kth) lim = lp_below(lp_key_value(kth));
+        }
 #pragma unroll
-        for (int i = 0; i < N; ++i) top.push(v[i] > top.thr, lp_key(v[i], col + i));
+        for (int i = 0; i < 2 * N; ++i) top.push(v[i] > lim, lp_key(v[i], col + (i < N ? i : LP_NEXT(T) + i - N)));
         top.refresh(a.k);
       }
     }
   });
   // the largest score of the workgroup decides, uniformly, whether the sums have to be taken again
-  float raw = acc.raw;
-  for (int x = 32; x > 0; x >>= 1) raw = fmaxf(raw, __shfl_xor(raw, x, 64));
+  float raw = lp_max<64>(acc.raw);
   if (lane == 0) sh[wave].raw = raw;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < W; ++w) raw = fmaxf(raw, sh[w].raw);
   __syncthreads();
   LpPart p;
-  if (fabsf(raw) > LP_BIG && fabsf(raw) < __builtin_inff()) {
+  const bool big = fabsf(raw) > LP_BIG && fabsf(raw) < __builtin_inff();
+  if (big) {
     acc.s = 0.f; acc.t = 0.f;
-    lp_stream<T>(l, n, split, n_split, [&](const float* v, int32_t) { acc.add_big<N>(v, raw); });
+    lp_stream<T>(l, n, split, n_split, [&](const float* v, int32_t) { acc.add_big<2 * N>(v, raw); });
     p.raw = raw; p.m2 = raw; p.s = acc.s; p.t = acc.t;
   } else {
     p.raw = acc.raw; p.m2 = acc.m2; p.s = acc.s; p.t = acc.t;
   }
-  p = lp_wave_join(p);
+  // a lane may have seen nothing but such scores under an ordinary maximum elsewhere: its sums are 0 then
+  p = lp_wave_join(p, false);
   if (lane == 0) sh[wave] = p;
   if constexpr (TOP) {
     top.flush();
@@ -458,20 +567,20 @@ lp_wide_kernel(rx_logprob_args a, LpPart* parts, uint64_t* lists, int n_split, i
   }
   const LpRow r = lp_finish(p.raw, p.m2, p.s, p.t);
   if (threadIdx.x == 0) lp_write_row(a, r, row);
-  for (int t = threadIdx.x; t < a.T; t += RX_BLOCK) lp_write_target<T>(a, r, l, n, row, t, err);
+  for (int t = threadIdx.x; t < a.T; t += LP_WIDE) lp_write_target<T>(a, r, l, n, row, t, err);
   if constexpr (TOP) {
     if (wave == 0 && lane < a.k) lp_write_top(a, r, row, lane, top.list);
   }
 }
 
-// One workgroup per row joins the splits.  A list's k-th key bounds the row's k-th key from below, so the largest of
-// them filters the candidates before anything is merged.
+// One workgroup per row joins the splits.  The k-th largest of the lists' first keys bounds the row's k-th key from
+// below (k lists have a key at least that large), which leaves about k of the n_split k candidates to be merged.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(RX_BLOCK)
 lp_join_kernel(rx_logprob_args a, const LpPart* parts, const uint64_t* lists, int n_split, int32_t* err) {
   constexpr int W = RX_BLOCK / 64;
   __shared__ LpPart sh[W];
-  __shared__ uint64_t bound[W];
+  __shared__ uint64_t heads[W][64];
   __shared__ uint64_t tops[TOP ? W : 1][TOP ? 128 : 1];
   const int64_t row = blockIdx.x;
   const int wave = threadIdx.x >> 6, lane = rx_lane();
@@ -480,12 +589,10 @@ lp_join_kernel(rx_logprob_args a, const LpPart* parts, const uint64_t* lists, in
   LpPart p;
   p.raw = LP_NINF; p.m2 = LP_NINF; p.s = 0.f; p.t = 0.f;
   if ((int)threadIdx.x < n_split) p = parts[row * n_split + threadIdx.x];
-  p = lp_wave_join(p);
+  p = lp_wave_join(p, __ballot(fabsf(p.raw) > LP_BIG && p.raw != LP_NINF) != 0);
   if (lane == 0) sh[wave] = p;
   if constexpr (TOP) {
-    uint64_t th = (int)threadIdx.x < n_split ? lists[(row * n_split + threadIdx.x) * a.k + a.k - 1] : 0;
-    for (int x = 32; x > 0; x >>= 1) { const uint64_t o = lp_shfl_xor64(th, x); th = th > o ? th : o; }
-    if (lane == 0) bound[wave] = th;
+    heads[wave][lane] = lp_sort_up((int)threadIdx.x < n_split ? lists[(row * n_split + threadIdx.x) * a.k] : 0);
   }
   __syncthreads();
   p = sh[0];
@@ -495,16 +602,18 @@ lp_join_kernel(rx_logprob_args a, const LpPart* parts, const uint64_t* lists, in
   if (threadIdx.x == 0) lp_write_row(a, r, row);
   for (int t = threadIdx.x; t < a.T; t += RX_BLOCK) lp_write_target<T>(a, r, l, n, row, t, err);
   if constexpr (TOP) {
-    uint64_t th = bound[0];
-#pragma unroll
-    for (int w = 1; w < W; ++w) th = th > bound[w] ? th : bound[w];
+    uint64_t best = heads[0][63 - lane];
+    for (int w = 1; w < W; ++w) best = lp_merge(best, heads[w][lane]);
+    const uint64_t th = lp_lane64(best, a.k - 1);            // 0 while there are fewer than k lists
     LpTop top;
     top.init(tops[wave]);
-    const int total = n_split * a.k;
-    const uint64_t* mine = lists + row * n_split * (int64_t)a.k;
-    for (int b = wave * 64; b < total; b += RX_BLOCK) {
-      const uint64_t key = b + lane < total ? mine[b + lane] : 0;
-      top.push(key != 0 && key >= th, key);
+    // a lane per list, which is sorted: down to the first key below the bound
+    const uint64_t* mine = lists + (row * n_split + threadIdx.x) * (int64_t)a.k;
+    bool more = (int)threadIdx.x < n_split;
+    for (int j = 0; j < a.k && __ballot(more); ++j) {
+      const uint64_t key = more ? mine[j] : 0;
+      more = key != 0 && key >= th;
+      top.push(more, key);
     }
     top.flush();
     tops[wave][lane] = top.list;
@@ -579,8 +688,7 @@ lp_bwd_small_kernel(rx_logprob_args a, const float* __restrict__ g, const float*
       int64_t y;
       if (lp_target_on(a, l, n, row, t, &y)) gs += g[row * a.T + t];
     }
-#pragma unroll
-  for (int x = G >> 1; x > 0; x >>= 1) gs += __shfl_xor(gs, x, 64);
+  gs = lp_sum<G>(gs);
   if (!on) return;
   const LpGrad r = lp_grad_row(a, gh, gl, gs, row);
   float v[PER];
@@ -638,7 +746,7 @@ lp_bwd_wide_kernel(rx_logprob_args a, const float* __restrict__ g, const float* 
     const int32_t c = head + q * N;
     float v[N];
     if (c + N <= n && !r.dead) {
-      if (same) lp_unpack<T>(*reinterpret_cast<const uint4*>(l + c), v);
+      if (same) lp_unpack<T>(*reinterpret_cast<const lp_u4*>(l + c), v);
       else {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = lp_elem(l + c + i);
@@ -733,12 +841,12 @@ static void lp_launch_fwd(const rx_logprob_args& a, void* ws, int32_t* err, hipS
   const int n = lp_splits(a.R, a.V);
   LpPart* parts = (LpPart*)ws;
   uint64_t* lists = (uint64_t*)(parts + (n > 1 ? a.R * n : 0));
-  const dim3 grid((unsigned)(a.R * n)), blk(RX_BLOCK);
+  const dim3 grid((unsigned)(a.R * n)), blk(RX_BLOCK), wide(LP_WIDE);
   if (a.k) {
-    hipLaunchKernelGGL((lp_wide_kernel<T, true>), grid, blk, 0, st, a, parts, lists, n, err);
+    hipLaunchKernelGGL((lp_wide_kernel<T, true>), grid, wide, 0, st, a, parts, lists, n, err);
     if (n > 1) hipLaunchKernelGGL((lp_join_kernel<T, true>), dim3((unsigned)a.R), blk, 0, st, a, parts, lists, n, err);
   } else {
-    hipLaunchKernelGGL((lp_wide_kernel<T, false>), grid, blk, 0, st, a, parts, lists, n, err);
+    hipLaunchKernelGGL((lp_wide_kernel<T, false>), grid, wide, 0, st, a, parts, lists, n, err);
     if (n > 1) hipLaunchKernelGGL((lp_join_kernel<T, false>), dim3((unsigned)a.R), blk, 0, st, a, parts, lists, n, err);
   }
 }
