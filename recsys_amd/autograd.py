@@ -1060,7 +1060,10 @@ def log_probs(logits: Tensor, targets: Tensor, lengths: Optional[Tensor] = None,
     ``lse`` are differentiable."""
     if logits.dim() == 2 and ((logits.shape[1] > 1 and logits.stride(1) != 1) or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1])):
         logits = logits.contiguous()
-    return ops.LogProbs(*LogProb.apply(logits, targets.contiguous(), None if lengths is None else lengths.contiguous(), k))
+    targets, lengths = targets.contiguous(), None if lengths is None else lengths.contiguous()
+    if not (logits.requires_grad and torch.is_grad_enabled()):
+        return ops.logprob_fwd(logits, targets, lengths, k)[0]
+    return ops.LogProbs(*LogProb.apply(logits, targets, lengths, k))
 
 
 class MeanNLL(Function):
@@ -1154,4 +1157,7 @@ def catalog_logprob(x: Tensor, table: Tensor, targets: Tensor, bias: Optional[Te
     takes its step, on every row)."""
     if x.dim() == 2 and ((x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
         x = x.contiguous()
-    return CatalogLogProb.apply(x, table, targets.contiguous(), bias)
+    targets = targets.contiguous()
+    if not (torch.is_grad_enabled() and (x.requires_grad or table.requires_grad or (bias is not None and bias.requires_grad))):
+        return ops.catalog_fwd(x, table, targets, bias)[:2]
+    return CatalogLogProb.apply(x, table, targets, bias)

@@ -61,7 +61,12 @@ def _after_index_op(device) -> None:
 
 
 # ------------------------------------------------------------------ small helpers
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # the handle without a Stream object around it: 0.2 against 2 us
+
+
 def _stream(t: Tensor):
+    if _raw_stream is not None:
+        return C.c_void_p(_raw_stream(_dev(t)))
     return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
