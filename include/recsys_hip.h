@@ -846,6 +846,7 @@ int rx_catalog_bwd(const rx_catalog_args* args, const float* d_stats, const floa
  *   A = X X^T,  X <- a X + (b A + c A A) X      (on G^T when rows > cols)
  * which drives the singular values of G towards 1 and leaves its singular vectors.  Products to fp32 accuracy.
  * At most RX_ORTHO_MAX matrices per call, none empty, rows and cols up to 16384.  A matrix of zeros gives zeros.
+ * Coefficients under which singular values in [0, 1] grow past 16 within the steps are refused.
  * The dense half of a train step (the reference steps every tower with Adam, recsys/pipelines/neuralcf/neumf.py:10). */
 #define RX_ORTHO_MAX 24
 typedef struct {

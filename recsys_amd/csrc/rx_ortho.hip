@@ -3,18 +3,22 @@
 //
 // The products take all the time: m^2 n + m^3 + 2 m^2 n operations per step, A and A A being symmetric (only tiles on and
 // below the diagonal are computed, the others are their mirror images).  Small singular values grow by up to a^steps = 485,
-// and so do rounding errors along them: bf16 products would leave errors of the size of the result there, so the products
+// and so do rounding errors along them: 16-bit products would leave errors of the size of the result there, so the products
 // keep fp32 accuracy.
 //   * Matrices that fit one workgroup's LDS take all steps in one launch, on fp32 matrix instructions: such lists are
 //     bound by launches, not by products.
-//   * The others share three launches per step, whatever their number.  X, X^T, A and B live in the workspace as three
-//     bf16 planes each (8 + 8 + 8 significant bits), cut once in the epilogue that makes them; six plane products give
-//     fp32 accuracy at 1/6 of the bf16 rate where fp32 matrix instructions have 1/16.  With X^T kept beside X
-//     all three products read both operands along the contraction.
+//   * The others share three launches per step, whatever their number.  X, X^T, A and B live in the workspace as two
+//     fp16 planes each (11 + 11 significant bits), cut once in the epilogue that makes them; high high + high low + low high
+//     gives fp32 accuracy (what is left out is below 2^-24 of a term) at a third of the 16-bit rate, where fp32 matrix
+//     instructions have a sixteenth.  fp16 lacks range, but the iteration does not use it: |X|_2 <= 1 at the start and the
+//     coefficients bound it from there on, so each array has one power-of-two scale that takes its bound to 2^15, found
+//     on the host.  With X^T kept beside X all three products read both operands along the contraction.
 #include "rx_common.h"
 
-typedef __bf16 ns_h8 __attribute__((ext_vector_type(8)));
-typedef __bf16 ns_h2 __attribute__((ext_vector_type(2)));
+#include <math.h>
+
+typedef _Float16 ns_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 ns_h2 __attribute__((ext_vector_type(2)));
 typedef float ns_f2 __attribute__((ext_vector_type(2)));
 typedef float ns_f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t ns_u4 __attribute__((ext_vector_type(4)));   // HIP's uint4 kept the prefetch registers in scratch
@@ -166,8 +170,8 @@ struct NsMat {
   float *out, *mom, *w;
   int32_t rows, cols;          // as given
   int32_t m, n, mp, np;        // working shape, and padded to the tile
-  uint16_t *x[2], *xt[2];      // [3][mp][np], [3][np][mp], alternating by step
-  uint16_t *A, *B;             // [3][mp][mp]
+  uint16_t *x[2], *xt[2];      // [2][mp][np], [2][np][mp], alternating by step
+  uint16_t *A, *B;             // [2][mp][mp]
   int32_t tiles_sym, tiles_x;
   float alpha;
 };
@@ -175,26 +179,29 @@ struct NsList {
   NsMat mat[RX_ORTHO_MAX];
   int32_t count, steps, tile, nesterov;
   float a, b, c, eps, mu;
+  float sx, sa, sb;            // scales of the X, A and B planes
   const float* scale;
   double* parts;               // [count][NS_PARTS]
 };
 
-__device__ __forceinline__ uint32_t ns_pk(float a, float b) {
-  ns_f2 v = {a, b};
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, ns_h2));
-}
-__device__ __forceinline__ float ns_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float ns_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// two values times a scale -> their words in the two planes
 __device__ __forceinline__ void ns_cut2(float a, float b, uint32_t* w) {
-#pragma unroll
-  for (int p = 0; p < 3; ++p) {
-    w[p] = ns_pk(a, b);
-    a -= ns_lo(w[p]);
-    b -= ns_hi(w[p]);
-  }
+  ns_f2 v = {a, b};
+  const ns_h2 h = __builtin_convertvector(v, ns_h2);
+  ns_f2 r = {a - (float)h.x, b - (float)h.y};
+  w[0] = __builtin_bit_cast(uint32_t, h);
+  w[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, ns_h2));
 }
-__device__ __forceinline__ float ns_join(const uint16_t* p, int64_t plane, int64_t at) {
-  return (__uint_as_float((uint32_t)p[2 * plane + at] << 16) + __uint_as_float((uint32_t)p[plane + at] << 16)) + __uint_as_float((uint32_t)p[at] << 16);
+// four neighbouring values from their planes
+__device__ __forceinline__ void ns_join4(const uint16_t* p, int64_t plane, float* v) {
+  const uint2 hi = *reinterpret_cast<const uint2*>(p), lo = *reinterpret_cast<const uint2*>(p + plane);
+  const uint32_t h[2] = {hi.x, hi.y}, l[2] = {lo.x, lo.y};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const ns_h2 a = __builtin_bit_cast(ns_h2, h[i]), b = __builtin_bit_cast(ns_h2, l[i]);
+    v[2 * i] = (float)a.x + (float)b.x;
+    v[2 * i + 1] = (float)a.y + (float)b.y;
+  }
 }
 
 __global__ void __launch_bounds__(RX_BLOCK) ns_norm_kernel(NsList a) {
@@ -258,23 +265,23 @@ __global__ void __launch_bounds__(RX_BLOCK) ns_init_kernel(NsList a) {
   const int64_t plane = (int64_t)t.mp * t.np;
   for (int i = threadIdx.x; i < 64 * 32; i += RX_BLOCK) {
     const int y = i / 32, x = i % 32 * 2;
-    uint32_t w[3];
-    ns_cut2(tl[y][x], tl[y][x + 1], w);
+    uint32_t w[2];
+    ns_cut2(tl[y][x] * a.sx, tl[y][x + 1] * a.sx, w);
 #pragma unroll
-    for (int p = 0; p < 3; ++p) *reinterpret_cast<uint32_t*>(t.x[0] + p * plane + (int64_t)(r0 + y) * t.np + c0 + x) = w[p];
-    ns_cut2(tl[x][y], tl[x + 1][y], w);
+    for (int p = 0; p < 2; ++p) *reinterpret_cast<uint32_t*>(t.x[0] + p * plane + (int64_t)(r0 + y) * t.np + c0 + x) = w[p];
+    ns_cut2(tl[x][y] * a.sx, tl[x + 1][y] * a.sx, w);
 #pragma unroll
-    for (int p = 0; p < 3; ++p) *reinterpret_cast<uint32_t*>(t.xt[0] + p * plane + (int64_t)(c0 + y) * t.mp + r0 + x) = w[p];
+    for (int p = 0; p < 2; ++p) *reinterpret_cast<uint32_t*>(t.xt[0] + p * plane + (int64_t)(c0 + y) * t.mp + r0 + x) = w[p];
   }
 }
 
-// One T x T tile of P Q^T from planes P [3][.][K], Q [3][.][K]: four wavefronts, (T / 2)^2 each.
-#define NS_BK 32
-#define NS_LDK (NS_BK + 8)
+// One T x T tile of P Q^T from planes P [2][.][K], Q [2][.][K]: four wavefronts, (T / 2)^2 each, BK of the contraction per
+// step.  Rows in LDS are an odd multiple of 16 bytes apart.
 template <int T>
 struct NsTile {
   static constexpr int NB = T / 64;
-  static constexpr int CH = 2 * 3 * T * (NS_BK / 8) / RX_BLOCK;       // 16-byte chunks per thread and step
+  static constexpr int BK = T == 64 ? 64 : 32, LDK = BK + 8;
+  static constexpr int CH = 4 * T * (BK / 8) / RX_BLOCK;              // 16-byte chunks per thread and step
 };
 
 enum { NS_MODE_A, NS_MODE_B, NS_MODE_X };
@@ -282,10 +289,11 @@ enum { NS_MODE_A, NS_MODE_B, NS_MODE_X };
 // chunk x of a step: 16 bytes of a row, the rows of a plane, the planes of an operand
 template <int T>
 __device__ __forceinline__ void ns_fetch(ns_u4 (&pre)[NsTile<T>::CH], const uint16_t* P, int64_t pp, const uint16_t* Q, int64_t pq, int K, int k0) {
+  constexpr int C = NsTile<T>::BK / 8;
 #pragma unroll
   for (int q = 0; q < NsTile<T>::CH; ++q) {
     const int x = q * RX_BLOCK + threadIdx.x;
-    const int ch = x % (NS_BK / 8), row = x / (NS_BK / 8) % T, pl = x / (NS_BK / 8) / T % 3, op = x / (NS_BK / 8) / T / 3;
+    const int ch = x % C, row = x / C % T, pl = x / C / T % 2, op = x / C / T / 2;
     const uint16_t* src = op ? Q + pl * pq : P + pl * pp;
     pre[q] = *reinterpret_cast<const ns_u4*>(src + (int64_t)row * K + k0 + ch * 8);
   }
@@ -293,8 +301,9 @@ __device__ __forceinline__ void ns_fetch(ns_u4 (&pre)[NsTile<T>::CH], const uint
 
 template <int T, int MODE>
 __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step) {
-  constexpr int NB = NsTile<T>::NB, CH = NsTile<T>::CH;
-  __shared__ __align__(16) uint16_t lds[2][3][T][NS_LDK];
+  typedef NsTile<T> Tile;
+  constexpr int NB = Tile::NB, CH = Tile::CH, BK = Tile::BK, LDK = Tile::LDK;
+  __shared__ __align__(16) uint16_t lds[2][2][T][LDK];
   // workgroups are dealt to the 8 XCDs in turn: each XCD takes a run of neighbouring tiles, which share operand rows in its L2
   const int per = (gridDim.x + 7) / 8;
   int mi = 0, b = (blockIdx.x % 8) * per + blockIdx.x / 8;
@@ -316,12 +325,13 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
     while (x > ti) x -= ++ti;
     tj = x;
   }
+  const int64_t pm = (int64_t)t.mp * t.mp, px = (int64_t)t.mp * t.np;
   const uint16_t *P, *Q;
   int64_t pp, pq;
   int K;
-  if (MODE == NS_MODE_A) { P = Q = t.x[cur]; pp = pq = (int64_t)t.mp * t.np; K = t.np; }
-  else if (MODE == NS_MODE_B) { P = Q = t.A; pp = pq = (int64_t)t.mp * t.mp; K = t.mp; }
-  else { P = t.B; pp = (int64_t)t.mp * t.mp; Q = t.xt[cur]; pq = (int64_t)t.np * t.mp; K = t.mp; }
+  if (MODE == NS_MODE_A) { P = Q = t.x[cur]; pp = pq = px; K = t.np; }
+  else if (MODE == NS_MODE_B) { P = Q = t.A; pp = pq = pm; K = t.mp; }
+  else { P = t.B; pp = pm; Q = t.xt[cur]; pq = px; K = t.mp; }
   P += (int64_t)ti * T * K;
   Q += (int64_t)tj * T * K;
   const int lane = rx_lane(), l31 = lane & 31, h = lane >> 5, wave = threadIdx.x >> 6;
@@ -329,52 +339,63 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
   ns_u4 pre[CH];
   ns_acc acc[NB][NB] = {};
   ns_fetch<T>(pre, P, pp, Q, pq, K, 0);
-  for (int k0 = 0; k0 < K; k0 += NS_BK) {
+  for (int k0 = 0; k0 < K; k0 += BK) {
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < CH; ++q) {
       const int x = q * RX_BLOCK + threadIdx.x;
-      const int ch = x % (NS_BK / 8), row = x / (NS_BK / 8) % T, pl = x / (NS_BK / 8) / T % 3, op = x / (NS_BK / 8) / T / 3;
+      const int ch = x % (BK / 8), row = x / (BK / 8) % T, pl = x / (BK / 8) / T % 2, op = x / (BK / 8) / T / 2;
       *reinterpret_cast<ns_u4*>(&lds[op][pl][row][ch * 8]) = pre[q];
     }
     __syncthreads();
-    if (k0 + NS_BK < K) ns_fetch<T>(pre, P, pp, Q, pq, K, k0 + NS_BK);
+    if (k0 + BK < K) ns_fetch<T>(pre, P, pp, Q, pq, K, k0 + BK);
 #pragma unroll
-    for (int ks = 0; ks < NS_BK; ks += 16) {
-      ns_h8 fa[NB][3], fb[NB][3];
+    for (int ks = 0; ks < BK; ks += 16) {
+      ns_h8 fa[NB][2], fb[NB][2];
 #pragma unroll
       for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {
+        for (int p = 0; p < 2; ++p) {
           fa[i][p] = *reinterpret_cast<const ns_h8*>(&lds[0][p][(wi * NB + i) * 32 + l31][ks + h * 8]);
           fb[i][p] = *reinterpret_cast<const ns_h8*>(&lds[1][p][(wj * NB + i) * 32 + l31][ks + h * 8]);
         }
-      constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
+      constexpr int PA[3] = {1, 0, 0}, PB[3] = {0, 1, 0};             // the smaller products first
 #pragma unroll
-      for (int u = 0; u < 6; ++u)
+      for (int u = 0; u < 3; ++u)
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
           for (int j = 0; j < NB; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i][PA[u]], fb[j][PB[u]], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][PA[u]], fb[j][PB[u]], acc[i][j], 0, 0, 0);
     }
   }
-  // lane: column tj * T + .. + l31, rows 8 q + 4 h + k
+  // lane: column tj * T + .. + l31, rows 8 q + 4 h + k.  The transposed image is written from the registers, four rows
+  // (8 bytes) at a time; the row-major one goes through LDS to be written 16 bytes at a time.
   const bool last = MODE == NS_MODE_X && step + 1 == a.steps;
   const bool flip = t.rows > t.cols;
+  const float undo = MODE == NS_MODE_A ? 1.f / (a.sx * a.sx) : MODE == NS_MODE_B ? 1.f / (a.sa * a.sa) : 1.f / (a.sb * a.sx);
+  const float scale = MODE == NS_MODE_A ? a.sa : MODE == NS_MODE_B ? a.sb : a.sx;
+  uint16_t* row_major = MODE == NS_MODE_A ? t.A : MODE == NS_MODE_B ? t.B : t.x[cur ^ 1];
+  uint16_t* mirror = MODE == NS_MODE_A ? t.A : MODE == NS_MODE_B ? t.B : t.xt[cur ^ 1];
+  const int64_t ldr = MODE == NS_MODE_X ? t.np : t.mp, plane = MODE == NS_MODE_X ? px : pm;
+  uint32_t (*turn)[36] = reinterpret_cast<uint32_t (*)[36]>(&lds[0][0][0][0]) + wave * 32;    // 32 x 32 words per wavefront
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < NB; ++i)
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
+    for (int j = 0; j < NB; ++j) {
+      const int r0 = ti * T + (wi * NB + i) * 32, c = tj * T + (wj * NB + j) * 32 + l31;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int r = ti * T + (wi * NB + i) * 32 + 8 * q + 4 * h, c = tj * T + (wj * NB + j) * 32 + l31;
-        float v[4];
+        const int r = r0 + 8 * q + 4 * h;
+        float v[4], e[4];
+        if (MODE == NS_MODE_B) ns_join4(t.A + (int64_t)c * t.mp + r, pm, e);         // A is its own mirror image
+        if (MODE == NS_MODE_X) ns_join4(t.xt[cur] + (int64_t)c * t.mp + r, px, e);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          v[k] = acc[i][j][4 * q + k];
-          if (MODE == NS_MODE_B) v[k] = fmaf(a.b, ns_join(t.A, (int64_t)t.mp * t.mp, (int64_t)(r + k) * t.mp + c), a.c * v[k]);
-          if (MODE == NS_MODE_X) v[k] = fmaf(a.a, ns_join(t.x[cur], (int64_t)t.mp * t.np, (int64_t)(r + k) * t.np + c), v[k]);
+          v[k] = acc[i][j][4 * q + k] * undo;
+          if (MODE == NS_MODE_B) v[k] = fmaf(a.b / a.sa, e[k], a.c * v[k]);
+          if (MODE == NS_MODE_X) v[k] = fmaf(a.a / a.sx, e[k], v[k]);
         }
         if (last) {
 #pragma unroll
@@ -386,24 +407,40 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
             }
           continue;
         }
-        uint32_t w0[3], w1[3];
-        ns_cut2(v[0], v[1], w0);
-        ns_cut2(v[2], v[3], w1);
-        uint16_t* row_major = MODE == NS_MODE_A ? t.A : MODE == NS_MODE_B ? t.B : t.x[cur ^ 1];
-        uint16_t* mirror = MODE == NS_MODE_A ? t.A : MODE == NS_MODE_B ? t.B : t.xt[cur ^ 1];
-        const int64_t ldr = MODE == NS_MODE_X ? t.np : t.mp, plane = (int64_t)t.mp * ldr;
+        uint32_t w0[2], w1[2];
+        ns_cut2(v[0] * scale, v[1] * scale, w0);
+        ns_cut2(v[2] * scale, v[3] * scale, w1);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) {
-          *reinterpret_cast<uint2*>(mirror + p * plane + (int64_t)c * t.mp + r) = make_uint2(w0[p], w1[p]);
-          if (MODE == NS_MODE_X || ti != tj) {           // a diagonal tile is its own mirror image
-            uint16_t* d = row_major + p * plane + (int64_t)r * ldr + c;
-            d[0] = (uint16_t)w0[p];
-            d[ldr] = (uint16_t)(w0[p] >> 16);
-            d[2 * ldr] = (uint16_t)w1[p];
-            d[3 * ldr] = (uint16_t)(w1[p] >> 16);
-          }
+        for (int p = 0; p < 2; ++p) *reinterpret_cast<uint2*>(mirror + p * plane + (int64_t)c * t.mp + r) = make_uint2(w0[p], w1[p]);
+        if (MODE == NS_MODE_X || ti != tj) {             // a diagonal tile is its own mirror image
+          const int y = 8 * q + 4 * h;
+          turn[y][l31] = (w0[0] & 0xffffu) | (w0[1] << 16);
+          turn[y + 1][l31] = (w0[0] >> 16) | (w0[1] & 0xffff0000u);
+          turn[y + 2][l31] = (w1[0] & 0xffffu) | (w1[1] << 16);
+          turn[y + 3][l31] = (w1[0] >> 16) | (w1[1] & 0xffff0000u);
         }
       }
+      if (last || !(MODE == NS_MODE_X || ti != tj)) continue;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const int y = lane >> 1, x = (lane & 1) * 16;      // half a row per lane
+      uint32_t u[16];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 f = *reinterpret_cast<const uint4*>(&turn[y][x + 4 * k]);
+        u[4 * k] = f.x; u[4 * k + 1] = f.y; u[4 * k + 2] = f.z; u[4 * k + 3] = f.w;
+      }
+      uint16_t* d = row_major + (int64_t)(r0 + y) * ldr + tj * T + (wj * NB + j) * 32 + x;
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          uint32_t o[4];
+#pragma unroll
+          for (int z = 0; z < 4; ++z) o[z] = __builtin_amdgcn_perm(u[8 * k + 2 * z + 1], u[8 * k + 2 * z], p ? 0x07060302u : 0x05040100u);
+          *reinterpret_cast<uint4*>(d + p * plane + 8 * k) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
 }
 
 // ---------------------------------------------------------------- host
@@ -414,6 +451,7 @@ struct NsArgs {                // rx_ortho_args and rx_muon_args in one form
   int32_t rows[RX_ORTHO_MAX], cols[RX_ORTHO_MAX];
   int32_t count, steps, nesterov;
   float a, b, c, eps, mu;
+  float sx, sa, sb;
   const float* scale;
 };
 
@@ -425,6 +463,39 @@ static int ns_check(const char* who, const int32_t* rows, const int32_t* cols, i
                rows[i], cols[i], NS_MAXDIM);
   return 0;
 }
+
+// Bounds of |X|_2, |A|_2 and |B|_2 over the steps, for singular values that start in [0, 1] (what the division by the norm
+// guarantees): the largest |a s + b s^3 + c s^5| over [0, bound so far], from its extrema; refuses coefficients that let
+// the bound grow past 16.
+static int ns_bounds(const char* who, double ca, double cb, double cc, int steps, float* x, float* a, float* b) {
+  double m = 1.0;
+  for (int k = 0; k < steps; ++k) {
+    double u[3] = {m * m, -1.0, -1.0};                   // s^2 of the candidates
+    if (cc != 0.0) {
+      const double d = 9.0 * cb * cb - 20.0 * ca * cc;
+      if (d >= 0.0) {
+        u[1] = (-3.0 * cb + sqrt(d)) / (10.0 * cc);
+        u[2] = (-3.0 * cb - sqrt(d)) / (10.0 * cc);
+      }
+    } else if (cb != 0.0) {
+      u[1] = -ca / (3.0 * cb);
+    }
+    double top = m;
+    for (int i = 0; i < 3; ++i)
+      if (u[i] > 0.0 && u[i] <= m * m) top = fmax(top, fabs(sqrt(u[i]) * (ca + u[i] * (cb + u[i] * cc))));
+    RX_REQUIRE(top <= 16.0 && isfinite(ca + cb + cc), "%s: coefficients (%g, %g, %g) let singular values in [0, 1] grow past 16 in %d steps",
+               who, ca, cb, cc, steps);
+    if (top == m) break;
+    m = top;
+  }
+  const double l = m * m, e = cc != 0.0 ? -cb / (2.0 * cc) : -1.0;
+  double q = fabs(l * (cb + l * cc));
+  if (e > 0.0 && e < l) q = fmax(q, fabs(e * (cb + e * cc)));
+  *x = (float)m; *a = (float)l; *b = (float)q;
+  return 0;
+}
+// power of two that takes a bound, with a margin for rounding, to at most 2^15
+static float ns_scale_of(float bound) { return bound > 0.f ? ldexpf(1.f, 14 - ilogbf(bound * 1.1f)) : 1.f; }
 
 // Tile: 128 once the largest product of the list fills the chip with such tiles, 64 for the parallelism otherwise.
 static void ns_plan(const NsArgs& a, NsList* l, size_t* bytes, uint8_t* ws) {
@@ -446,6 +517,7 @@ static void ns_plan(const NsArgs& a, NsList* l, size_t* bytes, uint8_t* ws) {
   l->mu = a.mu;
   l->scale = a.scale;
   l->a = a.a; l->b = a.b; l->c = a.c; l->eps = a.eps;
+  l->sx = a.sx; l->sa = a.sa; l->sb = a.sb;
   size_t at = 0;
   auto take = [&](size_t n) { uint8_t* p = ws ? ws + at : nullptr; at += rx_align_up(n, 256); return p; };
   l->parts = (double*)take(sizeof(double) * NS_PARTS * (size_t)k);
@@ -460,7 +532,7 @@ static void ns_plan(const NsArgs& a, NsList* l, size_t* bytes, uint8_t* ws) {
     const int tm = t.mp / l->tile;
     t.tiles_sym = tm * (tm + 1) / 2;
     t.tiles_x = tm * (t.np / l->tile);
-    const size_t mn = (size_t)t.mp * t.np * 6, mm = (size_t)t.mp * t.mp * 6;
+    const size_t mn = (size_t)t.mp * t.np * 4, mm = (size_t)t.mp * t.mp * 4;
     for (int q = 0; q < 2; ++q) { t.x[q] = (uint16_t*)take(mn); t.xt[q] = (uint16_t*)take(mn); }
     t.A = (uint16_t*)take(mm);
     t.B = (uint16_t*)take(mm);
@@ -482,7 +554,10 @@ static void ns_run(const NsList& l, hipStream_t st) {
   }
 }
 
-static int ns_go(const char* who, const NsArgs& a, void* ws, size_t ws_bytes, int device, void* stream) {
+static int ns_go(const char* who, NsArgs& a, void* ws, size_t ws_bytes, int device, void* stream) {
+  float bx, ba, bb;
+  if (ns_bounds(who, a.a, a.b, a.c, a.steps, &bx, &ba, &bb)) return 1;
+  a.sx = ns_scale_of(bx); a.sa = ns_scale_of(ba); a.sb = ns_scale_of(bb);
   NsList l;
   size_t need;
   ns_plan(a, &l, &need, (uint8_t*)ws);
