@@ -5,14 +5,14 @@
 // below the diagonal are computed, the others are their mirror images).  Small singular values grow by up to a^steps = 485,
 // and so do rounding errors along them: 16-bit products would leave errors of the size of the result there, so the products
 // keep fp32 accuracy.
-//   * Matrices that fit one workgroup's LDS take all steps in one launch, on fp32 matrix instructions: such lists are
-//     bound by launches, not by products.
-//   * The others share three launches per step, whatever their number.  X, X^T, A and B live in the workspace as two
-//     fp16 planes each (11 + 11 significant bits), cut once in the epilogue that makes them; high high + high low + low high
-//     gives fp32 accuracy (what is left out is below 2^-24 of a term) at a third of the 16-bit rate, where fp32 matrix
-//     instructions have a sixteenth.  fp16 lacks range, but the iteration does not use it: |X|_2 <= 1 at the start and the
-//     coefficients bound it from there on, so each array has one power-of-two scale that takes its bound to 2^15, found
-//     on the host.  With X^T kept beside X all three products read both operands along the contraction.
+// Operands are cut into two fp16 planes (11 + 11 significant bits); high high + high low + low high gives fp32 accuracy (what
+// is left out is below 2^-24 of a term) at a third of the 16-bit rate, where fp32 matrix instructions have a sixteenth.
+// fp16 lacks range, but the iteration does not use it: |X|_2 <= 1 at the start and the coefficients bound it from there
+// on, so each array has one power-of-two scale that takes its bound to 2^15, found on the host.
+//   * Matrices that fit one workgroup's LDS take all steps in one launch: such lists are bound by launches and latency.
+//   * The others share three launches per step, whatever their number.  X, X^T, A and B live in the workspace as planes, cut
+//     once in the epilogue that makes them; with X^T kept beside X all three products read both operands along the
+//     contraction.
 #include "rx_common.h"
 
 #include <math.h>
@@ -20,15 +20,36 @@
 typedef _Float16 ns_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 ns_h2 __attribute__((ext_vector_type(2)));
 typedef float ns_f2 __attribute__((ext_vector_type(2)));
-typedef float ns_f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t ns_u4 __attribute__((ext_vector_type(4)));   // HIP's uint4 kept the prefetch registers in scratch
+typedef float ns_f4 __attribute__((ext_vector_type(4)));
 typedef float ns_acc __attribute__((ext_vector_type(16)));
 
 #define NS_MAXDIM 16384
 #define NS_SMALL_M 96
 #define NS_SMALL_LDS (152 * 1024)
 #define NS_SMALL_THREADS 512
+#define NS_SMALL_JOBS 8          // tiles of A times shares of their contraction
 #define NS_PARTS 256           // norm partials per matrix
+
+// two values times a scale -> their words in the two planes
+__device__ __forceinline__ void ns_cut2(float a, float b, uint32_t* w) {
+  ns_f2 v = {a, b};
+  const ns_h2 h = __builtin_convertvector(v, ns_h2);
+  ns_f2 r = {a - (float)h.x, b - (float)h.y};
+  w[0] = __builtin_bit_cast(uint32_t, h);
+  w[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, ns_h2));
+}
+// four neighbouring values from their planes
+__device__ __forceinline__ void ns_join4(const uint16_t* p, int64_t plane, float* v) {
+  const uint2 hi = *reinterpret_cast<const uint2*>(p), lo = *reinterpret_cast<const uint2*>(p + plane);
+  const uint32_t h[2] = {hi.x, hi.y}, l[2] = {lo.x, lo.y};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const ns_h2 a = __builtin_bit_cast(ns_h2, h[i]), b = __builtin_bit_cast(ns_h2, l[i]);
+    v[2 * i] = (float)a.x + (float)b.x;
+    v[2 * i + 1] = (float)a.y + (float)b.y;
+  }
+}
 
 // ---------------------------------------------------------------- small matrices: one workgroup each
 struct NsSmall {
@@ -39,6 +60,7 @@ struct NsSmall {
   int32_t rows[RX_ORTHO_MAX], cols[RX_ORTHO_MAX];
   int32_t steps, nesterov;
   float a, b, c, eps, mu;
+  float sx, sa, sb;            // scales of X, A and B
   const float* scale;
 };
 // What is orthogonalised of a gradient value: the value itself, or with momentum (m: in the new, out the stored one)
@@ -48,38 +70,212 @@ __device__ __forceinline__ float ns_update(float g, float* m, float mu, int nest
   return nesterov ? fmaf(mu, *m, g) : *m;
 }
 static inline int ns_up(int x, int a) { return (x + a - 1) / a * a; }
+// LDS of one matrix: X as fp32 [mp][np + 4], A and B as planes [2][mp][mp + 8], and where fewer tiles of A than wavefronts
+// exist, a 32 x 36 partial tile per wavefront.  (m <= 16: see ns_tiny_run.)
 static size_t ns_small_lds(int rows, int cols) {
-  const int m = ns_up(rows < cols ? rows : cols, 16), n = ns_up(rows < cols ? cols : rows, 16);
-  return ((size_t)m * (n + 4) + 2 * (size_t)m * (m + 4)) * 4;
+  const int m = rows < cols ? rows : cols, mp = ns_up(m, 32), np = ns_up(rows < cols ? cols : rows, 32);
+  if (m <= 16) return ((size_t)m * (np + 4) + 320 * (2 + NS_SMALL_JOBS)) * 4;
+  return (size_t)mp * (np + 4) * 4 + (size_t)8 * mp * (mp + 8) + (mp < 96 ? (size_t)NS_SMALL_JOBS * 32 * 36 * 4 : 0);
 }
 static bool ns_is_small(int rows, int cols) {
   return (rows < cols ? rows : cols) <= NS_SMALL_M && ns_small_lds(rows, cols) <= NS_SMALL_LDS;
 }
 
-// C (m x m, symmetric) tiles on and below the diagonal of s U U^T + t W, both images written; U [m][K] in LDS
-__device__ __forceinline__ void ns_small_gram(const float* U, int ldu, int K, int mt, float s, float t, const float* W, float* C, int ldc) {
-  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = rx_lane(), l15 = lane & 15, q = lane >> 4;
-  const int tiles = mt * (mt + 1) / 2;
-  for (int x = wave; x < tiles; x += waves) {
-    int i = 0;
-    while ((i + 1) * (i + 2) / 2 <= x) ++i;
-    const int j = x - i * (i + 1) / 2;
-    const float* ui = U + (i * 16 + l15) * ldu + q;
-    const float* uj = U + (j * 16 + l15) * ldu + q;
-    ns_f4 acc0 = {}, acc1 = {};
-    int k = 0;
-    for (; k + 8 <= K; k += 8) {
-      acc0 = __builtin_amdgcn_mfma_f32_16x16x4f32(ui[k], uj[k], acc0, 0, 0, 0);
-      acc1 = __builtin_amdgcn_mfma_f32_16x16x4f32(ui[k + 4], uj[k + 4], acc1, 0, 0, 0);
-    }
+// eight fp32 values -> fragments of the two planes
+__device__ __forceinline__ void ns_cut8(const float* v, ns_h8* f) {
+  union { uint32_t w[4]; ns_h8 h; } p[2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = i * 16 + q * 4 + e, c = j * 16 + l15;
-      float v = s * (acc0[e] + acc1[e]);
-      if (W) v = fmaf(t, W[r * ldc + c], v);
-      C[r * ldc + c] = v;
-      C[c * ldc + r] = v;
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w[2];
+    ns_cut2(v[2 * i], v[2 * i + 1], w);
+    p[0].w[i] = w[0];
+    p[1].w[i] = w[1];
+  }
+  f[0] = p[0].h;
+  f[1] = p[1].h;
+}
+// one step of the contraction into three sums: a matrix instruction does not wait for the one before it
+struct NsSum {
+  ns_acc hh = {}, hl = {}, lh = {};
+  __device__ __forceinline__ void add(const ns_h8* a, const ns_h8* b) {
+    hh = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[0], hh, 0, 0, 0);
+    hl = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0], b[1], hl, 0, 0, 0);
+    lh = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1], b[0], lh, 0, 0, 0);
+  }
+  __device__ __forceinline__ ns_acc total() const { return hh + (hl + lh); }
+};
+
+// MB = m / 32, rounded up; rows past m hold zeros.  All arrays hold their values times their scale (X: sx, A: sa, B: sb).
+// All MB^2 tiles of A and B are computed: the lower and the upper one of a pair come out the same, bit for bit, and each
+// is written four rows at a time without a second, scattered image.
+template <int MB>
+__device__ __forceinline__ void ns_small_run(const NsSmall& a, float* X, int np) {
+  constexpr int MP = MB * 32, LDP = MP + 8, PLANE = MP * LDP, TILES = MB * MB, W = NS_SMALL_THREADS / 64;
+  constexpr int KS = NS_SMALL_JOBS / TILES < 1 ? 1 : NS_SMALL_JOBS / TILES;
+  const int ldx = np + 4, lane = rx_lane(), wave = threadIdx.x >> 6, l31 = lane & 31, h = lane >> 5;
+  uint16_t* A = reinterpret_cast<uint16_t*>(X + MP * ldx);
+  uint16_t* B = A + 2 * PLANE;
+  float* part = reinterpret_cast<float*>(B + 2 * PLANE);
+  auto planes_row = [&](const uint16_t* p, int row, int k, ns_h8* f) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) f[q] = *reinterpret_cast<const ns_h8*>(p + q * PLANE + row * LDP + k);
+  };
+  auto x_row = [&](int row, int k, ns_h8* f) {
+    const float4 lo = *reinterpret_cast<const float4*>(X + row * ldx + k), hi = *reinterpret_cast<const float4*>(X + row * ldx + k + 4);
+    const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    ns_cut8(v, f);
+  };
+  auto put4 = [&](uint16_t* p, int r, int c, const float* v) {      // rows r .. r + 3 of column c
+    uint32_t w0[2], w1[2];
+    ns_cut2(v[0], v[1], w0);
+    ns_cut2(v[2], v[3], w1);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) *reinterpret_cast<uint2*>(p + q * PLANE + c * LDP + r) = make_uint2(w0[q], w1[q]);
+  };
+  const float ua = a.sa / (a.sx * a.sx), ub = a.b * a.sb / a.sa, uc = a.c * a.sb / (a.sa * a.sa), ux = 1.f / a.sb;
+  const int shares = np >= 128 * KS ? KS : 1;          // a contraction of up to 8 steps is not worth the second pass
+  for (int step = 0; step < a.steps; ++step) {
+    // A = X X^T
+    for (int job = wave; job < TILES * shares; job += W) {
+      const int t = job / shares, s = job % shares, i = t / MB, j = t % MB;
+      const int steps = np / 16, lo = steps * s / shares, hi = steps * (s + 1) / shares;
+      NsSum sum;
+      for (int k = lo; k < hi; ++k) {
+        ns_h8 fi[2], fj[2];
+        x_row(i * 32 + l31, k * 16 + h * 8, fi);
+        if (i == j) sum.add(fi, fi);
+        else {
+          x_row(j * 32 + l31, k * 16 + h * 8, fj);
+          sum.add(fi, fj);
+        }
+      }
+      const ns_acc acc = sum.total();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float v[4] = {acc[4 * q] * ua, acc[4 * q + 1] * ua, acc[4 * q + 2] * ua, acc[4 * q + 3] * ua};
+        if (KS > 1 && shares > 1) *reinterpret_cast<float4*>(part + (job * 32 + l31) * 36 + 8 * q + 4 * h) = make_float4(v[0], v[1], v[2], v[3]);
+        else put4(A, i * 32 + 8 * q + 4 * h, j * 32 + l31, v);
+      }
     }
+    __syncthreads();
+    if (KS > 1 && shares > 1) {
+      for (int x = threadIdx.x; x < TILES * 256; x += NS_SMALL_THREADS) {
+        const int t = x >> 8, c = x & 31, r = (x >> 5 & 7) * 4;
+        float v[4] = {};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const float4 f = *reinterpret_cast<const float4*>(part + ((t * KS + s) * 32 + c) * 36 + r);
+          v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
+        }
+        put4(A, t / MB * 32 + r, t % MB * 32 + c, v);
+      }
+      __syncthreads();
+    }
+    // B = b A + c A A
+    for (int t = wave; t < TILES; t += W) {
+      const int i = t / MB, j = t % MB, c = j * 32 + l31;
+      NsSum sum;
+#pragma unroll
+      for (int k = 0; k < MP / 16; ++k) {
+        ns_h8 fi[2], fj[2];
+        planes_row(A, i * 32 + l31, k * 16 + h * 8, fi);
+        planes_row(A, c, k * 16 + h * 8, fj);
+        sum.add(fi, fj);
+      }
+      const ns_acc acc = sum.total();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = i * 32 + 8 * q + 4 * h;
+        float v[4];
+        ns_join4(A + c * LDP + r, PLANE, v);             // A is its own mirror image
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(ub, v[e], uc * acc[4 * q + e]);
+        put4(B, r, c, v);
+      }
+    }
+    __syncthreads();
+    // X = a X + B X: a wavefront owns 32 columns and has read all of them before it writes any
+    for (int cb = wave; cb < np / 32; cb += W) {
+      float* col = X + cb * 32 + l31;
+      ns_h8 fx[MP / 16][2];
+#pragma unroll
+      for (int k = 0; k < MP / 16; ++k) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = col[(k * 16 + h * 8 + e) * ldx];
+        ns_cut8(v, fx[k]);
+      }
+#pragma unroll 1
+      for (int i = 0; i < MB; ++i) {
+        NsSum sum;
+#pragma unroll
+        for (int k = 0; k < MP / 16; ++k) {
+          ns_h8 fb[2];
+          planes_row(B, i * 32 + l31, k * 16 + h * 8, fb);
+          sum.add(fb, fx[k]);
+        }
+        const ns_acc acc = sum.total();
+        float* p = col + (i * 32 + 4 * h) * ldx;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float* at = p + (8 * (e / 4) + e % 4) * ldx;
+          *at = fmaf(a.a, *at, acc[e] * ux);
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// m <= 16: one tile on fp32 matrix instructions, whose rate does not matter here; the contraction of A is shared out
+// among the wavefronts.  A [16][20] and B [16][20] behind X, the shares [waves][16][20] behind them.
+__device__ __forceinline__ void ns_tiny_run(const NsSmall& a, float* X, int m, int np) {
+  constexpr int W = NS_SMALL_JOBS;
+  const int ldx = np + 4, lane = rx_lane(), wave = threadIdx.x >> 6, l15 = lane & 15, q = lane >> 4;
+  float *A = X + m * ldx, *B = A + 320, *part = B + 320;
+  const float one = 1.f / (a.sx * a.sx);
+  for (int step = 0; step < a.steps; ++step) {
+    if (wave < W) {
+      ns_f4 acc[4] = {};
+      const int quads = np / 4, lo = quads * wave / W, hi = quads * (wave + 1) / W;
+      for (int k = lo; k < hi; k += 4)
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (k + u < hi) {
+            const float v = l15 < m ? X[l15 * ldx + (k + u) * 4 + q] : 0.f;
+            acc[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, v, acc[u], 0, 0, 0);
+          }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[wave * 320 + (q * 4 + e) * 20 + l15] = ((acc[0][e] + acc[1][e]) + (acc[2][e] + acc[3][e])) * one;
+    }
+    __syncthreads();
+    if (threadIdx.x < 256) {
+      const int at = (threadIdx.x >> 4) * 20 + (threadIdx.x & 15);
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) s += part[w * 320 + at];
+      A[at] = s;
+    }
+    __syncthreads();
+    if (wave == 0) {
+      ns_f4 acc = {};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(A[l15 * 20 + 4 * k + q], A[l15 * 20 + 4 * k + q], acc, 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) B[(q * 4 + e) * 20 + l15] = fmaf(a.b, A[(q * 4 + e) * 20 + l15], a.c * acc[e]);
+    }
+    __syncthreads();
+    for (int cb = wave; cb < np / 16; cb += NS_SMALL_THREADS / 64) {
+      float* col = X + cb * 16 + l15;
+      ns_f4 acc = {};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(B[l15 * 20 + 4 * k + q], 4 * k + q < m ? col[(4 * k + q) * ldx] : 0.f, acc, 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (q * 4 + e < m) col[(q * 4 + e) * ldx] = fmaf(a.a, col[(q * 4 + e) * ldx], acc[e]);
+    }
+    __syncthreads();
   }
 }
 
@@ -88,79 +284,69 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS) ns_small_kernel(NsSmall a) {
   __shared__ double part[NS_SMALL_THREADS / 64];
   const float* g = a.g[blockIdx.x];
   float* out = a.out[blockIdx.x];
+  float* mom = a.mom[blockIdx.x];
   const int rows = a.rows[blockIdx.x], cols = a.cols[blockIdx.x];
   const bool flip = rows > cols;
-  const int m = flip ? cols : rows, n = flip ? rows : cols;
-  const int mp = (m + 15) & ~15, np = (n + 15) & ~15, ldx = np + 4, ldc = mp + 4, mt = mp / 16;
+  const int m = flip ? cols : rows, n = flip ? rows : cols, np = (n + 31) & ~31, ldx = np + 4;
   float* X = ns_lds;
-  float* A = X + mp * ldx;
-  float* B = A + mp * ldc;
-  const int lane = rx_lane(), wave = threadIdx.x >> 6, waves = blockDim.x >> 6, l15 = lane & 15, q = lane >> 4;
-  for (int i = threadIdx.x; i < mp * ldx; i += blockDim.x) X[i] = 0.f;
-  __syncthreads();
-  double ss = 0.0;
-  float* mom = a.mom[blockIdx.x];
+  const int lane = rx_lane(), wave = threadIdx.x >> 6;
   const float sc = a.scale ? *a.scale : 1.f;
-  for (int i = threadIdx.x; i < rows * cols; i += blockDim.x) {
-    const int r = i / cols, c = i - r * cols;
-    float v = g[i];
-    if (mom) {
-      float m = mom[i];
-      v = ns_update(v * sc, &m, a.mu, a.nesterov);
-      mom[i] = m;
+  double ss = 0.0;
+  // along G, four values of a thread on their way at once
+  const int total = rows * cols, dr = NS_SMALL_THREADS / cols, dc = NS_SMALL_THREADS - dr * cols;
+  {
+    int r = threadIdx.x / cols, c = threadIdx.x - r * cols;
+    for (int i0 = threadIdx.x; i0 < total; i0 += 4 * NS_SMALL_THREADS) {
+      float v[4], mv[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * NS_SMALL_THREADS;
+        v[u] = i < total ? g[i] : 0.f;
+        mv[u] = mom && i < total ? mom[i] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * NS_SMALL_THREADS;
+        if (i < total) {
+          if (mom) {
+            v[u] = ns_update(v[u] * sc, &mv[u], a.mu, a.nesterov);
+            mom[i] = mv[u];
+          }
+          ss = fma((double)v[u], (double)v[u], ss);
+          X[flip ? c * ldx + r : r * ldx + c] = v[u];
+        }
+        r += dr;
+        c += dc;
+        if (c >= cols) { c -= cols; ++r; }
+      }
     }
-    ss = fma((double)v, (double)v, ss);
-    X[flip ? c * ldx + r : r * ldx + c] = v;
   }
+  for (int i = threadIdx.x; i < m * (ldx - n); i += NS_SMALL_THREADS) X[i / (ldx - n) * ldx + n + i % (ldx - n)] = 0.f;
+  if (m > 16)
+    for (int i = m * ldx + threadIdx.x; i < ((m + 31) & ~31) * ldx; i += NS_SMALL_THREADS) X[i] = 0.f;
   ss = rx_wave_sum_f64(ss);
   if (lane == 0) part[wave] = ss;
   __syncthreads();
   ss = 0.0;
-  for (int w = 0; w < waves; ++w) ss += part[w];
+  for (int w = 0; w < NS_SMALL_THREADS / 64; ++w) ss += part[w];
   const float div = (float)(sqrt(ss) + (double)a.eps);
-  for (int i = threadIdx.x; i < mp * ldx; i += blockDim.x) X[i] /= i % ldx < n && i / ldx < m ? div : 1.f;   // padding stays 0
+  for (int r = wave; r < m; r += NS_SMALL_THREADS / 64)
+    for (int c = lane; c < n; c += 64) X[r * ldx + c] = X[r * ldx + c] / div * a.sx;
   __syncthreads();
-  for (int step = 0; step < a.steps; ++step) {
-    ns_small_gram(X, ldx, np, mt, 1.f, 0.f, nullptr, A, ldc);
-    __syncthreads();
-    ns_small_gram(A, ldc, mp, mt, a.c, a.b, A, B, ldc);
-    __syncthreads();
-    // a wavefront owns 16 columns of X: all of them are read before any is written
-    for (int cb = wave; cb < np / 16; cb += waves) {
-      float x[NS_SMALL_M / 4];                     // rows q + 4 k of the lane's column
-      float* col = X + cb * 16 + l15;
-#pragma unroll
-      for (int k = 0; k < NS_SMALL_M / 4; ++k) x[k] = k * 4 < mp ? col[(k * 4 + q) * ldx] : 0.f;
-      ns_f4 acc[NS_SMALL_M / 16];
-#pragma unroll
-      for (int i = 0; i < NS_SMALL_M / 16; ++i) {
-        acc[i] = ns_f4{};
-        if (i < mt) {
-          const float* bi = B + (i * 16 + l15) * ldc + q;
-#pragma unroll
-          for (int k = 0; k < NS_SMALL_M / 4; ++k)
-            if (k * 4 < mp) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(bi[k * 4], x[k], acc[i], 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < NS_SMALL_M / 16; ++i)
-        if (i < mt) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float* p = col + (i * 16 + q * 4 + e) * ldx;
-            *p = fmaf(a.a, *p, acc[i][e]);
-          }
-        }
-    }
-    __syncthreads();
-  }
+  if (m <= 16) ns_tiny_run(a, X, m, np);
+  else if (m <= 32) ns_small_run<1>(a, X, np);
+  else if (m <= 64) ns_small_run<2>(a, X, np);
+  else ns_small_run<3>(a, X, np);
   float* w = a.w[blockIdx.x];
-  const float alpha = a.alpha[blockIdx.x];
-  for (int i = threadIdx.x; i < rows * cols; i += blockDim.x) {
-    const int r = i / cols, c = i - r * cols;
-    const float v = X[flip ? c * ldx + r : r * ldx + c];
+  const float alpha = a.alpha[blockIdx.x], undo = 1.f / a.sx;
+  int r = threadIdx.x / cols, c = threadIdx.x - r * cols;
+  for (int i = threadIdx.x; i < total; i += NS_SMALL_THREADS) {
+    const float v = X[flip ? c * ldx + r : r * ldx + c] * undo;
     if (w) w[i] = fmaf(-alpha, v, w[i]);
     else out[i] = v;
+    r += dr;
+    c += dc;
+    if (c >= cols) { c -= cols; ++r; }
   }
 }
 
@@ -183,26 +369,6 @@ struct NsList {
   const float* scale;
   double* parts;               // [count][NS_PARTS]
 };
-
-// two values times a scale -> their words in the two planes
-__device__ __forceinline__ void ns_cut2(float a, float b, uint32_t* w) {
-  ns_f2 v = {a, b};
-  const ns_h2 h = __builtin_convertvector(v, ns_h2);
-  ns_f2 r = {a - (float)h.x, b - (float)h.y};
-  w[0] = __builtin_bit_cast(uint32_t, h);
-  w[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, ns_h2));
-}
-// four neighbouring values from their planes
-__device__ __forceinline__ void ns_join4(const uint16_t* p, int64_t plane, float* v) {
-  const uint2 hi = *reinterpret_cast<const uint2*>(p), lo = *reinterpret_cast<const uint2*>(p + plane);
-  const uint32_t h[2] = {hi.x, hi.y}, l[2] = {lo.x, lo.y};
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const ns_h2 a = __builtin_bit_cast(ns_h2, h[i]), b = __builtin_bit_cast(ns_h2, l[i]);
-    v[2 * i] = (float)a.x + (float)b.x;
-    v[2 * i + 1] = (float)a.y + (float)b.y;
-  }
-}
 
 __global__ void __launch_bounds__(RX_BLOCK) ns_norm_kernel(NsList a) {
   const int mi = blockIdx.x / NS_PARTS, pt = blockIdx.x % NS_PARTS;
@@ -568,6 +734,7 @@ static int ns_go(const char* who, NsArgs& a, void* ws, size_t ws_bytes, int devi
   memset(&s, 0, sizeof(s));
   s.steps = a.steps; s.nesterov = a.nesterov; s.mu = a.mu; s.scale = a.scale;
   s.a = a.a; s.b = a.b; s.c = a.c; s.eps = a.eps;
+  s.sx = a.sx; s.sa = a.sa; s.sb = a.sb;
   int k = 0;
   size_t lds = 0;
   for (int i = 0; i < a.count; ++i)
