@@ -446,8 +446,11 @@ __global__ void __launch_bounds__(RX_BLOCK) ns_init_kernel(NsList a) {
 template <int T>
 struct NsTile {
   static constexpr int NB = T / 64;
-  static constexpr int BK = T == 64 ? 64 : 32, LDK = BK + 8;
+  static constexpr int BK = 64, LDK = BK + 8;
   static constexpr int CH = 4 * T * (BK / 8) / RX_BLOCK;              // 16-byte chunks per thread and step
+  // Steps in LDS: two where few workgroups hide little of the loads' latency, one where two workgroups share a CU.
+  static constexpr int BUF = T == 64 ? 2 : 1;
+  typedef uint16_t Lds[BUF][2][2][T][LDK];
 };
 
 enum { NS_MODE_A, NS_MODE_B, NS_MODE_X };
@@ -465,32 +468,91 @@ __device__ __forceinline__ void ns_fetch(ns_u4 (&pre)[NsTile<T>::CH], const uint
   }
 }
 
+template <int T>
+__device__ __forceinline__ void ns_put(const ns_u4 (&pre)[NsTile<T>::CH], typename NsTile<T>::Lds& lds, int buf) {
+  constexpr int C = NsTile<T>::BK / 8;
+#pragma unroll
+  for (int q = 0; q < NsTile<T>::CH; ++q) {
+    const int x = q * RX_BLOCK + threadIdx.x;
+    const int ch = x % C, row = x / C % T, pl = x / C / T % 2, op = x / C / T / 2;
+    *reinterpret_cast<ns_u4*>(&lds[buf][op][pl][row][ch * 8]) = pre[q];
+  }
+}
+template <int T>
+__device__ __forceinline__ void ns_step(const typename NsTile<T>::Lds& lds, int buf, int wi, int wj, ns_acc (&acc)[NsTile<T>::NB][NsTile<T>::NB]) {
+  constexpr int NB = NsTile<T>::NB;
+  const int l31 = rx_lane() & 31, h = rx_lane() >> 5;
+#pragma unroll
+  for (int ks = 0; ks < NsTile<T>::BK; ks += 16) {
+    ns_h8 fa[NB][2], fb[NB][2];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        fa[i][p] = *reinterpret_cast<const ns_h8*>(&lds[buf][0][p][(wi * NB + i) * 32 + l31][ks + h * 8]);
+        fb[i][p] = *reinterpret_cast<const ns_h8*>(&lds[buf][1][p][(wj * NB + i) * 32 + l31][ks + h * 8]);
+      }
+    constexpr int PA[3] = {1, 0, 0}, PB[3] = {0, 1, 0};               // the smaller products first
+#pragma unroll
+    for (int u = 0; u < 3; ++u)
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][PA[u]], fb[j][PB[u]], acc[i][j], 0, 0, 0);
+  }
+}
+
+// Tile b of a product: bands of 8 tile rows, each band column by column, so that the 64 tiles an XCD works on at a time
+// are about 8 x 8 and share operand rows.  FULL: all of tm x tn; otherwise the lower triangle of tm x tm.
+template <bool FULL>
+__device__ __forceinline__ void ns_tile(int b, int tm, int tn, int* ti, int* tj) {
+  for (int r0 = 0;; r0 += 8) {
+    const int rows = tm - r0 < 8 ? tm - r0 : 8;
+    const int square = rows * (FULL ? tn : r0), all = square + (FULL ? 0 : rows * (rows + 1) / 2);
+    if (b >= all && r0 + 8 < tm) { b -= all; continue; }
+    if (b < square) {
+      *ti = r0 + b % rows;
+      *tj = b / rows;
+      return;
+    }
+    b -= square;
+    int i = 0;
+    while (b > i) b -= ++i;
+    *ti = r0 + i;
+    *tj = r0 + b;
+    return;
+  }
+}
+
+// Workgroups are dealt to the 8 XCDs in turn.  Of a matrix's k tiles each XCD takes a run of neighbours, which share operand
+// rows in its L2; the runs one longer than the others go on where those of the matrix before ended (`off`: tiles so
+// far), so that every XCD has the same number of tiles, and as many of each length, to one.
+__host__ __device__ __forceinline__ int ns_run_of(int k, int xcd, int off, int* first) {
+  const int x = (xcd - off) & 7, rest = k & 7;
+  *first = x * (k >> 3) + (x < rest ? x : rest);
+  return (k >> 3) + (x < rest ? 1 : 0);
+}
+
 template <int T, int MODE>
 __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step) {
   typedef NsTile<T> Tile;
-  constexpr int NB = Tile::NB, CH = Tile::CH, BK = Tile::BK, LDK = Tile::LDK;
-  __shared__ __align__(16) uint16_t lds[2][2][T][LDK];
-  // workgroups are dealt to the 8 XCDs in turn: each XCD takes a run of neighbouring tiles, which share operand rows in its L2
-  const int per = (gridDim.x + 7) / 8;
-  int mi = 0, b = (blockIdx.x % 8) * per + blockIdx.x / 8;
+  constexpr int NB = Tile::NB, CH = Tile::CH, BK = Tile::BK;
+  __shared__ __align__(16) typename Tile::Lds lds;
+  int mi = 0, b = blockIdx.x / 8, off = 0;
   for (; mi < a.count; ++mi) {
     const int k = MODE == NS_MODE_X ? a.mat[mi].tiles_x : a.mat[mi].tiles_sym;
-    if (b < k) break;
-    b -= k;
+    int first;
+    const int run = ns_run_of(k, blockIdx.x % 8, off, &first);
+    if (b < run) { b += first; break; }
+    b -= run;
+    off += k;
   }
   if (mi == a.count) return;
   const NsMat& t = a.mat[mi];
   const int cur = step & 1;
   int ti, tj;
-  if (MODE == NS_MODE_X) {
-    ti = b / (t.np / T);
-    tj = b % (t.np / T);
-  } else {                     // lower triangle
-    ti = 0;
-    int x = b;
-    while (x > ti) x -= ++ti;
-    tj = x;
-  }
+  ns_tile<MODE == NS_MODE_X>(b, t.mp / T, t.np / T, &ti, &tj);
   const int64_t pm = (int64_t)t.mp * t.mp, px = (int64_t)t.mp * t.np;
   const uint16_t *P, *Q;
   int64_t pp, pq;
@@ -502,37 +564,38 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
   Q += (int64_t)tj * T * K;
   const int lane = rx_lane(), l31 = lane & 31, h = lane >> 5, wave = threadIdx.x >> 6;
   const int wi = wave >> 1, wj = wave & 1;
-  ns_u4 pre[CH];
+  // Two sets of registers: a step's loads are issued two steps before it goes into LDS.
+  ns_u4 even[CH], odd[CH];
   ns_acc acc[NB][NB] = {};
-  ns_fetch<T>(pre, P, pp, Q, pq, K, 0);
-  for (int k0 = 0; k0 < K; k0 += BK) {
+  // Past the end the last step is loaded again: with every load unconditional the compiler can count them, and waits for
+  // the older set alone.
+  const int steps = K / BK;
+  auto at = [&](int i) { return (i < steps ? i : steps - 1) * BK; };
+  ns_fetch<T>(even, P, pp, Q, pq, K, 0);
+  if constexpr (Tile::BUF == 2) {
+    ns_fetch<T>(odd, P, pp, Q, pq, K, at(1));
+    // one barrier per step: step i + 1 goes into the other buffer while step i is multiplied
+    ns_put<T>(even, lds, 0);
+    ns_fetch<T>(even, P, pp, Q, pq, K, at(2));
     __syncthreads();
-#pragma unroll
-    for (int q = 0; q < CH; ++q) {
-      const int x = q * RX_BLOCK + threadIdx.x;
-      const int ch = x % (BK / 8), row = x / (BK / 8) % T, pl = x / (BK / 8) / T % 2, op = x / (BK / 8) / T / 2;
-      *reinterpret_cast<ns_u4*>(&lds[op][pl][row][ch * 8]) = pre[q];
+    for (int i = 0; i < steps; i += 2) {
+      ns_put<T>(odd, lds, 1);
+      ns_fetch<T>(odd, P, pp, Q, pq, K, at(i + 3));
+      ns_step<T>(lds, 0, wi, wj, acc);
+      __syncthreads();
+      if (i + 1 == steps) break;
+      ns_put<T>(even, lds, 0);
+      ns_fetch<T>(even, P, pp, Q, pq, K, at(i + 4));
+      ns_step<T>(lds, 1, wi, wj, acc);
+      __syncthreads();
     }
-    __syncthreads();
-    if (k0 + BK < K) ns_fetch<T>(pre, P, pp, Q, pq, K, k0 + BK);
-#pragma unroll
-    for (int ks = 0; ks < BK; ks += 16) {
-      ns_h8 fa[NB][2], fb[NB][2];
-#pragma unroll
-      for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          fa[i][p] = *reinterpret_cast<const ns_h8*>(&lds[0][p][(wi * NB + i) * 32 + l31][ks + h * 8]);
-          fb[i][p] = *reinterpret_cast<const ns_h8*>(&lds[1][p][(wj * NB + i) * 32 + l31][ks + h * 8]);
-        }
-      constexpr int PA[3] = {1, 0, 0}, PB[3] = {0, 1, 0};             // the smaller products first
-#pragma unroll
-      for (int u = 0; u < 3; ++u)
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-          for (int j = 0; j < NB; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][PA[u]], fb[j][PB[u]], acc[i][j], 0, 0, 0);
+  } else {
+    for (int i = 0; i < steps; ++i) {
+      ns_put<T>(even, lds, 0);
+      __syncthreads();
+      ns_fetch<T>(even, P, pp, Q, pq, K, at(i + 1));
+      ns_step<T>(lds, 0, wi, wj, acc);
+      __syncthreads();
     }
   }
   // lane: column tj * T + .. + l31, rows 8 q + 4 h + k.  The transposed image is written from the registers, four rows
@@ -544,8 +607,7 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
   uint16_t* row_major = MODE == NS_MODE_A ? t.A : MODE == NS_MODE_B ? t.B : t.x[cur ^ 1];
   uint16_t* mirror = MODE == NS_MODE_A ? t.A : MODE == NS_MODE_B ? t.B : t.xt[cur ^ 1];
   const int64_t ldr = MODE == NS_MODE_X ? t.np : t.mp, plane = MODE == NS_MODE_X ? px : pm;
-  uint32_t (*turn)[36] = reinterpret_cast<uint32_t (*)[36]>(&lds[0][0][0][0]) + wave * 32;    // 32 x 32 words per wavefront
-  __syncthreads();
+  uint32_t (*turn)[36] = reinterpret_cast<uint32_t (*)[36]>(&lds[0][0][0][0][0]) + wave * 32;    // 32 x 32 words per wavefront
 #pragma unroll
   for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -709,11 +771,21 @@ static void ns_plan(const NsArgs& a, NsList* l, size_t* bytes, uint8_t* ws) {
 template <int T>
 static void ns_run(const NsList& l, hipStream_t st) {
   unsigned sym = 0, full = 0;
-  for (int i = 0; i < l.count; ++i) { sym += l.mat[i].tiles_sym; full += l.mat[i].tiles_x; }
-  sym = (sym + 7) / 8 * 8;
-  full = (full + 7) / 8 * 8;
+  for (int xcd = 0; xcd < 8; ++xcd) {
+    unsigned ns = 0, nf = 0;
+    int os = 0, of = 0, first;
+    for (int i = 0; i < l.count; ++i) {
+      ns += ns_run_of(l.mat[i].tiles_sym, xcd, os, &first);
+      nf += ns_run_of(l.mat[i].tiles_x, xcd, of, &first);
+      os += l.mat[i].tiles_sym;
+      of += l.mat[i].tiles_x;
+    }
+    if (ns > sym) sym = ns;
+    if (nf > full) full = nf;
+  }
+  sym *= 8;
+  full *= 8;
   for (int s = 0; s < l.steps; ++s) {
-    // a multiple of 8: the tiles are dealt to the XCDs in runs
     hipLaunchKernelGGL((ns_gemm_kernel<T, NS_MODE_A>), dim3(sym), dim3(RX_BLOCK), 0, st, l, s);
     hipLaunchKernelGGL((ns_gemm_kernel<T, NS_MODE_B>), dim3(sym), dim3(RX_BLOCK), 0, st, l, s);
     hipLaunchKernelGGL((ns_gemm_kernel<T, NS_MODE_X>), dim3(full), dim3(RX_BLOCK), 0, st, l, s);
