@@ -376,15 +376,24 @@ __global__ void __launch_bounds__(RX_BLOCK) ns_norm_kernel(NsList a) {
   const int64_t n = (int64_t)t.rows * t.cols;
   const float sc = a.scale ? *a.scale : 1.f;
   double s = 0.0;
-  for (int64_t i = (int64_t)pt * RX_BLOCK + threadIdx.x; i < n; i += (int64_t)NS_PARTS * RX_BLOCK) {
-    float u = t.g[i];
-    if (t.mom) {
-      float m = t.mom[i];
-      u = ns_update(u * sc, &m, a.mu, a.nesterov);
-      t.mom[i] = m;
+  const int64_t stride = (int64_t)NS_PARTS * RX_BLOCK;
+  for (int64_t i0 = (int64_t)pt * RX_BLOCK + threadIdx.x; i0 < n; i0 += 8 * stride) {
+    float u[8], m[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {              // eight values of a thread on their way at once
+      const int64_t i = i0 + k * stride;
+      u[k] = i < n ? t.g[i] : 0.f;
+      m[k] = t.mom && i < n ? t.mom[i] : 0.f;
     }
-    const double v = u;
-    s = fma(v, v, s);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int64_t i = i0 + k * stride;
+      if (t.mom && i < n) {
+        u[k] = ns_update(u[k] * sc, &m[k], a.mu, a.nesterov);
+        t.mom[i] = m[k];
+      }
+      s = fma((double)u[k], (double)u[k], s);
+    }
   }
   __shared__ double w[RX_BLOCK / 64];
   s = rx_wave_sum_f64(s);
@@ -414,30 +423,38 @@ __global__ void __launch_bounds__(RX_BLOCK) ns_init_kernel(NsList a) {
   const float sc = a.scale ? *a.scale : 1.f;
   const int r0 = b / (t.np / 64) * 64, c0 = b % (t.np / 64) * 64;      // of X
   const bool flip = t.rows > t.cols;
-  for (int i = threadIdx.x; i < 64 * 64; i += RX_BLOCK) {
-    const int y = i / 64, x = i % 64;
+  float v[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int i = k * RX_BLOCK + threadIdx.x, y = i / 64, x = i % 64;
     const int r = flip ? c0 + y : r0 + y, c = flip ? r0 + x : c0 + x;  // of G: rows of it are read along
-    float v = 0.f;
+    v[k] = 0.f;
     if (r < t.rows && c < t.cols) {
       const int64_t at = (int64_t)r * t.cols + c;
-      v = t.g[at];
-      if (t.mom) v = a.nesterov ? fmaf(a.mu, t.mom[at], v * sc) : t.mom[at];     // the norm's pass stored the new momentum
-      v /= div;
+      v[k] = t.g[at];
+      if (t.mom) v[k] = a.nesterov ? fmaf(a.mu, t.mom[at], v[k] * sc) : t.mom[at];     // the norm's pass stored the new momentum
     }
-    if (flip) tl[x][y] = v;
-    else tl[y][x] = v;
+  }
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int i = k * RX_BLOCK + threadIdx.x, y = i / 64, x = i % 64;
+    if (flip) tl[x][y] = v[k] / div * a.sx;
+    else tl[y][x] = v[k] / div * a.sx;
   }
   __syncthreads();
   const int64_t plane = (int64_t)t.mp * t.np;
-  for (int i = threadIdx.x; i < 64 * 32; i += RX_BLOCK) {
-    const int y = i / 32, x = i % 32 * 2;
-    uint32_t w[2];
-    ns_cut2(tl[y][x] * a.sx, tl[y][x + 1] * a.sx, w);
 #pragma unroll
-    for (int p = 0; p < 2; ++p) *reinterpret_cast<uint32_t*>(t.x[0] + p * plane + (int64_t)(r0 + y) * t.np + c0 + x) = w[p];
-    ns_cut2(tl[x][y] * a.sx, tl[x + 1][y] * a.sx, w);
+  for (int k = 0; k < 4; ++k) {
+    const int i = k * RX_BLOCK + threadIdx.x, y = i / 16, x = i % 16 * 4;
+    uint32_t w0[2], w1[2];
+    ns_cut2(tl[y][x], tl[y][x + 1], w0);
+    ns_cut2(tl[y][x + 2], tl[y][x + 3], w1);
 #pragma unroll
-    for (int p = 0; p < 2; ++p) *reinterpret_cast<uint32_t*>(t.xt[0] + p * plane + (int64_t)(c0 + y) * t.mp + r0 + x) = w[p];
+    for (int p = 0; p < 2; ++p) *reinterpret_cast<uint2*>(t.x[0] + p * plane + (int64_t)(r0 + y) * t.np + c0 + x) = make_uint2(w0[p], w1[p]);
+    ns_cut2(tl[x][y], tl[x + 1][y], w0);
+    ns_cut2(tl[x + 2][y], tl[x + 3][y], w1);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) *reinterpret_cast<uint2*>(t.xt[0] + p * plane + (int64_t)(c0 + y) * t.mp + r0 + x) = make_uint2(w0[p], w1[p]);
   }
 }
 
@@ -567,25 +584,22 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
   // Two sets of registers: a step's loads are issued two steps before it goes into LDS.
   ns_u4 even[CH], odd[CH];
   ns_acc acc[NB][NB] = {};
-  // Past the end the last step is loaded again: with every load unconditional the compiler can count them, and waits for
-  // the older set alone.
   const int steps = K / BK;
-  auto at = [&](int i) { return (i < steps ? i : steps - 1) * BK; };
   ns_fetch<T>(even, P, pp, Q, pq, K, 0);
   if constexpr (Tile::BUF == 2) {
-    ns_fetch<T>(odd, P, pp, Q, pq, K, at(1));
     // one barrier per step: step i + 1 goes into the other buffer while step i is multiplied
+    if (steps > 1) ns_fetch<T>(odd, P, pp, Q, pq, K, BK);
     ns_put<T>(even, lds, 0);
-    ns_fetch<T>(even, P, pp, Q, pq, K, at(2));
+    if (steps > 2) ns_fetch<T>(even, P, pp, Q, pq, K, 2 * BK);
     __syncthreads();
     for (int i = 0; i < steps; i += 2) {
-      ns_put<T>(odd, lds, 1);
-      ns_fetch<T>(odd, P, pp, Q, pq, K, at(i + 3));
+      if (i + 1 < steps) ns_put<T>(odd, lds, 1);
+      if (i + 3 < steps) ns_fetch<T>(odd, P, pp, Q, pq, K, (i + 3) * BK);
       ns_step<T>(lds, 0, wi, wj, acc);
       __syncthreads();
       if (i + 1 == steps) break;
-      ns_put<T>(even, lds, 0);
-      ns_fetch<T>(even, P, pp, Q, pq, K, at(i + 4));
+      if (i + 2 < steps) ns_put<T>(even, lds, 0);
+      if (i + 4 < steps) ns_fetch<T>(even, P, pp, Q, pq, K, (i + 4) * BK);
       ns_step<T>(lds, 1, wi, wj, acc);
       __syncthreads();
     }
@@ -593,7 +607,7 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
     for (int i = 0; i < steps; ++i) {
       ns_put<T>(even, lds, 0);
       __syncthreads();
-      ns_fetch<T>(even, P, pp, Q, pq, K, at(i + 1));
+      if (i + 1 < steps) ns_fetch<T>(even, P, pp, Q, pq, K, (i + 1) * BK);
       ns_step<T>(lds, 0, wi, wj, acc);
       __syncthreads();
     }
