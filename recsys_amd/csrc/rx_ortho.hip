@@ -5,8 +5,9 @@
 // below the diagonal are computed, the others are their mirror images).  Small singular values grow by up to a^steps = 485,
 // and so do rounding errors along them: 16-bit products would leave errors of the size of the result there, so the products
 // keep fp32 accuracy.
-// Operands are cut into two fp16 planes (11 + 11 significant bits); high high + high low + low high gives fp32 accuracy (what
-// is left out is below 2^-24 of a term) at a third of the 16-bit rate, where fp32 matrix instructions have a sixteenth.
+// Operands are cut into two fp16 planes (11 + 11 significant bits: the value to 2^-22) and multiplied as high high + high low
+// + low high.  What is left out is below 2^-22 of a term and differs in sign from term to term, so that the result is as near
+// the exact one as fp32 products leave it, at a third of the 16-bit rate, where fp32 matrix instructions have a sixteenth.
 // fp16 lacks range, but the iteration does not use it: |X|_2 <= 1 at the start and the coefficients bound it from there
 // on, so each array has one power-of-two scale that takes its bound to 2^15, found on the host.
 //   * Matrices that fit one workgroup's LDS take all steps in one launch: such lists are bound by launches and latency.
@@ -20,7 +21,6 @@
 typedef _Float16 ns_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 ns_h2 __attribute__((ext_vector_type(2)));
 typedef float ns_f2 __attribute__((ext_vector_type(2)));
-typedef uint32_t ns_u4 __attribute__((ext_vector_type(4)));   // HIP's uint4 kept the prefetch registers in scratch
 typedef float ns_f4 __attribute__((ext_vector_type(4)));
 typedef float ns_acc __attribute__((ext_vector_type(16)));
 
@@ -39,6 +39,9 @@ __device__ __forceinline__ void ns_cut2(float a, float b, uint32_t* w) {
   w[0] = __builtin_bit_cast(uint32_t, h);
   w[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, ns_h2));
 }
+// Planes in memory: the 32 high halves of a group of 32 elements, then its 32 low ones: 128 bytes, one cache line.  `ld`:
+// elements per row, a multiple of 32.
+__device__ __forceinline__ int64_t ns_at(int64_t row, int k, int ld) { return (row * ld + (k & ~31)) * 2 + (k & 31); }
 // four neighbouring values from their planes
 __device__ __forceinline__ void ns_join4(const uint16_t* p, int64_t plane, float* v) {
   const uint2 hi = *reinterpret_cast<const uint2*>(p), lo = *reinterpret_cast<const uint2*>(p + plane);
@@ -356,8 +359,8 @@ struct NsMat {
   float *out, *mom, *w;
   int32_t rows, cols;          // as given
   int32_t m, n, mp, np;        // working shape, and padded to the tile
-  uint16_t *x[2], *xt[2];      // [2][mp][np], [2][np][mp], alternating by step
-  uint16_t *A, *B;             // [2][mp][mp]
+  uint16_t *x[2], *xt[2];      // planes of [mp][np], [np][mp], alternating by step
+  uint16_t *A, *B;             // planes of [mp][mp]
   int32_t tiles_sym, tiles_x;
   float alpha;
 };
@@ -442,7 +445,6 @@ __global__ void __launch_bounds__(RX_BLOCK) ns_init_kernel(NsList a) {
     else tl[y][x] = v[k] / div * a.sx;
   }
   __syncthreads();
-  const int64_t plane = (int64_t)t.mp * t.np;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int i = k * RX_BLOCK + threadIdx.x, y = i / 16, x = i % 16 * 4;
@@ -450,74 +452,82 @@ __global__ void __launch_bounds__(RX_BLOCK) ns_init_kernel(NsList a) {
     ns_cut2(tl[y][x], tl[y][x + 1], w0);
     ns_cut2(tl[y][x + 2], tl[y][x + 3], w1);
 #pragma unroll
-    for (int p = 0; p < 2; ++p) *reinterpret_cast<uint2*>(t.x[0] + p * plane + (int64_t)(r0 + y) * t.np + c0 + x) = make_uint2(w0[p], w1[p]);
+    for (int p = 0; p < 2; ++p) *reinterpret_cast<uint2*>(t.x[0] + ns_at(r0 + y, c0 + x, t.np) + p * 32) = make_uint2(w0[p], w1[p]);
     ns_cut2(tl[x][y], tl[x + 1][y], w0);
     ns_cut2(tl[x + 2][y], tl[x + 3][y], w1);
 #pragma unroll
-    for (int p = 0; p < 2; ++p) *reinterpret_cast<uint2*>(t.xt[0] + p * plane + (int64_t)(c0 + y) * t.mp + r0 + x) = make_uint2(w0[p], w1[p]);
+    for (int p = 0; p < 2; ++p) *reinterpret_cast<uint2*>(t.xt[0] + ns_at(c0 + y, r0 + x, t.mp) + p * 32) = make_uint2(w0[p], w1[p]);
   }
 }
 
-// One T x T tile of P Q^T from planes P [2][.][K], Q [2][.][K]: four wavefronts, (T / 2)^2 each, BK of the contraction per
-// step.  Rows in LDS are an odd multiple of 16 bytes apart.
+// One T x T tile of P Q^T from the planes of P and Q: four wavefronts, (T / 2)^2 each, BK of the contraction per step.
+// A step of an operand lies in LDS as SUB groups of T rows of 128 bytes, brought there from memory without passing through
+// registers, 8 rows per instruction of a wavefront.  Such a load fills LDS in the order of the lanes, so rows cannot be padded
+// apart; instead the 16-byte chunks of row r change places by (r / 2) % 8, which has 16 neighbouring rows meet every bank.
 template <int T>
 struct NsTile {
   static constexpr int NB = T / 64;
-  static constexpr int BK = 64, LDK = BK + 8;
-  static constexpr int CH = 4 * T * (BK / 8) / RX_BLOCK;              // 16-byte chunks per thread and step
-  // Steps in LDS: two where few workgroups hide little of the loads' latency, one where two workgroups share a CU.
-  static constexpr int BUF = T == 64 ? 2 : 1;
-  typedef uint16_t Lds[BUF][2][2][T][LDK];
+  // Two steps of 32 KiB of both operands are in LDS, so that two workgroups share a CU.  Of a 3344 x 3344 product (T = 128)
+  // one workgroup per CU with four such steps took 411 us where two with two took 325, steps of 16 elements 390; of lists
+  // of 1024 x 1024 and less (T = 64) four steps were no faster.
+  static constexpr int SUB = T == 128 ? 1 : 2, BK = 32 * SUB;
+  static constexpr int OP = SUB * T * 64;                     // 16-bit elements of one operand's step
 };
 
 enum { NS_MODE_A, NS_MODE_B, NS_MODE_X };
 
-// chunk x of a step: 16 bytes of a row, the rows of a plane, the planes of an operand
-template <int T>
-__device__ __forceinline__ void ns_fetch(ns_u4 (&pre)[NsTile<T>::CH], const uint16_t* P, int64_t pp, const uint16_t* Q, int64_t pq, int K, int k0) {
-  constexpr int C = NsTile<T>::BK / 8;
-#pragma unroll
-  for (int q = 0; q < NsTile<T>::CH; ++q) {
-    const int x = q * RX_BLOCK + threadIdx.x;
-    const int ch = x % C, row = x / C % T, pl = x / C / T % 2, op = x / C / T / 2;
-    const uint16_t* src = op ? Q + pl * pq : P + pl * pp;
-    pre[q] = *reinterpret_cast<const ns_u4*>(src + (int64_t)row * K + k0 + ch * 8);
-  }
-}
+typedef __attribute__((address_space(3))) void* ns_shared;
 
+struct NsFeed {                // what a wavefront loads: its half of one operand's rows
+  const uint16_t* src;
+  int bytes;                   // of the half's rows: nothing behind them is read
+  int off[2];                  // of a lane, for even and odd groups of 8 rows
+  int rows8;                   // bytes from one group of 8 rows to the next
+};
+// 16 bytes per lane from src + lane_at + at (bytes) to 1 KiB of LDS, in the order of the lanes
+__device__ __forceinline__ void ns_load_lds(const uint16_t* src, int bytes, uint16_t* to, int lane_at, int at) {
+#ifdef __HIP_DEVICE_COMPILE__                                 // the host's pass does not know the type of a buffer descriptor
+  const auto d = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(src), 0, bytes, 0x27000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (ns_shared)to, 16, lane_at, at, 0, 0);
+#endif
+}
+// step i -> one LDS buffer
 template <int T>
-__device__ __forceinline__ void ns_put(const ns_u4 (&pre)[NsTile<T>::CH], typename NsTile<T>::Lds& lds, int buf) {
-  constexpr int C = NsTile<T>::BK / 8;
+__device__ __forceinline__ void ns_feed(const NsFeed& f, uint16_t* buf, int i) {
+  typedef NsTile<T> Tile;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint16_t* to = buf + (wave >> 1) * Tile::OP + (wave & 1) * (T / 2) * 64;
 #pragma unroll
-  for (int q = 0; q < NsTile<T>::CH; ++q) {
-    const int x = q * RX_BLOCK + threadIdx.x;
-    const int ch = x % C, row = x / C % T, pl = x / C / T % 2, op = x / C / T / 2;
-    *reinterpret_cast<ns_u4*>(&lds[buf][op][pl][row][ch * 8]) = pre[q];
-  }
+  for (int s = 0; s < Tile::SUB; ++s)
+#pragma unroll
+    for (int j = 0; j < T / 16; ++j)
+      ns_load_lds(f.src, f.bytes, to + s * T * 64 + j * 512, f.off[j & 1], j * f.rows8 + (i * Tile::SUB + s) * 128);
 }
 template <int T>
-__device__ __forceinline__ void ns_step(const typename NsTile<T>::Lds& lds, int buf, int wi, int wj, ns_acc (&acc)[NsTile<T>::NB][NsTile<T>::NB]) {
-  constexpr int NB = NsTile<T>::NB;
-  const int l31 = rx_lane() & 31, h = rx_lane() >> 5;
+__device__ __forceinline__ void ns_step(const uint16_t* buf, const int (&at)[2][2], int wi, int wj, ns_acc (&acc)[NsTile<T>::NB][NsTile<T>::NB]) {
+  typedef NsTile<T> Tile;
+  constexpr int NB = Tile::NB;
 #pragma unroll
-  for (int ks = 0; ks < NsTile<T>::BK; ks += 16) {
-    ns_h8 fa[NB][2], fb[NB][2];
+  for (int s = 0; s < Tile::SUB; ++s)
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        fa[i][p] = *reinterpret_cast<const ns_h8*>(&lds[buf][0][p][(wi * NB + i) * 32 + l31][ks + h * 8]);
-        fb[i][p] = *reinterpret_cast<const ns_h8*>(&lds[buf][1][p][(wj * NB + i) * 32 + l31][ks + h * 8]);
-      }
-    constexpr int PA[3] = {1, 0, 0}, PB[3] = {0, 1, 0};               // the smaller products first
-#pragma unroll
-    for (int u = 0; u < 3; ++u)
+    for (int ks = 0; ks < 2; ++ks) {
+      ns_h8 fa[NB][2], fb[NB][2];
 #pragma unroll
       for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][PA[u]], fb[j][PB[u]], acc[i][j], 0, 0, 0);
-  }
+        for (int p = 0; p < 2; ++p) {
+          fa[i][p] = *reinterpret_cast<const ns_h8*>(buf + (s * T + (wi * NB + i) * 32) * 64 + at[p][ks]);
+          fb[i][p] = *reinterpret_cast<const ns_h8*>(buf + Tile::OP + (s * T + (wj * NB + i) * 32) * 64 + at[p][ks]);
+        }
+      constexpr int PA[3] = {1, 0, 0}, PB[3] = {0, 1, 0};             // the smaller products first
+#pragma unroll
+      for (int u = 0; u < 3; ++u)
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int j = 0; j < NB; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][PA[u]], fb[j][PB[u]], acc[i][j], 0, 0, 0);
+    }
 }
 
 // Tile b of a product: bands of 8 tile rows, each band column by column, so that the 64 tiles an XCD works on at a time
@@ -554,8 +564,9 @@ __host__ __device__ __forceinline__ int ns_run_of(int k, int xcd, int off, int* 
 template <int T, int MODE>
 __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step) {
   typedef NsTile<T> Tile;
-  constexpr int NB = Tile::NB, CH = Tile::CH, BK = Tile::BK;
-  __shared__ __align__(16) typename Tile::Lds lds;
+  constexpr int NB = Tile::NB;
+  // two arrays: the compiler sees that loads into one and reads of the other do not meet
+  __shared__ __align__(128) uint16_t b0[2 * Tile::OP], b1[2 * Tile::OP];
   int mi = 0, b = blockIdx.x / 8, off = 0;
   for (; mi < a.count; ++mi) {
     const int k = MODE == NS_MODE_X ? a.mat[mi].tiles_x : a.mat[mi].tiles_sym;
@@ -570,48 +581,39 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
   const int cur = step & 1;
   int ti, tj;
   ns_tile<MODE == NS_MODE_X>(b, t.mp / T, t.np / T, &ti, &tj);
-  const int64_t pm = (int64_t)t.mp * t.mp, px = (int64_t)t.mp * t.np;
   const uint16_t *P, *Q;
-  int64_t pp, pq;
-  int K;
-  if (MODE == NS_MODE_A) { P = Q = t.x[cur]; pp = pq = px; K = t.np; }
-  else if (MODE == NS_MODE_B) { P = Q = t.A; pp = pq = pm; K = t.mp; }
-  else { P = t.B; pp = pm; Q = t.xt[cur]; pq = px; K = t.mp; }
-  P += (int64_t)ti * T * K;
-  Q += (int64_t)tj * T * K;
-  const int lane = rx_lane(), l31 = lane & 31, h = lane >> 5, wave = threadIdx.x >> 6;
+  int K, ld;
+  if (MODE == NS_MODE_A) { P = Q = t.x[cur]; K = t.np; ld = t.np; }
+  else if (MODE == NS_MODE_B) { P = Q = t.A; K = t.mp; ld = t.mp; }
+  else { P = t.B; Q = t.xt[cur]; K = t.mp; ld = t.mp; }
+  const int lane = rx_lane(), l31 = lane & 31, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave >> 1, wj = wave & 1;
-  // Two sets of registers: a step's loads are issued two steps before it goes into LDS.
-  ns_u4 even[CH], odd[CH];
+  NsFeed feed;
+  const uint16_t* mine = (wave >> 1 ? Q + (int64_t)tj * T * ld * 2 : P + (int64_t)ti * T * ld * 2) + (int64_t)(wave & 1) * (T / 2) * ld * 2;
+  feed.src = mine;
+  feed.bytes = (T / 2) * ld * 4;
+  feed.rows8 = 32 * ld;
+#pragma unroll
+  for (int o = 0; o < 2; ++o) feed.off[o] = (lane >> 3) * ld * 4 + ((lane & 7) ^ (o * 4 + (lane >> 4))) * 16;
+  int at[2][2];                // of a lane's fragment in a group of 32 rows, by plane and half of the 32
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) at[p][ks] = l31 * 64 + (((p * 4 + ks * 2 + h) ^ (l31 >> 1 & 7)) * 8);
   ns_acc acc[NB][NB] = {};
-  const int steps = K / BK;
-  ns_fetch<T>(even, P, pp, Q, pq, K, 0);
-  if constexpr (Tile::BUF == 2) {
-    // one barrier per step: step i + 1 goes into the other buffer while step i is multiplied
-    if (steps > 1) ns_fetch<T>(odd, P, pp, Q, pq, K, BK);
-    ns_put<T>(even, lds, 0);
-    if (steps > 2) ns_fetch<T>(even, P, pp, Q, pq, K, 2 * BK);
+  const int steps = K / Tile::BK;
+  ns_feed<T>(feed, b0, 0);
+  // One barrier per step: behind it step i is there for everybody (each wavefront has waited for its own loads) and everybody
+  // has done with step i - 1, whose buffer step i + 1 goes into.
+  auto stage = [&](int i, const uint16_t* now, uint16_t* next) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    for (int i = 0; i < steps; i += 2) {
-      if (i + 1 < steps) ns_put<T>(odd, lds, 1);
-      if (i + 3 < steps) ns_fetch<T>(odd, P, pp, Q, pq, K, (i + 3) * BK);
-      ns_step<T>(lds, 0, wi, wj, acc);
-      __syncthreads();
-      if (i + 1 == steps) break;
-      if (i + 2 < steps) ns_put<T>(even, lds, 0);
-      if (i + 4 < steps) ns_fetch<T>(even, P, pp, Q, pq, K, (i + 4) * BK);
-      ns_step<T>(lds, 1, wi, wj, acc);
-      __syncthreads();
-    }
-  } else {
-    for (int i = 0; i < steps; ++i) {
-      ns_put<T>(even, lds, 0);
-      __syncthreads();
-      if (i + 1 < steps) ns_fetch<T>(even, P, pp, Q, pq, K, (i + 1) * BK);
-      ns_step<T>(lds, 0, wi, wj, acc);
-      __syncthreads();
-    }
-  }
+    if (i + 1 < steps) ns_feed<T>(feed, next, i + 1);
+    ns_step<T>(now, at, wi, wj, acc);
+    return i + 1 < steps;
+  };
+  for (int i = 0; stage(i, b0, b1) && stage(i + 1, b1, b0); i += 2) {}
+  __syncthreads();
   // lane: column tj * T + .. + l31, rows 8 q + 4 h + k.  The transposed image is written from the registers, four rows
   // (8 bytes) at a time; the row-major one goes through LDS to be written 16 bytes at a time.
   const bool last = MODE == NS_MODE_X && step + 1 == a.steps;
@@ -620,8 +622,8 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
   const float scale = MODE == NS_MODE_A ? a.sa : MODE == NS_MODE_B ? a.sb : a.sx;
   uint16_t* row_major = MODE == NS_MODE_A ? t.A : MODE == NS_MODE_B ? t.B : t.x[cur ^ 1];
   uint16_t* mirror = MODE == NS_MODE_A ? t.A : MODE == NS_MODE_B ? t.B : t.xt[cur ^ 1];
-  const int64_t ldr = MODE == NS_MODE_X ? t.np : t.mp, plane = MODE == NS_MODE_X ? px : pm;
-  uint32_t (*turn)[36] = reinterpret_cast<uint32_t (*)[36]>(&lds[0][0][0][0][0]) + wave * 32;    // 32 x 32 words per wavefront
+  const int ldr = MODE == NS_MODE_X ? t.np : t.mp;
+  uint32_t (*turn)[36] = reinterpret_cast<uint32_t (*)[36]>(b0) + wave * 32;    // 32 x 32 words per wavefront
 #pragma unroll
   for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -631,8 +633,8 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
       for (int q = 0; q < 4; ++q) {
         const int r = r0 + 8 * q + 4 * h;
         float v[4], e[4];
-        if (MODE == NS_MODE_B) ns_join4(t.A + (int64_t)c * t.mp + r, pm, e);         // A is its own mirror image
-        if (MODE == NS_MODE_X) ns_join4(t.xt[cur] + (int64_t)c * t.mp + r, px, e);
+        if (MODE == NS_MODE_B) ns_join4(t.A + ns_at(c, r, t.mp), 32, e);         // A is its own mirror image
+        if (MODE == NS_MODE_X) ns_join4(t.xt[cur] + ns_at(c, r, t.mp), 32, e);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           v[k] = acc[i][j][4 * q + k] * undo;
@@ -653,7 +655,7 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
         ns_cut2(v[0] * scale, v[1] * scale, w0);
         ns_cut2(v[2] * scale, v[3] * scale, w1);
 #pragma unroll
-        for (int p = 0; p < 2; ++p) *reinterpret_cast<uint2*>(mirror + p * plane + (int64_t)c * t.mp + r) = make_uint2(w0[p], w1[p]);
+        for (int p = 0; p < 2; ++p) *reinterpret_cast<uint2*>(mirror + ns_at(c, r, t.mp) + p * 32) = make_uint2(w0[p], w1[p]);
         if (MODE == NS_MODE_X || ti != tj) {             // a diagonal tile is its own mirror image
           const int y = 8 * q + 4 * h;
           turn[y][l31] = (w0[0] & 0xffffu) | (w0[1] << 16);
@@ -671,7 +673,7 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
         const uint4 f = *reinterpret_cast<const uint4*>(&turn[y][x + 4 * k]);
         u[4 * k] = f.x; u[4 * k + 1] = f.y; u[4 * k + 2] = f.z; u[4 * k + 3] = f.w;
       }
-      uint16_t* d = row_major + (int64_t)(r0 + y) * ldr + tj * T + (wj * NB + j) * 32 + x;
+      uint16_t* d = row_major + ns_at(r0 + y, tj * T + (wj * NB + j) * 32 + x, ldr);
 #pragma unroll
       for (int p = 0; p < 2; ++p)
 #pragma unroll
@@ -679,7 +681,7 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
           uint32_t o[4];
 #pragma unroll
           for (int z = 0; z < 4; ++z) o[z] = __builtin_amdgcn_perm(u[8 * k + 2 * z + 1], u[8 * k + 2 * z], p ? 0x07060302u : 0x05040100u);
-          *reinterpret_cast<uint4*>(d + p * plane + 8 * k) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(d + p * 32 + 8 * k) = make_uint4(o[0], o[1], o[2], o[3]);
         }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
