@@ -13,9 +13,11 @@
 // are one number per lane, and the weights go straight back in as the other operand of the second product: its
 // contraction index may run in any order, and the transposed tile is laid out in the order the registers have.
 //
-// fp32 operands are cut into two fp16 planes (11 + 11 significant bits: the value to 2^-24) and multiplied as high high +
-// high low + low high in fp32: fp32 accuracy (what is left out is below 2^-24 of a term) from three products at the 16-bit
-// matrix rate, where fp32 matrix instructions run at 1/16 of it and three bf16 planes would take six products.  fp16 has no
+// fp32 operands are cut into two fp16 planes (11 + 11 significant bits: the value to 2^-22) and multiplied as high high +
+// high low + low high in fp32.  What is left out is below 2^-22 of a term, and such errors differ in sign from term to
+// term: sums of tens of terms come out as near the exact ones as fp32's own, whose additions round as often.  That takes
+// three products at the 16-bit matrix rate, where fp32 matrix instructions run at 1/16 of it and three bf16 planes would
+// take six products.  fp16 has no
 // range to spare, so everything is scaled by powers of two first, which costs no accuracy: a stationary vector by its
 // own largest element, a streaming tile by the tile's (both to 2^14 .. 2^15: elements down to 2^-15 of the largest keep
 // all their bits, smaller ones an absolute error of 2^-40 of it), and the weights by a running reference per stationary
@@ -43,11 +45,6 @@ typedef float ct_acc __attribute__((ext_vector_type(16)));
 // below 2^16 (a weight and a target's share on top of it), bf16 ones have room.
 #define CT_BASE(PL) ((PL) == 2 ? 6.f : 0.f)
 #define CT_TOP(PL) ((PL) == 2 ? 14.f : 24.f)
-#ifndef CT_NW64
-#define CT_NW64 4
-#define CT_NW32 4
-#define CT_OCC128 2
-#endif
 #define CT_THREADS 256
 #define CT_WAVES 4
 
@@ -207,7 +204,7 @@ __device__ __forceinline__ int ct_swz(int d, int c) {
   else return c ^ (((d & 2) | ((d >> 2) & 1)) ^ ((d >> 3) & 3));
 }
 
-template <typename T, int PL, int DP, int BN, bool TR, int NT>
+template <typename T, int PL, int DP, int BN, bool TR, int NT, bool MASK>
 struct CtStage {
   typedef CtTile<PL, DP, BN, TR, NT> Tile;
   // as they lie in memory: four floats, or four bf16 in two words, of four vectors
@@ -227,6 +224,24 @@ struct CtStage {
         else v[q][k] = ct_words4(base + (on ? row : 0) * ld, d, on ? D : 0, vec);
       }
     }
+  }
+  // Vectors whose item is out (bias -inf) become zeros, whatever they hold: their score is -inf all the same.
+  float bias[MASK ? Tile::PER : 1][4];
+  __device__ __forceinline__ void load_bias(const float* b, int64_t row0, int64_t rows) {
+#pragma unroll
+    for (int q = 0; q < Tile::PER; ++q)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t row = row0 + (q * NT + threadIdx.x) / (DP / 4) * 4 + k;
+        bias[q][k] = row < rows ? b[row] : 0.f;
+      }
+  }
+  __device__ __forceinline__ void drop() {
+#pragma unroll
+    for (int q = 0; q < Tile::PER; ++q)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (bias[q][k] == CT_NINF) v[q][k] = Quad{};
   }
   // bits of the largest magnitude the wavefront holds
   __device__ __forceinline__ uint32_t peak() const {
@@ -371,14 +386,16 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
   const int64_t row0 = ((int64_t)tile * NW + wave) * (32 * MB);
   const int64_t v0 = split * a.per_split, v1 = v0 + a.per_split < a.V ? v0 + a.per_split : a.V;
   const int n = (int)((v1 - v0 + BN - 1) / BN);             // tiles of this split, at least one
-  CtStage<T, PL, DP, BN, MEAN, NW * 64> stage;
+  CtStage<T, PL, DP, BN, MEAN, NW * 64, BIAS> stage;
   float nb = 0.f;
   auto fetch = [&](int i) {
     const int64_t v = v0 + (int64_t)i * BN;
     stage.load((const T*)a.t, a.ld_t, v, v1, a.D, a.vec);
+    if constexpr (BIAS) stage.load_bias(a.bias, v, v1);
     if (BIAS && threadIdx.x < BN) nb = v + threadIdx.x < v1 ? ct_bias2(a.bias[v + threadIdx.x]) : CT_NINF;
   };
   auto publish = [&](int i) {
+    if constexpr (BIAS) stage.drop();
     if constexpr (PL == 2) {
       const uint32_t m = stage.peak();
       if (rx_lane() == 0) lm[(i & 1) * NW + wave] = m;
@@ -650,7 +667,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
   const int64_t item0 = ((int64_t)tile * NW + wave) * (32 * MB);
   const int64_t r0 = split * a.per_split, r1 = r0 + a.per_split < a.R ? r0 + a.per_split : a.R;
   const int n = (int)((r1 - r0 + BN - 1) / BN);             // tiles of this split, at least one
-  CtStage<T, PL, DP, BN, true, NW * 64> stage;
+  CtStage<T, PL, DP, BN, true, NW * 64, false> stage;
   CtRow info;
   auto fetch = [&](int i) {
     const int64_t r = r0 + (int64_t)i * BN;
@@ -694,8 +711,9 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
     const int64_t item = item0 + mb * 32 + l31;
-    inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.t, a.ld_t, item, a.V, a.D, a.vec, st[mb]);
     b2[mb] = BIAS && item < a.V ? ct_bias2(a.bias[item]) : 0.f;
+    const bool out = b2[mb] == CT_NINF;                       // an item that is out may hold anything
+    inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.t, a.ld_t, item, out ? 0 : a.V, a.D, a.vec, st[mb]);
     dbias[mb] = 0.f;
     ref[mb] = PL == 2 ? CT_NINF : 0.f;
   }
@@ -860,9 +878,9 @@ static int ct_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 
           : dp == 64 ? X(uint16_t, 1, 64, 2, 64, 4, 2)                           \
           : dp == 128 ? X(uint16_t, 1, 128, 1, 64, 4, 2)                         \
                       : X(uint16_t, 1, 256, 1, 32, 4, 1)                         \
-   : dp == 32 ? X(float, 2, 32, 1, 64, CT_NW32, 2)                               \
-   : dp == 64 ? X(float, 2, 64, 1, 64, CT_NW64, 2)                               \
-   : dp == 128 ? X(float, 2, 128, 1, 32, 4, CT_OCC128)                           \
+   : dp == 32 ? X(float, 2, 32, 1, 64, 4, 2)                                     \
+   : dp == 64 ? X(float, 2, 64, 1, 64, 4, 2)                                     \
+   : dp == 128 ? X(float, 2, 128, 1, 32, 4, 2)                                   \
                : X(float, 2, 256, 1, 32, 4, 1))
 
 // stationary vectors per workgroup and streaming ones per tile, of the kernels in CT_KERNELS
@@ -928,7 +946,6 @@ extern "C" size_t rx_catalog_bwd_workspace_bytes(int64_t R, int64_t V, int32_t D
   return rx_align_up((size_t)R * sizeof(CtRow), 256) +
          (p.n_split > 1 ? rx_align_up((size_t)p.n_split * V * D * 4, 256) + (want_bias ? (size_t)p.n_split * V * 4 : 0) : 0);
 }
-
 
 template <typename K>
 static int ct_allow_lds(K kernel, int bytes) {
@@ -998,6 +1015,7 @@ extern "C" int rx_catalog_bwd(const rx_catalog_args* args, const float* d_stats,
   RX_REQUIRE(d_stats && ((uintptr_t)d_stats & 7) == 0, "rx_catalog_bwd: stats missing or not 8-byte aligned");
   RX_REQUIRE(!d_dx || d_mean, "rx_catalog_bwd: the gradient of x needs the means of the forward call");
   RX_REQUIRE(!d_dbias || (a.bias && d_dtable), "rx_catalog_bwd: the bias gradient needs a bias and comes with the table's");
+  RX_REQUIRE(!a.bias || !d_dtable || d_dbias, "rx_catalog_bwd: with a bias the table's gradient comes with the bias gradient");
   RX_REQUIRE(((uintptr_t)d_dtable & 15) == 0 && ((uintptr_t)d_dx & (a.bf16 ? 1 : 3)) == 0, "rx_catalog_bwd: gradient buffers not aligned");
   const bool want_t = d_dtable != nullptr;
   const size_t need = want_t ? rx_catalog_bwd_workspace_bytes(a.R, a.V, a.D, a.bf16, d_dbias != nullptr) : 0;
@@ -1017,10 +1035,8 @@ extern "C" int rx_catalog_bwd(const rx_catalog_args* args, const float* d_stats,
   const bool partial = p.n_split > 1;
   float* pt = (float*)w;
   float* pb = (float*)(w + rx_align_up((size_t)p.n_split * a.V * a.D * 4, 256));
-  // with a bias but no gradient asked for it, the pass still needs the bias: its sums then go to the partial's place
   CtBwd f = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, rows, a.D, p.tiles, p.n_split, p.per_split, ct_vec(&a),
              partial ? (void*)pt : d_dtable, partial ? (d_dbias ? pb : nullptr) : d_dbias, partial};
-  RX_REQUIRE(!a.bias || f.db, "rx_catalog_bwd: with a bias the table's gradient comes with the bias gradient");
 #define CT_GO(...) ct_pick_bwd<__VA_ARGS__>(f, st)
   const int rc = CT_KERNELS(CT_GO, a.bf16, ct_dp(a.D));
 #undef CT_GO

@@ -2,8 +2,9 @@
 
 A step amplifies an error along a small singular value by up to a = 3.44 and none by more than 4 (the largest slope of
 a s + b s^3 + c s^5 on [0, 1.2]), so no fixed multiple of 2^-24 describes the result: it is held to the error of the same
-iteration in plain fp32, whose products round K times per entry where these round 6 K / 16 times after plane products
-good to 2 u, times 4, plus 64 u of the result's norm for lists where the plain form happens to round to nothing."""
+iteration in plain fp32, whose products round K times per entry where these round 3 K / 16 times after plane products
+that hold a term to 12 u (two planes hold an operand to 2^-22 = 4 u, the product left out is below 4 u), times 4, plus 64 u
+of the result's norm: five steps at 12 u, for lists where the plain form happens to round to nothing."""
 import pytest
 import torch
 
