@@ -123,39 +123,72 @@ template <typename T> __device__ __forceinline__ float ct_elem(const T* p);
 template <> __device__ __forceinline__ float ct_elem<float>(const float* p) { return *p; }
 template <> __device__ __forceinline__ float ct_elem<uint16_t>(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
 
-// four consecutive elements [d, d + 4) of a row, zeros past D
+// four consecutive elements as they lie in memory, at any alignment of their own type: the hardware needs no more
+template <typename T> struct CtQuad;
+template <> struct CtQuad<float> { typedef float4 V; };
+template <> struct CtQuad<uint16_t> { typedef uint2 V; };
 template <typename T>
-__device__ __forceinline__ float4 ct_load4(const T* row, int d, int D, bool vec) {
-  if (vec && d + 4 <= D) {
-    if constexpr (sizeof(T) == 4) return *reinterpret_cast<const float4*>(row + d);
-    else {
-      const uint2 q = *reinterpret_cast<const uint2*>(row + d);
-      return make_float4(ct_lo(q.x), ct_hi(q.x), ct_lo(q.y), ct_hi(q.y));
-    }
+__device__ __forceinline__ typename CtQuad<T>::V ct_raw4(const T* p) {
+  typename CtQuad<T>::V v;
+  __builtin_memcpy(&v, p, sizeof(v));
+  return v;
+}
+__device__ __forceinline__ float4 ct_floats(const float4& q) { return q; }
+__device__ __forceinline__ float4 ct_floats(const uint2& q) { return make_float4(ct_lo(q.x), ct_hi(q.x), ct_lo(q.y), ct_hi(q.y)); }
+
+// `bytes` of memory: four elements from offset `at` on, zeros where that lies outside.  (The whole offset is in the vector
+// operand: the scalar one takes no part in the bounds check.)
+#define CT_MAXLD (1 << 22)       // 64 rows of four bytes apart at this distance: offsets stay below CT_OUTSIDE
+#define CT_OUTSIDE (1 << 30)
+struct CtBuffer {
+#ifdef __HIP_DEVICE_COMPILE__                                 // the host's pass does not know the type
+  __amdgpu_buffer_rsrc_t d;
+  __device__ __forceinline__ CtBuffer(const void* p, int bytes) : d(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x27000)) {}
+  __device__ __forceinline__ void load(float4& v, int at) const {
+    v = __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(d, at, 0, 0));
   }
+  __device__ __forceinline__ void load(uint2& v, int at) const {
+    v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(d, at, 0, 0));
+  }
+#else
+  __device__ CtBuffer(const void*, int) {}
+  template <typename V> __device__ void load(V&, int) const {}
+#endif
+};
+
+// elements [d, d + 4) of a row, zeros past D
+template <typename T>
+__device__ __forceinline__ float4 ct_load4(const T* row, int d, int D) {
+  if (d + 4 <= D) return ct_floats(ct_raw4(row + d));
   float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
   if (d < D) r.x = ct_elem(row + d);
   if (d + 1 < D) r.y = ct_elem(row + d + 1);
   if (d + 2 < D) r.z = ct_elem(row + d + 2);
-  if (d + 3 < D) r.w = ct_elem(row + d + 3);
   return r;
 }
-
-// the same four bf16 elements as two words
-__device__ __forceinline__ uint2 ct_words4(const uint16_t* row, int d, int D, bool vec) {
-  if (vec && d + 4 <= D) return *reinterpret_cast<const uint2*>(row + d);
+// the same of rows shorter than four elements, as it would lie in memory
+__device__ __forceinline__ float4 ct_short4(const float* row, int d, int D) { return ct_load4(row, d, D); }
+__device__ __forceinline__ uint2 ct_short4(const uint16_t* row, int d, int D) {
   uint2 r = make_uint2(0u, 0u);
   if (d < D) r.x = row[d];
   if (d + 1 < D) r.x |= (uint32_t)row[d + 1] << 16;
   if (d + 2 < D) r.y = row[d + 2];
-  if (d + 3 < D) r.y |= (uint32_t)row[d + 3] << 16;
   return r;
+}
+// elements moved down by n of four, zeros behind them
+__device__ __forceinline__ void ct_shift(float4& v, int n) {
+  if (n & 1) v = make_float4(v.y, v.z, v.w, 0.f);
+  if (n & 2) v = make_float4(v.z, v.w, 0.f, 0.f);
+}
+__device__ __forceinline__ void ct_shift(uint2& v, int n) {
+  const uint64_t u = ((uint64_t)v.y << 32 | v.x) >> (16 * n);
+  v = make_uint2((uint32_t)u, (uint32_t)(u >> 32));
 }
 
 // stationary operands of one block of 32 vectors: lane column l & 31, element ks * 16 + 8 (l >> 5) + j; returns what the
 // scores have to be multiplied with to undo the vector's scale
 template <typename T, int PL, int DP>
-__device__ __forceinline__ float ct_stationary(const T* base, int64_t ld, int64_t row, int64_t rows, int D, bool vec, CtFrag (*f)[PL]) {
+__device__ __forceinline__ float ct_stationary(const T* base, int64_t ld, int64_t row, int64_t rows, int D, CtFrag (*f)[PL]) {
   const int h = rx_lane() >> 5;
   const T* p = base + (row < rows ? row : 0) * ld;
   const int n = row < rows ? D : 0;
@@ -164,7 +197,7 @@ __device__ __forceinline__ float ct_stationary(const T* base, int64_t ld, int64_
     uint32_t peak = 0;
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
-      const float4 a = ct_load4(p, ks * 16 + h * 8, n, vec), b = ct_load4(p, ks * 16 + h * 8 + 4, n, vec);
+      const float4 a = ct_load4(p, ks * 16 + h * 8, n), b = ct_load4(p, ks * 16 + h * 8 + 4, n);
       peak = ct_umax(ct_umax(peak, ct_umax(ct_abs(a.x), ct_abs(a.y))), ct_umax(ct_abs(a.z), ct_abs(a.w)));
       peak = ct_umax(ct_umax(peak, ct_umax(ct_abs(b.x), ct_abs(b.y))), ct_umax(ct_abs(b.z), ct_abs(b.w)));
     }
@@ -172,7 +205,7 @@ __device__ __forceinline__ float ct_stationary(const T* base, int64_t ld, int64_
   }
 #pragma unroll
   for (int ks = 0; ks < DP / 16; ++ks) {
-    const float4 a = ct_load4(p, ks * 16 + h * 8, n, vec), b = ct_load4(p, ks * 16 + h * 8 + 4, n, vec);
+    const float4 a = ct_load4(p, ks * 16 + h * 8, n), b = ct_load4(p, ks * 16 + h * 8 + 4, n);
     float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
     if constexpr (PL == 2) {
 #pragma unroll
@@ -207,22 +240,33 @@ __device__ __forceinline__ int ct_swz(int d, int c) {
 template <typename T, int PL, int DP, int BN, bool TR, int NT, bool MASK>
 struct CtStage {
   typedef CtTile<PL, DP, BN, TR, NT> Tile;
-  // as they lie in memory: four floats, or four bf16 in two words, of four vectors
-  typedef typename std::conditional<sizeof(T) == 4, float4, uint2>::type Quad;
+  typedef typename CtQuad<T>::V Quad;          // as they lie in memory, of four vectors
   Quad v[Tile::PER][4];
-  // vectors [row0, row0 + BN) of the streaming side, zeros past `rows`
-  __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row0, int64_t rows, int D, bool vec) {
+  // Vectors [row0, row0 + BN) of the streaming side, zeros past `rows`.  A row's last, partial four elements are read as its
+  // last four and put in place by settle(): nothing here waits for what it loads.  The loads go through a buffer descriptor:
+  // what lies outside is zero without a branch, and one offset per block of a thread is all the registers they need.
+  __device__ __forceinline__ void load(const T* base, int64_t ld, int64_t row0, int64_t rows, int D) {
+    const int left = rows - row0 < BN ? (int)(rows - row0) : BN, step = (int)ld * (int)sizeof(T);
+    const CtBuffer b(base + row0 * ld, (left - 1) * step + D * (int)sizeof(T));
 #pragma unroll
     for (int q = 0; q < Tile::PER; ++q) {
       const int blk = q * NT + threadIdx.x;
-      const int d = blk % (DP / 4) * 4, i = blk / (DP / 4) * 4;
+      const int d = blk % (DP / 4) * 4, i = blk / (DP / 4) * 4, at = d + 4 <= D ? d : D - 4;
+      const bool on = d < D && (Tile::BLOCKS % NT == 0 || blk < Tile::BLOCKS);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int64_t row = row0 + i + k;
-        const bool on = row < rows && (Tile::BLOCKS % NT == 0 || blk < Tile::BLOCKS);
-        if constexpr (sizeof(T) == 4) v[q][k] = ct_load4(base + (on ? row : 0) * ld, d, on ? D : 0, vec);
-        else v[q][k] = ct_words4(base + (on ? row : 0) * ld, d, on ? D : 0, vec);
+        if (DP == 32 && D < 4) v[q][k] = i + k < left && on ? ct_short4(base + (row0 + i + k) * ld, d, D) : Quad{};
+        else b.load(v[q][k], on ? (i + k) * step + at * (int)sizeof(T) : CT_OUTSIDE);
       }
+    }
+  }
+  __device__ __forceinline__ void settle(int D) {
+    if (D % 4 == 0 || D < 4) return;
+#pragma unroll
+    for (int q = 0; q < Tile::PER; ++q) {
+      const int d = (q * NT + threadIdx.x) % (DP / 4) * 4, n = d < D && d + 4 > D ? d + 4 - D : 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) ct_shift(v[q][k], n);
     }
   }
   // Vectors whose item is out (bias -inf) become zeros, whatever they hold: their score is -inf all the same.
@@ -367,7 +411,6 @@ struct CtFwd {
   const float* bias;
   int D, tiles, n_split;
   int64_t per_split;           // items per split, a multiple of the tile
-  bool vec;
   float2* part;                // [n_split][R]: reference, sum
   float* out;                  // [n_split][R][D]: sum of weight * t_v
 };
@@ -390,11 +433,12 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
   float nb = 0.f;
   auto fetch = [&](int i) {
     const int64_t v = v0 + (int64_t)i * BN;
-    stage.load((const T*)a.t, a.ld_t, v, v1, a.D, a.vec);
+    stage.load((const T*)a.t, a.ld_t, v, v1, a.D);
     if constexpr (BIAS) stage.load_bias(a.bias, v, v1);
     if (BIAS && threadIdx.x < BN) nb = v + threadIdx.x < v1 ? ct_bias2(a.bias[v + threadIdx.x]) : CT_NINF;
   };
   auto publish = [&](int i) {
+    stage.settle(a.D);
     if constexpr (BIAS) stage.drop();
     if constexpr (PL == 2) {
       const uint32_t m = stage.peak();
@@ -422,7 +466,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
   float inv[MB], ref[MB], kr[MB], sum[MB];
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
-    inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.x, a.ld_x, row0 + mb * 32 + l31, a.R, a.D, a.vec, st[mb]);
+    inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.x, a.ld_x, row0 + mb * 32 + l31, a.R, a.D, st[mb]);
     ref[mb] = CT_NINF;
     kr[mb] = sum[mb] = 0.f;
   }
@@ -538,7 +582,9 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
   }
 }
 
-// One wavefront per row: joins the splits and takes the target's score as a plain dot product.
+// Joins a row's splits and takes the target's score as a plain dot product: TPR threads per row, which share out the splits as
+// well as the dimensions.  A wavefront per row (64) for up to 8 splits, where 8192 rows of 4 take 21 us against 29; a
+// workgroup (256) for more: 143 rows of 512 splits 50 us with the pass before it, against 170.
 struct CtJoin {
   const void *x, *t;
   int64_t ld_x, ld_t, R, V;
@@ -555,32 +601,57 @@ __device__ __forceinline__ float ct_dot(const T* x, const T* t, int D) {
   for (int d = rx_lane(); d < D; d += 64) s = fmaf(ct_elem(x + d), ct_elem(t + d), s);
   return rx_wave_sum(s);
 }
-template <typename T>
+// sum or maximum over a row's threads, in every one of them
+template <bool MAX, int TPR>
+__device__ __forceinline__ float ct_row(float v, float* w) {
+  for (int x = 32; x > 0; x >>= 1) v = MAX ? fmaxf(v, __shfl_xor(v, x, 64)) : v + __shfl_xor(v, x, 64);
+  if constexpr (TPR == 64) return v;
+  __syncthreads();
+  if (rx_lane() == 0) w[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return MAX ? fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])) : (w[0] + w[1]) + (w[2] + w[3]);
+}
+template <typename T, int TPR>
 __global__ void __launch_bounds__(CT_THREADS) ct_join_kernel(CtJoin a, int32_t* err) {
-  const int64_t row = (int64_t)blockIdx.x * CT_WAVES + (threadIdx.x >> 6);
-  if (row >= a.R) return;
-  const int lane = rx_lane();
+  __shared__ float w[CT_WAVES], sums[CT_THREADS];
+  const int64_t row = (int64_t)blockIdx.x * (CT_THREADS / TPR) + threadIdx.x / TPR;
+  const int lane = rx_lane(), tid = threadIdx.x % TPR;
+  if (TPR == 64 && row >= a.R) return;
   float ref = CT_NINF;
-  for (int q = lane; q < a.n_split; q += 64) ref = fmaxf(ref, a.part[(int64_t)q * a.R + row].x);
-  for (int x = 32; x > 0; x >>= 1) ref = fmaxf(ref, __shfl_xor(ref, x, 64));
+  for (int q = tid; q < a.n_split; q += TPR) ref = fmaxf(ref, a.part[(int64_t)q * a.R + row].x);
+  ref = ct_row<true, TPR>(ref, w);
   const float r0 = ref == CT_NINF ? 0.f : ref;
   float s = 0.f;
-  for (int q = lane; q < a.n_split; q += 64) {
+  for (int q = tid; q < a.n_split; q += TPR) {
     const float2 p = a.part[(int64_t)q * a.R + row];
     s += p.y * __builtin_amdgcn_exp2f(p.x - r0);
   }
-  s = rx_wave_sum(s);
+  s = ct_row<false, TPR>(s, w);
   const bool empty = s == 0.f;
   const float l2s = empty ? 0.f : log2f(s), lse = empty ? CT_NINF : (r0 + l2s) * CT_LN2;
   if (a.mean) {
-    const float inv = empty ? 0.f : 1.f / s;
-    for (int d = lane; d < a.D; d += 64) {
+    const int wide = a.D <= 32 ? 32 : a.D <= 64 ? 64 : a.D <= 128 ? 128 : 256;
+    const int dp = wide < TPR ? wide : TPR, groups = TPR / dp;      // threads along the dimensions, and along the splits
+    for (int d0 = 0; d0 < a.D; d0 += dp) {
+      const int d = d0 + tid % dp;
       float m = 0.f;
-      for (int q = 0; q < a.n_split; ++q)
-        m = fmaf(a.out[((int64_t)q * a.R + row) * a.D + d], __builtin_amdgcn_exp2f(a.part[(int64_t)q * a.R + row].x - r0), m);
-      a.mean[row * a.D + d] = m * inv;
+      if (d < a.D) {
+#pragma unroll 4
+        for (int q = tid / dp; q < a.n_split; q += groups)
+          m = fmaf(a.out[((int64_t)q * a.R + row) * a.D + d], __builtin_amdgcn_exp2f(a.part[(int64_t)q * a.R + row].x - r0), m);
+      }
+      if constexpr (TPR == 64) {
+        if (groups == 2) m += __shfl_xor(m, 32, 64);
+      } else {
+        sums[tid] = m;
+        __syncthreads();
+        if (tid < dp)
+          for (int k = 1; k < groups; ++k) m += sums[k * dp + tid];
+      }
+      if (tid < dp && d < a.D) a.mean[row * a.D + d] = empty ? 0.f : m / s;
     }
   }
+  if (tid >= 64) return;
   const int64_t y = a.targets[row];
   const bool ok = y >= 0 && y < a.V;
   float lp;
@@ -649,7 +720,6 @@ struct CtBwd {
   const CtRow* rows;
   int D, tiles, n_split;
   int64_t per_split;           // rows per split, a multiple of the tile
-  bool vec;
   void* dt;                    // [V][D] in the table's type, or fp32 [n_split][V][D]
   float* db;                   // [V], or [n_split][V]
   bool partial;
@@ -671,13 +741,14 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
   CtRow info;
   auto fetch = [&](int i) {
     const int64_t r = r0 + (int64_t)i * BN;
-    stage.load((const T*)a.x, a.ld_x, r, r1, a.D, a.vec);
+    stage.load((const T*)a.x, a.ld_x, r, r1, a.D);
     if (threadIdx.x < BN) {
       if (r + threadIdx.x < r1) info = a.rows[r + threadIdx.x];
       else { info.m2 = 0.f; info.l2s = info.z = __builtin_inff(); info.sgn = 1.f; info.g = 0.f; info.y = -1; }
     }
   };
   auto publish = [&](int i) {      // before the barrier in front of put(i): the largest magnitude, the sign words
+    stage.settle(a.D);
     if constexpr (PL == 2) {
       const uint32_t m = stage.peak();
       if (lane == 0) lm[(i & 1) * NW + wave] = m;
@@ -713,7 +784,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
     const int64_t item = item0 + mb * 32 + l31;
     b2[mb] = BIAS && item < a.V ? ct_bias2(a.bias[item]) : 0.f;
     const bool out = b2[mb] == CT_NINF;                       // an item that is out may hold anything
-    inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.t, a.ld_t, item, out ? 0 : a.V, a.D, a.vec, st[mb]);
+    inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.t, a.ld_t, item, out ? 0 : a.V, a.D, st[mb]);
     dbias[mb] = 0.f;
     ref[mb] = PL == 2 ? CT_NINF : 0.f;
   }
@@ -740,7 +811,8 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
     // rows of this tile whose target is among the wavefront's items
     const int64_t rel = lane < BN && ly[lane] >= 0 ? ly[lane] - item0 : -1;
     const uint64_t hits = __ballot(rel >= 0 && rel < 32 * MB);
-#pragma unroll
+  // bf16, 128 wide and with a bias: both halves of a tile at once spill 44 registers (1203 us against 721 at 8192 x 100k)
+#pragma unroll BIAS && PL == 1 && DP == 128 ? 1 : BN / 32
     for (int it = 0; it < BN / 32; ++it) {
       const bool hit = (uint32_t)(hits >> (it * 32)) != 0;
 #pragma unroll
@@ -863,6 +935,7 @@ __global__ void __launch_bounds__(CT_THREADS) ct_sum_kernel(const float* __restr
     const float* p = b ? part_b + (i - n) : part + i;
     const int64_t step = b ? nb : n;
     float s = 0.f;
+#pragma unroll 8
     for (int q = 0; q < n_split; ++q) s += p[q * step];
     if (b) out_b[i - n] = s;
     else if constexpr (sizeof(T) == 4) out[i] = s;
@@ -871,39 +944,53 @@ __global__ void __launch_bounds__(CT_THREADS) ct_sum_kernel(const float* __restr
 }
 
 // ---------------------------------------------------------------- host
-static int ct_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+static int ct_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : D <= 192 ? 192 : 256; }
 // X(T, PL, DP, MB, BN, NW, OCC): the kernels there are, one per element type and padded width
 #define CT_KERNELS(X, bf16, dp)                                                  \
   (bf16 ? dp == 32 ? X(uint16_t, 1, 32, 2, 64, 4, 2)                             \
           : dp == 64 ? X(uint16_t, 1, 64, 2, 64, 4, 2)                           \
+          : dp == 96 ? X(uint16_t, 1, 96, 1, 64, 4, 2)                           \
           : dp == 128 ? X(uint16_t, 1, 128, 1, 64, 4, 2)                         \
+          : dp == 192 ? X(uint16_t, 1, 192, 1, 32, 4, 1)                         \
                       : X(uint16_t, 1, 256, 1, 32, 4, 1)                         \
    : dp == 32 ? X(float, 2, 32, 1, 64, 4, 2)                                     \
    : dp == 64 ? X(float, 2, 64, 1, 64, 4, 2)                                     \
+   : dp == 96 ? X(float, 2, 96, 1, 32, 4, 2)                                     \
    : dp == 128 ? X(float, 2, 128, 1, 32, 4, 2)                                   \
+   : dp == 192 ? X(float, 2, 192, 1, 32, 4, 1)                                   \
                : X(float, 2, 256, 1, 32, 4, 1))
 
 // stationary vectors per workgroup and streaming ones per tile, of the kernels in CT_KERNELS
 #define CT_BM(T, PL, DP, MB, BN, NW, OCC) ((NW) * 32 * (MB))
 #define CT_BN(T, PL, DP, MB, BN, NW, OCC) (BN)
+#define CT_OCC(T, PL, DP, MB, BN, NW, OCC) (OCC)
 
 struct CtPlan {
   int tiles, n_split;
   int64_t per_split;
 };
-// `fixed` vectors are stationary, `moving` ones stream: enough splits of the stream for four workgroups per CU, each of
-// at least two tiles; multiples of 8 (one XCD each) where there are many.
-static CtPlan ct_plan(int64_t fixed, int64_t moving, int bm, int bn) {
+// `fixed` vectors are stationary, `moving` ones stream.  The number of splits is the one with the least time by this
+// estimate, in tiles of the stream: rounds of `slots` workgroups (what the chip holds at a time), each as long as its share of
+// the stream and two tiles more for the stationary vectors and the result; a last round that leaves every other workgroup
+// of a CU out takes 0.65 of one; a partial result on its way to memory and back costs 1/200, a pass that adds them up `join`.
+// At 372 x 17389 x 240 (fp32) this takes 85 splits where four workgroups per CU were 341: 91 against 169 us.
+static CtPlan ct_plan(int64_t fixed, int64_t moving, int bm, int bn, int slots, float join) {
   CtPlan p;
   p.tiles = (int)rx_cdiv(fixed, bm);
-  int64_t n = rx_cdiv(1024, p.tiles);
-  const int64_t most = rx_cdiv(moving, 2 * bn);
-  if (n > most) n = most;
-  if (n > 64) n = n / 8 * 8;
-  if (n < 1) n = 1;
-  p.per_split = rx_cdiv(rx_cdiv(moving, n), bn) * bn;
+  const int64_t stream = rx_cdiv(moving, bn);
+  const int64_t most = stream < 8 * slots / p.tiles + 1 ? stream : 8 * slots / p.tiles + 1;
+  float best = 0.f;
+  p.per_split = 0;
+  for (int64_t n = 1; n <= most; n += n < 64 ? 1 : 8) {
+    const int64_t per = rx_cdiv(stream, n), blocks = p.tiles * rx_cdiv(stream, per), rest = blocks % slots;
+    const float rounds = (float)(blocks / slots) + (rest == 0 ? 0.f : rest > slots / 2 || slots == 256 ? 1.f : 0.65f);
+    const float cost = rounds * (float)(per + 2) + (per < stream ? (float)blocks / 200.f + join : 0.f);
+    if (p.per_split == 0 || cost < best) {
+      best = cost;
+      p.per_split = per * bn;
+    }
+  }
   p.n_split = (int)rx_cdiv(moving, p.per_split);
-  if (p.n_split < 1) p.n_split = 1;
   return p;
 }
 
@@ -912,6 +999,8 @@ static int ct_check(const rx_catalog_args* a, const char* who) {
   RX_REQUIRE(a->R >= 0 && a->R <= (1 << 24) && a->V >= 1 && a->V <= (1ll << 30) && a->D >= 1 && a->D <= CT_MAXD,
              "%s: bad shape R=%lld V=%lld D=%d (R up to 2^24, V up to 2^30, D up to %d)", who, (long long)a->R, (long long)a->V, a->D, CT_MAXD);
   RX_REQUIRE(a->ld_x >= a->D && a->ld_t >= a->D, "%s: row strides %lld, %lld below D=%d", who, (long long)a->ld_x, (long long)a->ld_t, a->D);
+  RX_REQUIRE(a->ld_x <= CT_MAXLD && a->ld_t <= CT_MAXLD, "%s: rows %lld, %lld elements apart (at most %d)", who, (long long)a->ld_x,
+             (long long)a->ld_t, CT_MAXLD);
   RX_REQUIRE(a->bf16 == 0 || a->bf16 == 1, "%s: bad element type %d", who, a->bf16);
   if (a->R == 0) return 0;
   RX_REQUIRE(a->x && a->table && a->targets, "%s: null argument", who);
@@ -919,20 +1008,17 @@ static int ct_check(const rx_catalog_args* a, const char* who) {
   RX_REQUIRE(((uintptr_t)a->x & al) == 0 && ((uintptr_t)a->table & al) == 0, "%s: x or table not aligned to their elements", who);
   return 0;
 }
-static bool ct_vec(const rx_catalog_args* a) {      // 4-element loads
-  const uintptr_t al = a->bf16 ? 7 : 15;
-  return a->D % 4 == 0 && a->ld_x % 4 == 0 && a->ld_t % 4 == 0 && ((uintptr_t)a->x & al) == 0 && ((uintptr_t)a->table & al) == 0;
-}
-
 static CtPlan ct_fwd_plan(int64_t R, int64_t V, int D, int bf16) {
   const int dp = ct_dp(D);
-  return ct_plan(R, V, CT_KERNELS(CT_BM, bf16, dp), CT_KERNELS(CT_BN, bf16, dp));
+  return ct_plan(R, V, CT_KERNELS(CT_BM, bf16, dp), CT_KERNELS(CT_BN, bf16, dp), 256 * CT_KERNELS(CT_OCC, bf16, dp), 0.f);
 }
 static CtPlan ct_bwd_plan(int64_t R, int64_t V, int D, int bf16, bool bias) {
   const int dp = ct_dp(D);
   // two blocks and a bias do not fit the registers of two wavefronts per SIMD: one there (ct_pick_bwd)
   const int bm = CT_KERNELS(CT_BM, bf16, dp) / (bf16 && dp == 64 && bias ? 2 : 1);
-  return ct_plan(V, R, bm, CT_KERNELS(CT_BN, bf16, dp));
+  // the narrow fp32 kernel uses few enough registers for three workgroups per CU
+  const int occ = !bf16 && dp == 32 ? 3 : CT_KERNELS(CT_OCC, bf16, dp);
+  return ct_plan(V, R, bm, CT_KERNELS(CT_BN, bf16, dp), 256 * occ, 0.8f);
 }
 
 extern "C" size_t rx_catalog_fwd_workspace_bytes(int64_t R, int64_t V, int32_t D, int32_t bf16, int32_t want_mean) {
@@ -991,7 +1077,7 @@ extern "C" int rx_catalog_fwd(const rx_catalog_args* args, float* d_logprob, flo
   const CtPlan p = ct_fwd_plan(a.R, a.V, a.D, a.bf16);
   float2* part = (float2*)ws;
   float* out = d_mean ? (float*)((uint8_t*)ws + rx_align_up((size_t)p.n_split * a.R * sizeof(float2), 256)) : nullptr;
-  CtFwd f = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, a.D, p.tiles, p.n_split, p.per_split, ct_vec(&a), part, out};
+  CtFwd f = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, a.D, p.tiles, p.n_split, p.per_split, part, out};
   hipStream_t st = (hipStream_t)stream;
 #define CT_GO(...) ct_pick_fwd<__VA_ARGS__>(f, st)
   const int rc = CT_KERNELS(CT_GO, a.bf16, ct_dp(a.D));
@@ -999,9 +1085,10 @@ extern "C" int rx_catalog_fwd(const rx_catalog_args* args, float* d_logprob, flo
   if (rc) return rc;
   RX_LAUNCH_CHECK();
   CtJoin j = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, a.targets, a.D, p.n_split, part, out, d_logprob, d_lse, d_stats, d_mean};
-  const dim3 grid((unsigned)rx_cdiv(a.R, CT_WAVES));
-  if (a.bf16) hipLaunchKernelGGL(ct_join_kernel<uint16_t>, grid, dim3(CT_THREADS), 0, st, j, err_flag);
-  else hipLaunchKernelGGL(ct_join_kernel<float>, grid, dim3(CT_THREADS), 0, st, j, err_flag);
+  const bool few = p.n_split <= 8;
+  auto join = few ? (a.bf16 ? ct_join_kernel<uint16_t, 64> : ct_join_kernel<float, 64>)
+                  : (a.bf16 ? ct_join_kernel<uint16_t, 256> : ct_join_kernel<float, 256>);
+  hipLaunchKernelGGL(join, dim3((unsigned)(few ? rx_cdiv(a.R, CT_WAVES) : a.R)), dim3(CT_THREADS), 0, st, j, err_flag);
   RX_LAUNCH_CHECK();
   return 0;
 }
@@ -1035,7 +1122,7 @@ extern "C" int rx_catalog_bwd(const rx_catalog_args* args, const float* d_stats,
   const bool partial = p.n_split > 1;
   float* pt = (float*)w;
   float* pb = (float*)(w + rx_align_up((size_t)p.n_split * a.V * a.D * 4, 256));
-  CtBwd f = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, rows, a.D, p.tiles, p.n_split, p.per_split, ct_vec(&a),
+  CtBwd f = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, rows, a.D, p.tiles, p.n_split, p.per_split,
              partial ? (void*)pt : d_dtable, partial ? (d_dbias ? pb : nullptr) : d_dbias, partial};
 #define CT_GO(...) ct_pick_bwd<__VA_ARGS__>(f, st)
   const int rc = CT_KERNELS(CT_GO, a.bf16, ct_dp(a.D));
