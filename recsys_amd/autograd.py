@@ -1032,6 +1032,21 @@ def bce_with_logits(logits: Tensor, labels: Tensor) -> Tensor:
 
 
 # ------------------------------------------------------------------ list-wise log-probabilities
+def _mind_recordings(out: Tensor) -> None:
+    """A backward pass must not be recorded while an eager graph over the same leaves is alive: their accumulation nodes stay
+    bound to the legacy default stream, which the recording would drag in (graph.refuse_live_autograd_graphs).  Nodes seen
+    on that stream are marked, and a recording that meets a mark is refused."""
+    if ops.on_default_stream(out):
+        for node, _ in out.grad_fn.next_functions:
+            if type(node).__name__ == "AccumulateGrad":
+                node.metadata["rx_default_stream"] = True
+    elif torch.cuda.is_current_stream_capturing():
+        for node, _ in out.grad_fn.next_functions:
+            if type(node).__name__ == "AccumulateGrad" and "rx_default_stream" in node.metadata:
+                raise RuntimeError("cannot record this call: an autograd graph made on the default stream still references its "
+                                   "inputs (outputs kept alive?); delete or detach them first")
+
+
 class LogProb(Function):
     """ops.logprob_fwd with its gradient (rx_logprob_bwd) to the scores; the alternatives carry none."""
 
@@ -1063,7 +1078,9 @@ def log_probs(logits: Tensor, targets: Tensor, lengths: Optional[Tensor] = None,
     targets, lengths = targets.contiguous(), None if lengths is None else lengths.contiguous()
     if not (logits.requires_grad and torch.is_grad_enabled()):
         return ops.logprob_fwd(logits, targets, lengths, k)[0]
-    return ops.LogProbs(*LogProb.apply(logits, targets, lengths, k))
+    out = ops.LogProbs(*LogProb.apply(logits, targets, lengths, k))
+    _mind_recordings(out.logprob)
+    return out
 
 
 class MeanNLL(Function):
@@ -1095,33 +1112,27 @@ def gather_rows(table: Tensor, idx: Tensor) -> Tensor:
 
 
 # ------------------------------------------------------------------ softmax over a whole catalogue
-_ALL_ROWS: dict = {}
-
-
 def all_rows(n_rows: int, device) -> SortedIndex:
     """The index list 0 .. n_rows - 1 as its own sort, for a gradient that touches every row of a table."""
-    key = (int(n_rows), torch.device(device))
-    si = _ALL_ROWS.get(key)
-    if si is None:
-        i32 = torch.arange(n_rows + 1, dtype=torch.int32, device=device)
-        si = SortedIndex(n_rows, n_rows, i32[:n_rows], i32[:n_rows], torch.arange(n_rows, device=device), i32,
-                         torch.full((1,), n_rows, dtype=torch.int32, device=device))
-        if not (torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing()):
-            if torch.device(device).type == "cuda":
-                torch.cuda.current_stream(device).synchronize()      # once: any stream may read it from here on
-            _ALL_ROWS[key] = si          # a recording keeps its own copy in its pool
-            while len(_ALL_ROWS) > 16:
-                _ALL_ROWS.pop(next(iter(_ALL_ROWS)))
-    return si
+    i32 = torch.arange(n_rows + 1, dtype=torch.int32, device=device)
+    return SortedIndex(n_rows, n_rows, i32[:n_rows], i32[:n_rows], torch.arange(n_rows, device=device), i32,
+                       torch.full((1,), n_rows, dtype=torch.int32, device=device))
 
 
 def full_table_backward(param: Tensor, grad: Tensor):
     """A gradient for every row of ``param``: handed on as it is, or applied through the parameter's fused sparse
     rule (all rows touched) when it carries one."""
-    if getattr(param, "_rx_sparse", None) is None:
+    rule = getattr(param, "_rx_sparse", None)
+    if rule is None:
         return grad
-    rows = param.shape[0]
-    return table_backward(param, all_rows(rows, param.device), grad.reshape(rows, -1), dim=grad.numel() // rows)
+    rows, si = param.shape[0], rule.every_row
+    if si is None or si.n_rows != rows or si.sorted_pos.device != param.device:
+        si = all_rows(rows, param.device)
+        if not (param.is_cuda and torch.cuda.is_current_stream_capturing()):      # a recording keeps its own copy in its pool
+            if param.is_cuda:
+                torch.cuda.current_stream(param.device).synchronize()             # once: any stream may read it from here on
+            rule.every_row = si
+    return table_backward(param, si, grad.reshape(rows, -1), dim=grad.numel() // rows)
 
 
 class CatalogLogProb(Function):
@@ -1158,6 +1169,11 @@ def catalog_logprob(x: Tensor, table: Tensor, targets: Tensor, bias: Optional[Te
     if x.dim() == 2 and ((x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
         x = x.contiguous()
     targets = targets.contiguous()
+    _before_table_read(table)
+    if bias is not None:
+        _before_table_read(bias)
     if not (torch.is_grad_enabled() and (x.requires_grad or table.requires_grad or (bias is not None and bias.requires_grad))):
         return ops.catalog_fwd(x, table, targets, bias)[:2]
-    return CatalogLogProb.apply(x, table, targets, bias)
+    out = CatalogLogProb.apply(x, table, targets, bias)
+    _mind_recordings(out[0])
+    return out

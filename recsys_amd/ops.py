@@ -64,6 +64,11 @@ def _after_index_op(device) -> None:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # the handle without a Stream object around it: 0.2 against 2 us
 
 
+def on_default_stream(t: Tensor) -> bool:
+    """Whether the current stream of the tensor's device is the legacy default stream."""
+    return (_raw_stream(_dev(t)) if _raw_stream is not None else torch.cuda.current_stream(t.device).cuda_stream) == 0
+
+
 def _stream(t: Tensor):
     if _raw_stream is not None:
         return C.c_void_p(_raw_stream(_dev(t)))
@@ -1569,7 +1574,22 @@ def catalog_bwd(x: Tensor, table: Tensor, targets: Tensor, bias: Optional[Tensor
 
 
 # ------------------------------------------------------------------ orthogonalised updates
+ORTHO_MAX_DIM = 16384
 ORTHO_COEFFS = (3.4445, -4.7750, 2.0315)     # a, b, c of X <- a X + (b A + c A A) X, A = X X^T
+
+
+def _apart(who: str, reads: Sequence[Tensor], writes: Sequence[Tensor]) -> None:
+    """Lists of more than one chunk: no written tensor may overlap another tensor of the list (within a chunk the library looks)."""
+    if len(reads) <= _lib.RX_ORTHO_MAX:
+        return
+    spans = sorted([(t.data_ptr(), t.data_ptr() + 4 * t.numel(), False) for t in reads] +
+                   [(t.data_ptr(), t.data_ptr() + 4 * t.numel(), True) for t in writes])
+    end = wend = 0              # furthest ends so far, of all and of the written ones
+    for lo, hi, written in spans:
+        if lo < (end if written else wend):
+            raise ValueError(f"{who}: buffers overlap")
+        end = max(end, hi)
+        wend = max(wend, hi) if written else wend
 
 
 def orthogonalize(mats: Sequence[Tensor], steps: int = 5, coeffs=ORTHO_COEFFS, eps: float = 1e-7,
@@ -1595,6 +1615,7 @@ def orthogonalize(mats: Sequence[Tensor], steps: int = 5, coeffs=ORTHO_COEFFS, e
         if m.numel() == 0:
             raise ValueError(f"orthogonalize: matrix {i} is empty")
         _same_device(mats[0], m, o)
+    _apart("orthogonalize", mats, out)
     for i in range(0, len(mats), _lib.RX_ORTHO_MAX):
         a = OrthoArgs()
         part = list(zip(mats, out))[i:i + _lib.RX_ORTHO_MAX]
@@ -1630,6 +1651,7 @@ def muon_step(ws: Sequence[Tensor], gs: Sequence[Tensor], moms: Sequence[Tensor]
             raise ValueError("scale: one element")
         if n:
             _same_device(ws[0], scale)
+    _apart("muon_step", gs, list(ws) + list(moms))
     for i in range(0, n, _lib.RX_ORTHO_MAX):
         a = MuonArgs()
         c = min(n - i, _lib.RX_ORTHO_MAX)

@@ -44,6 +44,7 @@ class SparseRule:
     def __init__(self, kind: str, lr: float, eps: float, owner: "FusedOptimizer"):
         self.kind, self.mode, self.lr, self.eps, self.owner = kind, _MODES[kind], lr, eps, owner
         self.state: Optional[torch.Tensor] = None
+        self.every_row = None      # autograd.full_table_backward: the list of all rows, laid out once
 
     def _state_for(self, param):
         if self.kind == "sgd":
@@ -160,7 +161,7 @@ class FusedOptimizer:
     ``kind`` in {"sgd", "adagrad", "rowwise_adagrad"} applies to the parameters the model lists
     in ``model.sparse_parameters()``; all other parameters are stepped densely with
     ``dense_kind`` (default: "sgd" for sgd, "adagrad" otherwise; "adam" and "muon" allowed).
-    ``dense_kind="muon"``: weight matrices (both sides of two or more) take momentum steps along the orthogonalised
+    ``dense_kind="muon"``: weight matrices (both sides of 2 .. 16384) take momentum steps along the orthogonalised
     update (ops.muon_step: ``momentum``, Nesterov form, learning rate ``lr * sqrt(max(1, rows / cols))``), everything
     else (biases, normalisation, one-row layers) takes Adam with ``adam_lr`` (default ``lr``).
     ``speculative``: whether clipped SGD over field groups takes its step inside the backward's reduce and redoes
@@ -448,7 +449,7 @@ class FusedOptimizer:
         return out
 
     def _is_muon(self, p) -> bool:
-        return self.dense_kind == "muon" and p.dim() == 2 and min(p.shape) >= 2
+        return self.dense_kind == "muon" and p.dim() == 2 and min(p.shape) >= 2 and max(p.shape) <= ops.ORTHO_MAX_DIM
 
     def _dense_state_for(self, p):
         st = self._dense_state.get(id(p))

@@ -19,6 +19,7 @@ def _cat(**kw):
 
 @pytest.mark.parametrize("kw,text", [(dict(D=0), b"bad shape"), (dict(D=257, ld_x=257, ld_t=257), b"bad shape"), (dict(V=0), b"bad shape"),
                                      (dict(R=-1), b"bad shape"), (dict(R=(1 << 24) + 1), b"bad shape"), (dict(V=(1 << 30) + 1), b"bad shape"),
+                                     (dict(ld_x=(1 << 22) + 1), b"apart"), (dict(ld_t=1 << 40), b"apart"),
                                      (dict(ld_x=7), b"row strides"), (dict(ld_t=7), b"row strides"), (dict(bf16=3), b"element type"),
                                      (dict(x=0), b"null"), (dict(table=0), b"null"), (dict(targets=0), b"null"), (dict(table=4098), b"aligned")])
 def test_catalog_refusals(kw, text):
@@ -70,6 +71,21 @@ def test_ortho_and_muon_refusals():
     both(lambda a: a.cols.__setitem__(0, 16385), b"matrix 0")
     both(lambda a: a.g.__setitem__(0, 0), b"null")
     both(lambda a: a.g.__setitem__(0, (1 << 30) + 64), b"overlap")
+
+
+def test_overlaps_in_lists_longer_than_a_chunk():
+    import torch
+    from recsys_amd.ops import _apart
+    a = [torch.zeros(4, 5) for _ in range(30)]
+    b = [torch.zeros(4, 5) for _ in range(30)]
+    _apart("x", a, b)
+    _apart("x", a[:1] * 30, b)                    # what is only read may be the same
+    _apart("x", a[:5], a[:5])                     # short lists are the library's to check
+    flat = torch.zeros(2000)
+    for writes in (b[:29] + b[:1], b[:29] + a[:1], [flat[0:20].view(4, 5)] + b[:28] + [flat[19:39].view(4, 5)]):
+        with pytest.raises(ValueError, match="overlap"):
+            _apart("x", a, writes)
+    _apart("x", a, [flat[0:20].view(4, 5)] + b[:28] + [flat[20:40].view(4, 5)])
 
 
 def test_struct_layouts(tmp_path):
