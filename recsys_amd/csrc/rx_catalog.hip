@@ -778,14 +778,14 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
   };
   fetch(0);
   CtFrag st[MB][DP / 16][PL];
-  float inv[MB], b2[MB], dbias[MB], ref[MB];      // ref: of w = 2^(log2 (|c| p) + kt - ref); PL == 1 keeps it at 0
+  float inv[MB], b2[MB], dbias[MB], lost[MB], ref[MB];      // ref: of w = 2^(log2 (|c| p) + kt - ref); PL == 1 keeps it at 0
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
     const int64_t item = item0 + mb * 32 + l31;
     b2[mb] = BIAS && item < a.V ? ct_bias2(a.bias[item]) : 0.f;
     const bool out = b2[mb] == CT_NINF;                       // an item that is out may hold anything
     inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.t, a.ld_t, item, out ? 0 : a.V, a.D, st[mb]);
-    dbias[mb] = 0.f;
+    dbias[mb] = lost[mb] = 0.f;
     ref[mb] = PL == 2 ? CT_NINF : 0.f;
   }
   ct_acc o[MB][DP / 32] = {};
@@ -842,6 +842,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
               if (ref[mb] != CT_NINF) {
                 const float f = __builtin_amdgcn_exp2f(ref[mb] - (n - CT_BASE(PL)));
                 dbias[mb] *= f;
+                lost[mb] *= f;
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
@@ -862,9 +863,16 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
             if (ly[k] == mine) w[e] = fmaf(lg[k], up, w[e]);
           }
         }
-        if constexpr (BIAS) {
+        if constexpr (BIAS) {       // a sum over all rows: 16 at a time, each sum joined with the rounding that the last join lost
+          float part[4];
 #pragma unroll
-          for (int e = 0; e < 16; ++e) dbias[mb] = fmaf(w[e], ct_at(lsg + it * 32 + 8 * (e / 4) + 4 * h, e % 4), dbias[mb]);
+          for (int q = 0; q < 4; ++q) {
+            const float* sg = lsg + it * 32 + 8 * q + 4 * h;
+            part[q] = fmaf(w[4 * q + 1], ct_at(sg, 1), w[4 * q] * ct_at(sg, 0)) + fmaf(w[4 * q + 3], ct_at(sg, 3), w[4 * q + 2] * ct_at(sg, 2));
+          }
+          const float add = ((part[0] + part[1]) + (part[2] + part[3])) - lost[mb], sum = dbias[mb] + add;
+          lost[mb] = (sum - dbias[mb]) - add;
+          dbias[mb] = sum;
         }
         ct_weigh<PL, DP, BN>(tr, it, w, o[mb]);
         if (PL == 1 && hit) {     // a target's share is as large as the whole gradient: what bf16 dropped of these weights goes in too
