@@ -10,7 +10,7 @@
 // the exact one as fp32 products leave it, at a third of the 16-bit rate, where fp32 matrix instructions have a sixteenth.
 // fp16 lacks range, but the iteration does not use it: |X|_2 <= 1 at the start and the coefficients bound it from there
 // on, so each array has one power-of-two scale that takes its bound to 2^15, found on the host.
-//   * Matrices that fit one workgroup's LDS take all steps in one launch: such lists are bound by launches and latency.
+//   * Matrices that fit one workgroup's LDS take all steps in one launch (ns_split): such lists are bound by launches and latency.
 //   * The others share three launches per step, whatever their number.  X, X^T, A and B live in the workspace as planes, cut
 //     once in the epilogue that makes them; with X^T kept beside X all three products read both operands along the
 //     contraction.
@@ -741,12 +741,32 @@ static int ns_bounds(const char* who, double ca, double cb, double cc, int steps
 // power of two that takes a bound, with a margin for rounding, to at most 2^15
 static float ns_scale_of(float bound) { return bound > 0.f ? ldexpf(1.f, 14 - ilogbf(bound * 1.1f)) : 1.f; }
 
+// Which matrices take a workgroup of their own.  All that fit one do, but in a list that needs the large path anyway they join
+// it while all its 64 x 64 tiles are on the chip at once: its launches take little longer for them (845 x 13, 63 x 257, 300 x 7,
+// 1 x 1 and 129 x 130: 137 us, 162 with a launch for the small four).
+static void ns_split(const NsArgs& a, bool* small) {
+  int64_t big = 0, all = 0;
+  bool large = false;
+  for (int i = 0; i < a.count; ++i) {
+    small[i] = ns_is_small(a.rows[i], a.cols[i]);
+    all += rx_cdiv(a.rows[i], 64) * rx_cdiv(a.cols[i], 64);
+    if (!small[i]) {
+      large = true;
+      big += rx_cdiv(a.rows[i], 128) * rx_cdiv(a.cols[i], 128);
+    }
+  }
+  if (large && big < 256 && all <= 512)
+    for (int i = 0; i < a.count; ++i) small[i] = false;
+}
+
 // Tile: 128 once the largest product of the list fills the chip with such tiles, 64 for the parallelism otherwise.
 static void ns_plan(const NsArgs& a, NsList* l, size_t* bytes, uint8_t* ws) {
   memset(l, 0, sizeof(*l));
+  bool small[RX_ORTHO_MAX];
+  ns_split(a, small);
   int order[RX_ORTHO_MAX], k = 0;
   for (int i = 0; i < a.count; ++i)
-    if (!ns_is_small(a.rows[i], a.cols[i])) {
+    if (!small[i]) {
       int at = k++;
       auto cost = [&](int x) { return a.rows[x] < a.cols[x] ? a.rows[x] : a.cols[x]; };
       while (at > 0 && cost(order[at - 1]) < cost(i)) { order[at] = order[at - 1]; --at; }   // longest contractions first
@@ -823,10 +843,12 @@ static int ns_go(const char* who, NsArgs& a, void* ws, size_t ws_bytes, int devi
   s.steps = a.steps; s.nesterov = a.nesterov; s.mu = a.mu; s.scale = a.scale;
   s.a = a.a; s.b = a.b; s.c = a.c; s.eps = a.eps;
   s.sx = a.sx; s.sa = a.sa; s.sb = a.sb;
+  bool small[RX_ORTHO_MAX];
+  ns_split(a, small);
   int k = 0;
   size_t lds = 0;
   for (int i = 0; i < a.count; ++i)
-    if (ns_is_small(a.rows[i], a.cols[i])) {
+    if (small[i]) {
       s.g[k] = a.g[i]; s.out[k] = a.out[i]; s.mom[k] = a.mom[i]; s.w[k] = a.w[i]; s.alpha[k] = a.alpha[i];
       s.rows[k] = a.rows[i]; s.cols[k] = a.cols[i];
       const size_t b = ns_small_lds(a.rows[i], a.cols[i]);
