@@ -25,6 +25,9 @@
 // bf16 operands take one plane, exactly; there the weights of the second product are rounded to bf16 as well, 2^-9
 // relative and independent from term to term, as much as the result's own rounding.
 // Scores, references, sums, means and gradients accumulate in fp32.
+// Measured, where a large bf16 product reaches 1151 TFLOP/s: 2048 x 1000003 x 64 fp32 forward 1.72 ms, table gradient 1.83 (914 and
+// 860 TFLOP/s of plane products), 8192 x 100003 x 128 bf16 515 and 600 us (814 and 699).  What keeps them from more is the
+// work beside the products: an exponential, two cuts and a transposed copy.  1024 x 3706 x 64 fp32: 16 and 24 us, latency.
 #include "rx_common.h"
 
 #include <type_traits>
