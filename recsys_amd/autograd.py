@@ -1034,17 +1034,14 @@ def bce_with_logits(logits: Tensor, labels: Tensor) -> Tensor:
 # ------------------------------------------------------------------ list-wise log-probabilities
 def _mind_recordings(out: Tensor) -> None:
     """A backward pass must not be recorded while an eager graph over the same leaves is alive: their accumulation nodes stay
-    bound to the legacy default stream, which the recording would drag in (graph.refuse_live_autograd_graphs).  Nodes seen
-    on that stream are marked, and a recording that meets a mark is refused."""
-    if ops.on_default_stream(out):
-        for node, _ in out.grad_fn.next_functions:
-            if type(node).__name__ == "AccumulateGrad":
-                node.metadata["rx_default_stream"] = True
-    elif torch.cuda.is_current_stream_capturing():
-        for node, _ in out.grad_fn.next_functions:
-            if type(node).__name__ == "AccumulateGrad" and "rx_default_stream" in node.metadata:
-                raise RuntimeError("cannot record this call: an autograd graph made on the default stream still references its "
-                                   "inputs (outputs kept alive?); delete or detach them first")
+    bound to the legacy default stream, which the recording would drag in (graph.refuse_live_autograd_graphs).  A node is
+    marked with whether these calls first met it on that stream, and a recording that meets such a one is refused."""
+    default = ops.on_default_stream(out)
+    recording = not default and torch.cuda.is_current_stream_capturing()
+    for node, _ in out.grad_fn.next_functions:
+        if type(node).__name__ == "AccumulateGrad" and node.metadata.setdefault("rx_default_stream", default) and recording:
+            raise RuntimeError("cannot record this call: an autograd graph made on the default stream still references its "
+                               "inputs (outputs kept alive?); delete or detach them first")
 
 
 class LogProb(Function):
