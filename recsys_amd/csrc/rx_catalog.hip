@@ -55,7 +55,8 @@ struct CtRow {               // what the backward pass needs of a row
   float m2, l2s, z, sgn;     // p_rv |c_r| = 2^(s log2 e - m2 - l2s), z = m2 + l2s, sgn = sign of c_r
   float g;                   // gradient of logprob (0 where the row has no target)
   int32_t y;                 // target or -1
-  int32_t pad0, pad1;
+  float gl2;                // log2 |g|
+  int32_t pad;
 };
 
 union CtFrag { uint4 u; ct_h8 h; ct_f8 f; };
@@ -703,7 +704,8 @@ __global__ void __launch_bounds__(CT_THREADS) ct_prep_kernel(CtPrep a) {
     r.z = r.m2 + r.l2s;
     r.g = g;
     r.y = (int32_t)y;
-    r.pad0 = r.pad1 = 0;
+    r.gl2 = log2f(fabsf(g));
+    r.pad = 0;
     a.rows[row] = r;
   }
   if (a.dx) {
@@ -732,8 +734,8 @@ template <typename T, int PL, int DP, int MB, int BN, bool BIAS, int NW, int OCC
 __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
   typedef CtTile<PL, DP, BN, true, NW * 64> Tile;
   extern __shared__ __align__(16) uint8_t ct_lds[];
-  float* lz0 = reinterpret_cast<float*>(ct_lds + 2 * Tile::BYTES); // [2][6][BN], see below
-  uint32_t* lm = reinterpret_cast<uint32_t*>(lz0 + 12 * BN);       // [2][NW] largest magnitudes
+  float* lz0 = reinterpret_cast<float*>(ct_lds + 2 * Tile::BYTES); // [2][7][BN], see below
+  uint32_t* lm = reinterpret_cast<uint32_t*>(lz0 + 14 * BN);       // [2][NW] largest magnitudes
   int tile, split;
   ct_place(a.tiles, a.n_split, &tile, &split);
   const int wave = threadIdx.x >> 6, lane = rx_lane(), l31 = lane & 31, h = lane >> 5;
@@ -747,7 +749,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
     stage.load((const T*)a.x, a.ld_x, r, r1, a.D);
     if (threadIdx.x < BN) {
       if (r + threadIdx.x < r1) info = a.rows[r + threadIdx.x];
-      else { info.m2 = 0.f; info.l2s = info.z = __builtin_inff(); info.sgn = 1.f; info.g = 0.f; info.y = -1; }
+      else { info.m2 = 0.f; info.l2s = info.z = __builtin_inff(); info.sgn = 1.f; info.g = 0.f; info.gl2 = CT_NINF; info.y = -1; }
     }
   };
   auto publish = [&](int i) {      // before the barrier in front of put(i): the largest magnitude, the sign words
@@ -756,7 +758,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
       const uint32_t m = stage.peak();
       if (lane == 0) lm[(i & 1) * NW + wave] = m;
     }
-    if (threadIdx.x < BN) reinterpret_cast<uint32_t*>(lz0 + (i & 1) * 6 * BN)[5 * BN + threadIdx.x] = info.sgn < 0.f ? 0x80008000u : 0u;
+    if (threadIdx.x < BN) reinterpret_cast<uint32_t*>(lz0 + (i & 1) * 7 * BN)[5 * BN + threadIdx.x] = info.sgn < 0.f ? 0x80008000u : 0u;
   };
   auto put = [&](int i) -> float {
     float scale = 1.f;
@@ -767,13 +769,14 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
       scale = ct_scale(m);
     }
     const float kt = PL == 2 ? -ct_log2(scale) : 0.f;
-    float* lz = lz0 + (i & 1) * 6 * BN;
+    float* lz = lz0 + (i & 1) * 7 * BN;
     if (threadIdx.x < BN) {
       float* p = lz + threadIdx.x;
       p[0] = BIAS ? info.m2 : info.z - kt;
       if (BIAS) { p[BN] = info.l2s - kt; p[2 * BN] = info.sgn * scale; }     // sign of c, with the tile's scale undone
       p[3 * BN] = info.g * info.sgn;
       reinterpret_cast<int32_t*>(p)[4 * BN] = info.y;
+      p[6 * BN] = info.gl2 + kt;
     }
     uint16_t* rm = reinterpret_cast<uint16_t*>(ct_lds + (i & 1) * Tile::BYTES);
     stage.store(rm, rm + Tile::RM, reinterpret_cast<const uint32_t*>(lz + 5 * BN), scale);
@@ -807,12 +810,13 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
     }
     const uint16_t* rm = reinterpret_cast<const uint16_t*>(ct_lds + (i & 1) * Tile::BYTES);
     const uint16_t* tr = rm + Tile::RM;
-    const float* lz = lz0 + (i & 1) * 6 * BN;             // z, or m2 with a bias
-    const float *ll = lz + BN, *lsg = lz + 2 * BN, *lg = lz + 3 * BN;
-    const int32_t* ly = reinterpret_cast<const int32_t*>(lz + 4 * BN);
+    const float* lz = lz0 + (i & 1) * 7 * BN;             // z, or m2 with a bias
+    const float *ll = lz + BN, *lsg = lz + 2 * BN, *lg = lz + 3 * BN, *lgl = lz + 6 * BN;
+    const float* ly = lz + 4 * BN;                        // int32 targets
     const float kt = PL == 2 ? -ct_log2(scale) : 0.f, back = ct_inverse(scale);
     // rows of this tile whose target is among the wavefront's items
-    const int64_t rel = lane < BN && ly[lane] >= 0 ? ly[lane] - item0 : -1;
+    const int32_t of = lane < BN ? __float_as_int(ly[lane]) : -1;
+    const int64_t rel = of >= 0 ? of - item0 : -1;
     const uint64_t hits = __ballot(rel >= 0 && rel < 32 * MB);
   // bf16, 128 wide and with a bias: both halves of a tile at once spill 44 registers (1203 us against 721 at 8192 x 100k)
 #pragma unroll BIAS && PL == 1 && DP == 128 ? 1 : BN / 32
@@ -830,13 +834,13 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
           else w[e] = fmaf(s[e], mul, -ct_at(lz + k, e % 4));
           if (PL == 2) mx = fmaxf(mx, w[e]);
         }
-        const int64_t mine = item0 + mb * 32 + l31;
+        const int32_t mine = (int32_t)(item0 + mb * 32 + l31);
         if constexpr (PL == 2) {
           if (hit) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const int k = it * 32 + 8 * (e / 4) + 4 * h + e % 4;
-              if (ly[k] == mine) mx = fmaxf(mx, log2f(fabsf(lg[k])) + kt);
+              const int k = it * 32 + 8 * (e / 4) + 4 * h;
+              mx = fmaxf(mx, __float_as_int(ct_at(ly + k, e % 4)) == mine ? ct_at(lgl + k, e % 4) : CT_NINF);
             }
           }
           if (__ballot(mx > ref[mb] + CT_TOP(PL))) {
@@ -862,8 +866,9 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
           const float up = PL == 2 ? __builtin_amdgcn_exp2f(kt - rf) : 1.f;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int k = it * 32 + 8 * (e / 4) + 4 * h + e % 4;
-            if (ly[k] == mine) w[e] = fmaf(lg[k], up, w[e]);
+            const int k = it * 32 + 8 * (e / 4) + 4 * h;
+            const float share = fmaf(ct_at(lg + k, e % 4), up, w[e]);
+            w[e] = __float_as_int(ct_at(ly + k, e % 4)) == mine ? share : w[e];
           }
         }
         if constexpr (BIAS) {       // a sum over all rows: 16 at a time, each sum joined with the rounding that the last join lost
@@ -1065,7 +1070,7 @@ static int ct_pick_fwd(const CtFwd& f, hipStream_t st) {
 template <typename T, int PL, int DP, int MB, int BN, int NW, int OCC, bool BIAS>
 static int ct_go_bwd(const CtBwd& f, hipStream_t st) {
   auto kernel = ct_bwd_kernel<T, PL, DP, MB, BN, BIAS, NW, OCC>;
-  const int lds = 2 * CtTile<PL, DP, BN, true, NW * 64>::BYTES + 12 * BN * 4 + 2 * NW * 4;
+  const int lds = 2 * CtTile<PL, DP, BN, true, NW * 64>::BYTES + 14 * BN * 4 + 2 * NW * 4;
   if (ct_allow_lds(kernel, lds)) return 1;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(f.tiles * f.n_split)), dim3(NW * 64), lds, st, f);
   return 0;
