@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(RX_BLOCK) ns_init_kernel(NsList a) {
 // apart; instead the 16-byte chunks of row r change places by (r / 2) % 8, which has 16 neighbouring rows meet every bank.
 template <int T>
 struct NsTile {
-  static constexpr int NB = T / 64;
+  static constexpr int NB = T / 64, SUMS = T == 64 ? 3 : 2;
   // Two steps of 32 KiB of both operands are in LDS, so that two workgroups share a CU.  Of a 3344 x 3344 product (T = 128)
   // one workgroup per CU with four such steps took 411 us where two with two took 325, steps of 16 elements 390; of lists
   // of 1024 x 1024 and less (T = 64) four steps were no faster.
@@ -506,8 +506,10 @@ __device__ __forceinline__ void ns_feed(const NsFeed& f, uint16_t* buf, int i) {
     for (int j = 0; j < T / 16; ++j)
       ns_load_lds(f.src, f.bytes, to + s * T * 64 + j * 512, f.off[j & 1], j * f.rows8 + (i * Tile::SUB + s) * 128);
 }
+// acc: high high products, and the two others; of T = 64 the first in two sums.  Each addition into a sum rounds at its size:
+// with all in one, matrices of 33 x 1400 came out with 2.2 times the error of fp32 products.
 template <int T>
-__device__ __forceinline__ void ns_step(const uint16_t* buf, const int (&at)[2][2], int wi, int wj, ns_acc (&acc)[NsTile<T>::NB][NsTile<T>::NB]) {
+__device__ __forceinline__ void ns_step(const uint16_t* buf, const int (&at)[2][2], int wi, int wj, ns_acc (&acc)[NsTile<T>::SUMS][NsTile<T>::NB][NsTile<T>::NB]) {
   typedef NsTile<T> Tile;
   constexpr int NB = Tile::NB;
 #pragma unroll
@@ -522,14 +524,16 @@ __device__ __forceinline__ void ns_step(const uint16_t* buf, const int (&at)[2][
           fa[i][p] = *reinterpret_cast<const ns_h8*>(buf + (s * T + (wi * NB + i) * 32) * 64 + at[p][ks]);
           fb[i][p] = *reinterpret_cast<const ns_h8*>(buf + Tile::OP + (s * T + (wj * NB + i) * 32) * 64 + at[p][ks]);
         }
-      constexpr int PA[3] = {1, 0, 0}, PB[3] = {0, 1, 0};             // the smaller products first
+      constexpr int PA[3] = {1, 0, 0}, PB[3] = {0, 0, 1};
 #pragma unroll
       for (int u = 0; u < 3; ++u)
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
-          for (int j = 0; j < NB; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][PA[u]], fb[j][PB[u]], acc[i][j], 0, 0, 0);
+          for (int j = 0; j < NB; ++j) {
+            ns_acc& c = acc[u != 1 ? 0 : T == 64 ? 1 + ks : 1][i][j];
+            c = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i][PA[u]], fb[j][PB[u]], c, 0, 0, 0);
+          }
     }
 }
 
@@ -603,7 +607,7 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
   for (int p = 0; p < 2; ++p)
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) at[p][ks] = l31 * 64 + (((p * 4 + ks * 2 + h) ^ (l31 >> 1 & 7)) * 8);
-  ns_acc acc[NB][NB] = {};
+  ns_acc sums[Tile::SUMS][NB][NB] = {};
   const int steps = K / Tile::BK;
   ns_feed<T>(feed, b0, 0);
   // One barrier per step: behind it step i is there for everybody (each wavefront has waited for its own loads) and everybody
@@ -612,10 +616,12 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (i + 1 < steps) ns_feed<T>(feed, next, i + 1);
-    ns_step<T>(now, at, wi, wj, acc);
-    return i + 1 < steps;
+    ns_step<T>(now, at, wi, wj, sums);
   };
-  for (int i = 0; stage(i, b0, b1) && stage(i + 1, b1, b0); i += 2) {}
+  for (int i = 0; i < steps; i += 2) {
+    stage(i, b0, b1);
+    if (i + 1 < steps) stage(i + 1, b1, b0);
+  }
   __syncthreads();
   // lane: column tj * T + .. + l31, rows 8 q + 4 h + k.  The transposed image is written from the registers, four rows
   // (8 bytes) at a time; the row-major one goes through LDS to be written 16 bytes at a time.
@@ -640,7 +646,7 @@ __global__ void __launch_bounds__(RX_BLOCK, 2) ns_gemm_kernel(NsList a, int step
         if (MODE == NS_MODE_X) ns_join4(t.xt[cur] + ns_at(c, r, t.mp), 32, e);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          v[k] = acc[i][j][4 * q + k] * undo;
+          v[k] = (sums[0][i][j][4 * q + k] + (T == 64 ? sums[1][i][j][4 * q + k] + sums[Tile::SUMS - 1][i][j][4 * q + k] : sums[1][i][j][4 * q + k])) * undo;
           if (MODE == NS_MODE_B) v[k] = fmaf(a.b / a.sa, e[k], a.c * v[k]);
           if (MODE == NS_MODE_X) v[k] = fmaf(a.a / a.sx, e[k], v[k]);
         }
@@ -746,7 +752,8 @@ static float ns_scale_of(float bound) { return bound > 0.f ? ldexpf(1.f, 14 - il
 
 // Which matrices take a workgroup of their own.  All that fit one do, but in a list that needs the large path anyway they join
 // it while all its 64 x 64 tiles are on the chip at once: its launches take little longer for them (845 x 13, 63 x 257, 300 x 7,
-// 1 x 1 and 129 x 130: 137 us, 162 with a launch for the small four).
+// 1 x 1 and 129 x 130: 148 us with 63 x 257 there, 162 without).  Up to 16 rows stay apart in any case: with so few terms fp32
+// products leave an error that 22-bit planes would treble.
 static void ns_split(const NsArgs& a, bool* small) {
   int64_t big = 0, all = 0;
   bool large = false;
@@ -759,7 +766,7 @@ static void ns_split(const NsArgs& a, bool* small) {
     }
   }
   if (large && big < 256 && all <= 512)
-    for (int i = 0; i < a.count; ++i) small[i] = false;
+    for (int i = 0; i < a.count; ++i) small[i] = (a.rows[i] < a.cols[i] ? a.rows[i] : a.cols[i]) <= 16;
 }
 
 // Tile: 128 once the largest product of the list fills the chip with such tiles, 64 for the parallelism otherwise.
