@@ -45,8 +45,9 @@ typedef float ct_acc __attribute__((ext_vector_type(16)));
 #define CT_MAXD 256
 #define CT_LIM 3.0e38f       // |bias * log2 e| is held inside fp32: masks of the type's lowest value stay finite
 // A running reference is set so that the largest weight is 2^CT_BASE and moves when one passes 2^CT_TOP: fp16 weights stay
-// below 2^16 (a weight and a target's share on top of it), bf16 ones have room.
-#define CT_BASE(PL) ((PL) == 2 ? 6.f : 0.f)
+// below 2^16 (a weight and a target's share on top of it), bf16 ones have room.  The planes hold a weight to 2^-25, that is
+// to 2^-36 of the largest beside it.
+#define CT_BASE(PL) ((PL) == 2 ? 11.f : 0.f)
 #define CT_TOP(PL) ((PL) == 2 ? 14.f : 24.f)
 #define CT_THREADS 256
 #define CT_WAVES 4

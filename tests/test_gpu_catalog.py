@@ -8,7 +8,9 @@ lse moves by at most max delta, plus the sum of V weights in chains of at most `
 times vector entries; with M = sum |weight * entry| it may be off by M times the weights' error plus (terms / 2 + 32) u for
 the plane products.  bf16: the weights are rounded once (2^-8 of each term) and so is the result (2^-8 of the value).
 Weights and planes of weights below the smallest normal number, 2^-126, are held as zero: at most three times 2^-126 per
-term, whatever the term's size."""
+term, whatever the term's size.  fp32: the second product's weights are fp16 pairs under a reference that takes the largest of
+a vector's weights to at least 2^11, and the lower of a pair has steps of 2^-24, so that a weight is off by up to 2^-25, 2^-36 of
+the largest, on top of its relative error."""
 import math
 
 import pytest
@@ -75,6 +77,10 @@ def _ref(x, t, y, b, g=None, gl=None):
     tb = (aw.sum(0) + hot.abs().sum(0)) * acc_t + (aw * ew[:, None]).sum(0)
     out += [dx, dt, db]
     tiny = 3 * 2.0 ** -126
+    if not bf:
+        big = torch.maximum(aw, hot.abs())
+        tx = tx + 2.0 ** -36 * aw.max(1, keepdim=True).values * T.abs().sum(0)
+        tt = tt + 2.0 ** -36 * big.max(0).values[:, None] * X.abs().sum(0)
     tol += [tx + r * dx.abs() + tiny * T.abs().sum(0), tt + r * dt.abs() + tiny * X.abs().sum(0), tb + tiny * R]
     return out, tol
 
@@ -167,6 +173,17 @@ def test_masked_items_and_large_scores(dtype):
         _check(got, ref, tol)
         if case == 1:
             assert (got[1] == -INF).all() and (got[0] == -INF).all() and not any(v.any() for v in got[2:])
+
+
+def test_sharp_softmax_beside_targets_of_small_elements():
+    """Scores of several tens: an item's gradient is its target row's share plus weights 2^-20 of it times larger elements."""
+    for seed in range(30):
+        x, t, y, b = _make(16, 1710, 74, torch.float32, True, 400 + seed, scale=4.0)
+        x[:, ::5] *= 1e-4
+        g = torch.Generator().manual_seed(seed)
+        g, gl = torch.randn(16, generator=g).cuda(), torch.zeros(16, device="cuda")
+        ref, tol = _ref(x, t, y, b, g, gl)
+        _check(_run(x, t, y, b, g, gl), ref, tol)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
