@@ -812,7 +812,7 @@ int rx_logprob_bwd(const rx_logprob_args* args, const float* d_g_logprob, const 
  *   lse[r] = log sum_v exp s_rv,  logprob[r] = s_{r, y_r} - lse[r]     (natural logarithms, fp32)
  * x and the table are fp32, or bf16 with bf16 = 1; the bias is fp32 [V] or NULL.  D up to 256, any value; rows ld_x /
  * ld_t elements apart.  A product of fp32 operands is off by at most 12 * 2^-24 of itself, plus, where an element is below
- * 2^-15 of the largest one among its 64 neighbouring vectors, 2^-40 of that one times the other factor.  Non-finite elements make
+ * 2^-15 of the largest one among its 64 neighbouring vectors, 2^-39 of that one times the other factor.  Non-finite elements make
  * the rows that meet them NaN, and the table's gradient with them.  A target of -1 stands for "no target" (logprob 0, no
  * gradient through it); any other target outside [0, V) sets RX_ERR_INDEX and gives NaN.  A bias of -inf takes an item
  * out, whatever its vector holds; a target that is out gives -inf and no gradient, and a row with no item left gives lse -inf and no gradient.
@@ -836,7 +836,8 @@ int rx_catalog_fwd(const rx_catalog_args* args, float* d_logprob, float* d_lse, 
  *   dx_r = g_r t_{y_r} + c_r mean_r       dtable_v = sum_r c_r p_rv x_r + sum_{r: y_r = v} g_r x_r
  *   dbias_v = sum_r c_r p_rv + sum_{r: y_r = v} g_r
  * d_dx [R, D] / d_dtable [V, D] (the operands' type, 16-byte aligned table gradient, rows back to back) or NULL; with a bias
- * d_dbias [V] comes with d_dtable.  Deterministic: no atomics.  Workspace only with d_dtable. */
+ * d_dbias [V] comes with d_dtable.  fp32: beside their relative error the weights c_r p_rv, g_r (and p_rv in the mean) are held to
+ * 2^-36 of the largest of their item (row).  Deterministic: no atomics.  Workspace only with d_dtable. */
 size_t rx_catalog_bwd_workspace_bytes(int64_t R, int64_t V, int32_t D, int32_t bf16, int32_t want_bias);
 int rx_catalog_bwd(const rx_catalog_args* args, const float* d_stats, const float* d_mean, const float* d_g_logprob,
                    const float* d_g_lse, void* d_dx, void* d_dtable, float* d_dbias, void* ws, size_t ws_bytes, int device,

@@ -20,7 +20,7 @@
 // take six products.  fp16 has no
 // range to spare, so everything is scaled by powers of two first, which costs no accuracy: a stationary vector by its
 // own largest element, a streaming tile by the tile's (both to 2^14 .. 2^15: elements down to 2^-15 of the largest keep
-// all their bits, smaller ones an absolute error of 2^-40 of it), and the weights by a running reference per stationary
+// all their bits, smaller ones an absolute error of 2^-39 of it), and the weights by a running reference per stationary
 // vector (the softmax's own in the forward pass).  The factors fold into numbers the loop has anyway.
 // bf16 operands take one plane, exactly; there the weights of the second product are rounded to bf16 as well, 2^-9
 // relative and independent from term to term, as much as the result's own rounding.

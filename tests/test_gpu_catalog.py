@@ -10,7 +10,8 @@ the plane products.  bf16: the weights are rounded once (2^-8 of each term) and 
 Weights and planes of weights below the smallest normal number, 2^-126, are held as zero: at most three times 2^-126 per
 term, whatever the term's size.  fp32: the second product's weights are fp16 pairs under a reference that takes the largest of
 a vector's weights to at least 2^11, and the lower of a pair has steps of 2^-24, so that a weight is off by up to 2^-25, 2^-36 of
-the largest, on top of its relative error."""
+the largest, on top of its relative error.  Likewise an element of x or the table: scaled so that the largest of its vector, or of
+64 neighbours, is at least 2^14, it is off by up to 2^-25, 2^-39 of that one, on top of its relative 4 u."""
 import math
 
 import pytest
@@ -52,6 +53,8 @@ def _ref(x, t, y, b, g=None, gl=None):
     lp = torch.where(s.gather(1, yy[:, None])[:, 0] == -INF, torch.full_like(lp, -INF), lp)
     lp = torch.where(none, torch.zeros_like(lp), lp)
     delta = (D / 2 + 16) * U * torch.where(torch.isfinite(s), size, torch.zeros_like(size)).max(1).values
+    px, pt = (X.abs().max(), T.abs().max()) if not bf else (0.0, 0.0)
+    delta = delta + 2.0 ** -39 * (px * T.abs().sum(1).max() + pt * X.abs().sum(1))
     seq = max(64, V / 64)
     big = torch.where(torch.isfinite(lse), lse.abs(), torch.zeros_like(lse))
     t_lse = delta + (seq + 32) * U + 4 * U * big
@@ -79,8 +82,8 @@ def _ref(x, t, y, b, g=None, gl=None):
     tiny = 3 * 2.0 ** -126
     if not bf:
         big = torch.maximum(aw, hot.abs())
-        tx = tx + 2.0 ** -36 * aw.max(1, keepdim=True).values * T.abs().sum(0)
-        tt = tt + 2.0 ** -36 * big.max(0).values[:, None] * X.abs().sum(0)
+        tx = tx + 2.0 ** -36 * aw.max(1, keepdim=True).values * T.abs().sum(0) + 2.0 ** -39 * pt * aw.sum(1, keepdim=True)
+        tt = tt + 2.0 ** -36 * big.max(0).values[:, None] * X.abs().sum(0) + 2.0 ** -39 * px * (aw + hot.abs()).sum(0)[:, None]
     tol += [tx + r * dx.abs() + tiny * T.abs().sum(0), tt + r * dt.abs() + tiny * X.abs().sum(0), tb + tiny * R]
     return out, tol
 
