@@ -165,3 +165,38 @@ def test_adam_takes_the_matrices_muon_does_not():
     torch.cuda.synchronize()
     step = (before - m.a.detach()) * m.a.grad.sign()
     assert ((step - 0.01).abs() <= 1e-4).all()          # Adam's first step: lr sign(g), less 2e-8 of it for adam_eps
+
+
+def test_recordings_of_kernels_with_much_shared_memory(deferred):
+    """Launches that ask for more than 64 KiB of LDS, recorded, replayed three times beside eager calls."""
+    from recsys_amd import autograd as rxa, ops
+    torch.manual_seed(5)
+    mats = [torch.randn(90, 300, device="cuda"), torch.randn(700, 650, device="cuda"), torch.randn(16, 2200, device="cuda")]
+    y = torch.randint(0, 900, (70,), device="cuda")
+    b = torch.randn(900, device="cuda")
+
+    def step(x, t):
+        x, t = x.detach().requires_grad_(True), t.detach().requires_grad_(True)
+        lp, lse = rxa.catalog_logprob(x, t, y, bias=b)
+        return (lp, lse, *torch.autograd.grad(lp.sum() + 0.5 * lse.sum(), (x, t)), *ops.orthogonalize(mats[:1]), *ops.orthogonalize(mats))
+
+    for D, dtype in ((256, torch.float32), (190, torch.float32), (256, torch.bfloat16), (128, torch.float32)):
+        x, t = torch.randn(70, D, device="cuda").to(dtype), (0.1 * torch.randn(900, D, device="cuda")).to(dtype)
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            step(x, t)
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                rec = step(x, t)
+        torch.cuda.current_stream().wait_stream(stream)
+        for _ in range(3):
+            x.copy_(torch.randn(70, D, device="cuda"))
+            for m in mats:
+                m.normal_()
+            torch.cuda.synchronize()
+            graph.replay()
+            eager = step(x, t)
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(rec, eager))
