@@ -813,7 +813,8 @@ int rx_logprob_bwd(const rx_logprob_args* args, const float* d_g_logprob, const 
  * x and the table are fp32, or bf16 with bf16 = 1; the bias is fp32 [V] or NULL.  D up to 256, any value; rows ld_x /
  * ld_t elements apart.  A product of fp32 operands is off by at most 12 * 2^-24 of itself, plus, where an element is below
  * 2^-15 of the largest one among its 64 neighbouring vectors, 2^-39 of that one times the other factor.  Non-finite elements make
- * the rows that meet them NaN, and the table's gradient with them.  A target of -1 stands for "no target" (logprob 0, no
+ * the rows that meet them NaN, and the table's gradient with them, unless the row carries no gradient (no target and a zero
+ * or no gradient of its lse): such a row may hold anything.  A target of -1 stands for "no target" (logprob 0, no
  * gradient through it); any other target outside [0, V) sets RX_ERR_INDEX and gives NaN.  A bias of -inf takes an item
  * out, whatever its vector holds; a target that is out gives -inf and no gradient, and a row with no item left gives lse -inf and no gradient.
  * `stats` [R, 2] and `mean` [R, D] fp32 (both may be NULL) are what rx_catalog_bwd needs: the row's softmax

@@ -242,7 +242,7 @@ __device__ __forceinline__ int ct_swz(int d, int c) {
   else return c ^ (((d & 2) | ((d >> 2) & 1)) ^ ((d >> 3) & 3));
 }
 
-template <typename T, int PL, int DP, int BN, bool TR, int NT, bool MASK>
+template <typename T, int PL, int DP, int BN, bool TR, int NT>
 struct CtStage {
   typedef CtTile<PL, DP, BN, TR, NT> Tile;
   typedef typename CtQuad<T>::V Quad;          // as they lie in memory, of four vectors
@@ -274,8 +274,10 @@ struct CtStage {
       for (int k = 0; k < 4; ++k) ct_shift(v[q][k], n);
     }
   }
-  // Vectors whose item is out (bias -inf) become zeros, whatever they hold: their score is -inf all the same.
-  float bias[MASK ? Tile::PER : 1][4];
+  // Some vectors become zeros, whatever they hold: items that are out (bias -inf: their score is -inf all the same) in the
+  // forward pass, rows without a gradient (ct_prep_kernel's marks: their weights are 0) in the backward pass.
+  float bias[Tile::PER][4];
+  uint32_t mark[Tile::PER];    // a byte per vector: the branch below is rarely taken, and four floats cost 180 us of 590
   __device__ __forceinline__ void load_bias(const float* b, int64_t row0, int64_t rows) {
 #pragma unroll
     for (int q = 0; q < Tile::PER; ++q)
@@ -284,6 +286,24 @@ struct CtStage {
         const int64_t row = row0 + (q * NT + threadIdx.x) / (DP / 4) * 4 + k;
         bias[q][k] = row < rows ? b[row] : 0.f;
       }
+  }
+  __device__ __forceinline__ void load_marks(const uint8_t* m, int64_t row0) {     // of whole tiles, 4-byte aligned
+#pragma unroll
+    for (int q = 0; q < Tile::PER; ++q) {
+      const int blk = q * NT + threadIdx.x;
+      mark[q] = *reinterpret_cast<const uint32_t*>(m + row0 + (Tile::BLOCKS % NT == 0 || blk < Tile::BLOCKS ? blk / (DP / 4) * 4 : 0));
+    }
+  }
+  __device__ __forceinline__ void drop_marked() {
+    uint32_t any = 0;
+#pragma unroll
+    for (int q = 0; q < Tile::PER; ++q) any |= mark[q];
+    if (!__ballot(any != 0)) return;
+#pragma unroll
+    for (int q = 0; q < Tile::PER; ++q)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (mark[q] >> (8 * k) & 255) v[q][k] = Quad{};
   }
   __device__ __forceinline__ void drop() {
 #pragma unroll
@@ -434,7 +454,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
   const int64_t row0 = ((int64_t)tile * NW + wave) * (32 * MB);
   const int64_t v0 = split * a.per_split, v1 = v0 + a.per_split < a.V ? v0 + a.per_split : a.V;
   const int n = (int)((v1 - v0 + BN - 1) / BN);             // tiles of this split, at least one
-  CtStage<T, PL, DP, BN, MEAN, NW * 64, BIAS> stage;
+  CtStage<T, PL, DP, BN, MEAN, NW * 64> stage;
   float nb = 0.f;
   auto fetch = [&](int i) {
     const int64_t v = v0 + (int64_t)i * BN;
@@ -685,6 +705,7 @@ struct CtPrep {
   const float *stats, *mean, *g, *gl;
   void* dx;
   CtRow* rows;
+  uint8_t* marks;              // 1: nothing of the row reaches the table's gradient
 };
 // dx, and the rows as the table's pass wants them; one wavefront per row
 template <typename T>
@@ -708,6 +729,7 @@ __global__ void __launch_bounds__(CT_THREADS) ct_prep_kernel(CtPrep a) {
     r.gl2 = log2f(fabsf(g));
     r.pad = 0;
     a.rows[row] = r;
+    a.marks[row] = c == 0.f && g == 0.f;
   }
   if (a.dx) {
     const T* t = (const T*)a.t + (y < 0 ? 0 : y) * a.ld_t;
@@ -724,6 +746,7 @@ struct CtBwd {
   int64_t ld_x, ld_t, R, V;
   const float* bias;
   const CtRow* rows;
+  const uint8_t* marks;
   int D, tiles, n_split;
   int64_t per_split;           // rows per split, a multiple of the tile
   void* dt;                    // [V][D] in the table's type, or fp32 [n_split][V][D]
@@ -743,11 +766,12 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
   const int64_t item0 = ((int64_t)tile * NW + wave) * (32 * MB);
   const int64_t r0 = split * a.per_split, r1 = r0 + a.per_split < a.R ? r0 + a.per_split : a.R;
   const int n = (int)((r1 - r0 + BN - 1) / BN);             // tiles of this split, at least one
-  CtStage<T, PL, DP, BN, true, NW * 64, false> stage;
+  CtStage<T, PL, DP, BN, true, NW * 64> stage;
   CtRow info;
   auto fetch = [&](int i) {
     const int64_t r = r0 + (int64_t)i * BN;
     stage.load((const T*)a.x, a.ld_x, r, r1, a.D);
+    stage.load_marks(a.marks, r);
     if (threadIdx.x < BN) {
       if (r + threadIdx.x < r1) info = a.rows[r + threadIdx.x];
       else { info.m2 = 0.f; info.l2s = info.z = __builtin_inff(); info.sgn = 1.f; info.g = 0.f; info.gl2 = CT_NINF; info.y = -1; }
@@ -755,6 +779,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
   };
   auto publish = [&](int i) {      // before the barrier in front of put(i): the largest magnitude, the sign words
     stage.settle(a.D);
+    stage.drop_marked();
     if constexpr (PL == 2) {
       const uint32_t m = stage.peak();
       if (lane == 0) lm[(i & 1) * NW + wave] = m;
@@ -1046,7 +1071,7 @@ extern "C" size_t rx_catalog_fwd_workspace_bytes(int64_t R, int64_t V, int32_t D
 extern "C" size_t rx_catalog_bwd_workspace_bytes(int64_t R, int64_t V, int32_t D, int32_t bf16, int32_t want_bias) {
   if (R <= 0 || V <= 0 || D < 1 || D > CT_MAXD) return 0;
   const CtPlan p = ct_bwd_plan(R, V, D, bf16, want_bias != 0);
-  return rx_align_up((size_t)R * sizeof(CtRow), 256) +
+  return rx_align_up((size_t)R * sizeof(CtRow), 256) + rx_align_up((size_t)R, 256) +
          (p.n_split > 1 ? rx_align_up((size_t)p.n_split * V * D * 4, 256) + (want_bias ? (size_t)p.n_split * V * 4 : 0) : 0);
 }
 
@@ -1128,18 +1153,19 @@ extern "C" int rx_catalog_bwd(const rx_catalog_args* args, const float* d_stats,
   RX_GUARD_DEVICE(device);
   hipStream_t st = (hipStream_t)stream;
   CtRow* rows = want_t ? (CtRow*)ws : nullptr;
-  CtPrep q = {a.table, a.ld_t, a.R, a.V, a.bias, a.targets, a.D, d_stats, d_mean, d_g_logprob, d_g_lse, d_dx, rows};
+  uint8_t* marks = want_t ? (uint8_t*)ws + rx_align_up((size_t)a.R * sizeof(CtRow), 256) : nullptr;    // rounded up to whole tiles
+  CtPrep q = {a.table, a.ld_t, a.R, a.V, a.bias, a.targets, a.D, d_stats, d_mean, d_g_logprob, d_g_lse, d_dx, rows, marks};
   const dim3 grid((unsigned)rx_cdiv(a.R, CT_WAVES));
   if (a.bf16) hipLaunchKernelGGL(ct_prep_kernel<uint16_t>, grid, dim3(CT_THREADS), 0, st, q);
   else hipLaunchKernelGGL(ct_prep_kernel<float>, grid, dim3(CT_THREADS), 0, st, q);
   RX_LAUNCH_CHECK();
   if (!want_t) return 0;
   const CtPlan p = ct_bwd_plan(a.R, a.V, a.D, a.bf16, d_dbias != nullptr);
-  uint8_t* w = (uint8_t*)ws + rx_align_up((size_t)a.R * sizeof(CtRow), 256);
+  uint8_t* w = marks + rx_align_up((size_t)a.R, 256);
   const bool partial = p.n_split > 1;
   float* pt = (float*)w;
   float* pb = (float*)(w + rx_align_up((size_t)p.n_split * a.V * a.D * 4, 256));
-  CtBwd f = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, rows, a.D, p.tiles, p.n_split, p.per_split,
+  CtBwd f = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, rows, marks, a.D, p.tiles, p.n_split, p.per_split,
              partial ? (void*)pt : d_dtable, partial ? (d_dbias ? pb : nullptr) : d_dbias, partial};
 #define CT_GO(...) ct_pick_bwd<__VA_ARGS__>(f, st)
   const int rc = CT_KERNELS(CT_GO, a.bf16, ct_dp(a.D));

@@ -205,6 +205,26 @@ def test_items_that_are_out_may_hold_anything(dtype, D):
     assert not clean[3][out].any() and not clean[4][out].any()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,V,D", [(150, 700, 20), (65, 90, 64), (200, 3000, 190), (7, 40, 3)])
+def test_padded_rows_may_hold_anything(R, V, D, dtype):
+    """Rows without a target: zero gradient for them, the same bits for the others and the table as with zeros there."""
+    for bias in (False, True):
+        x, t, y, b = _make(R, V, D, dtype, bias, R + V)
+        pad = torch.rand(R, device="cuda") < 0.3
+        pad[-2:] = True
+        y[pad] = -1
+        x[pad] = 0
+        g, gl = torch.randn(R, device="cuda"), torch.zeros(R, device="cuda")
+        clean = _run(x, t, y, b, g, gl)
+        x[pad] = torch.tensor([float("nan"), INF, -INF, 3e38], device="cuda").to(dtype)[torch.randint(0, 4, (int(pad.sum()), 1), device="cuda")]
+        got = _run(x, t, y, b, g, gl)
+        assert torch.equal(got[0], clean[0]) and torch.equal(got[1][~pad], clean[1][~pad])
+        for p, q in zip(got[2:], clean[2:]):
+            assert p is None or torch.equal(p, q)
+        assert not got[2][pad].any()
+
+
 def test_a_nan_row_keeps_to_itself_in_the_forward_pass():
     from recsys_amd import autograd as rxa
     x, t, y, b = _make(100, 300, 20, torch.float32, False, 1)
