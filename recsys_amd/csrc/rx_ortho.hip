@@ -750,30 +750,53 @@ static int ns_bounds(const char* who, double ca, double cb, double cc, int steps
 // power of two that takes a bound, with a margin for rounding, to at most 2^15
 static float ns_scale_of(float bound) { return bound > 0.f ? ldexpf(1.f, 14 - ilogbf(bound * 1.1f)) : 1.f; }
 
-// Which matrices take a workgroup of their own.  All that fit one do, but in a list that needs the large path anyway they join
-// it while all its 64 x 64 tiles are on the chip at once: its launches take little longer for them (845 x 13, 63 x 257, 300 x 7,
-// 1 x 1 and 129 x 130: 148 us with 63 x 257 there, 162 without).  Up to 16 rows stay apart in any case: with so few terms fp32
-// products leave an error that 22-bit planes would treble.
-static void ns_split(const NsArgs& a, bool* small) {
-  int64_t big = 0, all = 0;
+// Time of a step's three products in tiles of t, in microseconds without the launches: each takes as long as its longest
+// contraction on a CU of its own, and as all its tiles' contractions shared out over 256 CUs (measured per 32 elements and tile:
+// with 128 0.8, and 0.8 to 1.09 where CUs have several; with 64 0.31).  Against the times of single matrices with both tiles: 2048 x 2048 841 us with 128
+// and 880 with 64, 1900 x 1900 792 and 643, 1500 x 3000 959 and 678, 1024 x 1024 483 and 238.
+static float ns_cost(const NsArgs& a, const bool* small, int t) {
+  float longest[3] = {}, shared[3] = {};
+  for (int i = 0; i < a.count; ++i) {
+    if (small[i]) continue;
+    const int lo = a.rows[i] < a.cols[i] ? a.rows[i] : a.cols[i], hi = a.rows[i] < a.cols[i] ? a.cols[i] : a.rows[i];
+    const int tm = (lo + t - 1) / t, tn = (hi + t - 1) / t;
+    const float sym = 0.5f * tm * (tm + 1), steps_m = tm * t / 32.f, steps_n = tn * t / 32.f;
+    const float tiles[3] = {sym, sym, (float)tm * tn}, steps[3] = {steps_n, steps_m, steps_m};
+    for (int p = 0; p < 3; ++p) {
+      if (steps[p] > longest[p]) longest[p] = steps[p];
+      shared[p] += tiles[p] * steps[p] / 256.f;
+    }
+  }
+  float sum = 0.f;
+  for (int p = 0; p < 3; ++p) {
+    const float one = longest[p] * (t == 128 ? 0.8f : 0.31f), all = shared[p] * (t == 128 ? 0.9f : 0.31f);
+    sum += one > all ? one : all;
+  }
+  return sum;
+}
+
+// Which matrices take a workgroup of their own; returns the tile of the others.  All that fit one do, but in a list that needs
+// the large path anyway they join it while all its 64 x 64 tiles are on the chip at once: its launches take little longer for
+// them (845 x 13, 63 x 257, 300 x 7, 1 x 1 and 129 x 130: 148 us with 63 x 257 there, 162 without).  Up to 16 rows stay apart in
+// any case: with so few terms fp32 products leave an error that 22-bit planes would treble.
+static int ns_split(const NsArgs& a, bool* small) {
+  int64_t all = 0;
   bool large = false;
   for (int i = 0; i < a.count; ++i) {
     small[i] = ns_is_small(a.rows[i], a.cols[i]);
     all += rx_cdiv(a.rows[i], 64) * rx_cdiv(a.cols[i], 64);
-    if (!small[i]) {
-      large = true;
-      big += rx_cdiv(a.rows[i], 128) * rx_cdiv(a.cols[i], 128);
-    }
+    large = large || !small[i];
   }
-  if (large && big < 256 && all <= 512)
+  const int tile = ns_cost(a, small, 128) < ns_cost(a, small, 64) ? 128 : 64;
+  if (large && tile == 64 && all <= 512)
     for (int i = 0; i < a.count; ++i) small[i] = (a.rows[i] < a.cols[i] ? a.rows[i] : a.cols[i]) <= 16;
+  return tile;
 }
 
-// Tile: 128 once the largest product of the list fills the chip with such tiles, 64 for the parallelism otherwise.
 static void ns_plan(const NsArgs& a, NsList* l, size_t* bytes, uint8_t* ws) {
   memset(l, 0, sizeof(*l));
   bool small[RX_ORTHO_MAX];
-  ns_split(a, small);
+  l->tile = ns_split(a, small);
   int order[RX_ORTHO_MAX], k = 0;
   for (int i = 0; i < a.count; ++i)
     if (!small[i]) {
@@ -782,9 +805,6 @@ static void ns_plan(const NsArgs& a, NsList* l, size_t* bytes, uint8_t* ws) {
       while (at > 0 && cost(order[at - 1]) < cost(i)) { order[at] = order[at - 1]; --at; }   // longest contractions first
       order[at] = i;
     }
-  int64_t big = 0;
-  for (int i = 0; i < k; ++i) big += rx_cdiv(a.rows[order[i]], 128) * rx_cdiv(a.cols[order[i]], 128);
-  l->tile = big >= 256 ? 128 : 64;
   l->count = k;
   l->steps = a.steps;
   l->nesterov = a.nesterov;
