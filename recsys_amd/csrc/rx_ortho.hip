@@ -777,8 +777,8 @@ static float ns_cost(const NsArgs& a, const bool* small, int t) {
 
 // Which matrices take a workgroup of their own; returns the tile of the others.  All that fit one do, but in a list that needs
 // the large path anyway they join it while all its 64 x 64 tiles are on the chip at once: its launches take little longer for
-// them (845 x 13, 63 x 257, 300 x 7, 1 x 1 and 129 x 130: 148 us with 63 x 257 there, 162 without).  Up to 16 rows stay apart in
-// any case: with so few terms fp32 products leave an error that 22-bit planes would treble.
+// them (845 x 13, 63 x 257, 300 x 7, 1 x 1 and 129 x 130: 148 us with 63 x 257 there, 162 without).  Up to 16 rows stay apart
+// where they fit: with so few terms fp32 products leave an error that 22-bit planes would treble.
 static int ns_split(const NsArgs& a, bool* small) {
   int64_t all = 0;
   bool large = false;
@@ -789,7 +789,7 @@ static int ns_split(const NsArgs& a, bool* small) {
   }
   const int tile = ns_cost(a, small, 128) < ns_cost(a, small, 64) ? 128 : 64;
   if (large && tile == 64 && all <= 512)
-    for (int i = 0; i < a.count; ++i) small[i] = (a.rows[i] < a.cols[i] ? a.rows[i] : a.cols[i]) <= 16;
+    for (int i = 0; i < a.count; ++i) small[i] = small[i] && (a.rows[i] < a.cols[i] ? a.rows[i] : a.cols[i]) <= 16;
   return tile;
 }
 

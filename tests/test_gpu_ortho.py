@@ -61,6 +61,16 @@ def test_lists_of_matrices(shapes):
             assert (alone.cpu().double() - o.cpu().double()).norm() <= 8e-6 * o.cpu().double().norm()
 
 
+def test_thin_matrices_on_either_side_of_a_workgroups_memory():
+    """Up to 16 rows beside a matrix of the large path: those that fit a workgroup's memory and those that do not."""
+    from recsys_amd import ops
+    shapes = [(150, 140), (16, 2300), (16, 2600), (2700, 16), (9, 4400), (5000, 9), (1, 16384), (2, 16384), (16384, 3)]
+    mats = [_grad(m, n, 31 * i + m) for i, (m, n) in enumerate(shapes)]
+    _check(mats, ops.orthogonalize(mats))
+    for m in mats:
+        _check([m], ops.orthogonalize([m]))
+
+
 def test_steps_and_coefficients():
     from recsys_amd import ops
     mats = [_grad(40, 90, 1), _grad(150, 140, 2)]
