@@ -128,16 +128,10 @@ template <typename T> __device__ __forceinline__ float ct_elem(const T* p);
 template <> __device__ __forceinline__ float ct_elem<float>(const float* p) { return *p; }
 template <> __device__ __forceinline__ float ct_elem<uint16_t>(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
 
-// four consecutive elements as they lie in memory, at any alignment of their own type: the hardware needs no more
+// four consecutive elements as they lie in memory, at any alignment of their own type: a buffer load needs no more
 template <typename T> struct CtQuad;
 template <> struct CtQuad<float> { typedef float4 V; };
 template <> struct CtQuad<uint16_t> { typedef uint2 V; };
-template <typename T>
-__device__ __forceinline__ typename CtQuad<T>::V ct_raw4(const T* p) {
-  typename CtQuad<T>::V v;
-  __builtin_memcpy(&v, p, sizeof(v));
-  return v;
-}
 __device__ __forceinline__ float4 ct_floats(const float4& q) { return q; }
 __device__ __forceinline__ float4 ct_floats(const uint2& q) { return make_float4(ct_lo(q.x), ct_hi(q.x), ct_lo(q.y), ct_hi(q.y)); }
 
@@ -161,18 +155,10 @@ struct CtBuffer {
 #endif
 };
 
-// elements [d, d + 4) of a row, zeros past D
-template <typename T>
-__device__ __forceinline__ float4 ct_load4(const T* row, int d, int D) {
-  if (d + 4 <= D) return ct_floats(ct_raw4(row + d));
-  float4 r = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (d < D) r.x = ct_elem(row + d);
-  if (d + 1 < D) r.y = ct_elem(row + d + 1);
-  if (d + 2 < D) r.z = ct_elem(row + d + 2);
-  return r;
+// a whole row of fewer than four elements (d = 0; zeros past it), as it would lie in memory
+__device__ __forceinline__ float4 ct_short4(const float* row, int d, int D) {
+  return make_float4(d < D ? row[d] : 0.f, d + 1 < D ? row[d + 1] : 0.f, d + 2 < D ? row[d + 2] : 0.f, 0.f);
 }
-// the same of rows shorter than four elements, as it would lie in memory
-__device__ __forceinline__ float4 ct_short4(const float* row, int d, int D) { return ct_load4(row, d, D); }
 __device__ __forceinline__ uint2 ct_short4(const uint16_t* row, int d, int D) {
   uint2 r = make_uint2(0u, 0u);
   if (d < D) r.x = row[d];
@@ -190,28 +176,52 @@ __device__ __forceinline__ void ct_shift(uint2& v, int n) {
   v = make_uint2((uint32_t)u, (uint32_t)(u >> 32));
 }
 
-// stationary operands of one block of 32 vectors: lane column l & 31, element ks * 16 + 8 (l >> 5) + j; returns what the
-// scores have to be multiplied with to undo the vector's scale
+// stationary operands of the 32 vectors from row0 on (uniform; zeros past `rows` and where `out`): lane column l & 31, element
+// ks * 16 + 8 (l >> 5) + j; returns what the scores have to be multiplied with to undo the vector's scale
 template <typename T, int PL, int DP>
-__device__ __forceinline__ float ct_stationary(const T* base, int64_t ld, int64_t row, int64_t rows, int D, CtFrag (*f)[PL]) {
-  const int h = rx_lane() >> 5;
-  const T* p = base + (row < rows ? row : 0) * ld;
-  const int n = row < rows ? D : 0;
+__device__ __forceinline__ float ct_stationary(const T* base, int64_t ld, int64_t row0, int64_t rows, int D, bool out, CtFrag (*f)[PL]) {
+  const int l31 = rx_lane() & 31, h = rx_lane() >> 5, step = (int)ld * (int)sizeof(T);
+  const int left = rows <= row0 ? 0 : rows - row0 < 32 ? (int)(rows - row0) : 32;
+  // in scalar registers for certain: a 64-bit comparison takes them out, and a descriptor elsewhere means a loop over its values
+  const uint64_t at0 = (uint64_t)(base + (left ? row0 : 0) * ld);
+  const T* first = (const T*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(at0 >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)at0));
+  const CtBuffer b(first, __builtin_amdgcn_readfirstlane(left ? (left - 1) * step + D * (int)sizeof(T) : 0));
+  const bool mine = l31 < left && !out;
+  typename CtQuad<T>::V raw[DP / 16][2];
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int d = ks * 16 + h * 8 + u * 4, at = d + 4 <= D ? d : D - 4;
+      const bool on = mine && d < D;
+      if (DP == 32 && D < 4) raw[ks][u] = on ? ct_short4(first + l31 * ld, d, D) : typename CtQuad<T>::V{};
+      else b.load(raw[ks][u], on ? l31 * step + at * (int)sizeof(T) : CT_OUTSIDE);
+    }
+  if (D % 4 != 0 && D >= 4) {
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int d = ks * 16 + h * 8 + u * 4;
+        ct_shift(raw[ks][u], d < D && d + 4 > D ? d + 4 - D : 0);
+      }
+  }
   float scale = 1.f;
   if constexpr (PL == 2) {
     uint32_t peak = 0;
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) {
-      const float4 a = ct_load4(p, ks * 16 + h * 8, n), b = ct_load4(p, ks * 16 + h * 8 + 4, n);
-      peak = ct_umax(ct_umax(peak, ct_umax(ct_abs(a.x), ct_abs(a.y))), ct_umax(ct_abs(a.z), ct_abs(a.w)));
-      peak = ct_umax(ct_umax(peak, ct_umax(ct_abs(b.x), ct_abs(b.y))), ct_umax(ct_abs(b.z), ct_abs(b.w)));
-    }
+    for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const float4 a = ct_floats(raw[ks][u]);
+        peak = ct_umax(ct_umax(peak, ct_umax(ct_abs(a.x), ct_abs(a.y))), ct_umax(ct_abs(a.z), ct_abs(a.w)));
+      }
     scale = ct_scale(ct_umax(peak, (uint32_t)__shfl_xor((int)peak, 32, 64)));
   }
 #pragma unroll
   for (int ks = 0; ks < DP / 16; ++ks) {
-    const float4 a = ct_load4(p, ks * 16 + h * 8, n), b = ct_load4(p, ks * 16 + h * 8 + 4, n);
-    float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    const float4 a = ct_floats(raw[ks][0]), c = ct_floats(raw[ks][1]);
+    float v[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
     if constexpr (PL == 2) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] *= scale;
@@ -450,7 +460,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
   uint32_t* lm = reinterpret_cast<uint32_t*>(lb + 2 * BN);                  // [2][NW] largest magnitudes
   int tile, split;
   ct_place(a.tiles, a.n_split, &tile, &split);
-  const int wave = threadIdx.x >> 6, l31 = rx_lane() & 31, h = rx_lane() >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l31 = rx_lane() & 31, h = rx_lane() >> 5;
   const int64_t row0 = ((int64_t)tile * NW + wave) * (32 * MB);
   const int64_t v0 = split * a.per_split, v1 = v0 + a.per_split < a.V ? v0 + a.per_split : a.V;
   const int n = (int)((v1 - v0 + BN - 1) / BN);             // tiles of this split, at least one
@@ -491,7 +501,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
   float inv[MB], ref[MB], kr[MB], sum[MB];
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
-    inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.x, a.ld_x, row0 + mb * 32 + l31, a.R, a.D, st[mb]);
+    inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.x, a.ld_x, row0 + mb * 32, a.R, a.D, false, st[mb]);
     ref[mb] = CT_NINF;
     kr[mb] = sum[mb] = 0.f;
   }
@@ -762,7 +772,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
   uint32_t* lm = reinterpret_cast<uint32_t*>(lz0 + 14 * BN);       // [2][NW] largest magnitudes
   int tile, split;
   ct_place(a.tiles, a.n_split, &tile, &split);
-  const int wave = threadIdx.x >> 6, lane = rx_lane(), l31 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = rx_lane(), l31 = lane & 31, h = lane >> 5;
   const int64_t item0 = ((int64_t)tile * NW + wave) * (32 * MB);
   const int64_t r0 = split * a.per_split, r1 = r0 + a.per_split < a.R ? r0 + a.per_split : a.R;
   const int n = (int)((r1 - r0 + BN - 1) / BN);             // tiles of this split, at least one
@@ -816,7 +826,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
     const int64_t item = item0 + mb * 32 + l31;
     b2[mb] = BIAS && item < a.V ? ct_bias2(a.bias[item]) : 0.f;
     const bool out = b2[mb] == CT_NINF;                       // an item that is out may hold anything
-    inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.t, a.ld_t, item, out ? 0 : a.V, a.D, st[mb]);
+    inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.t, a.ld_t, item0 + mb * 32, a.V, a.D, out, st[mb]);
     dbias[mb] = lost[mb] = 0.f;
     ref[mb] = PL == 2 ? CT_NINF : 0.f;
   }
