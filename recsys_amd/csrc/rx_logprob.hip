@@ -4,8 +4,11 @@
 //
 // Both directions read every score once and are bound by that read (and the write of dl): the softmax statistics are
 // online.  Each lane keeps its own running reference m (log2 units), sum s = sum 2^(l' - m) and t = sum 2^(l' - m) (l' - m)
-// with l' = l log2(e); the reference moves only when a score exceeds it by 2^4, so the rescale is off the common path,
-// and lanes, wavefronts and column splits are joined at the end.  All sums are fp32, whatever the scores' type.
+// with l' = l log2(e); the reference moves only when a score exceeds it by 2^4, so the rescale is off the common path.
+// m is a rounded number, and a score's distance from it is off by half of m's last step: no more than one up to LP_BIG, which is why
+// it is never below -LP_FLOOR (a lane that sees nothing but masks sums up zeros) and why rows whose largest score lies
+// beyond LP_BIG are read a second time.  What lanes, wavefronts and column splits join at the end is in score units, relative to
+// the largest score itself.  All sums are fp32, whatever the scores' type.
 // Alternatives: a wavefront keeps the 64 best keys (value, column) sorted across its lanes; scores that beat the k-th
 // one are collected in a small LDS buffer and merged 64 at a time, so a row costs one compare per 16 bytes in the
 // common case.  Keys order by value, then by the lower column, and are unique, so the result does not depend on
@@ -21,15 +24,16 @@
 #define LP_SPLIT_MAX 256
 #define LP_L2E 1.44269504088896340736f
 #define LP_LN2 0.69314718055994530942f
-#define LP_BIG 1e38f         // beyond this l * log2(e) leaves fp32: such rows take the form exp((l - m) log2 e)
+#define LP_BIG 16777216.f    // |largest score| up to which l * log2(e) - m is good to one; other rows take the form (l - m) log2(e)
+#define LP_FLOOR 33554432.f  // below -LP_BIG in log2 units, by more than any weight survives
 #define LP_NINF (-__builtin_inff())
 
 typedef uint32_t lp_u4 __attribute__((ext_vector_type(4)));
 
 struct LpPart {   // one split's share of a row
   float raw;      // largest score
-  float m2;       // reference of s and t (log2 units; the score itself when |raw| > LP_BIG)
-  float s, t;
+  float s, t;     // sums relative to it
+  float pad;
 };
 
 // ---------------------------------------------------------------- element access
@@ -205,35 +209,31 @@ struct LpTop {
 
 // ---------------------------------------------------------------- shared row pieces
 struct LpRow {
-  float raw, m2, s, t;   // final statistics of the row
+  float ref, l2s;        // final reference (a score) and log2 of the sum of weights relative to it
   float lse, H;
-  bool empty, big;
+  bool empty;
 };
 
-__device__ __forceinline__ LpRow lp_finish(float raw, float m2, float s, float t) {
+// raw: largest score; s, t relative to it
+__device__ __forceinline__ LpRow lp_finish(float raw, float s, float t) {
   LpRow r;
-  r.raw = raw; r.m2 = m2; r.s = s; r.t = t;
   r.empty = raw == LP_NINF && s == s;        // nothing above -inf (and no NaN): no distribution
-  r.big = fabsf(raw) > LP_BIG && fabsf(raw) < __builtin_inff();
-  if (r.empty) { r.lse = LP_NINF; r.H = 0.f; return r; }
-  const float l2s = log2f(s);
-  r.lse = r.big ? m2 + l2s * LP_LN2 : (m2 + l2s) * LP_LN2;
-  r.H = (l2s - t / s) * LP_LN2;
+  r.ref = raw == LP_NINF ? 0.f : raw;
+  r.l2s = log2f(s);
+  r.lse = r.empty ? LP_NINF : r.ref + r.l2s * LP_LN2;
+  r.H = r.empty ? 0.f : (r.l2s - t / s) * LP_LN2;
   return r;
 }
 // log-probability of a score, from the reference rather than from the rounded lse
 __device__ __forceinline__ float lp_of(const LpRow& r, float l) {
-  if (l == LP_NINF || r.empty) return LP_NINF;
-  if (!r.big && fabsf(l) > LP_BIG) return l - r.lse;     // a mask of the type's lowest value under an ordinary row
-  const float l2s = log2f(r.s);
-  return r.big ? (l - r.m2) - l2s * LP_LN2 : (fmaf(l, LP_L2E, -r.m2) - l2s) * LP_LN2;
+  return l == LP_NINF || r.empty ? LP_NINF : (l - r.ref) - r.l2s * LP_LN2;
 }
-// what the gradient needs of a row: (reference, log2 s, unit of the reference: 0 log2, 1 score; 2 = empty row, H).
-// Kept apart from lse, whose rounding would cost the probabilities a factor of 1 + |lse| 2^-24.
+// what the gradient needs of a row: (reference, log2 s, 1: empty row, H).  Kept apart from lse, whose rounding would cost the
+// probabilities a factor of 1 + |lse| 2^-24.
 __device__ __forceinline__ void lp_write_row(const rx_logprob_args& a, const LpRow& r, int64_t row) {
   a.lse[row] = r.lse;
   a.entropy[row] = r.H;
-  if (a.stats) reinterpret_cast<float4*>(a.stats)[row] = make_float4(r.m2, log2f(r.s), r.empty ? 2.f : r.big ? 1.f : 0.f, r.H);
+  if (a.stats) reinterpret_cast<float4*>(a.stats)[row] = make_float4(r.ref, r.l2s, r.empty ? 1.f : 0.f, r.H);
 }
 __device__ __forceinline__ int32_t lp_live(const rx_logprob_args& a, int64_t row) {
   if (!a.lengths) return (int32_t)a.V;
@@ -283,10 +283,7 @@ lp_small_kernel(rx_logprob_args a, int32_t* err) {
   }
   s = lp_sum<G>(s);
   t = lp_sum<G>(t);
-  // the reference is the score itself here, as for rows beyond LP_BIG
-  LpRow r = lp_finish(m, ref, s, t);
-  r.big = true;
-  if (!r.empty) r.lse = ref + log2f(s) * LP_LN2;
+  const LpRow r = lp_finish(m, s, t);
   if (on && sub == 0) lp_write_row(a, r, row);
   if (on)
     for (int q = sub; q < a.T; q += G) lp_write_target<T>(a, r, l, n, row, q, err);
@@ -334,13 +331,11 @@ lp_small_kernel(rx_logprob_args a, int32_t* err) {
 // ---------------------------------------------------------------- wide rows
 struct LpAcc {
   float raw, m2, s, t;
-  __device__ __forceinline__ void init() { raw = LP_NINF; m2 = LP_NINF; s = 0.f; t = 0.f; }
-  __device__ __forceinline__ void rebase(float n) {          // move the reference to n (log2 units, finite or +inf)
-    if (m2 != LP_NINF) {
-      const float f = lp_exp2(m2 - n);
-      t = (t + s * (m2 - n)) * f;
-      s *= f;
-    }
+  __device__ __forceinline__ void init() { raw = LP_NINF; m2 = -LP_FLOOR; s = 0.f; t = 0.f; }
+  __device__ __forceinline__ void rebase(float n) {          // move the reference up to n (log2 units)
+    const float d = fmaxf(m2 - n, -1e4f), f = lp_exp2(d);    // clamped: f is 0 there, and its factor stays finite
+    t = (t + s * d) * f;
+    s *= f;
     m2 = n;
   }
   template <int N>
@@ -355,17 +350,16 @@ struct LpAcc {
     if (__ballot(grow)) {
       if (grow) rebase(n2);
     }
-    const float ref = m2 == LP_NINF ? 0.f : -m2;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float d = fmaf(v[i], LP_L2E, ref), e = lp_exp2(d);
+      const float d = fmaf(v[i], LP_L2E, -m2), e = lp_exp2(d);
       s += e;
       t = fmaf(e, fmaxf(d, -1e4f), t);
     }
     return mx;
   }
-  // Scores whose products with log2(e) leave fp32 (e.g. masks of the type's lowest value with nothing else in the
-  // row): the same sums relative to the known maximum.
+  // rows beyond LP_BIG (e.g. masks of the type's lowest value with nothing else in the row): the same sums relative to
+  // the known maximum
   template <int N>
   __device__ __forceinline__ void add_big(const float* v, float m) {
 #pragma unroll
@@ -438,71 +432,20 @@ __device__ __forceinline__ void lp_stream(const T* l, int32_t n, int split, int 
   }
 }
 
-__device__ __forceinline__ void lp_join(LpPart& x, const LpPart& y) {
-  const float raw = fmaxf(x.raw, y.raw);
-  const bool big = fabsf(raw) > LP_BIG && fabsf(raw) < __builtin_inff();
-  // references in one unit: with the maximum beyond LP_BIG only sums taken relative to scores beyond it count
-  if (big) {
-    auto w = [&](const LpPart& p, float* s, float* t) {
-      if (p.raw == LP_NINF && p.s == p.s) { *s = 0.f; *t = 0.f; return; }
-      if (!(fabsf(p.raw) > LP_BIG)) {                    // ordinary scores below a maximum beyond LP_BIG
-        if (p.s == p.s && raw > 0.f) { *s = 0.f; *t = 0.f; } else { *s = p.s; *t = p.t; }
-        return;
-      }
-      const float d = (p.m2 - raw) * LP_L2E, f = lp_exp2(d);
-      *s = p.s * f;
-      *t = (p.t + p.s * fmaxf(d, -1e4f)) * f;
-    };
-    float s0, t0, s1, t1;
-    w(x, &s0, &t0);
-    w(y, &s1, &t1);
-    x.raw = raw; x.m2 = raw; x.s = s0 + s1; x.t = t0 + t1;
-    return;
-  }
-  auto scaled = [&](const LpPart& p, float m, float* s, float* t) {
-    if (p.m2 == LP_NINF || (fabsf(p.raw) > LP_BIG && p.raw < 0.f)) {   // empty, or far below the maximum (NaN goes through)
-      *s = p.s == p.s ? 0.f : p.s;
-      *t = p.s == p.s ? 0.f : p.t;
-      return;
-    }
-    const float f = lp_exp2(p.m2 - m);
-    *t = (p.t + p.s * (p.m2 - m)) * f;
-    *s = p.s * f;
-  };
-  const bool xb = fabsf(x.raw) > LP_BIG && x.raw < 0.f, yb = fabsf(y.raw) > LP_BIG && y.raw < 0.f;
-  const float m = fmaxf(xb ? LP_NINF : x.m2, yb ? LP_NINF : y.m2);
-  float s0, t0, s1, t1;
-  scaled(x, m, &s0, &t0);
-  scaled(y, m, &s1, &t1);
-  x.raw = raw; x.m2 = m; x.s = s0 + s1; x.t = t0 + t1;
-}
-// Joins the lanes' shares.  `big`: uniform, some share is relative to a score beyond LP_BIG.
-__device__ __forceinline__ LpPart lp_wave_join(LpPart p, bool big) {
-  if (!big) {
-    const float raw = lp_max<64>(p.raw), m = lp_max<64>(p.m2);
-    const bool none = p.m2 == LP_NINF;           // s is 0, or NaN
-    const float d = none ? 0.f : p.m2 - m, f = none ? 1.f : lp_exp2(d);
-    p.t = lp_sum<64>((p.t + p.s * d) * f);
-    p.s = lp_sum<64>(p.s * f);
-    p.raw = raw;
-    p.m2 = m;
-    return p;
-  }
-  for (int x = 32; x > 0; x >>= 1) {
-    LpPart o;
-    o.raw = __shfl_xor(p.raw, x, 64); o.m2 = __shfl_xor(p.m2, x, 64);
-    o.s = __shfl_xor(p.s, x, 64); o.t = __shfl_xor(p.t, x, 64);
-    // the same operand order on both sides keeps the lanes' copies bit-identical
-    if (rx_lane() & x) { LpPart q = o; lp_join(q, p); p = q; } else lp_join(p, o);
-  }
-  return p;
+// s and t, relative to a reference d log2 units away from the new one (-inf and NaN: nothing of them is left, but for NaN)
+__device__ __forceinline__ void lp_move(float d, float* s, float* t) {
+  d = fmaxf(d, -1e4f);
+  const float f = lp_exp2(d);
+  *t = (*t + *s * d) * f;
+  *s *= f;
 }
 
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(LP_WIDE)
 lp_wide_kernel(rx_logprob_args a, LpPart* parts, uint64_t* lists, int n_split, int32_t* err) {
   constexpr int N = LpVec<T>::N, W = LP_WIDE / 64;
-  __shared__ LpPart sh[W];
+  __shared__ float top_of[W];
+  __shared__ float2 sums[W];
   __shared__ uint64_t tops[TOP ? W : 1][TOP ? 128 : 1];
   const int64_t row = blockIdx.x / n_split;
   const int split = blockIdx.x % n_split;
@@ -529,33 +472,28 @@ lp_wide_kernel(rx_logprob_args a, LpPart* parts, uint64_t* lists, int n_split, i
       }
     }
   });
-  // the largest score of the workgroup decides, uniformly, whether the sums have to be taken again
+  // the largest score of the workgroup is its reference, and decides, uniformly, whether the sums have to be taken again
   float raw = lp_max<64>(acc.raw);
-  if (lane == 0) sh[wave].raw = raw;
+  if (lane == 0) top_of[wave] = raw;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < W; ++w) raw = fmaxf(raw, sh[w].raw);
-  __syncthreads();
-  LpPart p;
-  const bool big = fabsf(raw) > LP_BIG && fabsf(raw) < __builtin_inff();
-  if (big) {
+  for (int w = 0; w < W; ++w) raw = fmaxf(raw, top_of[w]);
+  if (fabsf(raw) > LP_BIG && fabsf(raw) < __builtin_inff()) {
     acc.s = 0.f; acc.t = 0.f;
     lp_stream<T>(l, n, split, n_split, [&](const float* v, int32_t) { acc.add_big<2 * N>(v, raw); });
-    p.raw = raw; p.m2 = raw; p.s = acc.s; p.t = acc.t;
   } else {
-    p.raw = acc.raw; p.m2 = acc.m2; p.s = acc.s; p.t = acc.t;
+    lp_move(-fmaf(raw == LP_NINF ? 0.f : raw, LP_L2E, -acc.m2), &acc.s, &acc.t);
   }
-  // a lane may have seen nothing but such scores under an ordinary maximum elsewhere: its sums are 0 then
-  p = lp_wave_join(p, false);
-  if (lane == 0) sh[wave] = p;
+  LpPart p = {raw, lp_sum<64>(acc.s), lp_sum<64>(acc.t), 0.f};
+  if (lane == 0) sums[wave] = make_float2(p.s, p.t);
   if constexpr (TOP) {
     top.flush();
     tops[wave][lane] = top.list;
   }
   __syncthreads();
-  p = sh[0];
+  p.s = p.t = 0.f;
 #pragma unroll
-  for (int w = 1; w < W; ++w) lp_join(p, sh[w]);
+  for (int w = 0; w < W; ++w) { p.s += sums[w].x; p.t += sums[w].y; }
   if constexpr (TOP) {
     if (wave == 0)
       for (int w = 1; w < W; ++w) top.list = lp_merge(top.list, tops[w][63 - lane]);
@@ -567,7 +505,7 @@ lp_wide_kernel(rx_logprob_args a, LpPart* parts, uint64_t* lists, int n_split, i
     }
     return;
   }
-  const LpRow r = lp_finish(p.raw, p.m2, p.s, p.t);
+  const LpRow r = lp_finish(p.raw, p.s, p.t);
   if (threadIdx.x == 0) lp_write_row(a, r, row);
   for (int t = threadIdx.x; t < a.T; t += LP_WIDE) lp_write_target<T>(a, r, l, n, row, t, err);
   if constexpr (TOP) {
@@ -581,26 +519,33 @@ template <typename T, bool TOP>
 __global__ void __launch_bounds__(RX_BLOCK)
 lp_join_kernel(rx_logprob_args a, const LpPart* parts, const uint64_t* lists, int n_split, int32_t* err) {
   constexpr int W = RX_BLOCK / 64;
-  __shared__ LpPart sh[W];
+  __shared__ float top_of[W];
+  __shared__ float2 sums[W];
   __shared__ uint64_t heads[W][64];
   __shared__ uint64_t tops[TOP ? W : 1][TOP ? 128 : 1];
   const int64_t row = blockIdx.x;
   const int wave = threadIdx.x >> 6, lane = rx_lane();
   const T* l = (const T*)a.logits + row * a.ld;
   const int32_t n = lp_live(a, row);
-  LpPart p;
-  p.raw = LP_NINF; p.m2 = LP_NINF; p.s = 0.f; p.t = 0.f;
+  LpPart p = {LP_NINF, 0.f, 0.f, 0.f};
   if ((int)threadIdx.x < n_split) p = parts[row * n_split + threadIdx.x];
-  p = lp_wave_join(p, __ballot(fabsf(p.raw) > LP_BIG && p.raw != LP_NINF) != 0);
-  if (lane == 0) sh[wave] = p;
+  float raw = lp_max<64>(p.raw);
+  if (lane == 0) top_of[wave] = raw;
   if constexpr (TOP) {
     heads[wave][lane] = lp_sort_up((int)threadIdx.x < n_split ? lists[(row * n_split + threadIdx.x) * a.k] : 0);
   }
   __syncthreads();
-  p = sh[0];
 #pragma unroll
-  for (int w = 1; w < W; ++w) lp_join(p, sh[w]);
-  const LpRow r = lp_finish(p.raw, p.m2, p.s, p.t);
+  for (int w = 0; w < W; ++w) raw = fmaxf(raw, top_of[w]);
+  lp_move((p.raw - raw) * LP_L2E, &p.s, &p.t);
+  p.s = lp_sum<64>(p.s);
+  p.t = lp_sum<64>(p.t);
+  if (lane == 0) sums[wave] = make_float2(p.s, p.t);
+  __syncthreads();
+  p.s = p.t = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) { p.s += sums[w].x; p.t += sums[w].y; }
+  const LpRow r = lp_finish(raw, p.s, p.t);
   if (threadIdx.x == 0) lp_write_row(a, r, row);
   for (int t = threadIdx.x; t < a.T; t += RX_BLOCK) lp_write_target<T>(a, r, l, n, row, t, err);
   if constexpr (TOP) {
@@ -632,13 +577,11 @@ lp_join_kernel(rx_logprob_args a, const LpPart* parts, const uint64_t* lists, in
 // probability (-1, a masked score, a column past the row's end) takes no part; a row with nothing left gets zeros.
 struct LpGrad {
   float ref, l2s, A, gh2;      // gh2 = g_H ln 2: log p is held in log2 units
-  bool dead, big;
-  template <bool BIG>
+  bool dead;
   __device__ __forceinline__ float of(float l) const {
-    const float d = (BIG ? (l - ref) * LP_L2E : fmaf(l, LP_L2E, -ref)) - l2s, p = lp_exp2(d);
+    const float d = fmaf(l - ref, LP_L2E, -l2s), p = lp_exp2(d);
     return p * fmaf(-gh2, fmaxf(d, -1e4f), A);
   }
-  __device__ __forceinline__ float any(float l) const { return big ? of<true>(l) : of<false>(l); }
 };
 template <typename T>
 __device__ __forceinline__ bool lp_target_on(const rx_logprob_args& a, const T* l, int32_t n, int64_t row, int t, int64_t* y) {
@@ -652,8 +595,7 @@ __device__ __forceinline__ LpGrad lp_grad_row(const rx_logprob_args& a, const fl
   r.ref = st.x; r.l2s = st.y;
   r.gh2 = h * LP_LN2;
   r.A = (gl ? gl[row] : 0.f) - gsum - h * st.w;
-  r.dead = st.z == 2.f;
-  r.big = st.z != 0.f;
+  r.dead = st.z != 0.f;
   return r;
 }
 // the whole gradient of target t's column: its share of the softmax and every gradient that names the column; written
@@ -669,7 +611,7 @@ __device__ __forceinline__ void lp_fix_target(const rx_logprob_args& a, const Lp
     if (u < t) return;
     sum += g[row * a.T + u];
   }
-  lp_put<T>(d + y, r.any(lp_elem(l + y)) + sum);
+  lp_put<T>(d + y, r.of(lp_elem(l + y)) + sum);
 }
 
 template <typename T, int G, int PER>
@@ -697,7 +639,7 @@ lp_bwd_small_kernel(rx_logprob_args a, const float* __restrict__ g, const float*
 #pragma unroll
   for (int q = 0; q < PER; ++q) {
     const int c = q * G + sub;
-    v[q] = c < n && !r.dead ? r.any(lp_elem(l + c)) : 0.f;
+    v[q] = c < n && !r.dead ? r.of(lp_elem(l + c)) : 0.f;
   }
   if (g && !r.dead) {
     // every lane looks at all targets: its own columns take their gradients in ascending target order
@@ -754,10 +696,10 @@ lp_bwd_wide_kernel(rx_logprob_args a, const float* __restrict__ g, const float* 
         for (int i = 0; i < N; ++i) v[i] = lp_elem(l + c + i);
       }
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = r.any(v[i]);
+      for (int i = 0; i < N; ++i) v[i] = r.of(v[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = c + i < n && !r.dead ? r.any(lp_elem(l + c + i)) : 0.f;
+      for (int i = 0; i < N; ++i) v[i] = c + i < n && !r.dead ? r.of(lp_elem(l + c + i)) : 0.f;
     }
     uint4 o;
     if constexpr (sizeof(T) == 4) {
@@ -774,11 +716,11 @@ lp_bwd_wide_kernel(rx_logprob_args a, const float* __restrict__ g, const float* 
   const int32_t tail = head + nvec * N;
   if (split == 0 && (int)threadIdx.x < head) {
     const int c = threadIdx.x;
-    lp_put<T>(d + c, c < n && !r.dead ? r.any(lp_elem(l + c)) : 0.f);
+    lp_put<T>(d + c, c < n && !r.dead ? r.of(lp_elem(l + c)) : 0.f);
   }
   if (split == n_split - 1 && (int)threadIdx.x < V - tail) {
     const int c = tail + threadIdx.x;
-    lp_put<T>(d + c, c < n && !r.dead ? r.any(lp_elem(l + c)) : 0.f);
+    lp_put<T>(d + c, c < n && !r.dead ? r.of(lp_elem(l + c)) : 0.f);
   }
   if (!g) return;
   __syncthreads();           // the targets' columns are written again, after everything else of this split
