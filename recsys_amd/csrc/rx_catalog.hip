@@ -55,7 +55,7 @@ typedef float ct_acc __attribute__((ext_vector_type(16)));
 struct CtRow {               // what the backward pass needs of a row
   float m2, l2s, z, sgn;     // p_rv |c_r| = 2^(s log2 e - m2 - l2s), z = m2 + l2s, sgn = sign of c_r
   float g;                   // gradient of logprob (0 where the row has no target)
-  int32_t y;                 // target or -1
+  int32_t y;                 // target whose share is g x, or -1
   float gl2;                // log2 |g|
   int32_t pad;
 };
@@ -735,7 +735,7 @@ __global__ void __launch_bounds__(CT_THREADS) ct_prep_kernel(CtPrep a) {
     r.l2s = c == 0.f ? __builtin_inff() : st.y - log2f(fabsf(c));
     r.z = r.m2 + r.l2s;
     r.g = g;
-    r.y = (int32_t)y;
+    r.y = g != 0.f ? (int32_t)y : -1;      // without a share the target may be as unlikely as it likes (NaN stays)
     r.gl2 = log2f(fabsf(g));
     r.pad = 0;
     a.rows[row] = r;
@@ -899,11 +899,12 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e] = __builtin_amdgcn_exp2f(PL == 2 ? w[e] - rf : w[e]);
         if (hit) {                // the target's own share: sgn(c) g on top of |c| p, both still to meet sgn(c) x
-          const float up = PL == 2 ? __builtin_amdgcn_exp2f(kt - rf) : 1.f;
+          // two factors: g 2^(kt - ref) is below 2^CT_TOP where g counts, 2^(kt - ref) alone is out of range for a g below 2^-114
+          const float up = PL == 2 ? __builtin_amdgcn_exp2f(0.5f * (kt - rf)) : 1.f;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int k = it * 32 + 8 * (e / 4) + 4 * h;
-            const float share = fmaf(ct_at(lg + k, e % 4), up, w[e]);
+            const float share = PL == 2 ? fmaf(ct_at(lg + k, e % 4) * up, up, w[e]) : ct_at(lg + k, e % 4) + w[e];
             w[e] = __float_as_int(ct_at(ly + k, e % 4)) == mine ? share : w[e];
           }
         }
