@@ -49,6 +49,10 @@ typedef float ct_acc __attribute__((ext_vector_type(16)));
 // to 2^-36 of the largest beside it.
 #define CT_BASE(PL) ((PL) == 2 ? 11.f : 0.f)
 #define CT_TOP(PL) ((PL) == 2 ? 14.f : 24.f)
+// Sums of weights are held times the tile's scale undone (at most 2^100: a tile of zeros), which 2^CT_TOP of 2^30 items would take
+// out of fp32: fp32 operands' sums are held times 2^-CT_DOWN.
+#define CT_DOWN(PL) ((PL) == 2 ? 20.f : 0.f)
+#define CT_UNIT 9.5367431640625e-7f       // 2^-CT_DOWN(2)
 #define CT_THREADS 256
 #define CT_WAVES 4
 
@@ -446,7 +450,7 @@ struct CtFwd {
   const float* bias;
   int D, tiles, n_split;
   int64_t per_split;           // items per split, a multiple of the tile
-  float2* part;                // [n_split][R]: reference, sum
+  float2* part;                // [n_split][R]: reference, sum times 2^-CT_DOWN
   float* out;                  // [n_split][R][D]: sum of weight * t_v
 };
 
@@ -496,7 +500,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
   fetch(0);
   CtFrag st[MB][DP / 16][PL];
   ct_acc o[MB][MEAN ? DP / 32 : 1] = {};
-  // w = 2^((score - ref) + (kt - kr)), kt the tile's scale undone; sum: of w / 2^kt.  Without a bias kt is part of the
+  // w = 2^((score - ref) + (kt - kr)), kt the tile's scale undone; sum: of w / 2^(kt + CT_DOWN).  Without a bias kt is part of the
   // score and kr stays 0: one operation less per score.  A bias may be a mask of 1e38, which would swallow it.
   float inv[MB], ref[MB], kr[MB], sum[MB];
 #pragma unroll
@@ -521,7 +525,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
     const uint16_t* rm = reinterpret_cast<const uint16_t*>(ct_lds + (i & 1) * Tile::BYTES);
     const uint16_t* tr = rm + Tile::RM;
     const float* bb = lb + (i & 1) * BN;
-    const float kt = PL == 2 ? -ct_log2(scale) : 0.f, back = ct_inverse(scale);
+    const float kt = PL == 2 ? -ct_log2(scale) : 0.f, back = ct_inverse(scale), unit = scale * CT_UNIT;
     const int64_t left = v1 - v0 - (int64_t)i * BN;
     const int live = left < BN ? (int)left : BN;
 #pragma unroll
@@ -574,7 +578,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           w[e] = __builtin_amdgcn_exp2f(!BIAS ? w[e] : PL == 2 ? (w[e] - r0) + dk : w[e] - r0);
-          sum[mb] = PL == 2 ? fmaf(w[e], scale, sum[mb]) : sum[mb] + w[e];
+          sum[mb] = PL == 2 ? fmaf(w[e], unit, sum[mb]) : sum[mb] + w[e];
         }
         if constexpr (MEAN) ct_weigh<PL, DP, BN>(tr, it, w, o[mb]);
       }
@@ -586,7 +590,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
     float total = sum[mb] + __shfl_xor(sum[mb], 32, 64);
-    if constexpr (PL == 2 && BIAS) {                          // back to plain 2^(score - ref)
+    if constexpr (PL == 2 && BIAS) {                          // back to 2^(score - ref)
       const float f = __builtin_amdgcn_exp2f(kr[mb]);
       total *= f;
       if constexpr (MEAN) {
@@ -662,8 +666,14 @@ __global__ void __launch_bounds__(CT_THREADS) ct_join_kernel(CtJoin a, int32_t* 
     s += p.y * __builtin_amdgcn_exp2f(p.x - r0);
   }
   s = ct_row<false, TPR>(s, w);
+  constexpr int PL = sizeof(T) == 4 ? 2 : 1;
   const bool empty = s == 0.f;
-  const float l2s = empty ? 0.f : log2f(s), lse = empty ? CT_NINF : (r0 + l2s) * CT_LN2;
+  // log2 of the sum to the reference and on top of it.  A reference holds the tile's scale undone, up to 100, and the sum makes up
+  // for it: their integer parts meet first (unless the reference is too large to take them, a mask), or both would round at that size.
+  const float up = empty ? 0.f : (float)__builtin_amdgcn_frexp_expf(s) + CT_DOWN(PL), near = r0 + up;
+  const bool fits = near - r0 == up;
+  const float l2s = empty ? 0.f : fits ? log2f(__builtin_amdgcn_frexp_mantf(s)) : log2f(s) + CT_DOWN(PL);
+  const float m2 = fits ? near : r0, lse = empty ? CT_NINF : (m2 + l2s) * CT_LN2;
   if (a.mean) {
     const int wide = a.D <= 32 ? 32 : a.D <= 64 ? 64 : a.D <= 128 ? 128 : 256;
     const int dp = wide < TPR ? wide : TPR, groups = TPR / dp;      // threads along the dimensions, and along the splits
@@ -683,7 +693,7 @@ __global__ void __launch_bounds__(CT_THREADS) ct_join_kernel(CtJoin a, int32_t* 
         if (tid < dp)
           for (int k = 1; k < groups; ++k) m += sums[k * dp + tid];
       }
-      if (tid < dp && d < a.D) a.mean[row * a.D + d] = empty ? 0.f : m / s;
+      if (tid < dp && d < a.D) a.mean[row * a.D + d] = empty ? 0.f : (PL == 2 ? m * CT_UNIT : m) / s;
     }
   }
   if (tid >= 64) return;
@@ -695,13 +705,13 @@ __global__ void __launch_bounds__(CT_THREADS) ct_join_kernel(CtJoin a, int32_t* 
     const float b = a.bias ? a.bias[y] : 0.f, b2 = ct_bias2(b);
     if (empty || b == CT_NINF) lp = CT_NINF;
     else if (fabsf(b2) == CT_LIM && fabsf(r0) < 1e38f) lp = dot + b - lse;      // a mask of the type's lowest value
-    else lp = (fmaf(dot, CT_L2E, b2) - r0 - l2s) * CT_LN2;
+    else lp = (fmaf(dot, CT_L2E, b2) - m2 - l2s) * CT_LN2;
   } else lp = y == -1 ? 0.f : __builtin_nanf("");
   if (lane == 0) {
     if (!ok && y != -1 && err) atomicOr(err, RX_ERR_INDEX);
     a.logprob[row] = lp;
     a.lse[row] = lse;
-    if (a.stats) reinterpret_cast<float2*>(a.stats)[row] = make_float2(r0, empty ? __builtin_inff() : l2s);
+    if (a.stats) reinterpret_cast<float2*>(a.stats)[row] = make_float2(empty ? CT_NINF : m2, l2s);      // -inf: no item left
   }
 }
 
@@ -724,14 +734,14 @@ __global__ void __launch_bounds__(CT_THREADS) ct_prep_kernel(CtPrep a) {
   if (row >= a.R) return;
   const float2 st = reinterpret_cast<const float2*>(a.stats)[row];
   int64_t y = a.targets[row];
-  const bool dead = st.y == __builtin_inff();
+  const bool dead = st.x == CT_NINF;
   if (dead || y < 0 || y >= a.V || (a.bias && a.bias[y] == CT_NINF)) y = -1;      // nothing depends on such a target
   const float g = y >= 0 && a.g ? a.g[row] : 0.f;
   const float c = dead ? 0.f : (a.gl ? a.gl[row] : 0.f) - g;
   if (rx_lane() == 0 && a.rows) {
     CtRow r;
     r.sgn = c < 0.f ? -1.f : 1.f;
-    r.m2 = st.x;
+    r.m2 = dead ? 0.f : st.x;
     r.l2s = c == 0.f ? __builtin_inff() : st.y - log2f(fabsf(c));
     r.z = r.m2 + r.l2s;
     r.g = g;
@@ -809,7 +819,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
     if (threadIdx.x < BN) {
       float* p = lz + threadIdx.x;
       p[0] = BIAS ? info.m2 : info.z - kt;
-      if (BIAS) { p[BN] = info.l2s - kt; p[2 * BN] = info.sgn * scale; }     // sign of c, with the tile's scale undone
+      if (BIAS) { p[BN] = info.l2s - kt; p[2 * BN] = info.sgn * (PL == 2 ? scale * CT_UNIT : scale); }   // sign of c, with the tile's scale undone
       p[3 * BN] = info.g * info.sgn;
       p[4 * BN] = __int_as_float(info.y);
       p[6 * BN] = info.gl2 + kt;
@@ -939,7 +949,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
       const float f = ref[mb] == CT_NINF ? 1.f : __builtin_amdgcn_exp2f(0.5f * ref[mb]);
-      dbias[mb] = dbias[mb] * f * f;
+      dbias[mb] = dbias[mb] * f * f / CT_UNIT;
 #pragma unroll
       for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
