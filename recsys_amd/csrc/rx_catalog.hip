@@ -443,6 +443,21 @@ __device__ __forceinline__ void ct_place(int tiles, int n_split, int* tile, int*
   }
 }
 
+// sum of 16 weights in four roundings
+__device__ __forceinline__ float ct_sum16(const float* w) {
+  float p[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p[i] = w[2 * i] + w[2 * i + 1];
+  return ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+}
+// sum += add, with the rounding that the last such addition lost: near-equal terms would all round the same way
+__device__ __forceinline__ void ct_add(float add, float* sum, float* lost) {
+  add -= *lost;
+  const float s = *sum + add;
+  *lost = (s - *sum) - add;
+  *sum = s;
+}
+
 // ---------------------------------------------------------------- forward
 struct CtFwd {
   const void *x, *t;
@@ -502,12 +517,12 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
   ct_acc o[MB][MEAN ? DP / 32 : 1] = {};
   // w = 2^((score - ref) + (kt - kr)), kt the tile's scale undone; sum: of w / 2^(kt + CT_DOWN).  Without a bias kt is part of the
   // score and kr stays 0: one operation less per score.  A bias may be a mask of 1e38, which would swallow it.
-  float inv[MB], ref[MB], kr[MB], sum[MB];
+  float inv[MB], ref[MB], kr[MB], sum[MB], lost[MB];
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
     inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.x, a.ld_x, row0 + mb * 32, a.R, a.D, false, st[mb]);
     ref[mb] = CT_NINF;
-    kr[mb] = sum[mb] = 0.f;
+    kr[mb] = sum[mb] = lost[mb] = 0.f;
   }
   publish(0);
   __syncthreads();
@@ -559,6 +574,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
             if (ref[mb] != CT_NINF) {
               const float f = __builtin_amdgcn_exp2f((ref[mb] - nr) + (kr[mb] - nk));
               sum[mb] *= f;
+              lost[mb] *= f;
               if constexpr (MEAN) {
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db)
@@ -576,10 +592,8 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
         }
         const float dk = kb - kr[mb];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          w[e] = __builtin_amdgcn_exp2f(!BIAS ? w[e] : PL == 2 ? (w[e] - r0) + dk : w[e] - r0);
-          sum[mb] = PL == 2 ? fmaf(w[e], unit, sum[mb]) : sum[mb] + w[e];
-        }
+        for (int e = 0; e < 16; ++e) w[e] = __builtin_amdgcn_exp2f(!BIAS ? w[e] : PL == 2 ? (w[e] - r0) + dk : w[e] - r0);
+        ct_add(PL == 2 ? ct_sum16(w) * unit : ct_sum16(w), &sum[mb], &lost[mb]);
         if constexpr (MEAN) ct_weigh<PL, DP, BN>(tr, it, w, o[mb]);
       }
     }
@@ -925,9 +939,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
             const float* sg = lsg + it * 32 + 8 * q + 4 * h;
             part[q] = fmaf(w[4 * q + 1], ct_at(sg, 1), w[4 * q] * ct_at(sg, 0)) + fmaf(w[4 * q + 3], ct_at(sg, 3), w[4 * q + 2] * ct_at(sg, 2));
           }
-          const float add = ((part[0] + part[1]) + (part[2] + part[3])) - lost[mb], sum = dbias[mb] + add;
-          lost[mb] = (sum - dbias[mb]) - add;
-          dbias[mb] = sum;
+          ct_add((part[0] + part[1]) + (part[2] + part[3]), &dbias[mb], &lost[mb]);
         }
         ct_weigh<PL, DP, BN>(tr, it, w, o[mb]);
         if (PL == 1 && hit) {     // a target's share is as large as the whole gradient: what bf16 dropped of these weights goes in too
