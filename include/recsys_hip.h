@@ -817,8 +817,9 @@ int rx_logprob_bwd(const rx_logprob_args* args, const float* d_g_logprob, const 
  * or no gradient of its lse): such a row may hold anything.  A target of -1 stands for "no target" (logprob 0, no
  * gradient through it); any other target outside [0, V) sets RX_ERR_INDEX and gives NaN.  A bias of -inf takes an item
  * out, whatever its vector holds; a target that is out gives -inf and no gradient, and a row with no item left gives lse -inf and no gradient.
- * `stats` [R, 2] and `mean` [R, D] fp32 (both may be NULL) are what rx_catalog_bwd needs: the row's softmax
- * reference and sum, and sum_v p_rv t_v (only for the gradient of x).
+ * `stats` [R, 4] (16-byte aligned) and `mean` [R, D] fp32 (both may be NULL) are what rx_catalog_bwd needs: the row's softmax
+ * reference and sum, rest_r = sum_{v != y_r} p_rv (of bf16's rounded weights with the mean), the smaller of p_{r, y_r} and
+ * -(1 - p_{r, y_r}) by size; and mean_r = sum_{v != y_r} p_rv t_v (only for the gradient of x).
  * The full-catalogue counterpart of the sampled BCE loss (recsys/models/matrix_factorization/vanilla_mf.py:35-39). */
 typedef struct {
   const void* x;
@@ -833,11 +834,13 @@ typedef struct {
 size_t rx_catalog_fwd_workspace_bytes(int64_t R, int64_t V, int32_t D, int32_t bf16, int32_t want_mean);
 int rx_catalog_fwd(const rx_catalog_args* args, float* d_logprob, float* d_lse, float* d_stats, float* d_mean, void* ws,
                    size_t ws_bytes, int32_t* err_flag, int device, void* stream);
-/* Gradients from those of logprob [R] and lse [R] (each may be NULL = zero), with c_r = g_lse_r - g_r:
- *   dx_r = g_r t_{y_r} + c_r mean_r       dtable_v = sum_r c_r p_rv x_r + sum_{r: y_r = v} g_r x_r
- *   dbias_v = sum_r c_r p_rv + sum_{r: y_r = v} g_r
+/* Gradients from those of logprob [R] and lse [R] (each may be NULL = zero), with c_r = g_lse_r - g_r and
+ * q_r = g_r + c_r p_{r, y_r}, taken as g_r rest_r + g_lse_r p_{r, y_r}:
+ *   dx_r = q_r t_{y_r} + c_r mean_r       dtable_v = sum_{r: y_r != v} c_r p_rv x_r + sum_{r: y_r = v} q_r x_r
+ *   dbias_v = sum_{r: y_r != v} c_r p_rv + sum_{r: y_r = v} q_r
+ * so that rows which are nearly sure of their target lose nothing.
  * d_dx [R, D] / d_dtable [V, D] (the operands' type, 16-byte aligned table gradient, rows back to back) or NULL; with a bias
- * d_dbias [V] comes with d_dtable.  fp32: beside their relative error the weights c_r p_rv, g_r (and p_rv in the mean) are held to
+ * d_dbias [V] comes with d_dtable.  fp32: beside their relative error the weights c_r p_rv, q_r (and p_rv in the mean) are held to
  * 2^-36 of the largest of their item (row).  Deterministic: no atomics.  Workspace only with d_dtable. */
 size_t rx_catalog_bwd_workspace_bytes(int64_t R, int64_t V, int32_t D, int32_t bf16, int32_t want_bias);
 int rx_catalog_bwd(const rx_catalog_args* args, const float* d_stats, const float* d_mean, const float* d_g_logprob,

@@ -1,10 +1,12 @@
 // Softmax over a whole item catalogue (gfx950): scores s_rv = x_r . t_v + b_v of rows x [R, D] against a table
 // t [V, D], never stored.
-//   forward   lse_r = log sum_v exp s_rv,  logprob_r = s_{r,y_r} - lse_r,  mean_r = sum_v p_rv t_v
-//   backward  dx_r = g_r t_{y_r} + c_r mean_r,   dt_v = sum_r c_r p_rv x_r + sum_{r: y_r = v} g_r x_r,   c_r = g_lse_r - g_r
-// The rows' expectation mean_r does not depend on the gradient, so the forward pass takes it along (online softmax with
+//   forward   lse_r = log sum_v exp s_rv,  logprob_r = s_{r,y_r} - lse_r,  mean_r = sum_{v != y_r} p_rv t_v,  rest_r = sum_{v != y_r} p_rv
+//   backward  dx_r = q_r t_{y_r} + c_r mean_r,   dt_v = sum_{r: y_r != v} c_r p_rv x_r + sum_{r: y_r = v} q_r x_r,
+//             c_r = g_lse_r - g_r,   q_r = g_r + c_r p_{r,y_r} = g_r rest_r + g_lse_r p_{r,y_r}
+// The rows' expectation does not depend on the gradient, so the forward pass takes it along (online softmax with
 // the table as keys and values) and a train step costs four products of 2 R V D operations: scores and mean forward,
-// scores and dt backward.
+// scores and dt backward.  A row's target stays out of its sums and joins them at their end: on a row that is nearly sure of it the
+// gradients are of the size of 1 - p_y, and so are all their errors then; g + c p_y would keep those of g.
 //
 // Both passes are one loop.  One side is stationary (forward: rows, backward: items): its vectors sit in registers as
 // matrix operands, 32 per wavefront and block, one per lane column.  The other side streams through LDS in tiles, kept
@@ -22,8 +24,10 @@
 // own largest element, a streaming tile by the tile's (both to 2^14 .. 2^15: elements down to 2^-15 of the largest keep
 // all their bits, smaller ones an absolute error of 2^-39 of it), and the weights by a running reference per stationary
 // vector (the softmax's own in the forward pass).  The factors fold into numbers the loop has anyway.
-// bf16 operands take one plane, exactly; there the weights of the second product are rounded to bf16 as well, 2^-9
-// relative and independent from term to term, as much as the result's own rounding.
+// bf16 operands take one plane, exactly; there the weights of the second product are rounded to bf16 as well, by up to 2^-8 of
+// each and independently from term to term.  Where they meet a large term of the other sign, the rounding is made good: dx takes the sum
+// of the rounded weights for rest, so that it is a sum of (t_y - t_v) under them, and the targets' shares q of the table's gradient come
+// with their low part.
 // Scores, references, sums, means and gradients accumulate in fp32.
 // Measured, where a large bf16 product reaches 1151 TFLOP/s: 2048 x 1000003 x 64 fp32 forward 1.72 ms, table gradient 1.83 (914 and
 // 860 TFLOP/s of plane products), 8192 x 100003 x 128 bf16 515 and 600 us (814 and 699).  What keeps them from more is the
@@ -58,9 +62,9 @@ typedef float ct_acc __attribute__((ext_vector_type(16)));
 
 struct CtRow {               // what the backward pass needs of a row
   float m2, l2s, z, sgn;     // p_rv |c_r| = 2^(s log2 e - m2 - l2s), z = m2 + l2s, sgn = sign of c_r
-  float g;                   // gradient of logprob (0 where the row has no target)
-  int32_t y;                 // target whose share is g x, or -1
-  float gl2;                // log2 |g|
+  float q;                   // what stands in for c p at the target
+  int32_t y;                 // target or -1
+  float ql2;                // log2 |q|
   int32_t pad;
 };
 
@@ -401,14 +405,22 @@ __device__ __forceinline__ ct_acc ct_scores(const uint16_t* rm, int it, const Ct
   return s;
 }
 // out[db] += transposed tile (dims db * 32 ..) x weights, w[16] in the scores' register order
-template <int PL, int DP, int BN>
-__device__ __forceinline__ void ct_weigh(const uint16_t* tr, int it, const float* w, ct_acc* out) {
+template <int PL, int DP, int BN, bool SUM = false>
+__device__ __forceinline__ void ct_weigh(const uint16_t* tr, int it, const float* w, ct_acc* out, float* sum = nullptr) {
   typedef CtTile<PL, DP, BN, true, 256> Tile;
   const int l31 = rx_lane() & 31, h = rx_lane() >> 5;
 #pragma unroll
   for (int k2 = 0; k2 < 2; ++k2) {
     CtFrag b[PL];
     ct_cut8<PL>(w + k2 * 8, b);
+    if constexpr (SUM) {                    // of the weights as they are used
+      const ct_h2 one = {(__bf16)1.f, (__bf16)1.f};
+      const uint32_t u[4] = {b[0].u.x, b[0].u.y, b[0].u.z, b[0].u.w};
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(ct_h2, u[i]), one, s, false);
+      *sum += s;
+    }
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) {
       CtFrag a[PL];
@@ -465,7 +477,9 @@ struct CtFwd {
   const float* bias;
   int D, tiles, n_split;
   int64_t per_split;           // items per split, a multiple of the tile
+  const int64_t* targets;      // a row's target takes no part in what follows
   float2* part;                // [n_split][R]: reference, sum times 2^-CT_DOWN
+  float* rest;                 // [n_split][R], bf16 with MEAN: the same sum, of the weights as out has them
   float* out;                  // [n_split][R][D]: sum of weight * t_v
 };
 
@@ -518,11 +532,15 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
   // w = 2^((score - ref) + (kt - kr)), kt the tile's scale undone; sum: of w / 2^(kt + CT_DOWN).  Without a bias kt is part of the
   // score and kr stays 0: one operation less per score.  A bias may be a mask of 1e38, which would swallow it.
   float inv[MB], ref[MB], kr[MB], sum[MB], lost[MB];
+  float rest[MB];                                          // bf16 with MEAN
+  int32_t target[MB];                                      // or -1; counted from the next tile's first item
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
     inv[mb] = CT_L2E * ct_stationary<T, PL, DP>((const T*)a.x, a.ld_x, row0 + mb * 32, a.R, a.D, false, st[mb]);
     ref[mb] = CT_NINF;
-    kr[mb] = sum[mb] = lost[mb] = 0.f;
+    kr[mb] = sum[mb] = lost[mb] = rest[mb] = 0.f;
+    const int64_t row = row0 + mb * 32 + l31, y = row < a.R ? a.targets[row] : -1;
+    target[mb] = y >= v0 && y < v1 ? (int32_t)(y - v0) : -1;
   }
   publish(0);
   __syncthreads();
@@ -543,6 +561,10 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
     const float kt = PL == 2 ? -ct_log2(scale) : 0.f, back = ct_inverse(scale), unit = scale * CT_UNIT;
     const int64_t left = v1 - v0 - (int64_t)i * BN;
     const int live = left < BN ? (int)left : BN;
+    bool mine = false;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) mine = mine || (uint32_t)target[mb] < (uint32_t)BN;
+    const bool special = live < BN || __ballot(mine) != 0;    // items past the end, or a row's target
 #pragma unroll
     for (int it = 0; it < BN / 32; ++it) {
 #pragma unroll
@@ -558,11 +580,14 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
           if constexpr (BIAS) w[e] = fmaf(s[e], mul, ct_at(bb + it * 32 + 8 * (e / 4) + 4 * h, e % 4));
           else w[e] = fmaf(s[e], mul, (PL == 2 ? kt : 0.f) - r0);
         }
-        if (live < BN) {
+        if (special) {
+          int end = live - (it * 32 + 4 * h), at = target[mb] - (it * 32 + 4 * h);
+          asm volatile("" : "+v"(end), "+v"(at));             // the comparisons are for few tiles only, and stay behind the branch
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (it * 32 + 8 * (e / 4) + 4 * h + e % 4 >= live) w[e] = CT_NINF;
-          asm volatile("");         // a branch: the comparisons are for the last tile only
+          for (int e = 0; e < 16; ++e) {
+            const int k = 8 * (e / 4) + e % 4;
+            if (k >= end || k == at) w[e] = CT_NINF;
+          }
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) mx = fmaxf(mx, w[e]);
@@ -575,6 +600,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
               const float f = __builtin_amdgcn_exp2f((ref[mb] - nr) + (kr[mb] - nk));
               sum[mb] *= f;
               lost[mb] *= f;
+              rest[mb] *= f;
               if constexpr (MEAN) {
 #pragma unroll
                 for (int db = 0; db < DP / 32; ++db)
@@ -594,9 +620,11 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e] = __builtin_amdgcn_exp2f(!BIAS ? w[e] : PL == 2 ? (w[e] - r0) + dk : w[e] - r0);
         ct_add(PL == 2 ? ct_sum16(w) * unit : ct_sum16(w), &sum[mb], &lost[mb]);
-        if constexpr (MEAN) ct_weigh<PL, DP, BN>(tr, it, w, o[mb]);
+        if constexpr (MEAN) ct_weigh<PL, DP, BN, PL == 1>(tr, it, w, o[mb], &rest[mb]);
       }
     }
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) target[mb] -= BN;
     if (i + 2 < n) publish(i);
     scale = next;
     __syncthreads();
@@ -604,6 +632,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
     float total = sum[mb] + __shfl_xor(sum[mb], 32, 64);
+    const float others = MEAN && PL == 1 ? rest[mb] + __shfl_xor(rest[mb], 32, 64) : 0.f;
     if constexpr (PL == 2 && BIAS) {                          // back to 2^(score - ref)
       const float f = __builtin_amdgcn_exp2f(kr[mb]);
       total *= f;
@@ -618,6 +647,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
     if (row >= a.R) continue;
     if (h == 0) a.part[(int64_t)split * a.R + row] = make_float2(ref[mb], total);
     if constexpr (MEAN) {
+      if (PL == 1 && h == 0) a.rest[(int64_t)split * a.R + row] = others;
       float* out = a.out + ((int64_t)split * a.R + row) * a.D;
       const bool v4 = a.D % 4 == 0;
 #pragma unroll
@@ -635,7 +665,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_fwd_kernel(CtFwd a) {
   }
 }
 
-// Joins a row's splits and takes the target's score as a plain dot product: TPR threads per row, which share out the splits as
+// Joins a row's splits and its target, whose score is a plain dot product: TPR threads per row, which share out the splits as
 // well as the dimensions.  A wavefront per row (64) for up to 8 splits, where 8192 rows of 4 take 21 us against 29; a
 // workgroup (256) for more: 143 rows of 512 splits 50 us with the pass before it, against 170.
 struct CtJoin {
@@ -645,7 +675,7 @@ struct CtJoin {
   const int64_t* targets;
   int D, n_split;
   const float2* part;
-  const float* out;
+  const float *rest, *out;
   float *logprob, *lse, *stats, *mean;
 };
 template <typename T>
@@ -670,24 +700,37 @@ __global__ void __launch_bounds__(CT_THREADS) ct_join_kernel(CtJoin a, int32_t* 
   const int64_t row = (int64_t)blockIdx.x * (CT_THREADS / TPR) + threadIdx.x / TPR;
   const int lane = rx_lane(), tid = threadIdx.x % TPR;
   if (TPR == 64 && row >= a.R) return;
+  constexpr int PL = sizeof(T) == 4 ? 2 : 1;
+  const int64_t y = a.targets[row];
+  const bool ok = y >= 0 && y < a.V;
+  const float bias = ok && a.bias ? a.bias[y] : 0.f, b2 = ct_bias2(bias);
+  const float dot = ok ? ct_dot((const T*)a.x + row * a.ld_x, (const T*)a.t + y * a.ld_t, a.D) : 0.f;
+  const float mine = ok && bias != CT_NINF ? fmaf(dot, CT_L2E, b2) : CT_NINF;      // the target's score, in log2 units
   float ref = CT_NINF;
   for (int q = tid; q < a.n_split; q += TPR) ref = fmaxf(ref, a.part[(int64_t)q * a.R + row].x);
   ref = ct_row<true, TPR>(ref, w);
   const float r0 = ref == CT_NINF ? 0.f : ref;
-  float s = 0.f;
+  float sum = 0.f, used = 0.f;             // of all but the target: their sum, and that of the weights as the mean has them
   for (int q = tid; q < a.n_split; q += TPR) {
     const float2 p = a.part[(int64_t)q * a.R + row];
-    s += p.y * __builtin_amdgcn_exp2f(p.x - r0);
+    const float f = __builtin_amdgcn_exp2f(p.x - r0);
+    sum += p.y * f;
+    if (PL == 1 && a.mean) used += a.rest[(int64_t)q * a.R + row] * f;
   }
-  s = ct_row<false, TPR>(s, w);
-  constexpr int PL = sizeof(T) == 4 ? 2 : 1;
-  const bool empty = s == 0.f;
-  // log2 of the sum to the reference and on top of it.  A reference holds the tile's scale undone, up to 100, and the sum makes up
-  // for it: their integer parts meet first (unless the reference is too large to take them, a mask), or both would round at that size.
-  const float up = empty ? 0.f : (float)__builtin_amdgcn_frexp_expf(s) + CT_DOWN(PL), near = r0 + up;
+  sum = ct_row<false, TPR>(sum, w);
+  used = PL == 1 && a.mean ? ct_row<false, TPR>(used, w) : sum;
+  // Weight of the others and of the target relative to the larger of the two, 2^m2.  A reference holds the tile's scale undone, up to
+  // 100, and the sum makes up for it: their integer parts meet first (unless the reference is too large to take them, a mask), or
+  // all that follows would round at that size.
+  const float up = (float)__builtin_amdgcn_frexp_expf(sum) + CT_DOWN(PL), near = r0 + up;
   const bool fits = near - r0 == up;
-  const float l2s = empty ? 0.f : fits ? log2f(__builtin_amdgcn_frexp_mantf(s)) : log2f(s) + CT_DOWN(PL);
-  const float m2 = fits ? near : r0, lse = empty ? CT_NINF : (m2 + l2s) * CT_LN2;
+  const float m2 = sum == 0.f ? (mine == CT_NINF ? 0.f : mine) : fmaxf(fits ? near : r0, mine);
+  const float others = sum == 0.f ? 0.f
+      : fits ? __builtin_amdgcn_frexp_mantf(sum) * __builtin_amdgcn_exp2f(near - m2) : sum * __builtin_amdgcn_exp2f(r0 - m2 + CT_DOWN(PL));
+  const float own = __builtin_amdgcn_exp2f(mine - m2), s = others + own;
+  const bool empty = s == 0.f;
+  const float l2s = empty ? 0.f : log2f(s), lse = empty ? CT_NINF : (m2 + l2s) * CT_LN2;
+  const float rest = empty ? 0.f : others / s;
   if (a.mean) {
     const int wide = a.D <= 32 ? 32 : a.D <= 64 ? 64 : a.D <= 128 ? 128 : 256;
     const int dp = wide < TPR ? wide : TPR, groups = TPR / dp;      // threads along the dimensions, and along the splits
@@ -707,25 +750,23 @@ __global__ void __launch_bounds__(CT_THREADS) ct_join_kernel(CtJoin a, int32_t* 
         if (tid < dp)
           for (int k = 1; k < groups; ++k) m += sums[k * dp + tid];
       }
-      if (tid < dp && d < a.D) a.mean[row * a.D + d] = empty ? 0.f : (PL == 2 ? m * CT_UNIT : m) / s;
+      if (tid < dp && d < a.D) a.mean[row * a.D + d] = sum == 0.f ? 0.f : (PL == 2 ? m * CT_UNIT : m) / sum * rest;
     }
   }
   if (tid >= 64) return;
-  const int64_t y = a.targets[row];
-  const bool ok = y >= 0 && y < a.V;
-  float lp;
+  float lp = y == -1 ? 0.f : __builtin_nanf("");
   if (ok) {
-    const float dot = ct_dot((const T*)a.x + row * a.ld_x, (const T*)a.t + y * a.ld_t, a.D);
-    const float b = a.bias ? a.bias[y] : 0.f, b2 = ct_bias2(b);
-    if (empty || b == CT_NINF) lp = CT_NINF;
-    else if (fabsf(b2) == CT_LIM && fabsf(r0) < 1e38f) lp = dot + b - lse;      // a mask of the type's lowest value
-    else lp = (fmaf(dot, CT_L2E, b2) - m2 - l2s) * CT_LN2;
-  } else lp = y == -1 ? 0.f : __builtin_nanf("");
+    if (empty || bias == CT_NINF) lp = CT_NINF;
+    else if (fabsf(b2) == CT_LIM && fabsf(m2) < 1e38f) lp = dot + bias - lse;      // a mask of the type's lowest value
+    else lp = (mine - m2 - l2s) * CT_LN2;
+  }
   if (lane == 0) {
     if (!ok && y != -1 && err) atomicOr(err, RX_ERR_INDEX);
     a.logprob[row] = lp;
     a.lse[row] = lse;
-    if (a.stats) reinterpret_cast<float2*>(a.stats)[row] = make_float2(empty ? CT_NINF : m2, l2s);      // -inf: no item left
+    // -inf: no item left.  Of p_y and 1 - p_y the smaller, the second one with its sign changed.
+    if (a.stats)
+      reinterpret_cast<float4*>(a.stats)[row] = make_float4(empty ? CT_NINF : m2, l2s, sum == 0.f ? 0.f : used / sum * rest, empty ? 0.f : own <= others ? own / s : -rest);
   }
 }
 
@@ -746,29 +787,35 @@ template <typename T>
 __global__ void __launch_bounds__(CT_THREADS) ct_prep_kernel(CtPrep a) {
   const int64_t row = (int64_t)blockIdx.x * CT_WAVES + (threadIdx.x >> 6);
   if (row >= a.R) return;
-  const float2 st = reinterpret_cast<const float2*>(a.stats)[row];
+  const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
   int64_t y = a.targets[row];
   const bool dead = st.x == CT_NINF;
   if (dead || y < 0 || y >= a.V || (a.bias && a.bias[y] == CT_NINF)) y = -1;      // nothing depends on such a target
   const float g = y >= 0 && a.g ? a.g[row] : 0.f;
-  const float c = dead ? 0.f : (a.gl ? a.gl[row] : 0.f) - g;
+  const float gl = dead || !a.gl ? 0.f : a.gl[row], c = gl - g;
+  const bool none = g == 0.f && gl == 0.f;                  // such a row may hold anything
+  const bool sure = __float_as_uint(st.w) >> 31;            // see the forward pass
+  const float py = sure ? 1.f + st.w : st.w, rest = sure ? -st.w : 1.f - st.w;
+  const float share = none || y < 0 ? 0.f : fmaf(g, rest, gl * py);
   if (rx_lane() == 0 && a.rows) {
     CtRow r;
     r.sgn = c < 0.f ? -1.f : 1.f;
-    r.m2 = dead ? 0.f : st.x;
+    r.m2 = dead || none ? 0.f : st.x;
     r.l2s = c == 0.f ? __builtin_inff() : st.y - log2f(fabsf(c));
     r.z = r.m2 + r.l2s;
-    r.g = g;
-    r.y = g != 0.f ? (int32_t)y : -1;      // without a share the target may be as unlikely as it likes (NaN stays)
-    r.gl2 = log2f(fabsf(g));
+    r.q = share;
+    r.y = (int32_t)y;
+    r.ql2 = log2f(fabsf(share));
     r.pad = 0;
     a.rows[row] = r;
-    a.marks[row] = c == 0.f && g == 0.f;
+    a.marks[row] = none;
   }
   if (a.dx) {
+    const float q = none || y < 0 ? 0.f : fmaf(g, st.z, gl * py);       // under the weights that the mean has
     const T* t = (const T*)a.t + (y < 0 ? 0 : y) * a.ld_t;
     for (int d = rx_lane(); d < a.D; d += 64) {
-      const float v = (y < 0 ? 0.f : g * ct_elem(t + d)) + (c == 0.f ? 0.f : c * a.mean[row * a.D + d]);
+      float v = c == 0.f ? 0.f : c * a.mean[row * a.D + d];
+      if (y >= 0 && !none) v = fmaf(q, ct_elem(t + d), v);
       if constexpr (sizeof(T) == 4) ((float*)a.dx)[row * a.D + d] = v;
       else ((uint16_t*)a.dx)[row * a.D + d] = (uint16_t)ct_pk(v, v);
     }
@@ -808,7 +855,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
     stage.load_marks(a.marks, r);
     if (threadIdx.x < BN) {
       if (r + threadIdx.x < r1) info = a.rows[r + threadIdx.x];
-      else { info.m2 = 0.f; info.l2s = info.z = __builtin_inff(); info.sgn = 1.f; info.g = 0.f; info.gl2 = CT_NINF; info.y = -1; }
+      else { info.m2 = 0.f; info.l2s = info.z = __builtin_inff(); info.sgn = 1.f; info.q = 0.f; info.ql2 = CT_NINF; info.y = -1; }
     }
   };
   auto publish = [&](int i) {      // before the barrier in front of put(i): the largest magnitude, the sign words
@@ -834,9 +881,9 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
       float* p = lz + threadIdx.x;
       p[0] = BIAS ? info.m2 : info.z - kt;
       if (BIAS) { p[BN] = info.l2s - kt; p[2 * BN] = info.sgn * (PL == 2 ? scale * CT_UNIT : scale); }   // sign of c, with the tile's scale undone
-      p[3 * BN] = info.g * info.sgn;
+      p[3 * BN] = info.q * info.sgn;
       p[4 * BN] = __int_as_float(info.y);
-      p[6 * BN] = info.gl2 + kt;
+      p[6 * BN] = info.ql2 + kt;
     }
     uint16_t* rm = reinterpret_cast<uint16_t*>(ct_lds + (i & 1) * Tile::BYTES);
     stage.store(rm, rm + Tile::RM, reinterpret_cast<const uint32_t*>(lz + 5 * BN), scale);
@@ -871,7 +918,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
     const uint16_t* rm = reinterpret_cast<const uint16_t*>(ct_lds + (i & 1) * Tile::BYTES);
     const uint16_t* tr = rm + Tile::RM;
     const float* lz = lz0 + (i & 1) * 7 * BN;             // z, or m2 with a bias
-    const float *ll = lz + BN, *lsg = lz + 2 * BN, *lg = lz + 3 * BN, *lgl = lz + 6 * BN;
+    const float *ll = lz + BN, *lsg = lz + 2 * BN, *lq = lz + 3 * BN, *lql = lz + 6 * BN;
     const float* ly = lz + 4 * BN;                        // int32 targets
     const float kt = PL == 2 ? -ct_log2(scale) : 0.f, back = ct_inverse(scale);
     // rows of this tile whose target is among the wavefront's items
@@ -892,7 +939,6 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
           const int k = it * 32 + 8 * (e / 4) + 4 * h;
           if constexpr (BIAS) w[e] = (fmaf(s[e], mul, b2[mb]) - ct_at(lz + k, e % 4)) - ct_at(ll + k, e % 4);
           else w[e] = fmaf(s[e], mul, -ct_at(lz + k, e % 4));
-          if (PL == 2) mx = fmaxf(mx, w[e]);
         }
         const int32_t mine = (int32_t)(item0 + mb * 32 + l31);
         if constexpr (PL == 2) {
@@ -900,9 +946,11 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const int k = it * 32 + 8 * (e / 4) + 4 * h;
-              mx = fmaxf(mx, __float_as_int(ct_at(ly + k, e % 4)) == mine ? ct_at(lgl + k, e % 4) : CT_NINF);
+              w[e] = __float_as_int(ct_at(ly + k, e % 4)) == mine ? ct_at(lql + k, e % 4) : w[e];
             }
           }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, w[e]);
           if (__ballot(mx > ref[mb] + CT_TOP(PL))) {
             const float n = fmaxf(mx, __shfl_xor(mx, 32, 64));
             if (n > ref[mb] + CT_TOP(PL)) {
@@ -922,13 +970,13 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
         const float rf = ref[mb] == CT_NINF ? 0.f : ref[mb];
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e] = __builtin_amdgcn_exp2f(PL == 2 ? w[e] - rf : w[e]);
-        if (hit) {                // the target's own share: sgn(c) g on top of |c| p, both still to meet sgn(c) x
-          // two factors: g 2^(kt - ref) is below 2^CT_TOP where g counts, 2^(kt - ref) alone is out of range for a g below 2^-114
-          const float up = PL == 2 ? __builtin_amdgcn_exp2f(0.5f * (kt - rf)) : 1.f;
+        if (hit) {                // a row's own target: sgn(c) q in place of |c| p, still to meet sgn(c) x
+          // two factors: q 2^(kt - ref) is below 2^CT_TOP, 2^(kt - ref) alone is out of range for a q below 2^-114 (and for 0 anything)
+          const float up = PL == 2 ? __builtin_amdgcn_exp2f(fminf(0.5f * (kt - rf), 126.f)) : 1.f;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int k = it * 32 + 8 * (e / 4) + 4 * h;
-            const float share = PL == 2 ? fmaf(ct_at(lg + k, e % 4) * up, up, w[e]) : ct_at(lg + k, e % 4) + w[e];
+            const float share = PL == 2 ? ct_at(lq + k, e % 4) * up * up : ct_at(lq + k, e % 4);
             w[e] = __float_as_int(ct_at(ly + k, e % 4)) == mine ? share : w[e];
           }
         }
@@ -942,7 +990,7 @@ __global__ void __launch_bounds__(NW * 64, OCC) ct_bwd_kernel(CtBwd a) {
           ct_add((part[0] + part[1]) + (part[2] + part[3]), &dbias[mb], &lost[mb]);
         }
         ct_weigh<PL, DP, BN>(tr, it, w, o[mb]);
-        if (PL == 1 && hit) {     // a target's share is as large as the whole gradient: what bf16 dropped of these weights goes in too
+        if (PL == 1 && hit) {     // a target's share may be as large as the whole gradient: what bf16 dropped of these weights goes in too
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             const uint32_t u = ct_pk(w[e], w[e + 1]);
@@ -1074,6 +1122,9 @@ static CtPlan ct_plan(int64_t fixed, int64_t moving, int bm, int bn, int slots, 
   return p;
 }
 
+static size_t ct_rest_at(const CtPlan& p, int64_t R) { return rx_align_up((size_t)p.n_split * R * sizeof(float2), 256); }
+static size_t ct_out_at(const CtPlan& p, int64_t R, int bf16) { return ct_rest_at(p, R) + (bf16 ? rx_align_up((size_t)p.n_split * R * 4, 256) : 0); }
+
 static int ct_check(const rx_catalog_args* a, const char* who) {
   RX_REQUIRE(a, "%s: null argument", who);
   RX_REQUIRE(a->R >= 0 && a->R <= (1 << 24) && a->V >= 1 && a->V <= (1ll << 30) && a->D >= 1 && a->D <= CT_MAXD,
@@ -1104,7 +1155,7 @@ static CtPlan ct_bwd_plan(int64_t R, int64_t V, int D, int bf16, bool bias) {
 extern "C" size_t rx_catalog_fwd_workspace_bytes(int64_t R, int64_t V, int32_t D, int32_t bf16, int32_t want_mean) {
   if (R <= 0 || V <= 0 || D < 1 || D > CT_MAXD) return 0;
   const CtPlan p = ct_fwd_plan(R, V, D, bf16);
-  return rx_align_up((size_t)p.n_split * R * sizeof(float2), 256) + (want_mean ? (size_t)p.n_split * R * D * 4 : 0);
+  return want_mean ? ct_out_at(p, R, bf16) + (size_t)p.n_split * R * D * 4 : ct_rest_at(p, R);
 }
 extern "C" size_t rx_catalog_bwd_workspace_bytes(int64_t R, int64_t V, int32_t D, int32_t bf16, int32_t want_bias) {
   if (R <= 0 || V <= 0 || D < 1 || D > CT_MAXD) return 0;
@@ -1150,21 +1201,22 @@ extern "C" int rx_catalog_fwd(const rx_catalog_args* args, float* d_logprob, flo
   const rx_catalog_args a = *args;
   if (a.R == 0) return 0;
   RX_REQUIRE(d_logprob && d_lse, "rx_catalog_fwd: null output");
-  RX_REQUIRE(((uintptr_t)d_stats & 7) == 0, "rx_catalog_fwd: stats must be 8-byte aligned");
+  RX_REQUIRE(((uintptr_t)d_stats & 15) == 0, "rx_catalog_fwd: stats must be 16-byte aligned");
   const size_t need = rx_catalog_fwd_workspace_bytes(a.R, a.V, a.D, a.bf16, d_mean != nullptr);
   RX_REQUIRE(ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0, "rx_catalog_fwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
   RX_GUARD_DEVICE(device);
   const CtPlan p = ct_fwd_plan(a.R, a.V, a.D, a.bf16);
   float2* part = (float2*)ws;
-  float* out = d_mean ? (float*)((uint8_t*)ws + rx_align_up((size_t)p.n_split * a.R * sizeof(float2), 256)) : nullptr;
-  CtFwd f = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, a.D, p.tiles, p.n_split, p.per_split, part, out};
+  float* rest = d_mean ? (float*)((uint8_t*)ws + ct_rest_at(p, a.R)) : nullptr;
+  float* out = d_mean ? (float*)((uint8_t*)ws + ct_out_at(p, a.R, a.bf16)) : nullptr;
+  CtFwd f = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, a.D, p.tiles, p.n_split, p.per_split, a.targets, part, rest, out};
   hipStream_t st = (hipStream_t)stream;
 #define CT_GO(...) ct_pick_fwd<__VA_ARGS__>(f, st)
   const int rc = CT_KERNELS(CT_GO, a.bf16, ct_dp(a.D));
 #undef CT_GO
   if (rc) return rc;
   RX_LAUNCH_CHECK();
-  CtJoin j = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, a.targets, a.D, p.n_split, part, out, d_logprob, d_lse, d_stats, d_mean};
+  CtJoin j = {a.x, a.table, a.ld_x, a.ld_t, a.R, a.V, a.bias, a.targets, a.D, p.n_split, part, rest, out, d_logprob, d_lse, d_stats, d_mean};
   const bool few = p.n_split <= 8;
   auto join = few ? (a.bf16 ? ct_join_kernel<uint16_t, 64> : ct_join_kernel<float, 64>)
                   : (a.bf16 ? ct_join_kernel<uint16_t, 256> : ct_join_kernel<float, 256>);
@@ -1179,7 +1231,7 @@ extern "C" int rx_catalog_bwd(const rx_catalog_args* args, const float* d_stats,
   if (ct_check(args, "rx_catalog_bwd")) return 1;
   const rx_catalog_args a = *args;
   if (a.R == 0) return 0;
-  RX_REQUIRE(d_stats && ((uintptr_t)d_stats & 7) == 0, "rx_catalog_bwd: stats missing or not 8-byte aligned");
+  RX_REQUIRE(d_stats && ((uintptr_t)d_stats & 15) == 0, "rx_catalog_bwd: stats missing or not 16-byte aligned");
   RX_REQUIRE(!d_dx || d_mean, "rx_catalog_bwd: the gradient of x needs the means of the forward call");
   RX_REQUIRE(!d_dbias || (a.bias && d_dtable), "rx_catalog_bwd: the bias gradient needs a bias and comes with the table's");
   RX_REQUIRE(!a.bias || !d_dtable || d_dbias, "rx_catalog_bwd: with a bias the table's gradient comes with the bias gradient");

@@ -1530,7 +1530,7 @@ def catalog_fwd(x: Tensor, table: Tensor, targets: Tensor, bias: Optional[Tensor
     dev = x.device
     f = lambda *shape: torch.empty(*shape, dtype=torch.float32, device=dev)
     logprob, lse = f(a.R), f(a.R)
-    stats = f(a.R, 2) if want_stats else None
+    stats = f(a.R, 4) if want_stats else None
     mean = f(a.R, a.D) if want_mean else None
     ws = _ws(int(lib.rx_catalog_fwd_workspace_bytes(a.R, a.V, a.D, a.bf16, int(want_mean))), dev)
     check(lib.rx_catalog_fwd(C.byref(a), _p(logprob), _p(lse), _p(stats), _p(mean), _p(ws), ws.numel(), _p(_err_flag(dev)), _dev(x),
@@ -1545,8 +1545,8 @@ def catalog_bwd(x: Tensor, table: Tensor, targets: Tensor, bias: Optional[Tensor
     forward call's stats and mean (rx_catalog_bwd).  With a bias its gradient comes with the table's."""
     a = _catalog_args(x, table, targets, bias)
     _req(stats, torch.float32, "stats", 2)
-    if tuple(stats.shape) != (a.R, 2):
-        raise ValueError(f"stats: expected shape [{a.R}, 2], got {tuple(stats.shape)}")
+    if tuple(stats.shape) != (a.R, 4):
+        raise ValueError(f"stats: expected shape [{a.R}, 4], got {tuple(stats.shape)}")
     if want_x:
         if mean is None:
             raise ValueError("the gradient of x needs the means of the forward call")
