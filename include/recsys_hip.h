@@ -817,6 +817,7 @@ int rx_logprob_bwd(const rx_logprob_args* args, const float* d_g_logprob, const 
  * or no gradient of its lse): such a row may hold anything.  A target of -1 stands for "no target" (logprob 0, no
  * gradient through it); any other target outside [0, V) sets RX_ERR_INDEX and gives NaN.  A bias of -inf takes an item
  * out, whatever its vector holds; a target that is out gives -inf and no gradient, and a row with no item left gives lse -inf and no gradient.
+ * A bias of NaN or +inf makes every row NaN; finite ones beyond +-2.07e38 count as that (masks of the type's lowest value).
  * `stats` [R, 4] (16-byte aligned) and `mean` [R, D] fp32 (both may be NULL) are what rx_catalog_bwd needs: the row's softmax
  * reference and sum, rest_r = sum_{v != y_r} p_rv (of bf16's rounded weights with the mean), the smaller of p_{r, y_r} and
  * -(1 - p_{r, y_r}) by size; and mean_r = sum_{v != y_r} p_rv t_v (only for the gradient of x).

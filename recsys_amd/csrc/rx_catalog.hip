@@ -438,8 +438,8 @@ __device__ __forceinline__ float ct_at(const float* p, int e) {
   const float4 f = *reinterpret_cast<const float4*>(p);
   return e == 0 ? f.x : e == 1 ? f.y : e == 2 ? f.z : f.w;
 }
-__device__ __forceinline__ float ct_bias2(float b) {      // bias in log2 units; -inf stays, anything else stays finite
-  return b == CT_NINF ? CT_NINF : fminf(fmaxf(b * CT_L2E, -CT_LIM), CT_LIM);
+__device__ __forceinline__ float ct_bias2(float b) {      // bias in log2 units; what is finite stays finite, infinities and NaN stay what they are
+  return fabsf(b) < __builtin_inff() ? fminf(fmaxf(b * CT_L2E, -CT_LIM), CT_LIM) : b;
 }
 
 // Which split and which stationary tile a workgroup takes.  Workgroups are dealt to the 8 XCDs in turn; with the splits
