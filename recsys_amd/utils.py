@@ -50,7 +50,8 @@ def recommend(model, inputs, k=10, exclude=None):
     """The ``k`` best items of every row of ``inputs`` with their log-probabilities: (codes [B, k] int64, logprob [B, k], entropy
     [B]), best first, the lower code first among equal scores; (-1, -inf) where a row has fewer items.  Over the whole
     catalogue when ``inputs["item_code"]`` is None (models that score every item then), else over each row's own candidates.
-    ``exclude`` [B, E]: positions in the score row (codes, for the whole catalogue) left out; -1 = nothing."""
+    ``exclude`` [B, E]: positions in the score row (codes, for the whole catalogue) left out; -1 = nothing.  One out of range
+    is an IndexError; a recording cannot raise, there it is nothing as well."""
     from . import autograd as rxa
     with torch.no_grad():
         scores = model(inputs)
@@ -61,9 +62,9 @@ def recommend(model, inputs, k=10, exclude=None):
                 raise ValueError(f"exclude: expected shape [{B}, E], got {tuple(exclude.shape)}")
             if not torch.cuda.is_current_stream_capturing() and exclude.numel() and bool(((exclude < -1) | (exclude >= V)).any()):
                 raise IndexError("exclude: position out of range")
-            # a spare last column takes the -1 entries
+            # a spare last column takes the -1 entries, and in a recording whatever a replay finds out of range
             wide = torch.cat([scores, scores.new_zeros(B, 1)], 1)
-            wide.scatter_(1, torch.where(exclude < 0, torch.full_like(exclude, V), exclude), float("-inf"))
+            wide.scatter_(1, torch.where((exclude < 0) | (exclude >= V), torch.full_like(exclude, V), exclude), float("-inf"))
             scores = wide[:, :V]
         none = torch.full((B,), -1, dtype=torch.int64, device=scores.device)
         out = rxa.log_probs(scores, none, k=k)
