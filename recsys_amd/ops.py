@@ -1592,6 +1592,14 @@ def _apart(who: str, reads: Sequence[Tensor], writes: Sequence[Tensor]) -> None:
         wend = max(wend, hi) if written else wend
 
 
+def _ortho_size(who: str, i: int, m: Tensor) -> None:
+    """Refused here, not by the library: it sees a long list chunk by chunk, the first of them stepped already."""
+    if m.numel() == 0:
+        raise ValueError(f"{who}: matrix {i} is empty")
+    if max(m.shape) > ORTHO_MAX_DIM:
+        raise RuntimeError(f"{who}: matrix {i} has shape {tuple(m.shape)}, at most {ORTHO_MAX_DIM} a side")
+
+
 def orthogonalize(mats: Sequence[Tensor], steps: int = 5, coeffs=ORTHO_COEFFS, eps: float = 1e-7,
                   out: Optional[Sequence[Tensor]] = None) -> List[Tensor]:
     """Newton-Schulz orthogonalisation of fp32 matrices (rx_orthogonalize): ``X = G / (|G|_F + eps)``, then ``steps`` times
@@ -1612,8 +1620,7 @@ def orthogonalize(mats: Sequence[Tensor], steps: int = 5, coeffs=ORTHO_COEFFS, e
         _req(o, torch.float32, f"out {i}", 2)
         if m.shape != o.shape:
             raise ValueError(f"orthogonalize: out {i} has shape {tuple(o.shape)}, the matrix {tuple(m.shape)}")
-        if m.numel() == 0:
-            raise ValueError(f"orthogonalize: matrix {i} is empty")
+        _ortho_size("orthogonalize", i, m)
         _same_device(mats[0], m, o)
     _apart("orthogonalize", mats, out)
     for i in range(0, len(mats), _lib.RX_ORTHO_MAX):
@@ -1642,9 +1649,10 @@ def muon_step(ws: Sequence[Tensor], gs: Sequence[Tensor], moms: Sequence[Tensor]
             _req(t, torch.float32, f"{name} {i}", 2)
             if t.shape != w.shape:
                 raise ValueError(f"muon_step: {name} {i} has shape {tuple(t.shape)}, the weight {tuple(w.shape)}")
-        if w.numel() == 0:
-            raise ValueError(f"muon_step: matrix {i} is empty")
+        _ortho_size("muon_step", i, w)
         _same_device(ws[0], w, g, m)
+    if not 1 <= steps <= 32:
+        raise ValueError(f"muon_step: steps={steps} (1..32)")
     if scale is not None:
         _req(scale, torch.float32, "scale")
         if scale.numel() != 1:
