@@ -855,7 +855,7 @@ int rx_catalog_bwd(const rx_catalog_args* args, const float* d_stats, const floa
  * which drives the singular values of G towards 1 and leaves its singular vectors.  Products to fp32 accuracy; the arrays of
  * matrices beyond one workgroup's reach are held to 2^-22 of each element or 2^-39 of their norm's bound, the larger (it is the
  * second for matrices whose norm is orders of magnitude below eps).
- * At most RX_ORTHO_MAX matrices per call, none empty, rows and cols up to 16384.  A matrix of zeros gives zeros.
+ * At most RX_ORTHO_MAX matrices per call, none empty, rows and cols up to 16384; eps >= 0.  A matrix of zeros gives zeros.
  * Coefficients under which singular values in [0, 1] grow past 16 within the steps are refused.
  * The dense half of a train step (the reference steps every tower with Adam, recsys/pipelines/neuralcf/neumf.py:10). */
 #define RX_ORTHO_MAX 24

@@ -75,6 +75,11 @@ __device__ __forceinline__ float ns_update(float g, float* m, float mu, int nest
   *m = fmaf(mu, *m, g);
   return nesterov ? fmaf(mu, *m, g) : *m;
 }
+// what a matrix is divided by; 1 for zeros without an eps
+__device__ __forceinline__ float ns_divisor(double ss, float eps) {
+  const float d = (float)(sqrt(ss) + (double)eps);
+  return d == 0.f ? 1.f : d;
+}
 static inline int ns_up(int x, int a) { return (x + a - 1) / a * a; }
 // LDS of one matrix: X as fp32 [mp][np + 4], A and B as planes [2][mp][mp + 8], and where fewer tiles of A than wavefronts
 // exist, a 32 x 36 partial tile per wavefront.  (m <= 16: see ns_tiny_run.)
@@ -335,7 +340,7 @@ __global__ void __launch_bounds__(NS_SMALL_THREADS) ns_small_kernel(NsSmall a) {
   __syncthreads();
   ss = 0.0;
   for (int w = 0; w < NS_SMALL_THREADS / 64; ++w) ss += part[w];
-  const float div = (float)(sqrt(ss) + (double)a.eps);
+  const float div = ns_divisor(ss, a.eps);
   for (int r = wave; r < m; r += NS_SMALL_THREADS / 64)
     for (int c = lane; c < n; c += 64) X[r * ldx + c] = X[r * ldx + c] / div * a.sx;
   __syncthreads();
@@ -425,7 +430,7 @@ __global__ void __launch_bounds__(RX_BLOCK) ns_init_kernel(NsList a) {
   if (rx_lane() == 0) wsum[threadIdx.x >> 6] = ss;
   __syncthreads();
   ss = ((wsum[0] + wsum[1]) + wsum[2]) + wsum[3];
-  const float div = (float)(sqrt(ss) + (double)a.eps);
+  const float div = ns_divisor(ss, a.eps);
   const float sc = a.scale ? *a.scale : 1.f;
   const int r0 = b / (t.np / 64) * 64, c0 = b % (t.np / 64) * 64;      // of X
   const bool flip = t.rows > t.cols;
@@ -708,6 +713,11 @@ struct NsArgs {                // rx_ortho_args and rx_muon_args in one form
   const float* scale;
 };
 
+static int ns_check_eps(const char* who, float eps) {
+  RX_REQUIRE(eps >= 0.f, "%s: eps=%g is negative", who, (double)eps);      // the scales count on |G|_F / (|G|_F + eps) <= 1
+  return 0;
+}
+
 static int ns_check(const char* who, const int32_t* rows, const int32_t* cols, int count, int steps) {
   RX_REQUIRE(count >= 0 && count <= RX_ORTHO_MAX, "%s: %d matrices (at most %d)", who, count, RX_ORTHO_MAX);
   RX_REQUIRE(steps >= 1 && steps <= 32, "%s: steps=%d (1..32)", who, steps);
@@ -925,7 +935,7 @@ extern "C" size_t rx_orthogonalize_workspace_bytes(const rx_ortho_args* a) {
 
 extern "C" int rx_orthogonalize(const rx_ortho_args* args, void* ws, size_t ws_bytes, int device, void* stream) {
   RX_REQUIRE(args, "rx_orthogonalize: null argument");
-  if (ns_check("rx_orthogonalize", args->rows, args->cols, args->count, args->steps)) return 1;
+  if (ns_check("rx_orthogonalize", args->rows, args->cols, args->count, args->steps) || ns_check_eps("rx_orthogonalize", args->eps)) return 1;
   NsArgs a;
   memset(&a, 0, sizeof(a));
   for (int i = 0; i < args->count; ++i) {
@@ -952,7 +962,7 @@ extern "C" size_t rx_muon_step_workspace_bytes(const rx_muon_args* a) {
 
 extern "C" int rx_muon_step(const rx_muon_args* args, void* ws, size_t ws_bytes, int device, void* stream) {
   RX_REQUIRE(args, "rx_muon_step: null argument");
-  if (ns_check("rx_muon_step", args->rows, args->cols, args->count, args->steps)) return 1;
+  if (ns_check("rx_muon_step", args->rows, args->cols, args->count, args->steps) || ns_check_eps("rx_muon_step", args->eps)) return 1;
   RX_REQUIRE(((uintptr_t)args->scale & 3) == 0, "rx_muon_step: unaligned scale");
   NsArgs a;
   memset(&a, 0, sizeof(a));
