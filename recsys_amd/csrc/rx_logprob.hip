@@ -331,12 +331,31 @@ lp_small_kernel(rx_logprob_args a, int32_t* err) {
 // ---------------------------------------------------------------- wide rows
 struct LpAcc {
   float raw, m2, s, t;
-  __device__ __forceinline__ void init() { raw = LP_NINF; m2 = -LP_FLOOR; s = 0.f; t = 0.f; }
+  float lost;                  // what the last addition to s rounded away
+  __device__ __forceinline__ void init() { raw = LP_NINF; m2 = -LP_FLOOR; clear(); }
+  __device__ __forceinline__ void clear() { s = 0.f; t = 0.f; lost = 0.f; }
   __device__ __forceinline__ void rebase(float n) {          // move the reference up to n (log2 units)
     const float d = fmaxf(m2 - n, -1e4f), f = lp_exp2(d);    // clamped: f is 0 there, and its factor stays finite
     t = (t + s * d) * f;
     s *= f;
+    lost *= f;
     m2 = n;
+  }
+  // s and t of N scores d log2 units from the reference: in four sums each, then with the rounding that the last addition to s
+  // lost.  One by one, near-equal weights would all round the same way (4e-5 of the sum after 4000 of them).
+  template <int N, typename F>
+  __device__ __forceinline__ void join(F distance) {
+    float a[4] = {}, b[4] = {};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float d = distance(i), e = lp_exp2(d);
+      a[i & 3] += e;
+      b[i & 3] = fmaf(e, fmaxf(d, -1e4f), b[i & 3]);       // a masked score: e = 0 times a finite number
+    }
+    const float add = ((a[0] + a[1]) + (a[2] + a[3])) - lost, n = s + add;
+    lost = (n - s) - add;
+    s = n;
+    t += (b[0] + b[1]) + (b[2] + b[3]);
   }
   template <int N>
   __device__ __forceinline__ float add(const float* v) {     // returns the largest of v
@@ -350,24 +369,14 @@ struct LpAcc {
     if (__ballot(grow)) {
       if (grow) rebase(n2);
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float d = fmaf(v[i], LP_L2E, -m2), e = lp_exp2(d);
-      s += e;
-      t = fmaf(e, fmaxf(d, -1e4f), t);
-    }
+    join<N>([&](int i) { return fmaf(v[i], LP_L2E, -m2); });
     return mx;
   }
   // rows beyond LP_BIG (e.g. masks of the type's lowest value with nothing else in the row): the same sums relative to
   // the known maximum
   template <int N>
   __device__ __forceinline__ void add_big(const float* v, float m) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float d = (v[i] - m) * LP_L2E, e = lp_exp2(d);
-      s += e;
-      t = fmaf(e, fmaxf(d, -1e4f), t);
-    }
+    join<N>([&](int i) { return (v[i] - m) * LP_L2E; });
   }
 };
 
@@ -479,7 +488,7 @@ lp_wide_kernel(rx_logprob_args a, LpPart* parts, uint64_t* lists, int n_split, i
 #pragma unroll
   for (int w = 0; w < W; ++w) raw = fmaxf(raw, top_of[w]);
   if (fabsf(raw) > LP_BIG && fabsf(raw) < __builtin_inff()) {
-    acc.s = 0.f; acc.t = 0.f;
+    acc.clear();
     lp_stream<T>(l, n, split, n_split, [&](const float* v, int32_t) { acc.add_big<2 * N>(v, raw); });
   } else {
     lp_move(-fmaf(raw == LP_NINF ? 0.f : raw, LP_L2E, -acc.m2), &acc.s, &acc.t);
