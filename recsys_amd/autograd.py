@@ -1108,6 +1108,28 @@ def gather_rows(table: Tensor, idx: Tensor) -> Tensor:
     return GatherConcat.apply([(0, idx, 0, 1, 1, 0, 0)], idx.shape[0], table.shape[1], table)
 
 
+class ScaleColumns(Function):
+    """x [B, D] times w [1, D].  The gradient of w is a product with a column of ones: torch's sum over the batch records a
+    memset from some thousand rows on, which a recorded step must not hold."""
+
+    @staticmethod
+    def forward(ctx, x, w):
+        ctx.save_for_backward(x, w)
+        return x * w
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x, w = ctx.saved_tensors
+        dx = g * w if ctx.needs_input_grad[0] else None
+        dw = ops.linear_bwd_w(torch.ones(x.shape[0], 1, device=x.device), g * x, want_bias=False)[0] if ctx.needs_input_grad[1] else None
+        return dx, dw
+
+
+def scale_columns(x: Tensor, w: Tensor) -> Tensor:
+    return ScaleColumns.apply(x, w)
+
+
 # ------------------------------------------------------------------ softmax over a whole catalogue
 def all_rows(n_rows: int, device) -> SortedIndex:
     """The index list 0 .. n_rows - 1 as its own sort, for a gradient that touches every row of a table."""

@@ -65,7 +65,7 @@ class GMF(HotPathModule):
 
     def _catalog_query(self, inputs):
         users = as_index(inputs["user_code"], "user_code")
-        return rxa.gather_rows(self.user_embedding.weight, users) * self.linear.weight, self.item_embedding.weight, None
+        return rxa.scale_columns(rxa.gather_rows(self.user_embedding.weight, users), self.linear.weight), self.item_embedding.weight, None
 
     def forward(self, inputs, pointwise=False):
         users = as_index(inputs["user_code"], "user_code")
