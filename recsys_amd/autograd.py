@@ -1154,6 +1154,11 @@ def full_table_backward(param: Tensor, grad: Tensor):
     return table_backward(param, si, grad.reshape(rows, -1), dim=grad.numel() // rows)
 
 
+def _moves(params):
+    """How often the fused optimizers of these parameters have stepped them."""
+    return tuple(rule.moves if rule is not None else 0 for rule in (getattr(p, "_rx_sparse", None) for p in params))
+
+
 class CatalogLogProb(Function):
     """ops.catalog_fwd with its gradients (rx_catalog_bwd) to x, the table and the bias."""
 
@@ -1164,6 +1169,7 @@ class CatalogLogProb(Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, table, targets, bias, stats, mean)
         ctx.params = (table, bias)         # the objects that may carry a sparse rule
+        ctx.moves = _moves(ctx.params)
         return logprob, lse
 
     @staticmethod
@@ -1173,6 +1179,9 @@ class CatalogLogProb(Function):
         need_x, need_t, _, need_b = ctx.needs_input_grad
         if g is None and gl is None:
             return None, None, None, None
+        if _moves(ctx.params) != ctx.moves:
+            raise RuntimeError("catalog_logprob: the table or the bias has moved since the forward pass (a fused optimizer without a "
+                               "clip steps inside the backward pass: one backward pass per forward pass, or a clip_norm)")
         g, gl = (None if t is None else t.contiguous() for t in (g, gl))
         dx, dt, db = ops.catalog_bwd(x, table, targets, bias, stats, mean, g, gl, want_x=need_x, want_table=need_t or need_b)
         dt = full_table_backward(ctx.params[0], dt) if need_t else None
@@ -1184,7 +1193,7 @@ def catalog_logprob(x: Tensor, table: Tensor, targets: Tensor, bias: Optional[Te
     """(logprob [R], lse [R]): log-probabilities of one item per row (-1 = none) under the softmax over all rows of ``table``
     of ``x @ table.T + bias``, and the log-sum-exp.  ``x`` [R, D] and ``table`` [V, D] both fp32 or both bf16, D <= 256,
     ``bias`` [V] fp32; the [R, V] scores are never stored.  Differentiable in all three (a table with a fused sparse rule
-    takes its step, on every row)."""
+    takes its step, on every row; a backward pass that finds the table moved since its forward pass is refused)."""
     if x.dim() == 2 and ((x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
         x = x.contiguous()
     targets = targets.contiguous()

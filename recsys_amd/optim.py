@@ -45,6 +45,7 @@ class SparseRule:
         self.kind, self.mode, self.lr, self.eps, self.owner = kind, _MODES[kind], lr, eps, owner
         self.state: Optional[torch.Tensor] = None
         self.every_row = None      # autograd.full_table_backward: the list of all rows, laid out once
+        self.moves = 0             # steps the table has taken: a backward pass that reads it again looks whether it moved
 
     def _state_for(self, param):
         if self.kind == "sgd":
@@ -53,6 +54,11 @@ class SparseRule:
             shape = param.shape if self.kind == "adagrad" else (param.shape[0],)
             self.state = torch.zeros(shape, dtype=torch.float32, device=param.device)
         return self.state
+
+    def _moved(self, companion=None):
+        self.moves += 1
+        if companion is not None:
+            companion.moves += 1
 
     def apply(self, param, occ, si, dim=None, occ_ld=None, param2=None, occ2=None):
         table = param.data
@@ -65,6 +71,7 @@ class SparseRule:
         if self.owner.clip_norm is None:
             ops.segreduce(occ, si, self.mode, table, state=state, lr=self.lr, eps=self.eps, dim=dim, occ_ld=occ_ld,
                           occ2=occ2, target2=table2, state2=state2)
+            self._moved(rule2)
             return
         # With a clip pending nothing can move before the global norm is known: the reduce itself is
         # left to step(), which takes the tables of equal width in one launch.
@@ -87,6 +94,7 @@ def _rule_apply_fm(self, feat, bias_table, si, tsum, g, n_fields_ex, deep=None, 
         if self.owner.clip_norm is None:
             ops.fg_reduce(tsum, g, si, self.mode, table, state=state, target2=table2, state2=state2,
                           lr=self.lr, eps=self.eps, deep=deep, premultiplied=premultiplied)
+            self._moved(rule2)
             return
         dim = tsum.shape[1]
         sq_out = self.owner._sq_slice(si.n, dim, table.device, ops.fg_reduce_grid(si.n, dim))
@@ -117,6 +125,7 @@ def _rule_apply_fm(self, feat, bias_table, si, tsum, g, n_fields_ex, deep=None, 
     if self.owner.clip_norm is None:
         ops.segreduce_fm(tsum, g, n_fields_ex, si, self.mode, table, state=state, target2=table2, state2=state2,
                          lr=self.lr, eps=self.eps, deep=deep)
+        self._moved(rule2)
         return
     dim = tsum.shape[1]
     if self.owner._pending:
@@ -548,6 +557,8 @@ class FusedOptimizer:
         scale = None
         if self._deferred:
             self._reduce_deferred()
+        for e in self._pending:
+            e[0]._moved(e[5][0] if e[5] is not None else None)
         if self.clip_norm is not None:
             # Global norm.  Dense gradients: one launch leaves fp64 partials for up to 24 tensors;
             # they and the per-block partials of the last table reduce ride in the launch that forms
