@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define RX_ABI_VERSION 1
+#define RX_ABI_VERSION 2      /* 2: stats of rx_catalog_fwd are [R, 4] */
 #define RX_ERR_INDEX 1    /* bit set in *err_flag when an index was out of range */
 #define RX_ERR_CAPACITY 2 /* bit set when a fixed-capacity exchange buffer was too small */
 
