@@ -29,9 +29,10 @@
 // of the rounded weights for rest, so that it is a sum of (t_y - t_v) under them, and the targets' shares q of the table's gradient come
 // with their low part.
 // Scores, references, sums, means and gradients accumulate in fp32.
-// Measured, where a large bf16 product reaches 1151 TFLOP/s: 2048 x 1000003 x 64 fp32 forward 1.72 ms, table gradient 1.83 (914 and
-// 860 TFLOP/s of plane products), 8192 x 100003 x 128 bf16 515 and 600 us (814 and 699).  What keeps them from more is the
-// work beside the products: an exponential, two cuts and a transposed copy.  1024 x 3706 x 64 fp32: 15 and 19 us, latency.
+// Measured under a kernel trace (the calls run about a tenth faster), where a large bf16 product reaches 1151 TFLOP/s and an fp16 one
+// 1105: 2048 x 1000003 x 64 fp32 forward 1.75 ms, table gradient 1.85 (900 and 852 TFLOP/s of plane products), 8192 x 100003 x 128
+// bf16 544 and 600 us (772 and 699).  Matrix unit, vector instructions (an exponential, two cuts, the sums) and LDS (a transposed copy)
+// are each busy for 37 to 55 % of that time; none of them alone is the bound.  1024 x 3706 x 64 fp32: 15 and 19 us, latency.
 #include "rx_common.h"
 
 #include <type_traits>

@@ -14,7 +14,7 @@
 // common case.  Keys order by value, then by the lower column, and are unique, so the result does not depend on
 // how the row was split.
 // Measured: 2048 x 50021 bf16, rows ending anywhere (half of all columns live): forward 30 us (3.4 TB/s), gradient 61 us (5.0 TB/s
-// read and written); 1 x 1000003 fp32, 50 alternatives: 12 us and 7 for the join; 6040 x 100, 10 alternatives: 9.4 us.
+// read and written); 1 x 1000003 fp32, 50 alternatives: 12 us and 6 for the join; 6040 x 100, 10 alternatives: 8.9 us.
 #include "rx_common.h"
 
 #define LP_SMALL 1024        // rows up to this width: one wavefront (or part of one) per row, scores in registers

@@ -14,8 +14,8 @@
 //   * The others share three launches per step, whatever their number.  X, X^T, A and B live in the workspace as planes, cut
 //     once in the epilogue that makes them; with X^T kept beside X all three products read both operands along the
 //     contraction.
-// Measured, where a large bf16 product reaches 1151 TFLOP/s: a step of 3344 x 3344, 1672 x 3344 and 836 x 1672 takes A 175, B 167
-// and X 337 us (821, 767 and 853 TFLOP/s of plane products); one of 1024 x 1024 16 us a product, of 256 x 256 7 us (a launch
+// Measured, where a large fp16 product reaches 1105 TFLOP/s: a step of 3344 x 3344, 1672 x 3344 and 836 x 1672 takes A 169, B 168
+// and X 338 us (850, 762 and 850 TFLOP/s of plane products); one of 1024 x 1024 16 us a product, of 256 x 256 7 us (a launch
 // is 4.5 of them); one workgroup's 64 x 128 33 us for all five steps.
 #include "rx_common.h"
 
