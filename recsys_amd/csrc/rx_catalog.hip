@@ -765,9 +765,10 @@ __global__ void __launch_bounds__(CT_THREADS) ct_join_kernel(CtJoin a, int32_t* 
     if (!ok && y != -1 && err) atomicOr(err, RX_ERR_INDEX);
     a.logprob[row] = lp;
     a.lse[row] = lse;
-    // -inf: no item left.  Of p_y and 1 - p_y the smaller, the second one with its sign changed.
-    if (a.stats)
-      reinterpret_cast<float4*>(a.stats)[row] = make_float4(empty ? CT_NINF : m2, l2s, sum == 0.f ? 0.f : used / sum * rest, empty ? 0.f : own <= others ? own / s : -rest);
+    if (a.stats) {                         // -inf: no item left.  Of p_y and 1 - p_y the smaller, the second one with its sign changed.
+      const float py = empty ? 0.f : own <= others ? own / s : -rest;
+      reinterpret_cast<float4*>(a.stats)[row] = make_float4(empty ? CT_NINF : m2, l2s, sum == 0.f ? 0.f : used / sum * rest, py);
+    }
   }
 }
 

@@ -1,8 +1,10 @@
 """Rows beyond 1024 columns with finite masks of any size, and with all scores far from zero: the results are those of the
-definition in fp64 on the same numbers, as for narrow rows.  Tolerances: those of test_gpu_logprob (its ``_tol`` and ``_ref_grad``),
-which count 8 u of a result's own size; a masked score has weight exp(-1e9) = 0 on both sides.  A weight below the smallest normal
-number, 2^-126 = e^-87.3, is held as zero: its whole gradient, that many times |g_lse| + sum |g| + |g_H| (88 + H), is left out.  A log-probability beyond the largest fp32 number (rows of +-2.3e38) is
--inf, as rounding has it."""
+definition in fp64 on the same numbers, as for narrow rows.
+
+Tolerances: those of test_gpu_logprob (its ``_tol`` and ``_ref_grad``), which count 8 u of a result's own size; a masked score has
+weight exp(-1e9) = 0 on both sides.  A weight below the smallest normal number, 2^-126 = e^-87.3, is held as zero: its whole gradient,
+that many times |g_lse| + sum |g| + |g_H| (88 + H), is left out.  A log-probability beyond the largest fp32 number (rows of
++-2.3e38) is -inf, as rounding has it."""
 import pytest
 import torch
 
